@@ -309,6 +309,91 @@ EBX_API ebx_status ebx_exchange_allreduce(ebx_exchange* ex, const float* partial
                                           int64_t N, const void* bias, void* y, float* y32,
                                           void* stream);
 
+/* ---- 8-bit paged key/value cache -------------------------------------------
+ * No reference counterpart: the reference's caches (mlbricks/cache.py) are whole
+ * 16-bit tensors.  A pool holds for keys and for values int8 codes
+ * [blocks][kv_heads][block_size][head_dim] and one fp32 scale for each (block,
+ * head); value = code * scale.  Row i of a block table (int32 [requests, width])
+ * names the blocks that hold request i's tokens, block_size tokens in each.
+ * All pointers are DEVICE memory; every call is stream-ordered on `device` and
+ * allocates nothing.  A number on the device that is out of range (a block id, a
+ * slot, a length) is never followed: such a token is not written, and not seen. */
+typedef struct {
+    void* k_codes;     /* int8, 16-byte aligned                                   */
+    float* k_scales;   /* fp32 [blocks][kv_heads]                                 */
+    void* v_codes;
+    float* v_scales;
+    int32_t blocks;    /* blocks * kv_heads * block_size <= 2^31 - 1              */
+    int32_t kv_heads;
+    int32_t block_size; /* 16, 32, 64 or 128 tokens                               */
+    int32_t head_dim;  /* 32, 64 or 128                                           */
+    int32_t device;
+    int32_t reserved;
+} ebx_kv_pool;
+
+/* Blocks and slots for one step, from the requests' lengths alone: request i holds
+ * past[i] tokens and adds added[i] >= 0; added[i] < 0 releases it.  Unused blocks
+ * wait in free_ring (int32 [free_size], room for every block of the pool) at places
+ * ring[0] .. ring[1] - 1 modulo free_size.  Requests are served in order: each takes
+ * the blocks that it lacks from the ring's front into its row of `tables`, or, when
+ * they are not there or its row is too short, nothing (its tokens get slot -1 and its
+ * length stays).  Released blocks join the ring's back, for later calls; a released
+ * row's entries are left as they are.
+ * Written: ring_out[4] = {front, back, blocks that were missing, tokens}, lengths
+ * [requests] (after the step; 0 when released), starts[requests + 1] (first token of
+ * each request among the step's tokens), and for t < `tokens` slots[t] = block *
+ * block_size + offset and positions[t] (slot -1, position 0 past the last token).
+ * ring_out and lengths must not overlap ring and past.  requests <= 16384. */
+EBX_API ebx_status ebx_kv_plan(const int32_t* past, const int32_t* added, int32_t requests,
+                               int32_t* tables, int32_t width, int32_t block_size, int32_t* free_ring,
+                               int32_t free_size, const int64_t* ring, int64_t* ring_out,
+                               int32_t* lengths, int32_t* starts, int64_t* slots, int32_t* positions,
+                               int64_t tokens, int32_t device, void* stream);
+
+/* Quantise `tokens` new keys and values [tokens, kv_heads, head_dim] (dtype 1 = fp16,
+ * 2 = bf16; token and head strides in elements, multiples of 8, 16-byte aligned) into
+ * their slots; tokens whose slot is negative or past the pool are skipped.  For each
+ * block and head: scale = max(old scale, max |x| / 127), code = rint(x / scale), where
+ * the old scale counts when the call's first token in the block is not the block's
+ * first; the tokens before it then move to a larger scale by rint(code * old / new).
+ * A block's tokens of one call are consecutive, and all behind those written before.
+ * A value that is not finite makes the scale of its block and head NaN. */
+EBX_API ebx_status ebx_kv_append(const ebx_kv_pool* pool, const void* k, int64_t k_token_stride,
+                                 int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                                 int64_t v_head_stride, const int64_t* slots, int64_t tokens,
+                                 int32_t dtype, void* stream);
+
+/* Keys and values back as code * scale, rounded once to dtype (0 = fp32, 1 = fp16,
+ * 2 = bf16): k, v [tokens, kv_heads, head_dim]; row t is place first[i] + t - starts[i]
+ * (first NULL: 0) of the request i with starts[i] <= t < starts[i + 1].  Rows of no
+ * request, and places without a block, are 0. */
+EBX_API ebx_status ebx_kv_materialize(const ebx_kv_pool* pool, const int32_t* tables, int32_t width,
+                                      const int32_t* starts, const int32_t* first, int32_t requests,
+                                      int64_t tokens, int32_t dtype, void* k, void* v, void* stream);
+
+/* Workspace bytes of ebx_kv_attention (partial results of split rows). */
+EBX_API uint64_t ebx_kv_attention_workspace_bytes(const ebx_kv_pool* pool);
+
+/* Attention of the new tokens' queries over the cache: request i's queries are rows
+ * starts[i] .. starts[i + 1] - 1 of q [tokens, heads, head_dim] (strides and dtype as in
+ * ebx_kv_append), at the last positions of its lengths[i] tokens; query head h reads
+ * key/value head h / (heads / kv_heads).  A query at position p sees keys j with
+ * first[i] <= j (first may be NULL) and j < lengths[i], and if causal j <= p, and if
+ * window > 0 (causal only) j > p - window.
+ *     out[t, h] = softmax_j(scale * q . k_j) v_j,  lse[t, h] = log sum_j exp(...)
+ * out [tokens, heads, head_dim] in q's dtype, lse fp32 (may be NULL); a query that sees
+ * nothing gets out = 0 and lse = -infinity.  Sums, maxima and scales are fp32, the
+ * weights of the values fp16.  max_new / max_length (0: unknown) are the largest number
+ * of new tokens and the largest length of a request where the caller knows them; they
+ * choose the kernel and never change what is computed. */
+EBX_API ebx_status ebx_kv_attention(const ebx_kv_pool* pool, const void* q, int64_t q_token_stride,
+                                    int64_t q_head_stride, int32_t heads, int32_t dtype,
+                                    const int32_t* tables, int32_t width, const int32_t* lengths,
+                                    const int32_t* starts, const int32_t* first, int32_t requests,
+                                    int64_t tokens, int32_t causal, int32_t window, float scale,
+                                    int32_t max_new, int32_t max_length, void* out, float* lse,
+                                    void* workspace, uint64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -51,6 +51,23 @@ class MatrixInfo(ctypes.Structure):
     ]
 
 
+class KVPool(ctypes.Structure):  # ebx_kv_pool
+    _fields_ = [
+        ("k_codes", ctypes.c_void_p),
+        ("k_scales", ctypes.c_void_p),
+        ("v_codes", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p),
+        ("blocks", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("device", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+_KV = ctypes.POINTER(KVPool)
+
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ebx_version": (ctypes.c_char_p, []),
     "ebx_last_error": (ctypes.c_size_t, [ctypes.c_char_p, ctypes.c_size_t]),
@@ -81,6 +98,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ebx_linear_allreduce": (_ST, [_P, _P, _I64, _P, _P, _P, _P, _P]),
     "ebx_exchange_allreduce": (_ST, [_P, _P, _I64, _I64, _P, _P, _P, _P]),
     "ebx_exchange_set_protocol": (_ST, [_P, _I32]),
+    "ebx_kv_plan": (
+        _ST, [_P, _P, _I32, _P, _I32, _I32, _P, _I32, _P, _P, _P, _P, _P, _P, _I64, _I32, _P]),
+    "ebx_kv_append": (_ST, [_KV, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I32, _P]),
+    "ebx_kv_materialize": (_ST, [_KV, _P, _I32, _P, _P, _I32, _I64, _I32, _P, _P, _P]),
+    "ebx_kv_attention_workspace_bytes": (_U64, [_KV]),
+    "ebx_kv_attention": (
+        _ST, [_KV, _P, _I64, _I64, _I32, _I32, _P, _I32, _P, _P, _P, _I32, _I64, _I32, _I32,
+              ctypes.c_float, _I32, _I32, _P, _P, _P, _U64, _P]),
     "ebx_elastic_linear_packed": (
         _ST, [_P, _I32, _I64, _P, _P, _I32, _P, _I32, _I64, _I64, _I64, _P, _P]),
 }
@@ -137,4 +162,4 @@ def stream_ptr(stream=None, device: int | None = None) -> int:
     return int(torch.cuda.current_stream(device).cuda_stream)
 
 
-__all__ = ["LIB_PATH", "MatrixInfo", "SIGNATURES", "load", "last_error", "check", "stream_ptr"]
+__all__ = ["LIB_PATH", "KVPool", "MatrixInfo", "SIGNATURES", "load", "last_error", "check", "stream_ptr"]

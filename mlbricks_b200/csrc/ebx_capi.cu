@@ -16,6 +16,7 @@
 #include "../../include/ebx.h"
 #include "ebx_common.cuh"
 #include "ebx_internal.h"
+#include "ebx_kv.h"
 
 struct ebx_matrix {
     ebx::Matrix m;
@@ -493,12 +494,13 @@ ebx_status ebx_device_status(int32_t device, int32_t* status, int32_t clear) {
     }
     DeviceGuard g(device);
     if (!g.ok) return cuda_fail(cudaErrorInvalidDevice, "cudaSetDevice");
-    int v = 0, vg = 0, vd = 0, vx = 0;
+    int v = 0, vg = 0, vd = 0, vx = 0, vk = 0;
     EBX_CUDA(ebx::read_device_status(&v, clear != 0, nullptr));
     EBX_CUDA(ebx::read_gemm_status(&vg, clear != 0, nullptr));
     EBX_CUDA(ebx::read_dgemm_status(&vd, clear != 0, nullptr));
     EBX_CUDA(ebx::read_xchg_status(&vx, clear != 0, nullptr));
-    *status = v ? v : (vg ? vg : (vd ? vd : vx));
+    EBX_CUDA(ebx::read_kv_status(&vk, clear != 0, nullptr));
+    *status = v ? v : (vg ? vg : (vd ? vd : (vx ? vx : vk)));
     return EBX_OK;
 }
 

@@ -1217,6 +1217,8 @@ bool gemm_supported(int K, const void* x, const void* w16) {
            (reinterpret_cast<uintptr_t>(w16) & 15) == 0 && encode_fn() != nullptr;
 }
 
+void* tensor_map_encoder() { return reinterpret_cast<void*>(encode_fn()); }
+
 int gemm_sm_count(int dev) {
     static std::atomic<int> cache[64];
     int sms = cache[dev & 63].load(std::memory_order_relaxed);

@@ -1,0 +1,79 @@
+// ebx_kv.h -- the 8-bit paged key/value cache: arguments and launchers shared by the
+// ebx_kv_*.cu translation units.
+//
+// A pool holds, for keys and for values, int8 codes [blocks][kv_heads][block_size][head_dim]
+// and one fp32 scale for each (block, head); value = code * scale.  A request's tokens lie in
+// the blocks that its row of the block table names, block_size of them in each.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace ebx {
+
+constexpr int kKvMaxRequests = 16384;  // ebx_kv_plan keeps 12 bytes a request in shared memory
+constexpr int kKvF32 = 0, kKvF16 = 1, kKvBF16 = 2;  // dtype codes of the C ABI
+
+struct KvPool {
+    int8_t* k_codes;
+    float* k_scales;
+    int8_t* v_codes;
+    float* v_scales;
+    int blocks, kv_heads, block_size, head_dim;
+    int shift;  // log2(block_size)
+};
+
+struct KvPlanArgs {
+    const int32_t* past;
+    const int32_t* added;
+    int32_t* tables;
+    int32_t* free_ring;
+    const int64_t* ring;
+    int64_t* ring_out;
+    int32_t* lengths;
+    int32_t* starts;
+    int64_t* slots;
+    int32_t* positions;
+    int64_t tokens;
+    int requests, width, shift, free_size;
+};
+
+// A 16-bit tensor [tokens, heads, head_dim] whose last dimension is contiguous; strides in elements.
+struct KvRows {
+    const uint16_t* p;
+    int64_t token_stride, head_stride;
+};
+
+struct KvAttnArgs {
+    KvPool pool;
+    KvRows q;
+    const int32_t* tables;
+    const int32_t* lengths;
+    const int32_t* starts;
+    const int32_t* first;  // may be null: every key from 0 on
+    void* out;
+    float* lse;            // may be null
+    int64_t tokens;
+    int requests, width, heads, group;
+    int causal, window;
+    float scale_log2;      // softmax scale * log2(e)
+    // partial results of row tiles that several CTAs share
+    float* part;           // [grid][2][rows][head_dim + 2]
+    int4* desc;            // [grid][2]
+};
+
+cudaError_t launch_kv_plan(const KvPlanArgs& a, cudaStream_t s);
+cudaError_t launch_kv_append(const KvPool& pool, const KvRows& k, const KvRows& v, const int64_t* slots,
+                             int64_t tokens, bool bf16, cudaStream_t s);
+cudaError_t launch_kv_materialize(const KvPool& pool, const int32_t* tables, int width,
+                                  const int32_t* starts, const int32_t* first, int requests,
+                                  int64_t tokens, int dtype, void* k, void* v, cudaStream_t s);
+uint64_t kv_attention_workspace_bytes(int head_dim);
+cudaError_t launch_kv_attention(KvAttnArgs a, bool bf16, void* ws, cudaStream_t s);
+cudaError_t read_kv_status(int* status, bool clear, cudaStream_t s);
+
+// ebx_gemm.cu: cuTensorMapEncodeTiled of the loaded driver (null without one).
+void* tensor_map_encoder();
+int gemm_sm_count(int dev);
+
+}  // namespace ebx

@@ -1,0 +1,255 @@
+"""An 8-bit paged key/value cache for the decoders that ElasticBit compresses.
+
+The weights of a compressed model are read as integer codes; at serving lengths the keys and
+values are the larger part of what a step reads, so they are kept as codes too: a block of 16 to
+128 tokens of one head is int8 under one fp32 scale (value = code * scale), half the bytes of a
+16-bit cache.  Blocks belong to requests through a block table, so that ragged requests share one
+pool.  Four operators (``libebx``, include/ebx.h ``ebx_kv_*``), all stream-ordered, none of which
+copies anything to the host:
+
+* ``plan``         blocks and slots of a step's new tokens, from the requests' lengths on the GPU;
+* ``append``       quantises the new keys and values into their slots;
+* ``attention``    new queries over the cache: decode steps, prompts, chunks, sliding windows;
+* ``materialize``  keys and values back in 16 or 32 bits.
+
+``KVCache`` holds a model's pools and tables and runs them together.  Inference only, as the rest
+of the native route: no autograd.  The reference has no counterpart (its caches,
+mlbricks/cache.py, are whole 16-bit tensors).
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import NamedTuple
+
+import torch
+
+from . import _ebx
+
+BLOCK_SIZES = (16, 32, 64, 128)
+HEAD_DIMS = (32, 64, 128)
+_ROW_DTYPES = {torch.float16: 1, torch.bfloat16: 2}
+_DTYPES = {torch.float32: 0, **_ROW_DTYPES}
+
+
+class KVPlan(NamedTuple):
+    """A step: what ``plan`` wrote (all on the GPU)."""
+
+    lengths: torch.Tensor    # int32 [requests], tokens held once the step's are appended
+    starts: torch.Tensor     # int32 [requests + 1], first token of each request in the step
+    slots: torch.Tensor      # int64 [tokens], where each token goes; -1: nowhere
+    positions: torch.Tensor  # int32 [tokens], its place in its request
+    ring: torch.Tensor       # int64 [4]: front, back, blocks that were missing, tokens
+
+
+def _check(cond: bool, msg: str) -> None:
+    if not cond:
+        raise ValueError(msg)
+
+
+def _check_int(t: torch.Tensor, dtype: torch.dtype, device: int, name: str) -> None:
+    if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor on cuda:{device}")
+
+
+class KVPool:
+    """One layer's cache: int8 codes [blocks, kv_heads, block_size, head_dim] and fp32 scales
+    [blocks, kv_heads], of keys and of values.  Holds the tensors; copies nothing."""
+
+    __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "device", "_c", "_ref")
+
+    def __init__(self, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
+                 v_scales: torch.Tensor) -> None:
+        shape, device = k_codes.shape, k_codes.get_device()
+        _check(k_codes.is_cuda and k_codes.dim() == 4, "codes must be CUDA tensors "
+               "[blocks, kv_heads, block_size, head_dim]")
+        for t, s, dtype, name in ((k_codes, shape, torch.int8, "k_codes"), (v_codes, shape, torch.int8, "v_codes"),
+                                  (k_scales, shape[:2], torch.float32, "k_scales"),
+                                  (v_scales, shape[:2], torch.float32, "v_scales")):
+            if t.dtype is not dtype or t.shape != s or t.get_device() != device or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous {dtype} tensor {tuple(s)} on cuda:{device}")
+        blocks, kv_heads, block_size, head_dim = shape
+        _check(block_size in BLOCK_SIZES, f"block_size must be one of {BLOCK_SIZES}, got {block_size}")
+        _check(head_dim in HEAD_DIMS, f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
+        _check(0 < blocks * kv_heads * block_size < 2**31, "need 0 < blocks * kv_heads * block_size < 2^31")
+        self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
+        self.device = device
+        self._c = _ebx.KVPool(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
+                              blocks, kv_heads, block_size, head_dim, device, 0)
+        self._ref = ctypes.byref(self._c)
+
+    @classmethod
+    def empty(cls, blocks: int, kv_heads: int, block_size: int, head_dim: int, device="cuda") -> "KVPool":
+        """A pool whose blocks hold nothing yet."""
+        shape = (blocks, kv_heads, block_size, head_dim)
+        return cls(*(t for _ in "kv" for t in (torch.zeros(shape, dtype=torch.int8, device=device),
+                                               torch.zeros(shape[:2], dtype=torch.float32, device=device))))
+
+    blocks = property(lambda self: self._c.blocks)
+    kv_heads = property(lambda self: self._c.kv_heads)
+    block_size = property(lambda self: self._c.block_size)
+    head_dim = property(lambda self: self._c.head_dim)
+
+    def _rows(self, x: torch.Tensor, heads: int | None, name: str) -> torch.Tensor:
+        """x [tokens, heads, head_dim] as the kernels read it: 16-byte aligned rows."""
+        if x.dtype not in _ROW_DTYPES or x.get_device() != self.device:
+            raise ValueError(f"{name} must be float16 or bfloat16 on cuda:{self.device}")
+        if x.dim() != 3 or x.shape[2] != self._c.head_dim or (heads is not None and x.shape[1] != heads):
+            raise ValueError(f"{name} must be [tokens, {'heads' if heads is None else heads}, "
+                             f"{self._c.head_dim}], got {tuple(x.shape)}")
+        s0, s1, s2 = x.stride()
+        if s2 != 1 or s0 % 8 or s1 % 8 or x.data_ptr() % 16:
+            return x.clone(memory_format=torch.contiguous_format)
+        return x
+
+
+def _stream(device: int) -> int:
+    return _ebx.stream_ptr(device=device)
+
+
+def plan(past: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, free: torch.Tensor, ring: torch.Tensor, *,
+         block_size: int, tokens: int) -> KVPlan:
+    """Blocks and slots of one step, on the GPU.
+
+    Request i holds ``past[i]`` tokens and brings ``new[i]``; ``new[i] < 0`` releases it.  Free
+    blocks wait in the ring ``free`` (int32, room for every block) from ``ring[0]`` up to
+    ``ring[1]``, modulo its size.  In order, each request takes the blocks that it lacks into its
+    row of ``tables`` (written in place) -- or nothing, if they are not all there or the row is too
+    short: its tokens then get slot -1, its length stays, and ``ring[2]`` of the result counts the
+    missing blocks.  Released blocks join the ring's back.  ``tokens`` is the room for slots and
+    positions: the sum of the new tokens, or more (the rest is slot -1, position 0).
+
+    The inputs ``past`` and ``ring`` are not changed; the next step takes the result's ``lengths``
+    and ``ring`` in their place."""
+    device = past.get_device()
+    if not past.is_cuda:
+        raise ValueError("plan needs CUDA tensors")
+    requests = past.numel()
+    _check_int(past, torch.int32, device, "past")
+    _check_int(new, torch.int32, device, "new")
+    _check_int(tables, torch.int32, device, "tables")
+    _check_int(free, torch.int32, device, "free")
+    _check_int(ring, torch.int64, device, "ring")
+    _check(new.numel() == requests and tables.dim() == 2 and tables.shape[0] == requests,
+           "past, new and the rows of tables must be as many")
+    _check(ring.numel() >= 2 and tokens >= 0, "ring holds at least its front and back, and tokens >= 0")
+    _check(block_size in BLOCK_SIZES, f"block_size must be one of {BLOCK_SIZES}, got {block_size}")
+    where = past.device
+    lengths = torch.empty(requests, dtype=torch.int32, device=where)
+    starts = torch.empty(requests + 1, dtype=torch.int32, device=where)
+    slots = torch.empty(tokens, dtype=torch.int64, device=where)
+    positions = torch.empty(tokens, dtype=torch.int32, device=where)
+    out = torch.empty(4, dtype=torch.int64, device=where)
+    st = _ebx.load().ebx_kv_plan(
+        past.data_ptr(), new.data_ptr(), requests, tables.data_ptr(), tables.shape[1], block_size,
+        free.data_ptr(), free.numel(), ring.data_ptr(), out.data_ptr(), lengths.data_ptr(), starts.data_ptr(),
+        slots.data_ptr(), positions.data_ptr(), tokens, device, _stream(device))
+    if st:
+        _ebx.check(st)
+    return KVPlan(lengths, starts, slots, positions, out)
+
+
+def append(k: torch.Tensor, v: torch.Tensor, pool: KVPool, slots: torch.Tensor) -> None:
+    """Quantise new keys and values [tokens, kv_heads, head_dim] (fp16 or bf16, any strides) into
+    their slots, in place.  For each block and head the scale is max(old, max |x| / 127) and a code
+    rint(x / scale); tokens that the block held before move to a larger scale.  Tokens with slot -1
+    are skipped; a value that is not finite makes the scale of its block NaN.  The tokens of one
+    block are consecutive, behind all that the block holds (as ``plan`` lays them)."""
+    heads = pool._c.kv_heads
+    k, v = pool._rows(k, heads, "k"), pool._rows(v, heads, "v")
+    tokens = k.shape[0]
+    if v.shape[0] != tokens or v.dtype is not k.dtype:
+        raise ValueError("k and v must have the same tokens and dtype")
+    _check_int(slots, torch.int64, pool.device, "slots")
+    if slots.numel() != tokens:
+        raise ValueError("slots must have one entry for each token")
+    if tokens == 0:
+        return
+    st = _ebx.load().ebx_kv_append(
+        pool._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+        slots.data_ptr(), tokens, _ROW_DTYPES[k.dtype], _stream(pool.device))
+    if st:
+        _ebx.check(st)
+
+
+def materialize(pool: KVPool, tables: torch.Tensor, starts: torch.Tensor, *, first: torch.Tensor | None = None,
+                tokens: int, dtype: torch.dtype = torch.float16) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values [tokens, kv_heads, head_dim] as code * scale, rounded once to ``dtype``:
+    rows starts[i] .. starts[i + 1] - 1 are the places first[i] (default 0) on of request i."""
+    if dtype not in _DTYPES:
+        raise ValueError("dtype must be float32, float16 or bfloat16")
+    requests = starts.numel() - 1
+    _check_int(starts, torch.int32, pool.device, "starts")
+    _check_int(tables, torch.int32, pool.device, "tables")
+    _check(requests >= 0 and tables.dim() == 2 and tables.shape[0] == requests and tokens >= 0,
+           "tables must have a row, and starts an entry, for each request (and one more); tokens >= 0")
+    if first is not None:
+        _check_int(first, torch.int32, pool.device, "first")
+        _check(first.numel() == requests, "first must have one entry for each request")
+    shape = (tokens, pool._c.kv_heads, pool._c.head_dim)
+    k = torch.empty(shape, dtype=dtype, device=starts.device)
+    v = torch.empty(shape, dtype=dtype, device=starts.device)
+    st = _ebx.load().ebx_kv_materialize(
+        pool._ref, tables.data_ptr(), tables.shape[1], starts.data_ptr(), None if first is None else first.data_ptr(),
+        requests, tokens, _DTYPES[dtype], k.data_ptr(), v.data_ptr(), _stream(pool.device))
+    if st:
+        _ebx.check(st)
+    return k, v
+
+
+def attention(q: torch.Tensor, pool: KVPool, tables: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor, *,
+              scale: float | None = None, causal: bool = True, window: int = 0, first: torch.Tensor | None = None,
+              max_new: int = 0, max_length: int = 0, out: torch.Tensor | None = None, return_lse: bool = False):
+    """Attention of new queries [tokens, heads, head_dim] (fp16 or bf16, any strides) over the cache.
+
+    Request i's queries are rows starts[i] .. starts[i + 1] - 1, at the last positions of its
+    lengths[i] tokens; heads / kv_heads query heads share a key/value head.  A query at position p
+    sees the keys j < lengths[i] with j >= first[i] (if given), j <= p (``causal``) and
+    j > p - window (``window`` > 0).  A query that sees nothing gets 0 (log-sum-exp -infinity); rows
+    of no request are left as they are.  ``scale`` defaults to 1 / sqrt(head_dim).  ``max_new`` and
+    ``max_length``, where the caller knows the largest number of new tokens and the largest length,
+    choose the kernel and change no result.  Returns out, or (out, lse [tokens, heads] fp32)."""
+    q = pool._rows(q, None, "q")
+    device = pool.device
+    tokens, heads, dim = q.shape
+    requests = lengths.numel()
+    _check_int(tables, torch.int32, device, "tables")
+    _check_int(lengths, torch.int32, device, "lengths")
+    _check_int(starts, torch.int32, device, "starts")
+    if heads == 0 or heads % pool._c.kv_heads:
+        raise ValueError(f"heads ({heads}) must be a multiple of kv_heads ({pool._c.kv_heads})")
+    if starts.numel() != requests + 1 or tables.dim() != 2 or tables.shape[0] != requests:
+        raise ValueError("lengths and the rows of tables must be as many, and starts one more")
+    if first is not None:
+        _check_int(first, torch.int32, device, "first")
+        _check(first.numel() == requests, "first must have one entry for each request")
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != device or not out.is_contiguous():
+        raise ValueError("out must be a contiguous tensor of q's shape and dtype")
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    if tokens and requests:
+        lib = _ebx.load()
+        nbytes = _workspace_bytes(lib, pool)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        st = lib.ebx_kv_attention(
+            pool._ref, q.data_ptr(), q.stride(0), q.stride(1), heads, _ROW_DTYPES[q.dtype], tables.data_ptr(),
+            tables.shape[1], lengths.data_ptr(), starts.data_ptr(), None if first is None else first.data_ptr(),
+            requests, tokens, causal, window, 1.0 / math.sqrt(dim) if scale is None else scale, max_new, max_length,
+            out.data_ptr(), None if lse is None else lse.data_ptr(), ws.data_ptr(), nbytes, _stream(device))
+        if st:
+            _ebx.check(st)
+    return out if lse is None else (out, lse)
+
+
+_WORKSPACE: dict[tuple[int, int], int] = {}
+
+
+def _workspace_bytes(lib, pool: KVPool) -> int:
+    key = (pool.device, pool._c.head_dim)  # what the size depends on
+    if key not in _WORKSPACE:
+        _WORKSPACE[key] = int(lib.ebx_kv_attention_workspace_bytes(pool._ref))
+    return _WORKSPACE[key]
+
+
+__all__ = ["BLOCK_SIZES", "HEAD_DIMS", "KVPlan", "KVPool", "append", "attention", "materialize", "plan"]
