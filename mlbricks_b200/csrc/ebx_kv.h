@@ -68,9 +68,14 @@ cudaError_t launch_kv_append(const KvPool& pool, const KvRows& k, const KvRows& 
 cudaError_t launch_kv_materialize(const KvPool& pool, const int32_t* tables, int width,
                                   const int32_t* starts, const int32_t* first, int requests,
                                   int64_t tokens, int dtype, void* k, void* v, cudaStream_t s);
-uint64_t kv_attention_workspace_bytes(int head_dim);
-cudaError_t launch_kv_attention(KvAttnArgs a, bool bf16, void* ws, cudaStream_t s);
+uint64_t kv_attention_workspace_bytes(int head_dim, int group, int64_t tokens, int max_new);
+cudaError_t launch_kv_attention(const KvAttnArgs& a, bool bf16, int max_new, void* ws, cudaStream_t s);
 cudaError_t read_kv_status(int* status, bool clear, cudaStream_t s);
+
+// ebx_kv_prompt.cu: the same for many rows.
+uint64_t kv_prompt_workspace_bytes(int head_dim, int sms);
+cudaError_t launch_kv_prompt(const KvAttnArgs& a, bool bf16, void* ws, int dev, cudaStream_t s);
+cudaError_t read_kv_prompt_status(int* status, bool clear, cudaStream_t s);
 
 // ebx_gemm.cu: cuTensorMapEncodeTiled of the loaded driver (null without one).
 void* tensor_map_encoder();

@@ -9,9 +9,6 @@
 // m near the running maximum of t, so that the weight w_j, which carries the value's scale, fits
 // fp16 for the second product whatever the scale's size, and one exponential serves both sums.  V scales
 // below 2^-100 count as 2^-100.  out = O / l and the log-sum-exp is ln2 * (m + log2 l).
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -23,21 +20,12 @@ namespace ebx {
 namespace {
 
 __device__ int g_kv_status = 0;
-// V scale of a key tile's 16 tokens that no block holds: its keys are not seen
-__device__ const float g_kv_none = -1.0f;
+__device__ const float kv_none = kKvNone;  // for the copies of scales
 
 __device__ __forceinline__ bool kv_wait(uint32_t bar, uint32_t parity) {
     if (mbar_wait_bounded(bar, parity)) return true;
     atomicExch(&g_kv_status, 0x7104);
     return false;
-}
-
-__device__ __forceinline__ void kv_tma_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4}], [%2];\n" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
-        : "memory");
 }
 
 // ---- few rows: decode ---------------------------------------------------------------------
@@ -46,11 +34,6 @@ constexpr int kRows = 16;        // rows of a tile: the M of mma.m16n8k16
 constexpr int kConsumers = 4;    // warps that compute; one more loads
 constexpr int kStepThreads = 32 * (kConsumers + 1);
 constexpr int kStages = 3;
-// Weights are 2^(t - m + kShift), m at most kLag below the maximum so far: the largest is below
-// 2^15, and of the fp16 range nothing is left unused below it (a weight 2^-22 of the largest
-// still has all its 11 bits).
-constexpr float kLag = 8.0f, kShift = 7.0f;
-
 template <int D>
 struct StepCfg {
     static constexpr int KT = 8192 / D;              // tokens of a key tile: 8 KB of codes a side
@@ -83,11 +66,6 @@ __device__ __forceinline__ void lds(uint32_t addr, uint32_t (&w)[BYTES / 4]) {
         asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
     else
         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
-}
-
-// Two int8 codes (already xor 0x80: code + 128) as fp16: 0x64 above a byte is 1024 + byte.
-__device__ __forceinline__ uint32_t codes_to_half2(uint32_t w, uint32_t sel) {
-    return hsub2_u(__byte_perm(w, 0x64646464u, sel), 0x64806480u);  // - 1152
 }
 
 template <int D, bool BF16>
@@ -175,7 +153,7 @@ __global__ void __launch_bounds__(kStepThreads)
                 }
                 if (sc) {
                     const int64_t cell = int64_t(sid) * a.pool.kv_heads + walk.head;
-                    const float* src = sid == none ? &g_kv_none : (sc_v ? a.pool.v_scales : a.pool.k_scales) + cell;
+                    const float* src = sid == none ? &kv_none : (sc_v ? a.pool.v_scales : a.pool.k_scales) + cell;
                     cp_async4(smem_u32(scales + (st * 2 + (sc_v ? 1 : 0)) * UNITS + sc_row / 16), src);
                 }
                 asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(bar) : "memory");
@@ -286,7 +264,7 @@ __global__ void __launch_bounds__(kStepThreads)
                         }
                     }
                 }
-                const bool none = vs < 0.0f;
+                const bool none = vs < 0.0f;  // kKvNone
                 const float vsc = vs < 0x1p-100f ? 0x1p-100f : vs;  // NaN stays
                 const float b = none ? -INFINITY : lg2(vsc);
                 const float inv = vs == vs ? 1.0f / vsc : 1.0f;  // NaN goes through t, where the mask stops it
@@ -430,88 +408,6 @@ __global__ void __launch_bounds__(kStepThreads)
     }
 }
 
-// Row tiles that several CTAs worked on: CTA (c, y) joins the one that begins in CTA c, its rows
-// y, y + gridDim.y, ..., reading c's part 1 and then part 0 of the CTAs after it until one ends it.
-template <int D, int RT, bool BF16>
-__global__ void __launch_bounds__(128) kv_join_kernel(const __grid_constant__ KvAttnArgs a, int ctas) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    constexpr int LANES = D / 4;            // threads of a row, 4 values each
-    constexpr int WAYS = 128 / LANES;       // parts of a row read at once
-    __shared__ float s_m[WAYS][LANES], s_l[WAYS][LANES];
-    __shared__ float4 s_o[WAYS][LANES];
-    __shared__ int s_last;
-    const int c = blockIdx.x;
-    const int4 d1 = a.desc[2 * c + 1];
-    if (d1.x == 0) return;
-    if (threadIdx.x == 0) s_last = ctas - 1;
-    for (int base = c + 1;; base += 128) {  // the CTA that ends the row tile
-        const int k = base + int(threadIdx.x);
-        const bool end = k >= ctas - 1 || (a.desc[2 * k].x & kKvEnds) != 0;
-        const bool any = __syncthreads_or(end);
-        if (end) atomicMin(&s_last, k);
-        if (any) break;
-    }
-    __syncthreads();
-    const int last = s_last;
-    const int lane = threadIdx.x % LANES, way = threadIdx.x / LANES;
-    for (int r = blockIdx.y; r < d1.w; r += gridDim.y) {
-        float m = -INFINITY, l = 0.0f;
-        float4 o = make_float4(0, 0, 0, 0);
-        for (int k = c + way; k <= last; k += WAYS) {
-            const float* src = a.part + ((2 * int64_t(k) + (k == c ? 1 : 0)) * RT + r) * (D + 2);
-            const float2 v0 = *reinterpret_cast<const float2*>(src + 4 * lane);
-            const float2 v1 = *reinterpret_cast<const float2*>(src + 4 * lane + 2);
-            const float2 ml = *reinterpret_cast<const float2*>(src + D);
-            const float mn = fmaxf(m, ml.x);
-            const float f0 = m == mn ? 1.0f : ex2(m - mn), f1 = ml.x == mn ? 1.0f : ex2(ml.x - mn);
-            o.x = o.x * f0 + v0.x * f1; o.y = o.y * f0 + v0.y * f1;
-            o.z = o.z * f0 + v1.x * f1; o.w = o.w * f0 + v1.y * f1;
-            l = l * f0 + ml.y * f1;
-            m = mn;
-        }
-        s_m[way][lane] = m;
-        s_l[way][lane] = l;
-        s_o[way][lane] = o;
-        __syncthreads();
-        if (way == 0) {
-#pragma unroll
-            for (int w = 1; w < WAYS; ++w) {
-                const float m1 = s_m[w][lane];
-                const float4 v = s_o[w][lane];
-                const float mn = fmaxf(m, m1);
-                const float f0 = m == mn ? 1.0f : ex2(m - mn), f1 = m1 == mn ? 1.0f : ex2(m1 - mn);
-                o.x = o.x * f0 + v.x * f1; o.y = o.y * f0 + v.y * f1;
-                o.z = o.z * f0 + v.z * f1; o.w = o.w * f0 + v.w * f1;
-                l = l * f0 + s_l[w][lane] * f1;
-                m = mn;
-            }
-            const int row = (d1.x & (kKvEnds - 1)) - 1 + r;
-            const int64_t at = int64_t(d1.y + row / a.group) * a.heads + d1.z * a.group + row % a.group;
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            uint2 pk;
-            pk.x = pack16<BF16>(o.x * inv, o.y * inv);
-            pk.y = pack16<BF16>(o.z * inv, o.w * inv);
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at * D + 4 * lane) = pk;
-            if (a.lse && lane == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + lg2(l)) * 0.6931471805599453f;
-        }
-        __syncthreads();
-    }
-}
-
-bool code_map(CUtensorMap* map, const int8_t* codes, const KvPool& p, int box_rows) {
-    auto fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encoder());
-    if (!fn) return false;
-    const cuuint64_t dims[2] = {cuuint64_t(p.head_dim), cuuint64_t(p.blocks) * p.kv_heads * p.block_size};
-    const cuuint64_t strides[1] = {cuuint64_t(p.head_dim)};
-    const cuuint32_t box[2] = {cuuint32_t(p.head_dim), cuuint32_t(box_rows)};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUtensorMapSwizzle sw = p.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
-                                  : p.head_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(codes), dims, strides, box, estr,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 constexpr int kStepPerSm = 2;   // CTAs of an SM
 constexpr int kStepLeast = 4;   // key tiles a CTA takes at least: a partial result costs about as much
 
@@ -536,32 +432,37 @@ cudaError_t launch_step(KvAttnArgs a, void* ws, int dev, cudaStream_t s) {
     kern<<<grid, kStepThreads, C::kSmem, s>>>(mk, mv, a, kStepLeast);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(grid), unsigned(std::min(kRows, a.group)));
-    cfg.blockDim = dim3(128);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kv_join_kernel<D, kRows, BF16>, a, grid);
+    return launch_join<D, kRows, BF16>(a, grid, std::min(kRows, a.group), s);
 }
 
 }  // namespace
 
-uint64_t kv_attention_workspace_bytes(int head_dim) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-    const uint64_t grid = uint64_t(gemm_sm_count(dev)) * kStepPerSm;
-    return uint64_t(round_up(int64_t(grid * 2 * (sizeof(int4) + kRows * (head_dim + 2) * sizeof(float))), 256));
+namespace {
+
+// Row tiles of 256 rows on tcgen05 from kPromptMin rows of a request on; below, tiles of 16.
+constexpr int kPromptMin = 33;
+
+bool takes_prompt(int group, int64_t tokens, int max_new) {
+    const int64_t most = max_new > 0 ? std::min<int64_t>(max_new, tokens) : tokens;
+    return most * group >= kPromptMin;
 }
 
-cudaError_t launch_kv_attention(KvAttnArgs a, bool bf16, void* ws, cudaStream_t s) {
+}  // namespace
+
+uint64_t kv_attention_workspace_bytes(int head_dim, int group, int64_t tokens, int max_new) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    const int sms = gemm_sm_count(dev);
+    if (takes_prompt(group, tokens, max_new)) return kv_prompt_workspace_bytes(head_dim, sms);
+    return uint64_t(round_up(int64_t(sms) * kStepPerSm * 2 * int64_t(sizeof(int4) + kRows * (head_dim + 2) * sizeof(float)), 256));
+}
+
+cudaError_t launch_kv_attention(const KvAttnArgs& a, bool bf16, int max_new, void* ws, cudaStream_t s) {
     if (a.tokens <= 0 || a.requests <= 0) return cudaSuccess;
     int dev = 0;
     const cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
+    if (takes_prompt(a.group, a.tokens, max_new)) return launch_kv_prompt(a, bf16, ws, dev, s);
     switch (a.pool.head_dim) {
         case 32: return bf16 ? launch_step<32, true>(a, ws, dev, s) : launch_step<32, false>(a, ws, dev, s);
         case 64: return bf16 ? launch_step<64, true>(a, ws, dev, s) : launch_step<64, false>(a, ws, dev, s);
@@ -570,13 +471,10 @@ cudaError_t launch_kv_attention(KvAttnArgs a, bool bf16, void* ws, cudaStream_t 
 }
 
 cudaError_t read_kv_status(int* status, bool clear, cudaStream_t s) {
-    cudaError_t e = cudaMemcpyFromSymbolAsync(status, g_kv_status, sizeof(int), 0, cudaMemcpyDeviceToHost, s);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-    if (e == cudaSuccess && clear) {
-        const int zero = 0;
-        e = cudaMemcpyToSymbolAsync(g_kv_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s);
-        if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-    }
+    int prompt = 0;
+    cudaError_t e = read_status_word(g_kv_status, status, clear, s);
+    if (e == cudaSuccess) e = read_kv_prompt_status(&prompt, clear, s);
+    if (*status == 0) *status = prompt;
     return e;
 }
 

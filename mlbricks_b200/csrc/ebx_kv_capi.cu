@@ -129,11 +129,12 @@ ebx_status ebx_kv_materialize(const ebx_kv_pool* pool, const int32_t* tables, in
                                                v, static_cast<cudaStream_t>(stream)), "ebx_kv_materialize");
 }
 
-uint64_t ebx_kv_attention_workspace_bytes(const ebx_kv_pool* pool) {
+uint64_t ebx_kv_attention_workspace_bytes(const ebx_kv_pool* pool, int32_t heads, int64_t tokens,
+                                          int32_t max_new) {
     ebx::KvPool p;
-    if (pool_of(pool, p)) return 0;
+    if (pool_of(pool, p) || heads < 1 || heads % p.kv_heads != 0 || tokens < 0 || max_new < 0) return 0;
     Device d(pool->device);
-    return d.err == cudaSuccess ? ebx::kv_attention_workspace_bytes(p.head_dim) : 0;
+    return d.err == cudaSuccess ? ebx::kv_attention_workspace_bytes(p.head_dim, heads / p.kv_heads, tokens, max_new) : 0;
 }
 
 ebx_status ebx_kv_attention(const ebx_kv_pool* pool, const void* q, int64_t q_token_stride,
@@ -162,7 +163,7 @@ ebx_status ebx_kv_attention(const ebx_kv_pool* pool, const void* q, int64_t q_to
         return invalid("ebx_kv_attention: out and workspace must be 16-byte aligned");
     Device d(pool->device);
     if (d.err != cudaSuccess) return launched(d.err, "cudaSetDevice");
-    if (!workspace || workspace_bytes < ebx::kv_attention_workspace_bytes(p.head_dim)) {
+    if (!workspace || workspace_bytes < ebx::kv_attention_workspace_bytes(p.head_dim, heads / p.kv_heads, tokens, max_new)) {
         ebx::set_error("ebx_kv_attention: workspace smaller than ebx_kv_attention_workspace_bytes");
         return EBX_ERR_WORKSPACE;
     }
@@ -183,7 +184,7 @@ ebx_status ebx_kv_attention(const ebx_kv_pool* pool, const void* q, int64_t q_to
     a.causal = causal != 0;
     a.window = window;
     a.scale_log2 = scale * 1.4426950408889634f;
-    return launched(ebx::launch_kv_attention(a, dtype == ebx::kKvBF16, workspace,
+    return launched(ebx::launch_kv_attention(a, dtype == ebx::kKvBF16, max_new, workspace,
                                              static_cast<cudaStream_t>(stream)), "ebx_kv_attention");
 }
 

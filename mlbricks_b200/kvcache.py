@@ -230,7 +230,7 @@ def attention(q: torch.Tensor, pool: KVPool, tables: torch.Tensor, lengths: torc
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
     if tokens and requests:
         lib = _ebx.load()
-        nbytes = _workspace_bytes(lib, pool)
+        nbytes = lib.ebx_kv_attention_workspace_bytes(pool._ref, heads, tokens, max_new)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         st = lib.ebx_kv_attention(
             pool._ref, q.data_ptr(), q.stride(0), q.stride(1), heads, _ROW_DTYPES[q.dtype], tables.data_ptr(),
@@ -240,16 +240,6 @@ def attention(q: torch.Tensor, pool: KVPool, tables: torch.Tensor, lengths: torc
         if st:
             _ebx.check(st)
     return out if lse is None else (out, lse)
-
-
-_WORKSPACE: dict[tuple[int, int], int] = {}
-
-
-def _workspace_bytes(lib, pool: KVPool) -> int:
-    key = (pool.device, pool._c.head_dim)  # what the size depends on
-    if key not in _WORKSPACE:
-        _WORKSPACE[key] = int(lib.ebx_kv_attention_workspace_bytes(pool._ref))
-    return _WORKSPACE[key]
 
 
 __all__ = ["BLOCK_SIZES", "HEAD_DIMS", "KVPlan", "KVPool", "append", "attention", "materialize", "plan"]
