@@ -57,9 +57,20 @@ struct KvAttnArgs {
     int requests, width, heads, group;
     int causal, window;
     float scale_log2;      // softmax scale * log2(e)
+    uint32_t group_mul, group_shift;  // n / group = n * group_mul >> group_shift
     // partial results of row tiles that several CTAs share
     float* part;           // [grid][2][rows][head_dim + 2]
     int4* desc;            // [grid][2]
+
+    // With 2^(k-1) < g <= 2^k and mul = ceil(2^(31+k) / g), mul * g exceeds 2^(31+k) by less than
+    // g <= 2^k, so n * mul >> (31 + k) is n / g for every n < 2^31.
+    void set_group(int g) {
+        group = g;
+        uint32_t k = 0;
+        while ((1u << k) < uint32_t(g)) ++k;
+        group_shift = 31 + k;
+        group_mul = uint32_t(((uint64_t(1) << group_shift) + uint32_t(g) - 1) / uint32_t(g));
+    }
 };
 
 cudaError_t launch_kv_plan(const KvPlanArgs& a, cudaStream_t s);

@@ -85,7 +85,6 @@ __global__ void __launch_bounds__(kStepThreads)
     float* scales = reinterpret_cast<float*>(smem + kStages * C::kStageBytes + C::kMergeBytes);  // [stage][k, v][unit]
     uint64_t* full = reinterpret_cast<uint64_t*>(scales + kStages * 2 * UNITS);
     uint64_t* empty = full + kStages;
-    __shared__ int64_t scratch[kStepThreads / 32 + 2];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -95,15 +94,12 @@ __global__ void __launch_bounds__(kStepThreads)
         }
         fence_proxy_async_smem();
     }
-    int request;
-    int64_t at, units;
-    kv_share<kRows, KT, kStepThreads>(a, least, scratch, request, at, units);
+    const KvShare share = kv_share<kRows, KT, kStepThreads>(a, least, reinterpret_cast<int*>(smem));
+    fence_proxy_async_smem();  // the ring's copies may overwrite what kv_share kept there
+    if (threadIdx.x < 2) a.desc[2 * blockIdx.x + threadIdx.x] = make_int4(0, 0, 0, 0);
     __syncthreads();
-    if (threadIdx.x < 2 && a.desc) a.desc[2 * blockIdx.x + threadIdx.x] = make_int4(0, 0, 0, 0);
-    __syncthreads();
-
     KvWalk<kRows, KT> walk;
-    walk.start(a, request, at, units);
+    walk.start(a, share);
     const int bsize = a.pool.block_size;
 
     if (warp == kConsumers) {
@@ -184,12 +180,12 @@ __global__ void __launch_bounds__(kStepThreads)
         for (int half = 0; half < 2; ++half) {
             const int r = walk.rt * kRows + n8 + 8 * half;
             const bool in = r < walk.r.rows;
-            const int token = in ? r / a.group : 0;
+            const int token = in ? by_group(a, r) : 0;
             const int place = walk.r.begin + token;
             hi[half] = !in ? INT_MAX : a.causal ? min(place + 1, walk.r.length) : walk.r.length;
             lo[half] = !in ? 0 : max(walk.r.first, a.window > 0 ? place - a.window + 1 : 0);
             const uint16_t* src = a.q.p + (walk.r.token0 + token) * a.q.token_stride +
-                                  (walk.head * a.group + (in ? r % a.group : 0)) * a.q.head_stride + c * KB;
+                                  (walk.head * a.group + (in ? r - token * a.group : 0)) * a.q.head_stride + c * KB;
 #pragma unroll
             for (int l = 0; l < KL; ++l)
 #pragma unroll
@@ -368,7 +364,6 @@ __global__ void __launch_bounds__(kStepThreads)
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kConsumers) : "memory");
         const bool whole = walk.begins && walk.ends;
         const int slot = walk.begins ? 1 : 0;
-        float* part = whole ? nullptr : a.part + (2 * int64_t(blockIdx.x) + slot) * kRows * (D + 2);
         for (int w = threadIdx.x; w < rows * (D / 4); w += 32 * kConsumers) {
             const int r = w / (D / 4), d = (w % (D / 4)) * 4;
             const float* src = merge + r * (D + 4);
@@ -388,7 +383,8 @@ __global__ void __launch_bounds__(kStepThreads)
             }
             if (whole) {
                 const int row = walk.rt * kRows + r;
-                const int64_t at_row = int64_t(walk.r.token0 + row / a.group) * a.heads + walk.head * a.group + row % a.group;
+                const int token = by_group(a, row);
+                const int64_t at_row = int64_t(walk.r.token0 + token) * a.heads + walk.head * a.group + row - token * a.group;
                 const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
                 uint2 pk;
                 pk.x = pack16<BF16>(sum.x * inv, sum.y * inv);
@@ -396,10 +392,8 @@ __global__ void __launch_bounds__(kStepThreads)
                 *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at_row * D + d) = pk;
                 if (a.lse && d == 0) a.lse[at_row] = ll == 0.0f ? -INFINITY : (mm + lg2(ll)) * 0.6931471805599453f;
             } else {
-                float* dst = part + r * (D + 2);
-                *reinterpret_cast<float2*>(dst + d) = make_float2(sum.x, sum.y);
-                *reinterpret_cast<float2*>(dst + d + 2) = make_float2(sum.z, sum.w);
-                if (d == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(mm, ll);
+                reinterpret_cast<float4*>(kv_part<D, kRows>(a, blockIdx.x, slot))[d / 4 * kRows + r] = sum;
+                if (d == 0) kv_part_ml<D, kRows>(a, blockIdx.x, slot)[r] = make_float2(mm, ll);
             }
         }
         if (!whole && threadIdx.x == 0)

@@ -180,7 +180,7 @@ ebx_status ebx_kv_attention(const ebx_kv_pool* pool, const void* q, int64_t q_to
     a.requests = requests;
     a.width = width;
     a.heads = heads;
-    a.group = heads / p.kv_heads;
+    a.set_group(heads / p.kv_heads);
     a.causal = causal != 0;
     a.window = window;
     a.scale_log2 = scale * 1.4426950408889634f;

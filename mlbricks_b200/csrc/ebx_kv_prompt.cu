@@ -10,9 +10,10 @@
 //   * one thread of warp 13 issues S = q k^T and O += w v.  The accumulators of both row tiles
 //     (S 2 x 128 columns, O 2 x 128) fill the tensor memory; the weights overwrite S as the second
 //     product's A operand.  While it works on one row tile, the other's weights are computed;
-//   * warps 0-3 and 4-7: a thread per row of each row tile.  One pass over S: t, its maximum, the
-//     weights and their sum.  Only if t grew by more than the lag is the pass done again and O
-//     rescaled, so O stays in tensor memory for nearly all of the row's life.
+//   * warps 0-3 and 4-7: a thread per row of each row tile, two passes over S in tensor memory: the
+//     largest t; the weights and their sum.  O is rescaled (in tensor memory) only when t grew by
+//     more than the lag.  (Holding the row in registers saves the second read of S but not its time:
+//     the unrolled code of 128 columns missed the instruction cache and spilled.)
 // Every mbarrier wait is bounded; a timeout sets the device status word and the roles leave.
 #include <algorithm>
 #include <atomic>
@@ -58,19 +59,26 @@ __device__ __forceinline__ bool pwait(const uint64_t* bar, int phase) {
 
 // 128-byte swizzled tile: rows of 128 bytes, 8-row groups 1024 bytes apart, 64-element blocks of
 // the contiguous dimension kHalf apart (used when that dimension is N; K steps inside one block).
+// An offset of b bytes is b / 16 more.
 __device__ __forceinline__ uint64_t tile_desc(uint32_t saddr) {
     return uint64_t((saddr & 0x3FFFFu) >> 4) | uint64_t(kHalf >> 4) << 16 | uint64_t(1024 >> 4) << 32 |
            uint64_t(1) << 46 | uint64_t(2) << 61;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+template <bool ACC>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-                 "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(acc)) : "memory");
+                 "l"(a), "l"(b), "r"(idesc), "n"(ACC ? 1 : 0) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-                 "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(acc)) : "memory");
+                 "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ bool elected() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ void commit(const uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar))
@@ -79,30 +87,52 @@ __device__ __forceinline__ void commit(const uint64_t* bar) {
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+// 32 columns of the thread's lane; valid after tmem_wait on the same registers.
+template <int N>
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[N], int at = 0) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
         "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
-        "tcgen05.wait::ld.sync.aligned;\n"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
-          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "=r"(v[at]), "=r"(v[at + 1]), "=r"(v[at + 2]), "=r"(v[at + 3]), "=r"(v[at + 4]), "=r"(v[at + 5]),
+          "=r"(v[at + 6]), "=r"(v[at + 7]), "=r"(v[at + 8]), "=r"(v[at + 9]), "=r"(v[at + 10]), "=r"(v[at + 11]),
+          "=r"(v[at + 12]), "=r"(v[at + 13]), "=r"(v[at + 14]), "=r"(v[at + 15]), "=r"(v[at + 16]),
+          "=r"(v[at + 17]), "=r"(v[at + 18]), "=r"(v[at + 19]), "=r"(v[at + 20]), "=r"(v[at + 21]),
+          "=r"(v[at + 22]), "=r"(v[at + 23]), "=r"(v[at + 24]), "=r"(v[at + 25]), "=r"(v[at + 26]),
+          "=r"(v[at + 27]), "=r"(v[at + 28]), "=r"(v[at + 29]), "=r"(v[at + 30]), "=r"(v[at + 31])
         : "r"(taddr) : "memory");
 }
-template <int AT, int N>
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[N]) {
+template <int N>
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[N], int at) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+        : "=r"(v[at]), "=r"(v[at + 1]), "=r"(v[at + 2]), "=r"(v[at + 3]), "=r"(v[at + 4]), "=r"(v[at + 5]),
+          "=r"(v[at + 6]), "=r"(v[at + 7]), "=r"(v[at + 8]), "=r"(v[at + 9]), "=r"(v[at + 10]), "=r"(v[at + 11]),
+          "=r"(v[at + 12]), "=r"(v[at + 13]), "=r"(v[at + 14]), "=r"(v[at + 15])
+        : "r"(taddr) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void tmem_wait(uint32_t (&v)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; i += 8)  // no use of the registers moves above the wait
+        asm volatile("" : "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3]), "+r"(v[i + 4]),
+                     "+r"(v[i + 5]), "+r"(v[i + 6]), "+r"(v[i + 7]));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};\n" ::"r"(v[AT + 0]),
-        "r"(v[AT + 1]), "r"(v[AT + 2]), "r"(v[AT + 3]), "r"(v[AT + 4]), "r"(v[AT + 5]), "r"(v[AT + 6]),
-        "r"(v[AT + 7]), "r"(v[AT + 8]), "r"(v[AT + 9]), "r"(v[AT + 10]), "r"(v[AT + 11]), "r"(v[AT + 12]),
-        "r"(v[AT + 13]), "r"(v[AT + 14]), "r"(v[AT + 15]), "r"(v[AT + 16]), "r"(v[AT + 17]), "r"(v[AT + 18]),
-        "r"(v[AT + 19]), "r"(v[AT + 20]), "r"(v[AT + 21]), "r"(v[AT + 22]), "r"(v[AT + 23]), "r"(v[AT + 24]),
-        "r"(v[AT + 25]), "r"(v[AT + 26]), "r"(v[AT + 27]), "r"(v[AT + 28]), "r"(v[AT + 29]), "r"(v[AT + 30]),
-        "r"(v[AT + 31]), "r"(taddr) : "memory");
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};\n" ::"r"(v[0]),
+        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),
+        "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]),
+        "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};\n" ::"r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(taddr) : "memory");
 }
 
 // Two fp32 values in one register pair.
@@ -127,63 +157,101 @@ struct Row {
     int lo, hi;   // it sees keys [lo, hi)
 };
 
-// One pass over a row of S: weights 2^(t - mr) as fp16 pairs, their sum over vs, and the largest
-// t - mr.  tab[u] = {ks * scale * log2 e, log2 vs, 1 / vs} of 16 tokens.  MASK: the row may not
-// see all of the tile, which begins at key0.
-template <bool MASK>
-__device__ __forceinline__ void weigh(uint32_t s, const float4* tab, const Row& row, float mr, int key0,
-                                      uint32_t (&p)[64], float& sum, float& top) {
-    top = -INFINITY;
-    sum = 0.0f;
-    const uint32_t from = uint32_t(row.lo - key0), width = row.hi > row.lo ? uint32_t(row.hi - row.lo) : 0u;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        uint32_t v[32];
-        tmem_ld32(s + c * 32, v);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const float4 e = tab[2 * c + u];
-            const float cf = e.x * row.unit, b = e.y - mr;
-            const uint64_t cf2 = pack2f(cf, cf), b2 = pack2f(b, b);
-            uint64_t w2 = 0;
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const uint64_t t2 = fma2(uint64_t(v[16 * u + i]) | uint64_t(v[16 * u + i + 1]) << 32, cf2, b2);
-                float t0 = lo2(t2), t1 = hi2(t2);
-                if constexpr (MASK) {
-                    const uint32_t k = uint32_t(32 * c + 16 * u + i);
-                    if (k - from >= width) t0 = -INFINITY;
-                    if (k + 1 - from >= width) t1 = -INFINITY;
-                }
-                top = fmaxf(top, fmaxf(t0, t1));
-                const float w0 = ex2(t0), w1 = ex2(t1);
-                w2 = add2(w2, pack2f(w0, w1));
-                p[16 * c + 8 * u + i / 2] = pack_half2(w0, w1);  // 11 bits, as the codes' operands need
-            }
-            sum = fmaf(lo2(w2) + hi2(w2), e.z, sum);
+// Bit i: the row sees key key0 + i.
+__device__ __forceinline__ uint32_t seen32(const Row& row, int key0) {
+    const int lo = min(max(row.lo - key0, 0), 32), hi = min(max(row.hi - key0, 0), 32);
+    return hi > lo ? (0xffffffffu >> (32 - (hi - lo))) << lo : 0u;
+}
+
+// Walks the row's 128 columns of S, a unit of 16 tokens at a time, the next on its way: f(v, e, at,
+// seen) with v the columns from `at` on, e = {ks * scale * log2 e, log2 vs, 1 / vs} of the unit, and
+// with MASK the columns that the row sees of the tile, which begins at key0.
+template <bool MASK, class F>
+__device__ __forceinline__ void columns(uint32_t s, const float4* tab, const Row& row, int key0, F f) {
+    uint32_t v[32];
+    float4 e0 = tab[0], e1;
+    tmem_ld16(s, v, 0);
+#pragma unroll 1
+    for (int c = 0; c < 128; c += 32) {
+        const uint32_t seen = MASK ? seen32(row, key0 + c) : 0u;
+        tmem_wait(v);
+        tmem_ld16(s + c + 16, v, 16);
+        e1 = tab[c / 16 + 1];
+        f(v, e0, c, seen);
+        tmem_wait(v);
+        if (c < 96) {
+            tmem_ld16(s + c + 32, v, 0);
+            e0 = tab[c / 16 + 2];
         }
+        f(v + 16, e1, c + 16, seen >> 16);
     }
 }
 
-// The largest t of a row of S.
-__device__ __forceinline__ float largest(uint32_t s, const float4* tab, const Row& row, int key0) {
-    float top = -INFINITY;
-    const uint32_t from = uint32_t(row.lo - key0), width = row.hi > row.lo ? uint32_t(row.hi - row.lo) : 0u;
-#pragma unroll 1
-    for (int c = 0; c < 4; ++c) {
-        uint32_t v[32];
-        tmem_ld32(s + c * 32, v);
+// t - mr of columns i and i + 1.
+template <bool MASK>
+__device__ __forceinline__ uint64_t t_pair(const uint32_t* v, int i, uint64_t c2, uint64_t b2, uint32_t seen) {
+    const uint64_t t2 = fma2(uint64_t(v[i]) | uint64_t(v[i + 1]) << 32, c2, b2);
+    if constexpr (!MASK) return t2;
+    return pack2f(seen & (1u << i) ? lo2(t2) : -INFINITY, seen & (2u << i) ? hi2(t2) : -INFINITY);
+}
+
+// The largest t - mr of the row.
+template <bool MASK>
+__device__ __forceinline__ float largest(uint32_t s, const float4* tab, const Row& row, float mr, int key0) {
+    float top0 = -INFINITY, top1 = -INFINITY;
+    columns<MASK>(s, tab, row, key0, [&](const uint32_t* v, const float4& e, int, uint32_t seen) {
+        const float c = e.x * row.unit, b = e.y - mr;
+        const uint64_t c2 = pack2f(c, c), b2 = pack2f(b, b);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const float4 e = tab[2 * c + u];
-            const float cf = e.x * row.unit;
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (uint32_t(32 * c + 16 * u + i) - from < width)
-                    top = fmaxf(top, fmaf(__uint_as_float(v[16 * u + i]), cf, e.y));
+        for (int i = 0; i < 16; i += 4) {
+            const uint64_t t = t_pair<MASK>(v, i, c2, b2, seen), u = t_pair<MASK>(v, i + 2, c2, b2, seen);
+            top0 = fmaxf(top0, fmaxf(lo2(t), hi2(t)));
+            top1 = fmaxf(top1, fmaxf(lo2(u), hi2(u)));
         }
-    }
-    return top;
+    });
+    return fmaxf(top0, top1);
+}
+
+// 2^t of two values on the FMA units: t = n + f with n its nearest integer (added to 1.5 * 2^23, so
+// that the sum's low bits are n), a polynomial of degree 4 for 2^f on [-1/2, 1/2] (minimax in the
+// relative error, 2.6e-6, by Remez' exchange) and n added to the exponent field.  t < -126 gives
+// 2^-126, and so does a NaN.
+__device__ __forceinline__ uint64_t ex2_pair(uint64_t t) {
+    const uint64_t x = pack2f(fmaxf(lo2(t), -126.0f), fmaxf(hi2(t), -126.0f));
+    const uint64_t n = add2(x, pack2f(12582912.0f, 12582912.0f));
+    const uint64_t f = fma2(add2(n, pack2f(-12582912.0f, -12582912.0f)), pack2f(-1.0f, -1.0f), x);
+    uint64_t p = fma2(f, pack2f(0x1.3997d6p-7f, 0x1.3997d6p-7f), pack2f(0x1.ca1440p-5f, 0x1.ca1440p-5f));
+    p = fma2(p, f, pack2f(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+    p = fma2(p, f, pack2f(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+    p = fma2(p, f, pack2f(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+    return uint64_t(uint32_t(p) + (uint32_t(n) << 23)) | uint64_t(uint32_t(p >> 32) + (uint32_t(n >> 32) << 23)) << 32;
+}
+
+// Weights 2^(t - mr) as fp16 pairs over the columns of S that were read, and their sum over vs.
+// Without a mask one pair in kPolyEvery goes to the FMA units: the exponential unit's 16 a clock
+// bound this loop.  (A NaN unit still shows through the other pairs.)
+constexpr int kPolyEvery = 4;
+
+template <bool MASK>
+__device__ __forceinline__ float weigh(uint32_t s, const float4* tab, const Row& row, float mr, int key0) {
+    float l = 0.0f;
+    columns<MASK>(s, tab, row, key0, [&](const uint32_t* v, const float4& e, int at, uint32_t seen) {
+        uint32_t p[8];
+        const float c = e.x * row.unit, b = e.y - mr;
+        const uint64_t c2 = pack2f(c, c), b2 = pack2f(b, b);
+        uint64_t w2 = 0;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const uint64_t t2 = t_pair<MASK>(v, i, c2, b2, seen);
+            const uint64_t w = !MASK && (i / 2) % kPolyEvery == kPolyEvery - 1 ? ex2_pair(t2)
+                                                                              : pack2f(ex2(lo2(t2)), ex2(hi2(t2)));
+            w2 = add2(w2, w);
+            p[i / 2] = pack_half2(lo2(w), hi2(w));  // 11 bits, as the codes' operands need
+        }
+        l = fmaf(lo2(w2) + hi2(w2), e.z, l);
+        tmem_st8(s + at / 2, p);
+    });
+    return l;
 }
 
 template <int D, bool BF16>
@@ -205,7 +273,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     uint64_t* p_full = s_full + 2;
     uint64_t* o_done = p_full + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
-    __shared__ int64_t scratch[kPromptThreads / 32 + 2];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp == 12) {
@@ -232,134 +299,308 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
-    int request;
-    int64_t at, units;
-    kv_share<kPromptRows, kPromptKeys, kPromptThreads>(a, least, scratch, request, at, units);
+    const KvShare share = kv_share<kPromptRows, kPromptKeys, kPromptThreads>(a, least, reinterpret_cast<int*>(smem));
+    fence_proxy_async_smem();  // copies will overwrite what kv_share kept there
     if (threadIdx.x < 2) a.desc[2 * blockIdx.x + threadIdx.x] = make_int4(0, 0, 0, 0);
     before_sync();
     __syncthreads();
     after_sync();
     const uint32_t tmem = *tmem_slot;
     KvWalk<kPromptRows, kPromptKeys> walk;
-    walk.start(a, request, at, units);
+    walk.start(a, share);
 
-    if (warp == 12) {
-        // ---------------- loader ----------------
-        const int bsize = a.pool.block_size, none = a.pool.blocks;
-        const int64_t past_pool = int64_t(none) * a.pool.kv_heads * bsize;  // TMA fills with zeros
-        const int boxes = kPromptKeys / bsize;  // at most 8
-        int it = 0;
+    if (warp < 8) {
+        // ---------------- a thread per row ----------------
+        const int x = warp >> 2;                               // row tile
+        const int rl = (warp & 3) * 32 + lane;                 // row in it = tensor memory lane
+        const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
+        const uint32_t s_addr = tmem + lane_base + kSCol + x * 128, o_addr = tmem + lane_base + kOCol + x * 128;
+        int g = 0;   // key tiles of this row tile so far
+        int gj = 0;  // key tiles of the CTA so far
         bool ok = true;
         for (; !walk.done() && ok; walk.next(a)) {
-            const int32_t* row = a.tables + int64_t(walk.request) * a.width;
-            auto block_of = [&](int token) {
-                const int column = token >> a.pool.shift;
-                if (token >= walk.r.length || column >= a.width) return none;
-                const int id = __ldg(row + column);
-                return id < 0 || id > none ? none : id;
+            if (x == 1 && walk.r.rows - walk.rt * kPromptRows <= 128) {
+                gj += walk.n;
+                continue;
+            }
+            const int r = walk.rt * kPromptRows + x * 128 + rl;
+            const bool live = r < walk.r.rows;
+            const int token = live ? by_group(a, r) : 0, head = walk.head * a.group + (live ? r - token * a.group : 0);
+            Row row;
+            row.unit = 1.0f;
+            row.mr = -INFINITY;
+            row.l = 0.0f;
+            const int place = walk.r.begin + token;
+            row.hi = !live ? INT_MAX : a.causal ? min(place + 1, walk.r.length) : walk.r.length;
+            row.lo = !live ? 0 : max(walk.r.first, a.window > 0 ? place - a.window + 1 : 0);
+            // q: PER lanes read a row together, 16 bytes each
+            constexpr int PER = D / 8, ROWS = 32 / PER;
+            const int row0 = walk.rt * kPromptRows + x * 128 + (warp & 3) * 32;  // the warp's first row
+            auto row_at = [&](int i, int64_t token_stride, int64_t head_stride) {  // its row i's offset; -1: past the last
+                const int ri = row0 + i;
+                if (ri >= walk.r.rows) return int64_t(-1);
+                const int t = by_group(a, ri);
+                return (walk.r.token0 + t) * token_stride + (walk.head * a.group + ri - t * a.group) * head_stride;
             };
-            const int box_row = (lane & 7) * bsize, unit_row = (lane & 7) * 16;
-            int id_next = lane < boxes ? block_of(walk.t0 * kPromptKeys + box_row) : none;
-            int sid_next = block_of(walk.t0 * kPromptKeys + unit_row);
-            for (int j = 0; j < walk.n && ok; ++j) {
-                const int key0 = (walk.t0 + j) * kPromptKeys;
-                const int id = id_next, sid = sid_next;
-                if (j + 1 < walk.n) {
-                    if (lane < boxes) id_next = block_of(key0 + kPromptKeys + box_row);
-                    sid_next = block_of(key0 + kPromptKeys + unit_row);
+            uint8_t* staged = smem + x * C::kTile + (warp & 3) * 32 * 128;  // q's rows, later the output's
+            const int mine = lane / PER, chunk = lane % PER;
+            auto stage_at = [&](int i) {  // this lane's 16 bytes of the warp's row i
+                return reinterpret_cast<uint4*>(staged + (chunk / 8) * kHalf + i * 128 + (((chunk & 7) ^ (i & 7)) << 4));
+            };
+            {
+                uint4 v[PER];
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    const int64_t off = row_at(i * ROWS + mine, a.q.token_stride, a.q.head_stride);
+                    v[i] = off >= 0 ? __ldg(reinterpret_cast<const uint4*>(a.q.p + off) + chunk) : make_uint4(0, 0, 0, 0);
                 }
-                for (int side = 0; side < 2; ++side, ++it) {
-                    const int st = it % kRaw;
-                    const bool free = it < kRaw || pwait(raw_empty + st, it / kRaw - 1);
-                    if (!__all_sync(0xffffffffu, free)) {
-                        ok = false;
-                        break;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    if constexpr (BF16) {
+                        // over the power of two at the row's largest element, as in ebx_kv_attention.cu
+                        const uint32_t m = 0x7fff7fffu;
+                        uint32_t top = __vmaxu2(__vmaxu2(v[i].x & m, v[i].y & m), __vmaxu2(v[i].z & m, v[i].w & m));
+                        top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+                        for (int d = 1; d < PER; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        const uint32_t e = min(max(top >> 7, 1u), 253u);
+                        const float down = __uint_as_float((254u - e) << 23);
+                        const uint32_t up = __shfl_sync(0xffffffffu, e << 23, (lane % ROWS) * PER);
+                        if (lane / ROWS == i) row.unit = __uint_as_float(up);
+                        auto half = [&](uint32_t b) {
+                            return pack_half2(__uint_as_float(b << 16) * down, __uint_as_float(b & 0xffff0000u) * down);
+                        };
+                        v[i] = make_uint4(half(v[i].x), half(v[i].y), half(v[i].z), half(v[i].w));
                     }
-                    const uint32_t bar = smem_u32(raw_full + st);
-                    if (lane == 0) mbar_expect_tx(bar, C::kRawTile);
-                    __syncwarp();
-                    if (lane < boxes)
-                        kv_tma_2d(smem_u32(smem + C::kRawOff + st * C::kRawTile + box_row * D), side ? &map_v : &map_k, 0,
-                                  int(id == none ? past_pool : (int64_t(id) * a.pool.kv_heads + walk.head) * bsize), bar);
-                    if (side == 0 && lane < 16) {  // both sides' scales travel with the keys
-                        const int64_t cell = int64_t(sid) * a.pool.kv_heads + walk.head;
-                        cp_async4(smem_u32(raw_scales + st * 16 + lane),
-                                  sid == none ? &kv_prompt_none : (lane < 8 ? a.pool.k_scales : a.pool.v_scales) + cell);
+                    *stage_at(i * ROWS + mine) = v[i];
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(q_full + x));
+            }
+            // keys that every row of the warp sees
+            const int all_lo = __reduce_max_sync(0xffffffffu, row.lo), all_hi = __reduce_min_sync(0xffffffffu, row.hi);
+            // moves mr of the rows whose t reached `top`, and what was summed with the old one
+            auto raise = [&](float top, int j) {
+                const bool up = top > row.mr + (kLag + kShift);
+                const float mr = up ? top - kShift : row.mr;
+                const float f = up ? ex2(row.mr - mr) : 1.0f;
+                row.mr = mr;
+                row.l *= f;
+                if (j == 0) return true;
+                if (!__all_sync(0xffffffffu, pwait(o_done + x, g - 1))) return false;
+                after_sync();
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t v[32];
+                    tmem_ld32(o_addr + c * 32, v);
+                    tmem_wait(v);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                    tmem_st32(o_addr + c * 32, v);
+                }
+                return true;
+            };
+            for (int j = 0; j < walk.n; ++j, ++g, ++gj) {
+                ok = pwait(s_full + x, g) && pwait(tab_full + gj % kTabs, gj / kTabs);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
+                }
+                after_sync();
+                const float4* tab = tabs + (gj % kTabs) * 8;
+                const int key0 = (walk.t0 + j) * kPromptKeys;
+                const bool mask = key0 < all_lo || key0 + kPromptKeys > all_hi;
+                const float mr = row.mr == -INFINITY ? 0.0f : row.mr;
+                const float top = mr + (mask ? largest<true>(s_addr, tab, row, mr, key0) : largest<false>(s_addr, tab, row, mr, key0));
+                if (__any_sync(0xffffffffu, top > row.mr + (kLag + kShift)))
+                    if (!(ok = raise(top, j))) break;
+                const float now = row.mr == -INFINITY ? 0.0f : row.mr;
+                row.l += mask ? weigh<true>(s_addr, tab, row, now, key0) : weigh<false>(s_addr, tab, row, now, key0);
+                asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+                before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(p_full + x));
+            }
+            if (!ok) break;
+            if (!__all_sync(0xffffffffu, pwait(o_done + x, g - 1))) {
+                ok = false;
+                break;
+            }
+            after_sync();
+            const bool whole = walk.begins && walk.ends;
+            const int slot = walk.begins ? 1 : 0;
+            const float inv = row.l == 0.0f ? 0.0f : 1.0f / row.l;
+            float4* part = whole ? nullptr
+                                 : reinterpret_cast<float4*>(kv_part<D, kPromptRows>(a, blockIdx.x, slot)) + x * 128 + rl;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t v[32];
+                tmem_ld32(o_addr + c * 32, v);
+                tmem_wait(v);
+                if (whole) {  // through shared memory, so that rows are written whole
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t h[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            h[k] = pack16<BF16>(__uint_as_float(v[8 * i + 2 * k]) * inv, __uint_as_float(v[8 * i + 2 * k + 1]) * inv);
+                        const int q = 4 * c + i;
+                        *reinterpret_cast<uint4*>(staged + (q / 8) * kHalf + lane * 128 + (((q & 7) ^ (lane & 7)) << 4)) =
+                            make_uint4(h[0], h[1], h[2], h[3]);
                     }
-                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(bar) : "memory");
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        part[(8 * c + i) * kPromptRows] =
+                            make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
+                                        __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
                 }
             }
+            __syncwarp();
+            if (whole) {
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    const int64_t off = row_at(i * ROWS + mine, int64_t(a.heads) * D, D);
+                    if (off >= 0) *(reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + off) + chunk) = *stage_at(i * ROWS + mine);
+                }
+            }
+            const int64_t at_row = int64_t(walk.r.token0 + token) * a.heads + head;
+            before_sync();
+            if (live && whole && a.lse)
+                a.lse[at_row] = row.l == 0.0f ? -INFINITY : (row.mr + lg2(row.l)) * 0.6931471805599453f;
+            if (!whole) kv_part_ml<D, kPromptRows>(a, blockIdx.x, slot)[x * 128 + rl] = make_float2(row.mr, row.l);
+            if (!whole && threadIdx.x == 0)
+                a.desc[2 * blockIdx.x + slot] = kv_desc(walk.r, walk.rt, kPromptRows, walk.head, walk.ends);
         }
-        asm volatile("cp.async.wait_all;\n" ::: "memory");
-    } else if (warp == 13) {
-        // ---------------- products ----------------
-        if (lane == 0) {
-            const uint32_t q0 = smem_u32(smem), bufs = smem_u32(smem + C::kBufOff);
+    } else if (warp >= 12) {
+        if (warp == 12) {
+            // ---------------- loader ----------------
+            const int bsize = a.pool.block_size, none = a.pool.blocks;
+            const int64_t past_pool = int64_t(none) * a.pool.kv_heads * bsize;  // TMA fills with zeros
+            const int boxes = kPromptKeys / bsize;  // at most 8
+            int it = 0;
+            bool ok = true;
+            for (; !walk.done() && ok; walk.next(a)) {
+                const int32_t* row = a.tables + int64_t(walk.request) * a.width;
+                auto block_of = [&](int token) {
+                    const int column = token >> a.pool.shift;
+                    if (token >= walk.r.length || column >= a.width) return none;
+                    const int id = __ldg(row + column);
+                    return id < 0 || id > none ? none : id;
+                };
+                const int box_row = (lane & 7) * bsize, unit_row = (lane & 7) * 16;
+                int id_next = lane < boxes ? block_of(walk.t0 * kPromptKeys + box_row) : none;
+                int sid_next = block_of(walk.t0 * kPromptKeys + unit_row);
+                for (int j = 0; j < walk.n && ok; ++j) {
+                    const int key0 = (walk.t0 + j) * kPromptKeys;
+                    const int id = id_next, sid = sid_next;
+                    if (j + 1 < walk.n) {
+                        if (lane < boxes) id_next = block_of(key0 + kPromptKeys + box_row);
+                        sid_next = block_of(key0 + kPromptKeys + unit_row);
+                    }
+                    for (int side = 0; side < 2; ++side, ++it) {
+                        const int st = it % kRaw;
+                        const bool free = it < kRaw || pwait(raw_empty + st, it / kRaw - 1);
+                        if (!__all_sync(0xffffffffu, free)) {
+                            ok = false;
+                            break;
+                        }
+                        const uint32_t bar = smem_u32(raw_full + st);
+                        if (lane == 0) mbar_expect_tx(bar, C::kRawTile);
+                        __syncwarp();
+                        if (lane < boxes)
+                            kv_tma_2d(smem_u32(smem + C::kRawOff + st * C::kRawTile + box_row * D), side ? &map_v : &map_k, 0,
+                                      int(id == none ? past_pool : (int64_t(id) * a.pool.kv_heads + walk.head) * bsize), bar);
+                        if (side == 0 && lane < 16) {  // both sides' scales travel with the keys
+                            const int64_t cell = int64_t(sid) * a.pool.kv_heads + walk.head;
+                            cp_async4(smem_u32(raw_scales + st * 16 + lane),
+                                      sid == none ? &kv_prompt_none : (lane < 8 ? a.pool.k_scales : a.pool.v_scales) + cell);
+                        }
+                        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(bar) : "memory");
+                    }
+                }
+            }
+            asm volatile("cp.async.wait_all;\n" ::: "memory");
+        } else if (warp == 13) {
+            // ---------------- products: the warp together, one elected lane issues ----------------
+            const uint64_t q0 = tile_desc(smem_u32(smem)), buf0 = tile_desc(smem_u32(smem + C::kBufOff));
             int it = 0;            // fp16 tiles used: key and value tiles in turn
             int seg = 0, segb = 0; // segments of either row tile
             int g[2] = {0, 0};     // key tiles of either row tile
             bool ok = true;
             auto scores = [&](int x, int buf) {
-                const uint32_t q = q0 + x * C::kTile, k = bufs + buf * C::kTile;
+                const uint64_t q = q0 + uint32_t(x * (C::kTile >> 4)), k = buf0 + uint32_t(buf * (C::kTile >> 4));
+                const uint32_t d = tmem + kSCol + x * 128;
+                if (elected()) {
+                    mma_ss<false>(d, q, k, C::kIdescS);
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    const uint32_t off = (i / 4) * kHalf + (i % 4) * 32;
-                    mma_ss(tmem + kSCol + x * 128, tile_desc(q + off), tile_desc(k + off), C::kIdescS, i != 0);
+                    for (int i = 1; i < D / 16; ++i) {
+                        constexpr uint32_t kBlock = kHalf >> 4;
+                        mma_ss<true>(d, q + (i / 4) * kBlock + (i % 4) * 2, k + (i / 4) * kBlock + (i % 4) * 2, C::kIdescS);
+                    }
+                    commit(s_full + x);
                 }
-                commit(s_full + x);
+                __syncwarp();
             };
             auto values = [&](int x, int buf, bool first) {
-                const uint32_t v = bufs + buf * C::kTile;
+                const uint64_t v = buf0 + uint32_t(buf * (C::kTile >> 4));
+                const uint32_t d = tmem + kOCol + x * 128, w = tmem + kSCol + x * 128;
+                if (elected()) {
 #pragma unroll
-                for (int i = 0; i < kPromptKeys / 16; ++i)
-                    mma_ts(tmem + kOCol + x * 128, tmem + kSCol + x * 128 + i * 8, tile_desc(v + i * 2048), C::kIdescO,
-                           !first || i != 0);
-                commit(o_done + x);
+                    for (int i = 0; i < kPromptKeys / 16; ++i)
+                        mma_ts(d, w + i * 8, v + i * (2048 >> 4), C::kIdescO, i == 0 ? !first : 1);
+                    commit(o_done + x);
+                }
+                __syncwarp();
+            };
+            auto release = [&](int buf) {
+                if (elected()) commit(buf_empty + buf);
+                __syncwarp();
+            };
+            auto wait = [&](const uint64_t* bar, int phase) {
+                const bool got = __all_sync(0xffffffffu, pwait(bar, phase));
+                after_sync();
+                return got;
             };
             for (; !walk.done() && ok; walk.next(a)) {
                 const bool two = walk.r.rows - walk.rt * kPromptRows > 128;
-                ok = pwait(buf_full + it % kBufs, it / kBufs) && pwait(q_full, seg);
+                ok = wait(buf_full + it % kBufs, it / kBufs) && wait(q_full, seg);
                 ++seg;
                 if (!ok) break;
-                after_sync();
                 scores(0, it % kBufs);
                 if (two) {
-                    if (!(ok = pwait(q_full + 1, segb))) break;
+                    if (!(ok = wait(q_full + 1, segb))) break;
                     ++segb;
-                    after_sync();
                     scores(1, it % kBufs);
                 }
-                commit(buf_empty + it % kBufs);
+                release(it % kBufs);
                 ++it;
                 for (int j = 0; j < walk.n; ++j) {
                     const int vb = it % kBufs, kb = (it + 1) % kBufs;
                     const bool more = j + 1 < walk.n;
-                    if (!(ok = pwait(buf_full + vb, it / kBufs) && pwait(p_full, g[0]))) break;
+                    if (!(ok = wait(buf_full + vb, it / kBufs) && wait(p_full, g[0]))) break;
                     ++g[0];
-                    after_sync();
                     values(0, vb, j == 0);
                     if (more) {
-                        if (!(ok = pwait(buf_full + kb, (it + 1) / kBufs))) break;
-                        after_sync();
+                        if (!(ok = wait(buf_full + kb, (it + 1) / kBufs))) break;
                         scores(0, kb);  // after the product above, which reads the same columns
                     }
                     if (two) {
-                        if (!(ok = pwait(p_full + 1, g[1]))) break;
+                        if (!(ok = wait(p_full + 1, g[1]))) break;
                         ++g[1];
-                        after_sync();
                         values(1, vb, j == 0);
                     }
-                    commit(buf_empty + vb);
+                    release(vb);
                     if (more) {
                         if (two) scores(1, kb);
-                        commit(buf_empty + kb);
+                        release(kb);
                     }
                     it += more ? 2 : 1;
                 }
             }
         }
-        __syncwarp();
-    } else if (warp >= 8) {
+    } else {
         // ---------------- codes to fp16 ----------------
         const int w = warp - 8;
         int it = 0, gj = 0;
@@ -379,8 +620,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                             const bool none = vs < 0.0f;                        // kKvNone
                             const float vsc = vs < 0x1p-100f ? 0x1p-100f : vs;  // NaN stays
                             // NaN goes through t, where the mask stops it, and not through 1 / vs
-                            tabs[(gj % kTabs) * 8 + lane] = make_float4(
-                                none ? 0.0f : ks * a.scale_log2, none ? -INFINITY : lg2(vsc), vs == vs ? 1.0f / vsc : 1.0f, 0.0f);
+                            tabs[(gj % kTabs) * 8 + lane] =
+                                make_float4(none ? 0.0f : ks * a.scale_log2, none ? -INFINITY : lg2(vsc),
+                                            none ? 0.0f : vs == vs ? 1.0f / vsc : 1.0f, 0.0f);
                         }
                         __syncwarp();
                         if (lane == 0) mbar_arrive(smem_u32(tab_full + gj % kTabs));
@@ -389,7 +631,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     uint8_t* out = smem + C::kBufOff + buf * C::kTile;
                     constexpr int CH = D / 16 < 4 ? D / 16 : 4;  // 16-byte chunks of a row that neighbouring lanes read
                     constexpr int STEP = 32 / CH;                // rows of a warp's load
-#pragma unroll
+#pragma unroll 2
                     for (int g = 0; g < 32 / STEP; ++g)
 #pragma unroll
                         for (int h = 0; h < C::HALVES; ++h) {
@@ -420,162 +662,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     }
                 }
             }
-        }
-    } else {
-        // ---------------- a thread per row ----------------
-        const int x = warp >> 2;                               // row tile
-        const int rl = (warp & 3) * 32 + lane;                 // row in it = tensor memory lane
-        const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
-        const uint32_t s_addr = tmem + lane_base + kSCol + x * 128, o_addr = tmem + lane_base + kOCol + x * 128;
-        int g = 0;   // key tiles of this row tile so far
-        int gj = 0;  // key tiles of the CTA so far
-        bool ok = true;
-        for (; !walk.done() && ok; walk.next(a)) {
-            if (x == 1 && walk.r.rows - walk.rt * kPromptRows <= 128) {
-                gj += walk.n;
-                continue;
-            }
-            const int r = walk.rt * kPromptRows + x * 128 + rl;
-            const bool live = r < walk.r.rows;
-            const int token = live ? r / a.group : 0, head = walk.head * a.group + (live ? r % a.group : 0);
-            Row row;
-            row.unit = 1.0f;
-            row.mr = -INFINITY;
-            row.l = 0.0f;
-            const int place = walk.r.begin + token;
-            row.hi = !live ? INT_MAX : a.causal ? min(place + 1, walk.r.length) : walk.r.length;
-            row.lo = !live ? 0 : max(walk.r.first, a.window > 0 ? place - a.window + 1 : 0);
-            {
-                const uint16_t* src = a.q.p + (walk.r.token0 + token) * a.q.token_stride + head * a.q.head_stride;
-                uint4 v[D / 8];
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i)
-                    v[i] = live ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
-                if constexpr (BF16) {
-                    // over the power of two at the row's largest element, as in ebx_kv_attention.cu
-                    uint32_t top = 0;
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i) {
-                        const uint32_t m = 0x7fff7fffu;
-                        top = __vmaxu2(top, __vmaxu2(__vmaxu2(v[i].x & m, v[i].y & m), __vmaxu2(v[i].z & m, v[i].w & m)));
-                    }
-                    top = max(top & 0xffffu, top >> 16);
-                    const uint32_t e = min(max(top >> 7, 1u), 253u);
-                    const float down = __uint_as_float((254u - e) << 23);
-                    row.unit = __uint_as_float(e << 23);
-                    auto half = [&](uint32_t b) {
-                        return pack_half2(__uint_as_float(b << 16) * down, __uint_as_float(b & 0xffff0000u) * down);
-                    };
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i) v[i] = make_uint4(half(v[i].x), half(v[i].y), half(v[i].z), half(v[i].w));
-                }
-                uint8_t* dst = smem + x * C::kTile + rl * 128;
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i)
-                    *reinterpret_cast<uint4*>(dst + (i / 8) * kHalf + (((i & 7) ^ (rl & 7)) << 4)) = v[i];
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(q_full + x));
-            }
-            // keys that every row of the warp sees
-            const int all_lo = __reduce_max_sync(0xffffffffu, row.lo), all_hi = __reduce_min_sync(0xffffffffu, row.hi);
-            // moves mr of the rows whose t reached `top`, and what was summed with the old one
-            auto raise = [&](float top, int j) {
-                const bool up = top > row.mr + (kLag + kShift);
-                const float mr = up ? top - kShift : row.mr;
-                const float f = up ? ex2(row.mr - mr) : 1.0f;
-                row.mr = mr;
-                row.l *= f;
-                if (j == 0) return true;
-                if (!__all_sync(0xffffffffu, pwait(o_done + x, g - 1))) return false;
-                after_sync();
-#pragma unroll 1
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t v[32];
-                    tmem_ld32(o_addr + c * 32, v);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-                    tmem_st32<0>(o_addr + c * 32, v);
-                }
-                return true;
-            };
-            for (int j = 0; j < walk.n; ++j, ++g, ++gj) {
-                ok = pwait(s_full + x, g) && pwait(tab_full + gj % kTabs, gj / kTabs);
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
-                    break;
-                }
-                after_sync();
-                const float4* tab = tabs + (gj % kTabs) * 8;
-                const int key0 = (walk.t0 + j) * kPromptKeys;
-                const bool mask = key0 < all_lo || key0 + kPromptKeys > all_hi;
-                uint32_t p[64];
-                float sum, top;
-                if (__any_sync(0xffffffffu, row.mr == -INFINITY)) {
-                    ok = raise(largest(s_addr, tab, row, key0), j);
-                    if (!__all_sync(0xffffffffu, ok)) {
-                        ok = false;
-                        break;
-                    }
-                }
-                for (int again = 0; again < 2; ++again) {
-                    const float mr = row.mr == -INFINITY ? 0.0f : row.mr;
-                    if (mask) weigh<true>(s_addr, tab, row, mr, key0, p, sum, top);
-                    else weigh<false>(s_addr, tab, row, mr, key0, p, sum, top);
-                    if (!__any_sync(0xffffffffu, top > kLag + kShift)) break;
-                    if (again == 0 && !__all_sync(0xffffffffu, raise(top + mr, j))) {
-                        ok = false;
-                        break;
-                    }
-                }
-                if (!ok) break;
-                row.l += sum;
-                tmem_st32<0>(s_addr, p);
-                tmem_st32<32>(s_addr + 32, p);
-                asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
-                before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(p_full + x));
-            }
-            if (!ok) break;
-            if (!__all_sync(0xffffffffu, pwait(o_done + x, g - 1))) {
-                ok = false;
-                break;
-            }
-            after_sync();
-            const bool whole = walk.begins && walk.ends;
-            const int slot = walk.begins ? 1 : 0;
-            const float inv = row.l == 0.0f ? 0.0f : 1.0f / row.l;
-            const int64_t at_row = int64_t(walk.r.token0 + token) * a.heads + head;
-            float* part = whole ? nullptr
-                                : a.part + ((2 * int64_t(blockIdx.x) + slot) * kPromptRows + x * 128 + rl) * (D + 2);
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-                uint32_t v[32];
-                tmem_ld32(o_addr + c * 32, v);
-                if (live && whole) {
-                    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at_row * D + c * 32);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t h[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            h[k] = pack16<BF16>(__uint_as_float(v[8 * i + 2 * k]) * inv, __uint_as_float(v[8 * i + 2 * k + 1]) * inv);
-                        dst[i] = make_uint4(h[0], h[1], h[2], h[3]);
-                    }
-                } else if (live) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2)
-                        *reinterpret_cast<uint2*>(part + c * 32 + i) = make_uint2(v[i], v[i + 1]);
-                }
-                __syncwarp();
-            }
-            before_sync();
-            if (live && whole && a.lse)
-                a.lse[at_row] = row.l == 0.0f ? -INFINITY : (row.mr + lg2(row.l)) * 0.6931471805599453f;
-            if (live && !whole) *reinterpret_cast<float2*>(part + D) = make_float2(row.mr, row.l);
-            if (!whole && threadIdx.x == 0)
-                a.desc[2 * blockIdx.x + slot] = kv_desc(walk.r, walk.rt, kPromptRows, walk.head, walk.ends);
         }
     }
 
@@ -610,7 +696,7 @@ cudaError_t launch_prompt(KvAttnArgs a, void* ws, int dev, cudaStream_t s) {
     kern<<<grid, kPromptThreads, C::kSmem, s>>>(mk, mv, a, kPromptLeast);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    return launch_join<D, kPromptRows, BF16>(a, grid, 16, s);
+    return launch_join<D, kPromptRows, BF16>(a, grid, kPromptRows, s);
 }
 
 }  // namespace

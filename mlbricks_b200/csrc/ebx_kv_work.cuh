@@ -43,12 +43,17 @@ __device__ __forceinline__ KvRequest kv_request(const KvAttnArgs& a, int i) {
     return r;
 }
 
+// n / group for 0 <= n < 2^31 (KvAttnArgs::set_group).
+__device__ __forceinline__ int by_group(const KvAttnArgs& a, int n) {
+    return int(uint64_t(uint32_t(n)) * a.group_mul >> a.group_shift);
+}
+
 // Keys [lo, hi) that some row of the tile sees, as key tiles [t0, t0 + n), n >= 1 (a tile that
 // sees nothing still has its zeros to write).
 template <int RT, int KT>
 __device__ __forceinline__ void kv_key_tiles(const KvAttnArgs& a, const KvRequest& r, int rt, int& t0, int& n) {
     const int last = min((rt + 1) * RT, r.rows) - 1;
-    const int p0 = r.begin + rt * RT / a.group, p1 = r.begin + last / a.group;
+    const int p0 = r.begin + by_group(a, rt * RT), p1 = r.begin + by_group(a, last);
     const int hi = a.causal ? min(p1 + 1, r.length) : r.length;
     const int lo = max(r.first, a.window > 0 ? p0 - a.window + 1 : 0);
     t0 = max(lo, 0) / KT;
@@ -56,17 +61,12 @@ __device__ __forceinline__ void kv_key_tiles(const KvAttnArgs& a, const KvReques
     n = max(n, 1);
 }
 
-// Units of one head of the request.
-template <int RT, int KT>
-__device__ __forceinline__ int64_t kv_head_units(const KvAttnArgs& a, const KvRequest& r) {
-    int64_t sum = 0;
-    for (int rt = 0; rt * RT < r.rows; ++rt) {
-        int t0, n;
-        kv_key_tiles<RT, KT>(a, r, rt, t0, n);
-        sum += n;
-    }
-    return sum;
-}
+// Where a CTA's share of the line begins, and how long it is.
+struct KvShare {
+    int64_t units;
+    int request, head, rt;
+    int skip;  // key tiles of that row tile that belong to the CTA before
+};
 
 // A CTA's walk along the line: which (request, head, row tile) it is at, and which of its key
 // tiles are the CTA's.  Every warp keeps its own copy.
@@ -75,28 +75,19 @@ struct KvWalk {
     int64_t left;        // units from here to the CTA's end
     int request, head, rt;
     KvRequest r;
-    int64_t head_units;
-    int skip;            // key tiles of the current row tile that belong to the CTA before
+    int skip;
     // the current segment
     int t0, n;           // its key tiles
     bool begins, ends;   // it holds the row tile's first / last key tile
 
-    // at: the unit of the line at which this CTA begins, counted from the start of `req`
-    __device__ __forceinline__ void start(const KvAttnArgs& a, int req, int64_t at, int64_t units) {
-        left = units;
-        request = req;
-        head = rt = skip = 0;
+    __device__ __forceinline__ void start(const KvAttnArgs& a, const KvShare& s) {
+        left = s.units;
+        request = s.request;
+        head = s.head;
+        rt = s.rt;
+        skip = s.skip;
         if (left <= 0) return;
         r = kv_request(a, request);
-        head_units = kv_head_units<RT, KT>(a, r);
-        head = int(at / head_units);
-        int64_t rest = at - head * head_units;
-        for (;; ++rt) {
-            kv_key_tiles<RT, KT>(a, r, rt, t0, n);
-            if (rest < n) break;
-            rest -= n;
-        }
-        skip = int(rest);
         segment(a);
     }
     __device__ __forceinline__ void segment(const KvAttnArgs& a) {
@@ -126,66 +117,139 @@ struct KvWalk {
     }
 };
 
-// Where this CTA's share begins: `request`, `at` units into it, `units` long.  Called by all
-// NT threads of the block; `scratch` holds NT / 32 + 2 int64.
+// This CTA's share.  Called by all NT threads of the block.  Two steps over windows of requests:
+// a thread per request counts its row tiles, then a thread per row tile counts its key tiles, so
+// that one long prompt and many short requests cost the same few loads a thread.  `scratch`:
+// kShareInts ints of shared memory, free again when the last barrier in here is passed.
+constexpr int kShareWindow = 1024;
+constexpr int kShareInts = 2 * kShareWindow + 128;
+
 template <int RT, int KT, int NT>
-__device__ __forceinline__ void kv_share(const KvAttnArgs& a, int64_t least, int64_t* scratch, int& request,
-                                         int64_t& at, int64_t& units) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+__device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, int* scratch) {
     constexpr int W = NT / 32;
-    auto request_units = [&](int i) {
-        if (i >= a.requests) return int64_t(0);
-        const KvRequest r = kv_request(a, i);
-        return kv_head_units<RT, KT>(a, r) * a.pool.kv_heads;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int* tiles = scratch;                       // row tiles of the window's requests ahead of i
+    int* units = scratch + kShareWindow;        // key tiles of one head of request i
+    int64_t* sums = reinterpret_cast<int64_t*>(scratch + 2 * kShareWindow);  // [W] and the answer
+    static_assert(W + 4 <= 64, "scratch of kv_share");
+    // exclusive scan over the block; total receives the sum
+    auto scan = [&](int64_t v, int64_t& total) {
+        int64_t x = v;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t o = __shfl_up_sync(0xffffffffu, x, d);
+            if (lane >= d) x += o;
+        }
+        __syncthreads();
+        if (lane == 31) sums[warp] = x;
+        __syncthreads();
+        total = 0;
+        int64_t ahead = x - v;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            if (w < warp) ahead += sums[w];
+            total += sums[w];
+        }
+        return ahead;
     };
-    int64_t mine = 0;
-    for (int i = tid; i < a.requests; i += NT) mine += request_units(i);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
-    if (lane == 0) scratch[warp] = mine;
-    __syncthreads();
+    // fills `units` for the requests [i0, i0 + n)
+    auto count = [&](int i0, int n) {
+        int64_t all = 0;
+        for (int b = 0; b < n; b += NT) {
+            const int i = b + tid;
+            int64_t rts = 0, total;
+            if (i < n) {
+                const int64_t s0 = max(a.starts[i0 + i], 0), s1 = min(int64_t(a.starts[i0 + i + 1]), a.tokens);
+                rts = s1 > s0 ? ((s1 - s0) * a.group + RT - 1) / RT : 0;
+            }
+            const int64_t ahead = all + scan(rts, total);
+            if (i < n) {
+                tiles[i] = int(ahead);
+                units[i] = 0;
+            }
+            all += total;
+        }
+        __syncthreads();
+        for (int64_t x = tid; x < all; x += NT) {
+            int lo = 0, hi = n;  // the last request with tiles[lo] <= x: it has row tiles
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (tiles[mid] <= x) lo = mid; else hi = mid;
+            }
+            int t0, k;
+            kv_key_tiles<RT, KT>(a, kv_request(a, i0 + lo), int(x) - tiles[lo], t0, k);
+            atomicAdd(units + lo, k);
+        }
+        __syncthreads();
+    };
     int64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < W; ++w) total += scratch[w];
+    for (int i0 = 0; i0 < a.requests; i0 += kShareWindow) {
+        const int n = min(kShareWindow, a.requests - i0);
+        count(i0, n);
+        int64_t mine = 0, all;
+        for (int i = tid; i < n; i += NT) mine += units[i];
+        scan(mine, all);
+        total += all * a.pool.kv_heads;
+    }
     int64_t per = (total + gridDim.x - 1) / gridDim.x;
     per = per < least ? least : per;
     const int64_t w0 = per * blockIdx.x;
-    units = total - w0 < per ? total - w0 : per;
-    request = 0;
-    at = 0;
-    if (units <= 0) {
-        units = 0;
-        return;
+    KvShare out;
+    out.units = total - w0 < per ? total - w0 : per;
+    out.request = out.head = out.rt = out.skip = 0;
+    if (out.units <= 0) {
+        out.units = 0;
+        __syncthreads();
+        return out;
     }
-    // the request that holds unit w0: scan the requests' units NT at a time
-    int64_t base = 0;
-    for (int i0 = 0;; i0 += NT) {
-        const int64_t u = request_units(i0 + tid);
-        int64_t v = u;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int64_t o = __shfl_up_sync(0xffffffffu, v, d);
-            if (lane >= d) v += o;
+    int64_t base = 0;  // units ahead of the window
+    for (int i0 = 0;; i0 += kShareWindow) {
+        const int n = min(kShareWindow, a.requests - i0);
+        if (a.requests > kShareWindow) count(i0, n);  // else they are still there
+        bool found = false;
+        for (int b = 0; b < n; b += NT) {
+            const int i = b + tid;
+            const int64_t u = i < n ? int64_t(units[i]) * a.pool.kv_heads : 0;
+            int64_t all;
+            const int64_t begin = base + scan(u, all);
+            if (u > 0 && begin <= w0 && w0 < begin + u) {  // exactly one thread
+                const int64_t at = w0 - begin;
+                sums[W] = i0 + i;
+                sums[W + 1] = at / units[i];
+                sums[W + 2] = at % units[i];
+            }
+            base += all;
+            found = base > w0;
+            if (found) break;
         }
-        __syncthreads();
-        if (lane == 31) scratch[warp] = v;
-        __syncthreads();
-        int64_t ahead = base;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            if (w < warp) ahead += scratch[w];
-            base += scratch[w];
-        }
-        const int64_t begin = ahead + v - u;
-        if (u > 0 && begin <= w0 && w0 < begin + u) {  // exactly one thread
-            scratch[W] = i0 + tid;
-            scratch[W + 1] = w0 - begin;
-        }
-        if (base > w0) break;
+        if (found) break;
     }
     __syncthreads();
-    request = int(scratch[W]);
-    at = scratch[W + 1];
+    out.request = int(sums[W]);
+    out.head = int(sums[W + 1]);
+    // the row tile: each warp for itself, 32 at a time
+    int rest = int(sums[W + 2]);
+    const KvRequest r = kv_request(a, out.request);
+    for (int rt0 = 0;; rt0 += 32) {
+        int t0, k = 0;
+        if ((rt0 + lane) * RT < r.rows) kv_key_tiles<RT, KT>(a, r, rt0 + lane, t0, k);
+        int x = k;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, x, d);
+            if (lane >= d) x += o;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, x > rest);
+        if (past) {
+            const int f = __ffs(past) - 1;
+            out.rt = rt0 + f;
+            out.skip = rest - __shfl_sync(0xffffffffu, x - k, f);
+            break;
+        }
+        rest -= __shfl_sync(0xffffffffu, x, 31);
+    }
+    __syncthreads();
+    return out;
 }
 
 // ---- partial results ----------------------------------------------------------------------
@@ -205,6 +269,17 @@ __device__ __forceinline__ int4 kv_desc(const KvRequest& r, int rt, int rt_rows,
 constexpr float kLag = 8.0f, kShift = 7.0f;
 // V scale of 16 tokens that no block holds: their keys are not seen.
 constexpr float kKvNone = -1.0f;
+
+// A part: O as float4 [head_dim / 4][RT] (neighbouring rows are neighbours, for threads that hold a
+// row each), then {m, l} [RT].
+template <int D, int RT>
+__device__ __forceinline__ float* kv_part(const KvAttnArgs& a, int cta, int slot) {
+    return a.part + (2 * int64_t(cta) + slot) * RT * (D + 2);
+}
+template <int D, int RT>
+__device__ __forceinline__ float2* kv_part_ml(const KvAttnArgs& a, int cta, int slot) {
+    return reinterpret_cast<float2*>(kv_part<D, RT>(a, cta, slot) + RT * D);
+}
 
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
@@ -240,69 +315,82 @@ __device__ __forceinline__ uint32_t codes_to_half2(uint32_t w, uint32_t sel) {
     return hsub2_u(__byte_perm(w, 0x64646464u, sel), 0x64806480u);  // - 1152
 }
 
-// Row tiles that several CTAs worked on: CTA (c, y) joins the one that begins in CTA c, its rows
-// y, y + gridDim.y, ..., reading c's part 1 and then part 0 of the CTAs after it until one ends it.
+// Row tiles that several CTAs worked on: CTA (c, y) joins rows 4 y .. 4 y + 3 (and so on, gridDim.y
+// fours at a time) of the one that begins in CTA c, reading c's part 1 and then part 0 of the CTAs
+// after it until one ends it.  Threads: 4 rows x 8 ways (parts taken in turn) x 8 column groups.
 template <int D, int RT, bool BF16>
-__global__ void __launch_bounds__(128) kv_join_kernel(const __grid_constant__ KvAttnArgs a, int ctas) {
+__global__ void __launch_bounds__(256) kv_join_kernel(const __grid_constant__ KvAttnArgs a, int ctas) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    constexpr int LANES = D / 4;            // threads of a row, 4 values each
-    constexpr int WAYS = 128 / LANES;       // parts of a row read at once
-    __shared__ float s_m[WAYS][LANES], s_l[WAYS][LANES];
-    __shared__ float4 s_o[WAYS][LANES];
+    constexpr int COLS = D / 32;  // float4 columns of a thread: groups of 8 apart
+    __shared__ float2 s_ml[8][8][4];
+    __shared__ float4 s_o[COLS][8][8][4];
     __shared__ int s_last;
     const int c = blockIdx.x;
     const int4 d1 = a.desc[2 * c + 1];
-    if (d1.x == 0) return;
+    if (d1.x == 0 || int(blockIdx.y) * 4 >= d1.w) return;
     if (threadIdx.x == 0) s_last = ctas - 1;
-    for (int base = c + 1;; base += 128) {  // the CTA that ends the row tile
+    __syncthreads();
+    for (int base = c + 1;; base += 256) {  // the CTA that ends the row tile
         const int k = base + int(threadIdx.x);
         const bool end = k >= ctas - 1 || (a.desc[2 * k].x & kKvEnds) != 0;
-        const bool any = __syncthreads_or(end);
         if (end) atomicMin(&s_last, k);
-        if (any) break;
+        if (__syncthreads_or(end)) break;
     }
-    __syncthreads();
     const int last = s_last;
-    const int lane = threadIdx.x % LANES, way = threadIdx.x / LANES;
-    for (int r = blockIdx.y; r < d1.w; r += gridDim.y) {
+    const int ri = threadIdx.x & 3, col = (threadIdx.x >> 2) & 7, way = threadIdx.x >> 5;
+    for (int r0 = blockIdx.y * 4; r0 < d1.w; r0 += gridDim.y * 4) {
+        const int r = r0 + ri;
         float m = -INFINITY, l = 0.0f;
-        float4 o = make_float4(0, 0, 0, 0);
-        for (int k = c + way; k <= last; k += WAYS) {
-            const float* src = a.part + ((2 * int64_t(k) + (k == c ? 1 : 0)) * RT + r) * (D + 2);
-            const float2 v0 = *reinterpret_cast<const float2*>(src + 4 * lane);
-            const float2 v1 = *reinterpret_cast<const float2*>(src + 4 * lane + 2);
-            const float2 ml = *reinterpret_cast<const float2*>(src + D);
-            const float mn = fmaxf(m, ml.x);
-            const float f0 = m == mn ? 1.0f : ex2(m - mn), f1 = ml.x == mn ? 1.0f : ex2(ml.x - mn);
-            o.x = o.x * f0 + v0.x * f1; o.y = o.y * f0 + v0.y * f1;
-            o.z = o.z * f0 + v1.x * f1; o.w = o.w * f0 + v1.y * f1;
-            l = l * f0 + ml.y * f1;
-            m = mn;
-        }
-        s_m[way][lane] = m;
-        s_l[way][lane] = l;
-        s_o[way][lane] = o;
-        __syncthreads();
-        if (way == 0) {
+        float4 o[COLS];
 #pragma unroll
-            for (int w = 1; w < WAYS; ++w) {
-                const float m1 = s_m[w][lane];
-                const float4 v = s_o[w][lane];
-                const float mn = fmaxf(m, m1);
-                const float f0 = m == mn ? 1.0f : ex2(m - mn), f1 = m1 == mn ? 1.0f : ex2(m1 - mn);
-                o.x = o.x * f0 + v.x * f1; o.y = o.y * f0 + v.y * f1;
-                o.z = o.z * f0 + v.z * f1; o.w = o.w * f0 + v.w * f1;
-                l = l * f0 + s_l[w][lane] * f1;
-                m = mn;
+        for (int x = 0; x < COLS; ++x) o[x] = make_float4(0, 0, 0, 0);
+        auto join = [&](float m1, float l1, const float4 (&v)[COLS]) {
+            const float mn = fmaxf(m, m1);
+            const float f0 = m == mn ? 1.0f : ex2(m - mn), f1 = m1 == mn ? 1.0f : ex2(m1 - mn);
+#pragma unroll
+            for (int x = 0; x < COLS; ++x) {
+                o[x].x = o[x].x * f0 + v[x].x * f1;
+                o[x].y = o[x].y * f0 + v[x].y * f1;
+                o[x].z = o[x].z * f0 + v[x].z * f1;
+                o[x].w = o[x].w * f0 + v[x].w * f1;
+            }
+            l = l * f0 + l1 * f1;
+            m = mn;
+        };
+        if (r < d1.w) {
+            for (int k = c + way; k <= last; k += 8) {
+                const int slot = k == c ? 1 : 0;
+                const float4* src = reinterpret_cast<const float4*>(kv_part<D, RT>(a, k, slot));
+                float4 v[COLS];
+#pragma unroll
+                for (int x = 0; x < COLS; ++x) v[x] = src[(x * 8 + col) * RT + r];
+                const float2 ml = kv_part_ml<D, RT>(a, k, slot)[r];
+                join(ml.x, ml.y, v);
+            }
+        }
+        s_ml[way][col][ri] = make_float2(m, l);
+#pragma unroll
+        for (int x = 0; x < COLS; ++x) s_o[x][way][col][ri] = o[x];
+        __syncthreads();
+        if (way == 0 && r < d1.w) {
+            for (int w = 1; w < min(8, last - c + 1); ++w) {
+                float4 v[COLS];
+#pragma unroll
+                for (int x = 0; x < COLS; ++x) v[x] = s_o[x][w][col][ri];
+                join(s_ml[w][col][ri].x, s_ml[w][col][ri].y, v);
             }
             const int row = (d1.x & (kKvEnds - 1)) - 1 + r;
-            const int64_t at = int64_t(d1.y + row / a.group) * a.heads + d1.z * a.group + row % a.group;
+            const int token = by_group(a, row);
+            const int64_t at = int64_t(d1.y + token) * a.heads + d1.z * a.group + row - token * a.group;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            uint2 pk;
-            pk.x = pack16<BF16>(o.x * inv, o.y * inv);
-            pk.y = pack16<BF16>(o.z * inv, o.w * inv);
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at * D + 4 * lane) = pk;
-            if (a.lse && lane == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + lg2(l)) * 0.6931471805599453f;
+#pragma unroll
+            for (int x = 0; x < COLS; ++x) {
+                uint2 pk;
+                pk.x = pack16<BF16>(o[x].x * inv, o[x].y * inv);
+                pk.y = pack16<BF16>(o[x].z * inv, o[x].w * inv);
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at * D + 4 * (x * 8 + col)) = pk;
+            }
+            if (a.lse && col == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + lg2(l)) * 0.6931471805599453f;
         }
         __syncthreads();
     }
@@ -324,12 +412,12 @@ inline bool code_map(CUtensorMap* map, const int8_t* codes, const KvPool& p, int
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The join of a launch of `ctas` CTAs, started while the last of them still run.
+// The join of a launch of `ctas` CTAs whose row tiles have up to `rows` rows.
 template <int D, int RT, bool BF16>
-cudaError_t launch_join(const KvAttnArgs& a, int ctas, int ways, cudaStream_t s) {
+cudaError_t launch_join(const KvAttnArgs& a, int ctas, int rows, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(ctas), unsigned(ways));
-    cfg.blockDim = dim3(128);
+    cfg.gridDim = dim3(unsigned(ctas), unsigned((rows + 3) / 4));
+    cfg.blockDim = dim3(256);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
