@@ -30,17 +30,22 @@ __device__ __forceinline__ bool kv_wait(uint32_t bar, uint32_t parity) {
 
 // ---- few rows: decode ---------------------------------------------------------------------
 
-constexpr int kRows = 16;        // rows of a tile: the M of mma.m16n8k16
 constexpr int kConsumers = 4;    // warps that compute; one more loads
 constexpr int kStepThreads = 32 * (kConsumers + 1);
 constexpr int kStages = 3;
-template <int D>
+constexpr int kStepLeast = 4;   // key tiles a CTA takes at least: a partial result costs about as much
+
+// D: head_dim; NQ: blocks of 8 rows (queries) in a row tile, the N of mma.m16n8k16, whose M is 16
+// keys of the first product and 16 dimensions of the second.
+template <int D, int NQ>
 struct StepCfg {
+    static constexpr int ROWS = 8 * NQ;
+    static constexpr int PER_SM = NQ == 1 ? 3 : 2;   // CTAs of an SM that the registers allow
     static constexpr int KT = 8192 / D;              // tokens of a key tile: 8 KB of codes a side
     static constexpr int UNITS = KT / 16;            // 16 tokens lie in one block: one scale
     static constexpr int PER_WARP = UNITS / kConsumers;
     static constexpr int kStageBytes = 2 * 8192;
-    static constexpr int kMergeBytes = kConsumers * kRows * (D + 4) * 4;
+    static constexpr int kMergeBytes = kConsumers * ROWS * (D + 4) * 4;
     static constexpr int kSmem = 1024 + kStages * kStageBytes + kMergeBytes + kStages * 2 * UNITS * 4 + 256;
 };
 
@@ -51,9 +56,9 @@ __device__ __forceinline__ uint32_t swz(int r, int b) {
     return uint32_t(r * D + (b ^ (x << 4)));
 }
 
-// Column n of an 8-key product is key {0,5,2,7,1,4,3,6}[n] of its eight: with this order the
-// loads of K rows (by n) and of V rows (by n / 2, for n even and odd) are free of bank conflicts
-// under each of the three swizzles.
+// Row i of an 8-key block of the first product is key {0,5,2,7,1,4,3,6}[i] of its eight: with this
+// order the loads of K rows (by i) and of V rows (by i / 2, for i even and odd) are free of bank
+// conflicts under each of the three swizzles.
 __device__ __forceinline__ int key_even(int c) { return ((c & 1) << 1) | (c >> 1); }        // 0 2 1 3
 __device__ __forceinline__ int key_odd(int c) { return 4 + (key_even(c) ^ 1); }             // 5 7 4 6
 
@@ -68,17 +73,23 @@ __device__ __forceinline__ void lds(uint32_t addr, uint32_t (&w)[BYTES / 4]) {
         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
 }
 
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kStepThreads)
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+template <int D, int NQ, bool BF16>
+__global__ void __launch_bounds__(kStepThreads, (StepCfg<D, NQ>::PER_SM))
     kv_step_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                    const __grid_constant__ KvAttnArgs a, int least) {
-    using C = StepCfg<D>;
-    constexpr int KT = C::KT, UNITS = C::UNITS;
+    using C = StepCfg<D, NQ>;
+    constexpr int KT = C::KT, UNITS = C::UNITS, kRows = C::ROWS;
     constexpr int KB = D >= 64 ? 16 : 8;        // bytes of a K row that a lane loads at once
     constexpr int KL = D / (4 * KB);            // such loads for a row
     constexpr int KW = KB / 4;                  // words of it = products of depth 16
     constexpr int VB = D / 8;                   // bytes of a V row that a lane loads
-    constexpr int NT = VB;                      // 8-wide column tiles of O
+    constexpr int MT = D / 16;                  // 16-dimension tiles of O
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float* merge = reinterpret_cast<float*>(smem + kStages * C::kStageBytes);
@@ -163,75 +174,89 @@ __global__ void __launch_bounds__(kStepThreads)
     const int c = lane & 3, n8 = lane >> 2;
     const int krow = (n8 & 1) ? key_odd(n8 >> 1) : key_even(n8 >> 1);
     const int vrow0 = key_even(c), vrow1 = key_odd(c);
-    // the D / 8 bytes of a V row that this lane's column n8 of each of the NT column tiles holds
+    // the D / 8 bytes of a V row, and dimensions of O, of this lane
     const int vbyte = D == 128 ? 16 * ((n8 >> 1) | ((n8 & 1) << 2))
                       : D == 64 ? 8 * (2 * ((((n8 >> 1) & 1) << 1) | (n8 >> 2)) + (n8 & 1)) : 4 * n8;
-    // O: column tile t of columns 2c and 2c + 1 is dimension odim0 + t and odim1 + t
-    const int odim0 = D == 128 ? 16 * c : D == 64 ? 16 * (((c & 1) << 1) | (c >> 1)) : 8 * c;
-    const int odim1 = D == 128 ? odim0 + 64 : odim0 + VB;
     int it = 0;
     bool ok = true;
     for (; !walk.done(); walk.next(a)) {
-        // q: rows n8 and n8 + 8, this lane's 4 KL KW products of depth 16
-        uint32_t qa[KL * KW][4];
-        float unit[2] = {1.0f, 1.0f};  // what q was divided by
-        int lo[2], hi[2];              // the row sees keys [lo, hi); a row past the last is not kept
+        // q: row n8 of each block of 8, this lane's dimensions of the KL KW products of depth 16
+        uint32_t qb[NQ][KL * KW][2];
+        float unit[NQ][2];               // what the rows 2c and 2c + 1 of q were divided by
+        int lo[NQ][2], hi[NQ][2];        // they see keys [lo, hi); a row past the last is not kept
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int r = walk.rt * kRows + n8 + 8 * half;
-            const bool in = r < walk.r.rows;
-            const int token = in ? by_group(a, r) : 0;
-            const int place = walk.r.begin + token;
-            hi[half] = !in ? INT_MAX : a.causal ? min(place + 1, walk.r.length) : walk.r.length;
-            lo[half] = !in ? 0 : max(walk.r.first, a.window > 0 ? place - a.window + 1 : 0);
-            const uint16_t* src = a.q.p + (walk.r.token0 + token) * a.q.token_stride +
-                                  (walk.head * a.group + (in ? r - token * a.group : 0)) * a.q.head_stride + c * KB;
+        for (int nq = 0; nq < NQ; ++nq) {
+            {
+                const int r = walk.rt * kRows + 8 * nq + n8;
+                const bool in = r < walk.r.rows;
+                const int token = in ? by_group(a, r) : 0;
+                const uint16_t* src = a.q.p + (walk.r.token0 + token) * a.q.token_stride +
+                                      (walk.head * a.group + (in ? r - token * a.group : 0)) * a.q.head_stride + c * KB;
 #pragma unroll
-            for (int l = 0; l < KL; ++l)
+                for (int l = 0; l < KL; ++l)
 #pragma unroll
-                for (int q = 0; q < KW; q += 2) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (in) v = __ldg(reinterpret_cast<const uint4*>(src + l * 4 * KB + q * 4));
-                    qa[l * KW + q][half] = v.x;
-                    qa[l * KW + q][half + 2] = v.y;
-                    qa[l * KW + q + 1][half] = v.z;
-                    qa[l * KW + q + 1][half + 2] = v.w;
-                }
-        }
-        if constexpr (BF16) {
-            // fp16 operands: each row over the power of two at its largest element, so that every
-            // element of at least 2^-14 of it is exact and the others are off by 2^-25 of it
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
+                    for (int q = 0; q < KW; q += 2) {
+                        uint4 v = make_uint4(0, 0, 0, 0);
+                        if (in) v = __ldg(reinterpret_cast<const uint4*>(src + l * 4 * KB + q * 4));
+                        qb[nq][l * KW + q][0] = v.x;
+                        qb[nq][l * KW + q][1] = v.y;
+                        qb[nq][l * KW + q + 1][0] = v.z;
+                        qb[nq][l * KW + q + 1][1] = v.w;
+                    }
+            }
+            if constexpr (BF16) {
+                // fp16 operands: each row over the power of two at its largest element, so that every
+                // element of at least 2^-14 of it is exact and the others are off by 2^-25 of it
                 uint32_t top = 0;
 #pragma unroll
                 for (int i = 0; i < KL * KW; ++i)
-                    top = __vmaxu2(top, __vmaxu2(qa[i][half] & 0x7fff7fffu, qa[i][half + 2] & 0x7fff7fffu));
+                    top = __vmaxu2(top, __vmaxu2(qb[nq][i][0] & 0x7fff7fffu, qb[nq][i][1] & 0x7fff7fffu));
                 top = max(top & 0xffffu, top >> 16);
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const uint32_t e = min(max(top >> 7, 1u), 253u);  // 2^(e - 127)
                 const float down = __uint_as_float((254u - e) << 23);
-                unit[half] = __uint_as_float(e << 23);
 #pragma unroll
                 for (int i = 0; i < KL * KW; ++i)
 #pragma unroll
-                    for (int q = half; q < 4; q += 2) {
-                        const uint32_t v = qa[i][q];
-                        qa[i][q] = pack_half2(__uint_as_float(v << 16) * down,
-                                              __uint_as_float(v & 0xffff0000u) * down);
+                    for (int q = 0; q < 2; ++q) {
+                        const uint32_t v = qb[nq][i][q];
+                        qb[nq][i][q] = pack_half2(__uint_as_float(v << 16) * down, __uint_as_float(v & 0xffff0000u) * down);
                     }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) unit[nq][i] = __uint_as_float(__shfl_sync(0xffffffffu, e << 23, (2 * c + i) * 4));
+            } else {
+                unit[nq][0] = unit[nq][1] = 1.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = walk.rt * kRows + 8 * nq + 2 * c + i;
+                const bool in = r < walk.r.rows;
+                const int place = walk.r.begin + by_group(a, r);
+                hi[nq][i] = !in ? INT_MAX : a.causal ? min(place + 1, walk.r.length) : walk.r.length;
+                lo[nq][i] = !in ? 0 : max(walk.r.first, a.window > 0 ? place - a.window + 1 : 0);
             }
         }
-        float o[NT][4];
+        float o[NQ][MT][4];
+        float m[NQ][2], l[NQ][2];
+        int all_lo = 0, all_hi = INT_MAX;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[t][i] = 0.0f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[nq][t][i] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                m[nq][i] = -INFINITY;
+                l[nq][i] = 0.0f;
+                all_lo = max(all_lo, lo[nq][i]);
+                all_hi = min(all_hi, hi[nq][i]);
+            }
+        }
         // the keys that every row of the tile sees
-        const int all_lo = __reduce_max_sync(0xffffffffu, max(lo[0], lo[1]));
-        const int all_hi = __reduce_min_sync(0xffffffffu, min(hi[0], hi[1]));
+        all_lo = __reduce_max_sync(0xffffffffu, all_lo);
+        all_hi = __reduce_min_sync(0xffffffffu, all_hi);
 
         for (int j = 0; j < walk.n; ++j, ++it) {
             const int st = it % kStages;
@@ -243,74 +268,24 @@ __global__ void __launch_bounds__(kStepThreads)
                 const int u = warp * C::PER_WARP + u0;
                 const int key0 = (walk.t0 + j) * KT + u * 16;
                 const float ks = scales[st * 2 * UNITS + u], vs = scales[(st * 2 + 1) * UNITS + u];
-                float s[2][4];
+                // S^T: 16 keys (rows) by 8 queries; this lane's keys krow, krow + 8, queries 2c, 2c + 1
+                float s[NQ][4];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[h][i] = 0.0f;
-                    const int r = u * 16 + h * 8 + krow;
+                    for (int i = 0; i < 4; ++i) s[nq][i] = 0.0f;
 #pragma unroll
-                    for (int x = 0; x < KL; ++x) {
-                        uint32_t w[KW];
-                        lds<KB>(kbase + swz<D>(r, x * 4 * KB + c * KB), w);
+                for (int x = 0; x < KL; ++x) {
+                    uint32_t w0[KW], w1[KW];
+                    lds<KB>(kbase + swz<D>(u * 16 + krow, x * 4 * KB + c * KB), w0);
+                    lds<KB>(kbase + swz<D>(u * 16 + 8 + krow, x * 4 * KB + c * KB), w1);
 #pragma unroll
-                        for (int q = 0; q < KW; ++q) {
-                            const uint32_t v = w[q] ^ 0x80808080u;
-                            mma_16816(s[h], qa[x * KW + q], codes_to_half2(v, 0x4140), codes_to_half2(v, 0x4342));
-                        }
-                    }
-                }
-                const bool none = vs < 0.0f;  // kKvNone
-                const float vsc = vs < 0x1p-100f ? 0x1p-100f : vs;  // NaN stays
-                const float b = none ? -INFINITY : lg2(vsc);
-                const float inv = vs == vs ? 1.0f / vsc : 1.0f;  // NaN goes through t, where the mask stops it
-                const float cs = none ? 0.0f : ks * a.scale_log2;
-                const bool edge = key0 < all_lo || key0 + 16 > all_hi;
-                float top[2];
+                    for (int q = 0; q < KW; ++q) {
+                        const uint32_t v0 = w0[q] ^ 0x80808080u, v1 = w1[q] ^ 0x80808080u;
+                        const uint32_t ka[4] = {codes_to_half2(v0, 0x4140), codes_to_half2(v1, 0x4140),
+                                                codes_to_half2(v0, 0x4342), codes_to_half2(v1, 0x4342)};
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const float cf = cs * unit[half];
-                    top[half] = -INFINITY;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            float& t = s[h][2 * half + i];
-                            t = fmaf(t, cf, b);
-                            if (edge) {
-                                const int key = key0 + h * 8 + (i ? vrow1 : vrow0);
-                                if (key < lo[half] || key >= hi[half]) t = -INFINITY;
-                            }
-                            top[half] = fmaxf(top[half], t);
-                        }
-                    top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
-                    top[half] = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 2));
-                }
-                // the running maximum moves only when it grew by more than 2^kLag, so that most
-                // tiles rescale nothing
-                if (__any_sync(0xffffffffu, top[0] > m[0] + kLag || top[1] > m[1] + kLag)) {
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const float mn = fmaxf(m[half], top[half]);
-                        const float f = mn == m[half] ? 1.0f : ex2(m[half] - mn);
-                        m[half] = mn;
-                        l[half] *= f;
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            o[t][2 * half] *= f;
-                            o[t][2 * half + 1] *= f;
-                        }
-                    }
-                }
-                uint32_t p[4];
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const float mr = m[half] == -INFINITY ? 0.0f : m[half] - kShift;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float w0 = ex2(s[h][2 * half] - mr), w1 = ex2(s[h][2 * half + 1] - mr);
-                        l[half] = fmaf(w0 + w1, inv, l[half]);
-                        p[2 * h + half] = pack_half2(w0, w1);  // 11 bits, as the codes' operands need
+                        for (int nq = 0; nq < NQ; ++nq) mma_16816(s[nq], ka, qb[nq][x * KW + q][0], qb[nq][x * KW + q][1]);
                     }
                 }
                 uint32_t v00[VB / 4], v01[VB / 4], v10[VB / 4], v11[VB / 4];
@@ -318,15 +293,78 @@ __global__ void __launch_bounds__(kStepThreads)
                 lds<VB>(vbase + swz<D>(u * 16 + vrow1, vbyte), v01);
                 lds<VB>(vbase + swz<D>(u * 16 + 8 + vrow0, vbyte), v10);
                 lds<VB>(vbase + swz<D>(u * 16 + 8 + vrow1, vbyte), v11);
+                const bool none = vs < 0.0f;  // kKvNone
+                const float vsc = vs < 0x1p-100f ? 0x1p-100f : vs;  // NaN stays
+                const float b = none ? -INFINITY : lg2(vsc);
+                const float inv = vs == vs ? rcp(vsc) : 1.0f;  // NaN goes through t, where the mask stops it
+                const float cs = none ? 0.0f : ks * a.scale_log2;
+                const bool edge = key0 < all_lo || key0 + 16 > all_hi;
+                uint32_t p[NQ][2];  // w^T as the second product's keys-by-queries operand
+                float top[NQ][2];
+                bool grew = false;
+#pragma unroll
+                for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float cf = cs * unit[nq][i];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float& t = s[nq][2 * h + i];
+                            t = fmaf(t, cf, b);
+                            if (edge) {
+                                const int key = key0 + 8 * h + krow;
+                                if (key < lo[nq][i] || key >= hi[nq][i]) t = -INFINITY;
+                            }
+                        }
+                        top[nq][i] = fmaxf(s[nq][i], s[nq][2 + i]);
+                        grew |= top[nq][i] > m[nq][i] + kLag;
+                    }
+                // the running maximum moves only when it grew by more than 2^kLag, so that most
+                // tiles rescale nothing (and need not agree on their largest)
+                if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+                    for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float t = top[nq][i];
+                            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+                            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+                            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+                            const float mn = fmaxf(m[nq][i], t);
+                            const float f = mn == m[nq][i] ? 1.0f : ex2(m[nq][i] - mn);
+                            m[nq][i] = mn;
+                            l[nq][i] *= f;
+#pragma unroll
+                            for (int y = 0; y < MT; ++y) {
+                                o[nq][y][i] *= f;
+                                o[nq][y][2 + i] *= f;
+                            }
+                        }
+                }
+#pragma unroll
+                for (int nq = 0; nq < NQ; ++nq) {
+                    float w[4];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float mr = m[nq][i] == -INFINITY ? 0.0f : m[nq][i] - kShift;
+                        w[i] = ex2(s[nq][i] - mr);
+                        w[2 + i] = ex2(s[nq][2 + i] - mr);
+                        l[nq][i] = fmaf(w[i] + w[2 + i], inv, l[nq][i]);
+                    }
+                    p[nq][0] = transpose8x8(pack_half2(w[0], w[1]));  // 11 bits, as the codes' operands need
+                    p[nq][1] = transpose8x8(pack_half2(w[2], w[3]));
+                }
 #pragma unroll
                 for (int q = 0; q < VB / 4; ++q) {
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) {  // dimensions 4q + 2y and 4q + 2y + 1
+                    for (int y = 0; y < 2; ++y) {  // dimensions 4q + 2y and 4q + 2y + 1 of the lane's
                         const uint32_t sel = y ? 0x7362 : 0x5140;  // {even key, odd key} of each
                         const uint32_t x0 = __byte_perm(v00[q], v01[q], sel) ^ 0x80808080u;
                         const uint32_t x1 = __byte_perm(v10[q], v11[q], sel) ^ 0x80808080u;
-                        mma_16816(o[4 * q + 2 * y], p, codes_to_half2(x0, 0x4140), codes_to_half2(x1, 0x4140));
-                        mma_16816(o[4 * q + 2 * y + 1], p, codes_to_half2(x0, 0x4342), codes_to_half2(x1, 0x4342));
+                        const uint32_t va[4] = {codes_to_half2(x0, 0x4140), codes_to_half2(x0, 0x4342),
+                                                codes_to_half2(x1, 0x4140), codes_to_half2(x1, 0x4342)};
+#pragma unroll
+                        for (int nq = 0; nq < NQ; ++nq) mma_16816(o[nq][2 * q + y], va, p[nq][0], p[nq][1]);
                     }
                 }
             }
@@ -335,32 +373,29 @@ __global__ void __launch_bounds__(kStepThreads)
         }
 
         // ---- the four warps' results become one ----
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
-            l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-        }
         const int rows = min(kRows, walk.r.rows - walk.rt * kRows);
         float* mine = merge + warp * kRows * (D + 4);  // row: D values, m, l
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int r = n8 + 8 * half;
-            if (r < rows) {
-                float* dst = mine + r * (D + 4);
+        for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-                for (int t = 0; t < NT; t += 4) {
-                    *reinterpret_cast<float4*>(dst + odim0 + t) =
-                        make_float4(o[t][2 * half], o[t + 1][2 * half], o[t + 2][2 * half], o[t + 3][2 * half]);
-                    *reinterpret_cast<float4*>(dst + odim1 + t) =
-                        make_float4(o[t][2 * half + 1], o[t + 1][2 * half + 1], o[t + 2][2 * half + 1],
-                                    o[t + 3][2 * half + 1]);
-                }
-                if (c == 0) {
-                    dst[D] = m[half] - kShift;
-                    dst[D + 1] = l[half];
+            for (int i = 0; i < 2; ++i) {
+                float sum = l[nq][i];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                const int r = 8 * nq + 2 * c + i;
+                if (r < rows) {
+                    float* dst = mine + r * (D + 4);
+#pragma unroll
+                    for (int t = 0; t < MT; t += 2)
+                        *reinterpret_cast<float4*>(dst + vbyte + 2 * t) =
+                            make_float4(o[nq][t][i], o[nq][t][2 + i], o[nq][t + 1][i], o[nq][t + 1][2 + i]);
+                    if (n8 == 0) {
+                        dst[D] = m[nq][i] - kShift;
+                        dst[D + 1] = sum;
+                    }
                 }
             }
-        }
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kConsumers) : "memory");
         const bool whole = walk.begins && walk.ends;
         const int slot = walk.begins ? 1 : 0;
@@ -402,13 +437,10 @@ __global__ void __launch_bounds__(kStepThreads)
     }
 }
 
-constexpr int kStepPerSm = 2;   // CTAs of an SM
-constexpr int kStepLeast = 4;   // key tiles a CTA takes at least: a partial result costs about as much
-
-template <int D, bool BF16>
+template <int D, int NQ, bool BF16>
 cudaError_t launch_step(KvAttnArgs a, void* ws, int dev, cudaStream_t s) {
-    using C = StepCfg<D>;
-    auto kern = kv_step_kernel<D, BF16>;
+    using C = StepCfg<D, NQ>;
+    auto kern = kv_step_kernel<D, NQ, BF16>;
     static std::atomic<uint64_t> configured{0};
     const uint64_t bit = 1ull << (dev & 63);
     if (!(configured.load(std::memory_order_relaxed) & bit)) {
@@ -420,25 +452,25 @@ cudaError_t launch_step(KvAttnArgs a, void* ws, int dev, cudaStream_t s) {
     const int box = std::min(a.pool.block_size, C::KT);
     if (!code_map(&mk, a.pool.k_codes, a.pool, box) || !code_map(&mv, a.pool.v_codes, a.pool, box))
         return cudaErrorInvalidValue;
-    const int grid = gemm_sm_count(dev) * kStepPerSm;
+    const int grid = gemm_sm_count(dev) * C::PER_SM;
     a.desc = static_cast<int4*>(ws);
     a.part = reinterpret_cast<float*>(a.desc + 2 * grid);
     kern<<<grid, kStepThreads, C::kSmem, s>>>(mk, mv, a, kStepLeast);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    return launch_join<D, kRows, BF16>(a, grid, std::min(kRows, a.group), s);
+    return launch_join<D, C::ROWS, BF16>(a, grid, C::ROWS, s);
 }
 
 }  // namespace
 
 namespace {
 
-// Row tiles of 256 rows on tcgen05 from kPromptMin rows of a request on; below, tiles of 16.
+// Row tiles of 256 rows on tcgen05 from kPromptMin rows of a request on; below, tiles of 8 or 16.
 constexpr int kPromptMin = 33;
 
-bool takes_prompt(int group, int64_t tokens, int max_new) {
-    const int64_t most = max_new > 0 ? std::min<int64_t>(max_new, tokens) : tokens;
-    return most * group >= kPromptMin;
+// Rows of one request and key/value head, at most.
+int64_t most_rows(int group, int64_t tokens, int max_new) {
+    return (max_new > 0 ? std::min<int64_t>(max_new, tokens) : tokens) * group;
 }
 
 }  // namespace
@@ -447,8 +479,10 @@ uint64_t kv_attention_workspace_bytes(int head_dim, int group, int64_t tokens, i
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 0;
     const int sms = gemm_sm_count(dev);
-    if (takes_prompt(group, tokens, max_new)) return kv_prompt_workspace_bytes(head_dim, sms);
-    return uint64_t(round_up(int64_t(sms) * kStepPerSm * 2 * int64_t(sizeof(int4) + kRows * (head_dim + 2) * sizeof(float)), 256));
+    const int64_t most = most_rows(group, tokens, max_new);
+    if (most >= kPromptMin) return kv_prompt_workspace_bytes(head_dim, sms);
+    const int nq = most <= 8 ? 1 : 2, ctas = sms * (nq == 1 ? StepCfg<32, 1>::PER_SM : StepCfg<32, 2>::PER_SM);
+    return uint64_t(round_up(int64_t(ctas) * 2 * int64_t(sizeof(int4) + 8 * nq * (head_dim + 2) * sizeof(float)), 256));
 }
 
 cudaError_t launch_kv_attention(const KvAttnArgs& a, bool bf16, int max_new, void* ws, cudaStream_t s) {
@@ -456,12 +490,17 @@ cudaError_t launch_kv_attention(const KvAttnArgs& a, bool bf16, int max_new, voi
     int dev = 0;
     const cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    if (takes_prompt(a.group, a.tokens, max_new)) return launch_kv_prompt(a, bf16, ws, dev, s);
+    if (most_rows(a.group, a.tokens, max_new) >= kPromptMin) return launch_kv_prompt(a, bf16, ws, dev, s);
+#define EBX_KV_STEP(DD)                                                                              \
+    (few ? (bf16 ? launch_step<DD, 1, true>(a, ws, dev, s) : launch_step<DD, 1, false>(a, ws, dev, s)) \
+         : (bf16 ? launch_step<DD, 2, true>(a, ws, dev, s) : launch_step<DD, 2, false>(a, ws, dev, s)))
+    const bool few = most_rows(a.group, a.tokens, max_new) <= 8;
     switch (a.pool.head_dim) {
-        case 32: return bf16 ? launch_step<32, true>(a, ws, dev, s) : launch_step<32, false>(a, ws, dev, s);
-        case 64: return bf16 ? launch_step<64, true>(a, ws, dev, s) : launch_step<64, false>(a, ws, dev, s);
-        default: return bf16 ? launch_step<128, true>(a, ws, dev, s) : launch_step<128, false>(a, ws, dev, s);
+        case 32: return EBX_KV_STEP(32);
+        case 64: return EBX_KV_STEP(64);
+        default: return EBX_KV_STEP(128);
     }
+#undef EBX_KV_STEP
 }
 
 cudaError_t read_kv_status(int* status, bool clear, cudaStream_t s) {
