@@ -56,11 +56,12 @@ struct KvAttnArgs {
     int64_t tokens;
     int requests, width, heads, group;
     int causal, window;
+    int whole;             // row tiles are not shared among CTAs
     float scale_log2;      // softmax scale * log2(e)
     uint32_t group_mul, group_shift;  // n / group = n * group_mul >> group_shift
     // partial results of row tiles that several CTAs share
     float* part;           // [grid][2][rows][head_dim + 2]
-    int4* desc;            // [grid][2]
+    int4* desc;            // [grid]
 
     // With 2^(k-1) < g <= 2^k and mul = ceil(2^(31+k) / g), mul * g exceeds 2^(31+k) by less than
     // g <= 2^k, so n * mul >> (31 + k) is n / g for every n < 2^31.
@@ -80,7 +81,7 @@ cudaError_t launch_kv_materialize(const KvPool& pool, const int32_t* tables, int
                                   const int32_t* starts, const int32_t* first, int requests,
                                   int64_t tokens, int dtype, void* k, void* v, cudaStream_t s);
 uint64_t kv_attention_workspace_bytes(int head_dim, int group, int64_t tokens, int max_new);
-cudaError_t launch_kv_attention(const KvAttnArgs& a, bool bf16, int max_new, void* ws, cudaStream_t s);
+cudaError_t launch_kv_attention(KvAttnArgs a, bool bf16, int max_new, int max_length, void* ws, cudaStream_t s);
 cudaError_t read_kv_status(int* status, bool clear, cudaStream_t s);
 
 // ebx_kv_prompt.cu: the same for many rows.

@@ -33,7 +33,8 @@ __device__ __forceinline__ bool kv_wait(uint32_t bar, uint32_t parity) {
 constexpr int kConsumers = 4;    // warps that compute; one more loads
 constexpr int kStepThreads = 32 * (kConsumers + 1);
 constexpr int kStages = 3;
-constexpr int kStepLeast = 4;   // key tiles a CTA takes at least: a partial result costs about as much
+constexpr int kStepLeast = 4;   // units a CTA takes at least: a partial result costs about as much
+constexpr int kStepExtra = 1;   // a row tile's begin and end, in key tiles
 
 // D: head_dim; NQ: blocks of 8 rows (queries) in a row tile, the N of mma.m16n8k16, whose M is 16
 // keys of the first product and 16 dimensions of the second.
@@ -105,11 +106,12 @@ __global__ void __launch_bounds__(kStepThreads, (StepCfg<D, NQ>::PER_SM))
         }
         fence_proxy_async_smem();
     }
-    const KvShare share = kv_share<kRows, KT, kStepThreads>(a, least, reinterpret_cast<int*>(smem));
+    const KvShare share = kv_share<kRows, KT, kStepExtra, kStepThreads>(a, least, reinterpret_cast<int*>(smem));
     fence_proxy_async_smem();  // the ring's copies may overwrite what kv_share kept there
-    if (threadIdx.x < 2) a.desc[2 * blockIdx.x + threadIdx.x] = make_int4(0, 0, 0, 0);
+    if (threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join waits for this grid's end
     __syncthreads();
-    KvWalk<kRows, KT> walk;
+    KvWalk<kRows, KT, kStepExtra> walk;
     walk.start(a, share);
     const int bsize = a.pool.block_size;
 
@@ -397,7 +399,7 @@ __global__ void __launch_bounds__(kStepThreads, (StepCfg<D, NQ>::PER_SM))
                 }
             }
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kConsumers) : "memory");
-        const bool whole = walk.begins && walk.ends;
+        const bool whole = walk.whole();
         const int slot = walk.begins ? 1 : 0;
         for (int w = threadIdx.x; w < rows * (D / 4); w += 32 * kConsumers) {
             const int r = w / (D / 4), d = (w % (D / 4)) * 4;
@@ -431,8 +433,8 @@ __global__ void __launch_bounds__(kStepThreads, (StepCfg<D, NQ>::PER_SM))
                 if (d == 0) kv_part_ml<D, kRows>(a, blockIdx.x, slot)[r] = make_float2(mm, ll);
             }
         }
-        if (!whole && threadIdx.x == 0)
-            a.desc[2 * blockIdx.x + slot] = kv_desc(walk.r, walk.rt, kRows, walk.head, walk.ends);
+        if (walk.begins && !whole && threadIdx.x == 0)
+            a.desc[blockIdx.x] = kv_desc(walk.r, walk.rt, kRows, walk.head, walk.last() - int(blockIdx.x));
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kConsumers) : "memory");  // merge is free again
     }
 }
@@ -454,11 +456,11 @@ cudaError_t launch_step(KvAttnArgs a, void* ws, int dev, cudaStream_t s) {
         return cudaErrorInvalidValue;
     const int grid = gemm_sm_count(dev) * C::PER_SM;
     a.desc = static_cast<int4*>(ws);
-    a.part = reinterpret_cast<float*>(a.desc + 2 * grid);
+    a.part = reinterpret_cast<float*>(a.desc + grid);
     kern<<<grid, kStepThreads, C::kSmem, s>>>(mk, mv, a, kStepLeast);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    return launch_join<D, C::ROWS, BF16>(a, grid, C::ROWS, s);
+    return launch_join<D, C::ROWS, 16, BF16>(a, grid, s);
 }
 
 }  // namespace
@@ -467,6 +469,7 @@ namespace {
 
 // Row tiles of 256 rows on tcgen05 from kPromptMin rows of a request on; below, tiles of 8 or 16.
 constexpr int kPromptMin = 33;
+constexpr int kWholeTiles = 4;
 
 // Rows of one request and key/value head, at most.
 int64_t most_rows(int group, int64_t tokens, int max_new) {
@@ -482,10 +485,10 @@ uint64_t kv_attention_workspace_bytes(int head_dim, int group, int64_t tokens, i
     const int64_t most = most_rows(group, tokens, max_new);
     if (most >= kPromptMin) return kv_prompt_workspace_bytes(head_dim, sms);
     const int nq = most <= 8 ? 1 : 2, ctas = sms * (nq == 1 ? StepCfg<32, 1>::PER_SM : StepCfg<32, 2>::PER_SM);
-    return uint64_t(round_up(int64_t(ctas) * 2 * int64_t(sizeof(int4) + 8 * nq * (head_dim + 2) * sizeof(float)), 256));
+    return uint64_t(round_up(int64_t(ctas) * int64_t(sizeof(int4) + 2 * 8 * nq * (head_dim + 2) * sizeof(float)), 256));
 }
 
-cudaError_t launch_kv_attention(const KvAttnArgs& a, bool bf16, int max_new, void* ws, cudaStream_t s) {
+cudaError_t launch_kv_attention(KvAttnArgs a, bool bf16, int max_new, int max_length, void* ws, cudaStream_t s) {
     if (a.tokens <= 0 || a.requests <= 0) return cudaSuccess;
     int dev = 0;
     const cudaError_t e = cudaGetDevice(&dev);
@@ -495,6 +498,8 @@ cudaError_t launch_kv_attention(const KvAttnArgs& a, bool bf16, int max_new, voi
     (few ? (bf16 ? launch_step<DD, 1, true>(a, ws, dev, s) : launch_step<DD, 1, false>(a, ws, dev, s)) \
          : (bf16 ? launch_step<DD, 2, true>(a, ws, dev, s) : launch_step<DD, 2, false>(a, ws, dev, s)))
     const bool few = most_rows(a.group, a.tokens, max_new) <= 8;
+    // short requests: a second launch would cost more than it spreads
+    a.whole = max_length > 0 && max_length <= kWholeTiles * (8192 / a.pool.head_dim);
     switch (a.pool.head_dim) {
         case 32: return EBX_KV_STEP(32);
         case 64: return EBX_KV_STEP(64);

@@ -184,7 +184,7 @@ ebx_status ebx_kv_attention(const ebx_kv_pool* pool, const void* q, int64_t q_to
     a.causal = causal != 0;
     a.window = window;
     a.scale_log2 = scale * 1.4426950408889634f;
-    return launched(ebx::launch_kv_attention(a, dtype == ebx::kKvBF16, max_new, workspace,
+    return launched(ebx::launch_kv_attention(a, dtype == ebx::kKvBF16, max_new, max_length, workspace,
                                              static_cast<cudaStream_t>(stream)), "ebx_kv_attention");
 }
 

@@ -29,6 +29,7 @@ constexpr int kPromptRows = 256;
 constexpr int kPromptKeys = 128;
 constexpr int kPromptThreads = 14 * 32;
 constexpr int kHalf = 128 * 128;   // bytes of 128 rows x 64 fp16
+constexpr int kPromptExtra = 3;    // a row tile's begin and end, in key tiles
 constexpr int kRaw = 4;            // int8 tiles in flight
 constexpr int kBufs = 3;           // fp16 tiles: a value tile, the next key tile, and one being filled
 constexpr int kTabs = 4;           // scale tables of key tiles
@@ -299,14 +300,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
-    const KvShare share = kv_share<kPromptRows, kPromptKeys, kPromptThreads>(a, least, reinterpret_cast<int*>(smem));
+    const KvShare share = kv_share<kPromptRows, kPromptKeys, kPromptExtra, kPromptThreads>(a, least, reinterpret_cast<int*>(smem));
     fence_proxy_async_smem();  // copies will overwrite what kv_share kept there
-    if (threadIdx.x < 2) a.desc[2 * blockIdx.x + threadIdx.x] = make_int4(0, 0, 0, 0);
+    if (threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join waits for this grid's end
     before_sync();
     __syncthreads();
     after_sync();
     const uint32_t tmem = *tmem_slot;
-    KvWalk<kPromptRows, kPromptKeys> walk;
+    KvWalk<kPromptRows, kPromptKeys, kPromptExtra> walk;
     walk.start(a, share);
 
     if (warp < 8) {
@@ -428,7 +430,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 break;
             }
             after_sync();
-            const bool whole = walk.begins && walk.ends;
+            const bool whole = walk.whole();
             const int slot = walk.begins ? 1 : 0;
             const float inv = row.l == 0.0f ? 0.0f : 1.0f / row.l;
             float4* part = whole ? nullptr
@@ -470,8 +472,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             if (live && whole && a.lse)
                 a.lse[at_row] = row.l == 0.0f ? -INFINITY : (row.mr + lg2(row.l)) * 0.6931471805599453f;
             if (!whole) kv_part_ml<D, kPromptRows>(a, blockIdx.x, slot)[x * 128 + rl] = make_float2(row.mr, row.l);
-            if (!whole && threadIdx.x == 0)
-                a.desc[2 * blockIdx.x + slot] = kv_desc(walk.r, walk.rt, kPromptRows, walk.head, walk.ends);
+            if (walk.begins && !whole && threadIdx.x == 0)
+                a.desc[blockIdx.x] = kv_desc(walk.r, walk.rt, kPromptRows, walk.head, walk.last() - int(blockIdx.x));
         }
     } else if (warp >= 12) {
         if (warp == 12) {
@@ -673,7 +675,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
 }
 
-constexpr int kPromptLeast = 4;  // key tiles a CTA takes at least
+constexpr int kPromptLeast = 8;  // units a CTA takes at least
 
 template <int D, bool BF16>
 cudaError_t launch_prompt(KvAttnArgs a, void* ws, int dev, cudaStream_t s) {
@@ -692,17 +694,17 @@ cudaError_t launch_prompt(KvAttnArgs a, void* ws, int dev, cudaStream_t s) {
         return cudaErrorInvalidValue;
     const int grid = gemm_sm_count(dev);
     a.desc = static_cast<int4*>(ws);
-    a.part = reinterpret_cast<float*>(a.desc + 2 * grid);
+    a.part = reinterpret_cast<float*>(a.desc + grid);
     kern<<<grid, kPromptThreads, C::kSmem, s>>>(mk, mv, a, kPromptLeast);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    return launch_join<D, kPromptRows, BF16>(a, grid, kPromptRows, s);
+    return launch_join<D, kPromptRows, 4, BF16>(a, grid, s);
 }
 
 }  // namespace
 
 uint64_t kv_prompt_workspace_bytes(int head_dim, int sms) {
-    return uint64_t(round_up(int64_t(sms) * 2 * int64_t(sizeof(int4) + kPromptRows * (head_dim + 2) * sizeof(float)), 256));
+    return uint64_t(round_up(int64_t(sms) * int64_t(sizeof(int4) + 2 * kPromptRows * (head_dim + 2) * sizeof(float)), 256));
 }
 
 cudaError_t launch_kv_prompt(const KvAttnArgs& a, bool bf16, void* ws, int dev, cudaStream_t s) {

@@ -4,10 +4,12 @@
 // The rows of request i and key/value head h are its new tokens times the `group` query heads
 // that share h (row r: token r / group, head h * group + r % group), in tiles of RT rows.  A row
 // tile reads the key tiles of KT tokens between the first and the last key that one of its rows
-// sees.  All (request, head, row tile, key tile) units lie on one line in that order, and every
-// CTA takes the same length of it, so that ragged requests, causal masks and single long
-// requests all fill the GPU alike.  A row tile that crosses the end of a CTA's length is left as
-// partial results {O, m, l}, which kv_join_kernel adds up in order: no atomics, no waiting.
+// sees.  All (request, head, row tile, key tile) units lie on one line in that order, EXTRA more
+// for the begin and the end of each row tile, and every CTA takes the same length of it, so that
+// ragged requests, causal masks and single long requests all fill the GPU alike.  A row tile that
+// crosses the end of a CTA's length is left as partial results {O, m, l}, which kv_join_kernel adds
+// up in order: no atomics, no waiting.  With `whole`, the line's units are row tiles: nothing is
+// left for a join.
 #pragma once
 
 #include <cuda.h>
@@ -64,24 +66,27 @@ __device__ __forceinline__ void kv_key_tiles(const KvAttnArgs& a, const KvReques
 // Where a CTA's share of the line begins, and how long it is.
 struct KvShare {
     int64_t units;
+    int per;     // every CTA's length
     int request, head, rt;
-    int skip;  // key tiles of that row tile that belong to the CTA before
+    int skip;    // units of that row tile that belong to the CTA before
 };
 
 // A CTA's walk along the line: which (request, head, row tile) it is at, and which of its key
 // tiles are the CTA's.  Every warp keeps its own copy.
-template <int RT, int KT>
+template <int RT, int KT, int EXTRA>
 struct KvWalk {
     int64_t left;        // units from here to the CTA's end
-    int request, head, rt;
+    int per, request, head, rt;
     KvRequest r;
     int skip;
     // the current segment
     int t0, n;           // its key tiles
-    bool begins, ends;   // it holds the row tile's first / last key tile
+    int rest;            // key tiles of the row tile behind it, for the next CTAs
+    bool begins;         // it holds the row tile's first key tile
 
     __device__ __forceinline__ void start(const KvAttnArgs& a, const KvShare& s) {
         left = s.units;
+        per = s.per;
         request = s.request;
         head = s.head;
         rt = s.rt;
@@ -92,15 +97,27 @@ struct KvWalk {
     }
     __device__ __forceinline__ void segment(const KvAttnArgs& a) {
         kv_key_tiles<RT, KT>(a, r, rt, t0, n);
-        begins = skip == 0;
-        t0 += skip;
-        n -= skip;
-        ends = n <= left;
-        if (!ends) n = int(left);
+        rest = 0;
+        begins = true;
+        if (a.whole) return;
+        const int before = max(skip - EXTRA, 0);
+        begins = before == 0;
+        t0 += before;
+        n -= before;
+        const int64_t room = left - max(EXTRA - skip, 0);
+        if (room < n) {
+            rest = n - max(int(room), 0);
+            n -= rest;
+            if (n == 0) left = 0;  // the share ends ahead of the first key tile
+        }
     }
     __device__ __forceinline__ bool done() const { return left <= 0; }
+    __device__ __forceinline__ bool whole() const { return begins && rest == 0; }
+    // the last CTA that works on the row tile
+    __device__ __forceinline__ int last() const { return int(blockIdx.x) + (rest + per - 1) / per; }
     __device__ __forceinline__ void next(const KvAttnArgs& a) {
-        left -= n;
+        left -= a.whole ? 1 : n + max(EXTRA - skip, 0);
+        if (rest > 0) left = 0;
         if (left <= 0) return;
         skip = 0;
         ++rt;
@@ -124,7 +141,7 @@ struct KvWalk {
 constexpr int kShareWindow = 1024;
 constexpr int kShareInts = 2 * kShareWindow + 128;
 
-template <int RT, int KT, int NT>
+template <int RT, int KT, int EXTRA, int NT>
 __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, int* scratch) {
     constexpr int W = NT / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -178,7 +195,7 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, 
             }
             int t0, k;
             kv_key_tiles<RT, KT>(a, kv_request(a, i0 + lo), int(x) - tiles[lo], t0, k);
-            atomicAdd(units + lo, k);
+            atomicAdd(units + lo, a.whole ? 1 : k + EXTRA);
         }
         __syncthreads();
     };
@@ -192,10 +209,11 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, 
         total += all * a.pool.kv_heads;
     }
     int64_t per = (total + gridDim.x - 1) / gridDim.x;
-    per = per < least ? least : per;
+    per = per < least && !a.whole ? least : per;
     const int64_t w0 = per * blockIdx.x;
     KvShare out;
     out.units = total - w0 < per ? total - w0 : per;
+    out.per = int(per < INT32_MAX ? per : INT32_MAX);
     out.request = out.head = out.rt = out.skip = 0;
     if (out.units <= 0) {
         out.units = 0;
@@ -232,7 +250,10 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, 
     const KvRequest r = kv_request(a, out.request);
     for (int rt0 = 0;; rt0 += 32) {
         int t0, k = 0;
-        if ((rt0 + lane) * RT < r.rows) kv_key_tiles<RT, KT>(a, r, rt0 + lane, t0, k);
+        if ((rt0 + lane) * RT < r.rows) {
+            kv_key_tiles<RT, KT>(a, r, rt0 + lane, t0, k);
+            k = a.whole ? 1 : k + EXTRA;
+        }
         int x = k;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -253,14 +274,11 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, 
 }
 
 // ---- partial results ----------------------------------------------------------------------
-// CTA c leaves at most two: part 0, which continues a row tile of the CTA before, and part 1,
-// which begins one that the next CTA continues.  desc = {1 + row tile's first row and ends flag
-// (0: none), first token row, head, rows}.
-constexpr int kKvEnds = 1 << 30;
-
-__device__ __forceinline__ int4 kv_desc(const KvRequest& r, int rt, int rt_rows, int head, bool ends) {
-    return make_int4((rt * rt_rows + 1) | (ends ? kKvEnds : 0), r.token0, head,
-                     min(rt_rows, r.rows - rt * rt_rows));
+// CTA c leaves at most two: part 0, which continues a row tile of a CTA before, and part 1, which
+// begins one that later CTAs continue.  desc[c] tells of part 1: {1 + the row tile's first row (0:
+// none), first token row, head, rows | CTAs behind c << 16}.
+__device__ __forceinline__ int4 kv_desc(const KvRequest& r, int rt, int rt_rows, int head, int behind) {
+    return make_int4(rt * rt_rows + 1, r.token0, head, min(rt_rows, r.rows - rt * rt_rows) | behind << 16);
 }
 
 // Weights are 2^(t - m + kShift), m at most kLag below the maximum so far: the largest is below
@@ -320,31 +338,22 @@ __device__ __forceinline__ uint32_t codes_to_half2(uint32_t w, uint32_t sel) {
     return hsub2_u(__byte_perm(w, 0x64646464u, sel), 0x64806480u);  // - 1152
 }
 
-// Row tiles that several CTAs worked on: CTA (c, y) joins rows 4 y .. 4 y + 3 (and so on, gridDim.y
-// fours at a time) of the one that begins in CTA c, reading c's part 1 and then part 0 of the CTAs
-// after it until one ends it.  Threads: 4 rows x 8 ways (parts taken in turn) x 8 column groups.
-template <int D, int RT, bool BF16>
-__global__ void __launch_bounds__(256) kv_join_kernel(const __grid_constant__ KvAttnArgs a, int ctas) {
+// Row tiles that several CTAs worked on: CTA (c, y) joins rows 4 y .. 4 y + 3 of the one that begins
+// in CTA c, c's part 1 and then part 0 of the CTAs behind it.  Threads: 4 rows x 8 column groups x
+// WAYS parts at a time.
+template <int D, int RT, int WAYS, bool BF16>
+__global__ void __launch_bounds__(32 * WAYS) kv_join_kernel(const __grid_constant__ KvAttnArgs a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     constexpr int COLS = D / 32;  // float4 columns of a thread: groups of 8 apart
-    __shared__ float2 s_ml[8][8][4];
-    __shared__ float4 s_o[COLS][8][8][4];
-    __shared__ int s_last;
+    __shared__ float2 s_ml[WAYS][8][4];
+    __shared__ float4 s_o[COLS][WAYS][8][4];
     const int c = blockIdx.x;
-    const int4 d1 = a.desc[2 * c + 1];
-    if (d1.x == 0 || int(blockIdx.y) * 4 >= d1.w) return;
-    if (threadIdx.x == 0) s_last = ctas - 1;
-    __syncthreads();
-    for (int base = c + 1;; base += 256) {  // the CTA that ends the row tile
-        const int k = base + int(threadIdx.x);
-        const bool end = k >= ctas - 1 || (a.desc[2 * k].x & kKvEnds) != 0;
-        if (end) atomicMin(&s_last, k);
-        if (__syncthreads_or(end)) break;
-    }
-    const int last = s_last;
+    const int4 d = a.desc[c];
+    const int rows = d.w & 0xffff, last = c + (d.w >> 16);
+    if (d.x == 0 || int(blockIdx.y) * 4 >= rows) return;
     const int ri = threadIdx.x & 3, col = (threadIdx.x >> 2) & 7, way = threadIdx.x >> 5;
-    for (int r0 = blockIdx.y * 4; r0 < d1.w; r0 += gridDim.y * 4) {
-        const int r = r0 + ri;
+    {
+        const int r = blockIdx.y * 4 + ri;
         float m = -INFINITY, l = 0.0f;
         float4 o[COLS];
 #pragma unroll
@@ -362,8 +371,8 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const __grid_constant__ Kv
             l = l * f0 + l1 * f1;
             m = mn;
         };
-        if (r < d1.w) {
-            for (int k = c + way; k <= last; k += 8) {
+        if (r < rows) {
+            for (int k = c + way; k <= last; k += WAYS) {
                 const int slot = k == c ? 1 : 0;
                 const float4* src = reinterpret_cast<const float4*>(kv_part<D, RT>(a, k, slot));
                 float4 v[COLS];
@@ -377,16 +386,16 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const __grid_constant__ Kv
 #pragma unroll
         for (int x = 0; x < COLS; ++x) s_o[x][way][col][ri] = o[x];
         __syncthreads();
-        if (way == 0 && r < d1.w) {
-            for (int w = 1; w < min(8, last - c + 1); ++w) {
+        if (way == 0 && r < rows) {
+            for (int w = 1; w < min(WAYS, last - c + 1); ++w) {
                 float4 v[COLS];
 #pragma unroll
                 for (int x = 0; x < COLS; ++x) v[x] = s_o[x][w][col][ri];
                 join(s_ml[w][col][ri].x, s_ml[w][col][ri].y, v);
             }
-            const int row = (d1.x & (kKvEnds - 1)) - 1 + r;
+            const int row = d.x - 1 + r;
             const int token = by_group(a, row);
-            const int64_t at = int64_t(d1.y + token) * a.heads + d1.z * a.group + row - token * a.group;
+            const int64_t at = int64_t(d.y + token) * a.heads + d.z * a.group + row - token * a.group;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
             for (int x = 0; x < COLS; ++x) {
@@ -397,7 +406,6 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const __grid_constant__ Kv
             }
             if (a.lse && col == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + lg2(l)) * 0.6931471805599453f;
         }
-        __syncthreads();
     }
 }
 
@@ -417,19 +425,20 @@ inline bool code_map(CUtensorMap* map, const int8_t* codes, const KvPool& p, int
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The join of a launch of `ctas` CTAs whose row tiles have up to `rows` rows.
-template <int D, int RT, bool BF16>
-cudaError_t launch_join(const KvAttnArgs& a, int ctas, int rows, cudaStream_t s) {
+// The join of a launch of `ctas` CTAs.
+template <int D, int RT, int WAYS, bool BF16>
+cudaError_t launch_join(const KvAttnArgs& a, int ctas, cudaStream_t s) {
+    if (a.whole) return cudaSuccess;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(ctas), unsigned((rows + 3) / 4));
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3(unsigned(ctas), unsigned((RT + 3) / 4));
+    cfg.blockDim = dim3(32 * WAYS);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kv_join_kernel<D, RT, BF16>, a, ctas);
+    return cudaLaunchKernelEx(&cfg, kv_join_kernel<D, RT, WAYS, BF16>, a);
 }
 
 // Reads (and clears) a translation unit's status word; synchronizes `s`.

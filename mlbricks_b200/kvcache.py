@@ -61,17 +61,21 @@ class KVPool:
     def __init__(self, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
                  v_scales: torch.Tensor) -> None:
         shape, device = k_codes.shape, k_codes.get_device()
-        _check(k_codes.is_cuda and k_codes.dim() == 4, "codes must be CUDA tensors "
-               "[blocks, kv_heads, block_size, head_dim]")
-        for t, s, dtype, name in ((k_codes, shape, torch.int8, "k_codes"), (v_codes, shape, torch.int8, "v_codes"),
-                                  (k_scales, shape[:2], torch.float32, "k_scales"),
-                                  (v_scales, shape[:2], torch.float32, "v_scales")):
-            if t.dtype is not dtype or t.shape != s or t.get_device() != device or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous {dtype} tensor {tuple(s)} on cuda:{device}")
+        if device < 0 or len(shape) != 4:
+            raise ValueError("codes must be CUDA tensors [blocks, kv_heads, block_size, head_dim]")
+        for t, dtype, name in ((k_codes, torch.int8, "k_codes"), (v_codes, torch.int8, "v_codes"),
+                               (k_scales, torch.float32, "k_scales"), (v_scales, torch.float32, "v_scales")):
+            if (t.dtype is not dtype or t.get_device() != device or not t.is_contiguous()
+                    or t.shape != (shape if dtype is torch.int8 else shape[:2])):
+                raise ValueError(f"{name} must be a contiguous {dtype} tensor "
+                                 f"{tuple(shape if dtype is torch.int8 else shape[:2])} on cuda:{device}")
         blocks, kv_heads, block_size, head_dim = shape
-        _check(block_size in BLOCK_SIZES, f"block_size must be one of {BLOCK_SIZES}, got {block_size}")
-        _check(head_dim in HEAD_DIMS, f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
-        _check(0 < blocks * kv_heads * block_size < 2**31, "need 0 < blocks * kv_heads * block_size < 2^31")
+        if block_size not in BLOCK_SIZES:
+            raise ValueError(f"block_size must be one of {BLOCK_SIZES}, got {block_size}")
+        if head_dim not in HEAD_DIMS:
+            raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
+        if not 0 < blocks * kv_heads * block_size < 2**31:
+            raise ValueError("need 0 < blocks * kv_heads * block_size < 2^31")
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
         self.device = device
         self._c = _ebx.KVPool(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
