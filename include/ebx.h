@@ -371,10 +371,11 @@ EBX_API ebx_status ebx_kv_materialize(const ebx_kv_pool* pool, const int32_t* ta
                                       const int32_t* starts, const int32_t* first, int32_t requests,
                                       int64_t tokens, int32_t dtype, void* k, void* v, void* stream);
 
-/* Workspace bytes of an ebx_kv_attention call (partial results of split rows); 0 for
- * arguments that it refuses. */
+/* Workspace bytes of an ebx_kv_attention call with these arguments (partial results of
+ * rows that several CTAs share); 0 when it needs none, or refuses them. */
 EBX_API uint64_t ebx_kv_attention_workspace_bytes(const ebx_kv_pool* pool, int32_t heads,
-                                                  int64_t tokens, int32_t max_new);
+                                                  int64_t tokens, int32_t max_new,
+                                                  int32_t max_length);
 
 /* Attention of the new tokens' queries over the cache: request i's queries are rows
  * starts[i] .. starts[i + 1] - 1 of q [tokens, heads, head_dim] (strides and dtype as in

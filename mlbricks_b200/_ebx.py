@@ -102,7 +102,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _ST, [_P, _P, _I32, _P, _I32, _I32, _P, _I32, _P, _P, _P, _P, _P, _P, _I64, _I32, _P]),
     "ebx_kv_append": (_ST, [_KV, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I32, _P]),
     "ebx_kv_materialize": (_ST, [_KV, _P, _I32, _P, _P, _I32, _I64, _I32, _P, _P, _P]),
-    "ebx_kv_attention_workspace_bytes": (_U64, [_KV, _I32, _I64, _I32]),
+    "ebx_kv_attention_workspace_bytes": (_U64, [_KV, _I32, _I64, _I32, _I32]),
     "ebx_kv_attention": (
         _ST, [_KV, _P, _I64, _I64, _I32, _I32, _P, _I32, _P, _P, _P, _I32, _I64, _I32, _I32,
               ctypes.c_float, _I32, _I32, _P, _P, _P, _U64, _P]),

@@ -80,7 +80,7 @@ cudaError_t launch_kv_append(const KvPool& pool, const KvRows& k, const KvRows& 
 cudaError_t launch_kv_materialize(const KvPool& pool, const int32_t* tables, int width,
                                   const int32_t* starts, const int32_t* first, int requests,
                                   int64_t tokens, int dtype, void* k, void* v, cudaStream_t s);
-uint64_t kv_attention_workspace_bytes(int head_dim, int group, int64_t tokens, int max_new);
+uint64_t kv_attention_workspace_bytes(int head_dim, int group, int64_t tokens, int max_new, int max_length);
 cudaError_t launch_kv_attention(KvAttnArgs a, bool bf16, int max_new, int max_length, void* ws, cudaStream_t s);
 cudaError_t read_kv_status(int* status, bool clear, cudaStream_t s);
 

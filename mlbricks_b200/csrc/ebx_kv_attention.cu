@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(kStepThreads, (StepCfg<D, NQ>::PER_SM))
     }
     const KvShare share = kv_share<kRows, KT, kStepExtra, kStepThreads>(a, least, reinterpret_cast<int*>(smem));
     fence_proxy_async_smem();  // the ring's copies may overwrite what kv_share kept there
-    if (threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (threadIdx.x == 0 && !a.whole) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join waits for this grid's end
     __syncthreads();
     KvWalk<kRows, KT, kStepExtra> walk;
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(kStepThreads, (StepCfg<D, NQ>::PER_SM))
 }
 
 template <int D, int NQ, bool BF16>
-cudaError_t launch_step(KvAttnArgs a, void* ws, int dev, cudaStream_t s) {
+cudaError_t launch_step(KvAttnArgs a, int rows, void* ws, int dev, cudaStream_t s) {
     using C = StepCfg<D, NQ>;
     auto kern = kv_step_kernel<D, NQ, BF16>;
     static std::atomic<uint64_t> configured{0};
@@ -460,7 +460,7 @@ cudaError_t launch_step(KvAttnArgs a, void* ws, int dev, cudaStream_t s) {
     kern<<<grid, kStepThreads, C::kSmem, s>>>(mk, mv, a, kStepLeast);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    return launch_join<D, C::ROWS, 16, BF16>(a, grid, s);
+    return launch_join<D, C::ROWS, 4, BF16>(a, grid, std::min(rows, C::ROWS), s);
 }
 
 }  // namespace
@@ -469,7 +469,12 @@ namespace {
 
 // Row tiles of 256 rows on tcgen05 from kPromptMin rows of a request on; below, tiles of 8 or 16.
 constexpr int kPromptMin = 33;
-constexpr int kWholeTiles = 4;
+
+// Short requests: a second launch, to join, would cost more than sharing row tiles gains.
+bool takes_whole(int head_dim, int max_length) {
+    constexpr int kTiles = 4;
+    return max_length > 0 && max_length <= kTiles * (8192 / head_dim);
+}
 
 // Rows of one request and key/value head, at most.
 int64_t most_rows(int group, int64_t tokens, int max_new) {
@@ -478,12 +483,13 @@ int64_t most_rows(int group, int64_t tokens, int max_new) {
 
 }  // namespace
 
-uint64_t kv_attention_workspace_bytes(int head_dim, int group, int64_t tokens, int max_new) {
+uint64_t kv_attention_workspace_bytes(int head_dim, int group, int64_t tokens, int max_new, int max_length) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 0;
     const int sms = gemm_sm_count(dev);
     const int64_t most = most_rows(group, tokens, max_new);
     if (most >= kPromptMin) return kv_prompt_workspace_bytes(head_dim, sms);
+    if (takes_whole(head_dim, max_length)) return 0;
     const int nq = most <= 8 ? 1 : 2, ctas = sms * (nq == 1 ? StepCfg<32, 1>::PER_SM : StepCfg<32, 2>::PER_SM);
     return uint64_t(round_up(int64_t(ctas) * int64_t(sizeof(int4) + 2 * 8 * nq * (head_dim + 2) * sizeof(float)), 256));
 }
@@ -495,11 +501,11 @@ cudaError_t launch_kv_attention(KvAttnArgs a, bool bf16, int max_new, int max_le
     if (e != cudaSuccess) return e;
     if (most_rows(a.group, a.tokens, max_new) >= kPromptMin) return launch_kv_prompt(a, bf16, ws, dev, s);
 #define EBX_KV_STEP(DD)                                                                              \
-    (few ? (bf16 ? launch_step<DD, 1, true>(a, ws, dev, s) : launch_step<DD, 1, false>(a, ws, dev, s)) \
-         : (bf16 ? launch_step<DD, 2, true>(a, ws, dev, s) : launch_step<DD, 2, false>(a, ws, dev, s)))
-    const bool few = most_rows(a.group, a.tokens, max_new) <= 8;
-    // short requests: a second launch would cost more than it spreads
-    a.whole = max_length > 0 && max_length <= kWholeTiles * (8192 / a.pool.head_dim);
+    (few ? (bf16 ? launch_step<DD, 1, true>(a, rows, ws, dev, s) : launch_step<DD, 1, false>(a, rows, ws, dev, s)) \
+         : (bf16 ? launch_step<DD, 2, true>(a, rows, ws, dev, s) : launch_step<DD, 2, false>(a, rows, ws, dev, s)))
+    const int rows = int(most_rows(a.group, a.tokens, max_new));
+    const bool few = rows <= 8;
+    a.whole = takes_whole(a.pool.head_dim, max_length);
     switch (a.pool.head_dim) {
         case 32: return EBX_KV_STEP(32);
         case 64: return EBX_KV_STEP(64);

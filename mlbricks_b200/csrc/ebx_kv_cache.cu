@@ -155,10 +155,37 @@ __device__ __forceinline__ float2 unpack16(uint32_t v) {
     }
 }
 
-// rint(x / s) of two values as int8 codes in the low two bytes.
-__device__ __forceinline__ uint32_t quant2(float2 x, float s) {
-    const int a = __float2int_rn(__fdiv_rn(x.x, s)), b = __float2int_rn(__fdiv_rn(x.y, s));
-    return (uint32_t(min(max(a, -127), 127)) & 0xffu) | (uint32_t(min(max(b, -127), 127)) & 0xffu) << 8;
+// rint(x / s) of eight values of one 16-byte load as int8 codes.  r = 1 / s, so y = x * r is within
+// 2^-22 |y| < 2^-15 of the correctly rounded x / s (|y| <= 127): unless y is that near to a tie, both
+// round to the same integer.  Near one, or where r is infinite (a subnormal s), the division is done.
+// Rounding adds 1.5 * 2^23; the low byte of the sum is the code.
+template <bool BF16>
+__device__ __forceinline__ uint2 quant8(const uint4& x, float s, float r) {
+    constexpr float kMagic = 12582912.0f;
+    const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+    uint32_t c[8];
+    float off = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack16<BF16>(in[i]);
+        const float y0 = f.x * r, y1 = f.y * r;
+        const float n0 = y0 + kMagic, n1 = y1 + kMagic;
+        off = fmaxf(off, fmaxf(fabsf(y0 - (n0 - kMagic)), fabsf(y1 - (n1 - kMagic))));
+        c[2 * i] = __float_as_uint(n0);
+        c[2 * i + 1] = __float_as_uint(n1);
+    }
+    if (off > 0.5f - 0x1p-15f || isinf(r)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack16<BF16>(in[i]);
+            c[2 * i] = uint32_t(min(max(__float2int_rn(__fdiv_rn(f.x, s)), -127), 127));
+            c[2 * i + 1] = uint32_t(min(max(__float2int_rn(__fdiv_rn(f.y, s)), -127), 127));
+        }
+    }
+    uint2 out;
+    out.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+    out.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
+    return out;
 }
 
 // A run is a maximal sequence of tokens whose slots follow one another inside one block; a
@@ -178,7 +205,6 @@ __global__ void __launch_bounds__(kAppendWarps * 32)
     const int h = int(item % pool.kv_heads);
     const int64_t t0 = item / pool.kv_heads * span;
     if (t0 >= tokens) return;
-    const int64_t t1 = min(t0 + span, tokens);
     const bool values = blockIdx.y != 0;
     const KvRows x = values ? v : k;
     int8_t* codes = values ? pool.v_codes : pool.k_codes;
@@ -187,18 +213,27 @@ __global__ void __launch_bounds__(kAppendWarps * 32)
     const int64_t most = int64_t(pool.blocks) << pool.shift;
     const int part = lane % kLanes, sub = lane / kLanes;
 
-    for (int64_t t = t0; t < t1; ++t) {
-        const int64_t slot = slots[t];
-        if (slot < 0 || slot >= most) continue;
+    // the window's tokens, a lane each: which begin a run, which go on with one
+    const int64_t mine = t0 + lane < tokens ? slots[t0 + lane] : -1;
+    int64_t prev = __shfl_up_sync(0xffffffffu, mine, 1);
+    if (lane == 0) prev = t0 > 0 ? slots[t0 - 1] : -1;
+    const bool held = mine >= 0 && mine < most;
+    const bool goes_on = held && (mine & (bsize - 1)) != 0 && prev == mine - 1;
+    const unsigned going = __ballot_sync(0xffffffffu, goes_on);
+    unsigned begin = __ballot_sync(0xffffffffu, held && !goes_on && lane < span);
+    for (; begin != 0; begin &= begin - 1) {
+        const int first = __ffs(begin) - 1;
+        const int64_t t = t0 + first, slot = __shfl_sync(0xffffffffu, mine, first);
         const int off = int(slot & (bsize - 1));
-        if (off != 0 && t > 0 && slots[t - 1] == slot - 1) continue;  // inside a run
-        int n = 1;  // the run's length
-        for (int base = 0; base < bsize; base += 32) {
-            const int j = base + lane;
-            const bool in = j < bsize - off && t + j < tokens && slots[t + j] == slot + j;
-            const unsigned m = __ballot_sync(0xffffffffu, in);
-            n = base + (m == 0xffffffffu ? 32 : __ffs(~m) - 1);
-            if (m != 0xffffffffu) break;
+        int n = first == 31 ? 1 : __ffs(~(going >> (first + 1)));  // the run's length in the window
+        if (first + n == 32) {
+            for (int base = 32;; base += 32) {
+                const int j = base - first + lane;
+                const bool in = off + j < bsize && t + j < tokens && slots[t + j] == slot + j;
+                const unsigned m = __ballot_sync(0xffffffffu, in);
+                n = base - first + (m == 0xffffffffu ? 32 : __ffs(~m) - 1);
+                if (m != 0xffffffffu) break;
+            }
         }
         const uint16_t* src = x.p + t * x.token_stride + h * x.head_stride + part * 8;
         uint4 hold[kHold];
@@ -230,17 +265,24 @@ __global__ void __launch_bounds__(kAppendWarps * 32)
         int8_t* dst = codes + (cell << pool.shift) * D;
         if (off != 0 && s > old) {  // the block's earlier tokens move to the larger scale
             const float ratio = __fdiv_rn(old, s);
-            uint32_t* w = reinterpret_cast<uint32_t*>(dst);
-            for (int j = lane; j < off * (D / 4); j += 32) {
-                const uint32_t c = w[j];
-                uint32_t r = 0;
+            uint4* w = reinterpret_cast<uint4*>(dst);
+#pragma unroll 4
+            for (int j = lane; j < off * (D / 16); j += 32) {
+                const uint4 c = w[j];
+                uint32_t in[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-                for (int b = 0; b < 4; ++b)
-                    r |= (uint32_t(__float2int_rn(float(int8_t(c >> (8 * b))) * ratio)) & 0xffu) << (8 * b);
-                w[j] = r;
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t r = 0;
+#pragma unroll
+                    for (int b = 0; b < 4; ++b)
+                        r |= (uint32_t(__float2int_rn(float(int8_t(in[q] >> (8 * b))) * ratio)) & 0xffu) << (8 * b);
+                    in[q] = r;
+                }
+                w[j] = make_uint4(in[0], in[1], in[2], in[3]);
             }
         }
         const bool live = s > 0.0f;  // neither an all-zero block nor NaN
+        const float r = __frcp_rn(s);
         for (int base = 0; base < n; base += kHold * kPer) {
             if (n > kHold * kPer) {  // the run did not fit the registers: read it again (L2)
 #pragma unroll
@@ -253,11 +295,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32)
             for (int i = 0; i < kHold; ++i) {
                 const int j = base + i * kPer + sub;
                 if (j >= n) continue;
-                uint2 c = make_uint2(0, 0);
-                if (live) {
-                    c.x = quant2(unpack16<BF16>(hold[i].x), s) | quant2(unpack16<BF16>(hold[i].y), s) << 16;
-                    c.y = quant2(unpack16<BF16>(hold[i].z), s) | quant2(unpack16<BF16>(hold[i].w), s) << 16;
-                }
+                const uint2 c = live ? quant8<BF16>(hold[i], s, r) : make_uint2(0, 0);
                 *reinterpret_cast<uint2*>(dst + (off + j) * D + part * 8) = c;
             }
         }

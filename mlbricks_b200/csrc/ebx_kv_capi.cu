@@ -130,11 +130,13 @@ ebx_status ebx_kv_materialize(const ebx_kv_pool* pool, const int32_t* tables, in
 }
 
 uint64_t ebx_kv_attention_workspace_bytes(const ebx_kv_pool* pool, int32_t heads, int64_t tokens,
-                                          int32_t max_new) {
+                                          int32_t max_new, int32_t max_length) {
     ebx::KvPool p;
-    if (pool_of(pool, p) || heads < 1 || heads % p.kv_heads != 0 || tokens < 0 || max_new < 0) return 0;
+    if (pool_of(pool, p) || heads < 1 || heads % p.kv_heads != 0 || tokens < 0 || max_new < 0 || max_length < 0)
+        return 0;
     Device d(pool->device);
-    return d.err == cudaSuccess ? ebx::kv_attention_workspace_bytes(p.head_dim, heads / p.kv_heads, tokens, max_new) : 0;
+    if (d.err != cudaSuccess) return 0;
+    return ebx::kv_attention_workspace_bytes(p.head_dim, heads / p.kv_heads, tokens, max_new, max_length);
 }
 
 ebx_status ebx_kv_attention(const ebx_kv_pool* pool, const void* q, int64_t q_token_stride,
@@ -163,7 +165,8 @@ ebx_status ebx_kv_attention(const ebx_kv_pool* pool, const void* q, int64_t q_to
         return invalid("ebx_kv_attention: out and workspace must be 16-byte aligned");
     Device d(pool->device);
     if (d.err != cudaSuccess) return launched(d.err, "cudaSetDevice");
-    if (!workspace || workspace_bytes < ebx::kv_attention_workspace_bytes(p.head_dim, heads / p.kv_heads, tokens, max_new)) {
+    const uint64_t need = ebx::kv_attention_workspace_bytes(p.head_dim, heads / p.kv_heads, tokens, max_new, max_length);
+    if (need > 0 && (!workspace || workspace_bytes < need)) {
         ebx::set_error("ebx_kv_attention: workspace smaller than ebx_kv_attention_workspace_bytes");
         return EBX_ERR_WORKSPACE;
     }

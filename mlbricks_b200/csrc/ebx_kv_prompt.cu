@@ -698,7 +698,7 @@ cudaError_t launch_prompt(KvAttnArgs a, void* ws, int dev, cudaStream_t s) {
     kern<<<grid, kPromptThreads, C::kSmem, s>>>(mk, mv, a, kPromptLeast);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    return launch_join<D, kPromptRows, 4, BF16>(a, grid, s);
+    return launch_join<D, kPromptRows, 4, BF16>(a, grid, kPromptRows, s);
 }
 
 }  // namespace

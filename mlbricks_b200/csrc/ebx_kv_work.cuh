@@ -372,14 +372,23 @@ __global__ void __launch_bounds__(32 * WAYS) kv_join_kernel(const __grid_constan
             m = mn;
         };
         if (r < rows) {
-            for (int k = c + way; k <= last; k += WAYS) {
-                const int slot = k == c ? 1 : 0;
-                const float4* src = reinterpret_cast<const float4*>(kv_part<D, RT>(a, k, slot));
-                float4 v[COLS];
+            constexpr int AHEAD = 4;  // parts on their way at once
+            for (int k0 = c + way; k0 <= last; k0 += AHEAD * WAYS) {
+                float4 v[AHEAD][COLS];
+                float2 ml[AHEAD];
 #pragma unroll
-                for (int x = 0; x < COLS; ++x) v[x] = src[(x * 8 + col) * RT + r];
-                const float2 ml = kv_part_ml<D, RT>(a, k, slot)[r];
-                join(ml.x, ml.y, v);
+                for (int i = 0; i < AHEAD; ++i) {
+                    const int k = k0 + i * WAYS, slot = k == c ? 1 : 0;
+                    ml[i] = make_float2(-INFINITY, 0.0f);
+                    if (k > last) continue;
+                    const float4* src = reinterpret_cast<const float4*>(kv_part<D, RT>(a, k, slot));
+#pragma unroll
+                    for (int x = 0; x < COLS; ++x) v[i][x] = src[(x * 8 + col) * RT + r];
+                    ml[i] = kv_part_ml<D, RT>(a, k, slot)[r];
+                }
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i)
+                    if (k0 + i * WAYS <= last) join(ml[i].x, ml[i].y, v[i]);
             }
         }
         s_ml[way][col][ri] = make_float2(m, l);
@@ -425,12 +434,12 @@ inline bool code_map(CUtensorMap* map, const int8_t* codes, const KvPool& p, int
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The join of a launch of `ctas` CTAs.
+// The join of a launch of `ctas` CTAs whose row tiles have at most `rows` rows.
 template <int D, int RT, int WAYS, bool BF16>
-cudaError_t launch_join(const KvAttnArgs& a, int ctas, cudaStream_t s) {
+cudaError_t launch_join(const KvAttnArgs& a, int ctas, int rows, cudaStream_t s) {
     if (a.whole) return cudaSuccess;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(ctas), unsigned((RT + 3) / 4));
+    cfg.gridDim = dim3(unsigned(ctas), unsigned((rows + 3) / 4));
     cfg.blockDim = dim3(32 * WAYS);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];

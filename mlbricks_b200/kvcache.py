@@ -138,12 +138,9 @@ def plan(past: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, free: torc
            "past, new and the rows of tables must be as many")
     _check(ring.numel() >= 2 and tokens >= 0, "ring holds at least its front and back, and tokens >= 0")
     _check(block_size in BLOCK_SIZES, f"block_size must be one of {BLOCK_SIZES}, got {block_size}")
-    where = past.device
-    lengths = torch.empty(requests, dtype=torch.int32, device=where)
-    starts = torch.empty(requests + 1, dtype=torch.int32, device=where)
-    slots = torch.empty(tokens, dtype=torch.int64, device=where)
-    positions = torch.empty(tokens, dtype=torch.int32, device=where)
-    out = torch.empty(4, dtype=torch.int64, device=where)
+    # new_empty: the cheapest way to a tensor, and this call is made every step
+    lengths, starts, positions = past.new_empty(requests), past.new_empty(requests + 1), past.new_empty(tokens)
+    slots, out = ring.new_empty(tokens), ring.new_empty(4)
     st = _ebx.load().ebx_kv_plan(
         past.data_ptr(), new.data_ptr(), requests, tables.data_ptr(), tables.shape[1], block_size,
         free.data_ptr(), free.numel(), ring.data_ptr(), out.data_ptr(), lengths.data_ptr(), starts.data_ptr(),
@@ -191,8 +188,7 @@ def materialize(pool: KVPool, tables: torch.Tensor, starts: torch.Tensor, *, fir
         _check_int(first, torch.int32, pool.device, "first")
         _check(first.numel() == requests, "first must have one entry for each request")
     shape = (tokens, pool._c.kv_heads, pool._c.head_dim)
-    k = torch.empty(shape, dtype=dtype, device=starts.device)
-    v = torch.empty(shape, dtype=dtype, device=starts.device)
+    k, v = starts.new_empty(shape, dtype=dtype), starts.new_empty(shape, dtype=dtype)
     st = _ebx.load().ebx_kv_materialize(
         pool._ref, tables.data_ptr(), tables.shape[1], starts.data_ptr(), None if first is None else first.data_ptr(),
         requests, tokens, _DTYPES[dtype], k.data_ptr(), v.data_ptr(), _stream(pool.device))
@@ -228,19 +224,20 @@ def attention(q: torch.Tensor, pool: KVPool, tables: torch.Tensor, lengths: torc
         _check_int(first, torch.int32, device, "first")
         _check(first.numel() == requests, "first must have one entry for each request")
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+        out = q.new_empty((tokens, heads, dim))
     elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != device or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor of q's shape and dtype")
-    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
     if tokens and requests:
         lib = _ebx.load()
-        nbytes = lib.ebx_kv_attention_workspace_bytes(pool._ref, heads, tokens, max_new)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        nbytes = lib.ebx_kv_attention_workspace_bytes(pool._ref, heads, tokens, max_new, max_length)
+        ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         st = lib.ebx_kv_attention(
             pool._ref, q.data_ptr(), q.stride(0), q.stride(1), heads, _ROW_DTYPES[q.dtype], tables.data_ptr(),
             tables.shape[1], lengths.data_ptr(), starts.data_ptr(), None if first is None else first.data_ptr(),
             requests, tokens, causal, window, 1.0 / math.sqrt(dim) if scale is None else scale, max_new, max_length,
-            out.data_ptr(), None if lse is None else lse.data_ptr(), ws.data_ptr(), nbytes, _stream(device))
+            out.data_ptr(), None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
+            _stream(device))
         if st:
             _ebx.check(st)
     return out if lse is None else (out, lse)
