@@ -2,19 +2,22 @@
 // formulas of ebx_kv_attention.cu on the 5th-generation tensor cores.
 //
 // A row tile is 256 rows (two of 128: the M of tcgen05.mma), a key tile 128 tokens.  One CTA per
-// SM, 14 warps:
-//   * warp 12 loads int8 key and value tiles (TMA, a box per block) and their scales;
-//   * warps 8-11 turn codes into fp16 tiles [64 dimensions][128 rows of 128 bytes] with the
+// SM, 24 warps (two idle):
+//   * warp 20 loads int8 key and value tiles (TMA, a box per block) and their scales;
+//   * warps 16-19 turn codes into fp16 tiles [64 dimensions][128 rows of 128 bytes] with the
 //     128-byte swizzle: exact integers, so the scales stay out of the products.  The same layout
 //     is K-major for q . k (rows = N) and N-major for w . v (rows = K), so values need no transpose;
-//   * one thread of warp 13 issues S = q k^T and O += w v.  The accumulators of both row tiles
-//     (S 2 x 128 columns, O 2 x 128) fill the tensor memory; the weights overwrite S as the second
-//     product's A operand.  While it works on one row tile, the other's weights are computed;
-//   * warps 0-3 and 4-7: a thread per row of each row tile, two passes over S in tensor memory: the
-//     largest t; the weights and their sum.  O is rescaled (in tensor memory) only when t grew by
-//     more than the lag.  (Holding the row in registers saves the second read of S but not its time:
-//     the unrolled code of 128 columns missed the instruction cache and spilled.)
-// Every mbarrier wait is bounded; a timeout sets the device status word and the roles leave.
+//   * warp 21 issues S = q k^T and O += w v.  The accumulators of both row tiles (S 2 x 128 columns,
+//     O 2 x 128) fill the tensor memory; the weights overwrite S as the second product's A operand.
+//     While it works on one row tile, the other's weights are computed;
+//   * warps 0-7 and 8-15: two threads per row of each row tile, 64 keys of the tile each, in two
+//     passes over S in tensor memory: the largest t; the weights and their sum.  O is rescaled (in
+//     tensor memory) only when t grew by more than the lag.
+// What bounds it: the chain S -> weights -> O of a row tile, of which the products of the other row
+// tile cover only a part.  Two threads a row halve the weights' part of it (one thread a row: 570 +
+// 1500 clocks for 128 keys, where the exponential unit alone would take 1000).
+// Every mbarrier wait is bounded; a timeout sets the device status word, after which the row warps
+// wait no more but still meet each other's barriers, and the other roles leave.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -27,7 +30,8 @@ namespace {
 
 constexpr int kPromptRows = 256;
 constexpr int kPromptKeys = 128;
-constexpr int kPromptThreads = 14 * 32;
+constexpr int kRowWarps = 16, kConvert = 16, kLoad = 20, kIssue = 21;  // first warps of the roles
+constexpr int kPromptThreads = 24 * 32;
 constexpr int kHalf = 128 * 128;   // bytes of 128 rows x 64 fp16
 constexpr int kPromptExtra = 3;    // a row tile's begin and end, in key tiles
 constexpr int kRaw = 4;            // int8 tiles in flight
@@ -44,7 +48,7 @@ struct PromptCfg {
     static constexpr int kRawOff = kBufOff + kBufs * kTile;
     static constexpr int kTabOff = kRawOff + kRaw * kRawTile;
     static constexpr int kBytes = kTabOff + kTabs * 8 * 16 + kRaw * 16 * 4 + 256;
-    static constexpr int kSmem = kBytes + 1024;
+    static constexpr int kSmem = kBytes + 2 * 2 * 128 * 4;  // and what the two threads of a row tell each other
     static constexpr uint32_t kIdescS = (1u << 4) | (uint32_t(kPromptKeys >> 3) << 17) | (8u << 24);
     static constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | (uint32_t(D >> 3) << 17) | (8u << 24);
 };
@@ -88,21 +92,7 @@ __device__ __forceinline__ void commit(const uint64_t* bar) {
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 
-// 32 columns of the thread's lane; valid after tmem_wait on the same registers.
-template <int N>
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[N], int at = 0) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
-        : "=r"(v[at]), "=r"(v[at + 1]), "=r"(v[at + 2]), "=r"(v[at + 3]), "=r"(v[at + 4]), "=r"(v[at + 5]),
-          "=r"(v[at + 6]), "=r"(v[at + 7]), "=r"(v[at + 8]), "=r"(v[at + 9]), "=r"(v[at + 10]), "=r"(v[at + 11]),
-          "=r"(v[at + 12]), "=r"(v[at + 13]), "=r"(v[at + 14]), "=r"(v[at + 15]), "=r"(v[at + 16]),
-          "=r"(v[at + 17]), "=r"(v[at + 18]), "=r"(v[at + 19]), "=r"(v[at + 20]), "=r"(v[at + 21]),
-          "=r"(v[at + 22]), "=r"(v[at + 23]), "=r"(v[at + 24]), "=r"(v[at + 25]), "=r"(v[at + 26]),
-          "=r"(v[at + 27]), "=r"(v[at + 28]), "=r"(v[at + 29]), "=r"(v[at + 30]), "=r"(v[at + 31])
-        : "r"(taddr) : "memory");
-}
+// 16 columns of the thread's lane; valid after tmem_wait on the same registers.
 template <int N>
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[N], int at) {
     asm volatile(
@@ -113,23 +103,20 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[N], int 
           "=r"(v[at + 12]), "=r"(v[at + 13]), "=r"(v[at + 14]), "=r"(v[at + 15])
         : "r"(taddr) : "memory");
 }
-template <int N>
-__device__ __forceinline__ void tmem_wait(uint32_t (&v)[N]) {
+template <int COUNT, int N>
+__device__ __forceinline__ void tmem_wait(uint32_t (&v)[N], int at = 0) {
     asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < N; i += 8)  // no use of the registers moves above the wait
+    for (int i = at; i < at + COUNT; i += 8)  // no use of the registers moves above the wait
         asm volatile("" : "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3]), "+r"(v[i + 4]),
                      "+r"(v[i + 5]), "+r"(v[i + 6]), "+r"(v[i + 7]));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};\n" ::"r"(v[0]),
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};\n" ::"r"(v[0]),
         "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),
-        "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]),
-        "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr) : "memory");
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};\n" ::"r"(v[0]),
@@ -164,7 +151,7 @@ __device__ __forceinline__ uint32_t seen32(const Row& row, int key0) {
     return hi > lo ? (0xffffffffu >> (32 - (hi - lo))) << lo : 0u;
 }
 
-// Walks the row's 128 columns of S, a unit of 16 tokens at a time, the next on its way: f(v, e, at,
+// Walks 64 columns of the row's S, a unit of 16 tokens at a time, the next on its way: f(v, e, at,
 // seen) with v the columns from `at` on, e = {ks * scale * log2 e, log2 vs, 1 / vs} of the unit, and
 // with MASK the columns that the row sees of the tile, which begins at key0.
 template <bool MASK, class F>
@@ -173,14 +160,14 @@ __device__ __forceinline__ void columns(uint32_t s, const float4* tab, const Row
     float4 e0 = tab[0], e1;
     tmem_ld16(s, v, 0);
 #pragma unroll 1
-    for (int c = 0; c < 128; c += 32) {
+    for (int c = 0; c < 64; c += 32) {
         const uint32_t seen = MASK ? seen32(row, key0 + c) : 0u;
-        tmem_wait(v);
+        tmem_wait<16>(v, 0);
         tmem_ld16(s + c + 16, v, 16);
         e1 = tab[c / 16 + 1];
         f(v, e0, c, seen);
-        tmem_wait(v);
-        if (c < 96) {
+        tmem_wait<16>(v, 16);
+        if (c == 0) {
             tmem_ld16(s + c + 32, v, 0);
             e0 = tab[c / 16 + 2];
         }
@@ -196,7 +183,7 @@ __device__ __forceinline__ uint64_t t_pair(const uint32_t* v, int i, uint64_t c2
     return pack2f(seen & (1u << i) ? lo2(t2) : -INFINITY, seen & (2u << i) ? hi2(t2) : -INFINITY);
 }
 
-// The largest t - mr of the row.
+// The largest t - mr of the 64 columns.
 template <bool MASK>
 __device__ __forceinline__ float largest(uint32_t s, const float4* tab, const Row& row, float mr, int key0) {
     float top0 = -INFINITY, top1 = -INFINITY;
@@ -255,13 +242,21 @@ __device__ __forceinline__ float weigh(uint32_t s, const float4* tab, const Row&
     return l;
 }
 
+// Barriers of the two warps that share 32 rows.
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ bool pair_any(int id, bool mine) {
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.or.pred p, %2, 64, q;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(any) : "r"(uint32_t(mine)), "r"(id) : "memory");
+    return any != 0;
+}
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kPromptThreads, 1)
     kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                      const __grid_constant__ KvAttnArgs a, int least) {
     using C = PromptCfg<D>;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];
     float4* tabs = reinterpret_cast<float4*>(smem + C::kTabOff);             // [kTabs][8]
     float* raw_scales = reinterpret_cast<float*>(tabs + kTabs * 8);          // [kRaw][k, v][8]
     uint64_t* raw_full = reinterpret_cast<uint64_t*>(raw_scales + kRaw * 16);
@@ -274,9 +269,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     uint64_t* p_full = s_full + 2;
     uint64_t* o_done = p_full + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
+    float* told = reinterpret_cast<float*>(smem + C::kBytes);               // [row tile][half][row]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp == 12) {
+    if (warp == kLoad) {
         if (lane == 0) {
             for (int i = 0; i < kRaw; ++i) {
                 mbar_init(smem_u32(raw_full + i), 1 + 32);  // the copies' bytes, and each lane's scales
@@ -288,9 +284,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
             for (int i = 0; i < kTabs; ++i) mbar_init(smem_u32(tab_full + i), 1);
             for (int i = 0; i < 2; ++i) {
-                mbar_init(smem_u32(q_full + i), 4);
+                mbar_init(smem_u32(q_full + i), 8);
                 mbar_init(smem_u32(s_full + i), 1);
-                mbar_init(smem_u32(p_full + i), 4);
+                mbar_init(smem_u32(p_full + i), 8);
                 mbar_init(smem_u32(o_done + i), 1);
             }
             fence_proxy_async_smem();
@@ -311,53 +307,63 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     KvWalk<kPromptRows, kPromptKeys, kPromptExtra> walk;
     walk.start(a, share);
 
-    if (warp < 8) {
-        // ---------------- a thread per row ----------------
-        const int x = warp >> 2;                               // row tile
-        const int rl = (warp & 3) * 32 + lane;                 // row in it = tensor memory lane
-        const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
-        const uint32_t s_addr = tmem + lane_base + kSCol + x * 128, o_addr = tmem + lane_base + kOCol + x * 128;
+    if (warp < kRowWarps) {
+        // ---------------- two threads per row ----------------
+        const int x = warp >> 3;                               // row tile
+        const int half = (warp >> 2) & 1;                      // 64 of the 128 keys, half of O's columns
+        const int quarter = warp & 3;                          // the warp's 32 lanes of tensor memory
+        const int pair = 1 + x * 4 + quarter;                  // barrier of the two warps that share them
+        const uint32_t lane_base = uint32_t(quarter * 32) << 16;
+        const uint32_t s_addr = tmem + lane_base + kSCol + x * 128 + half * 64;
+        const uint32_t o_addr = tmem + lane_base + kOCol + x * 128 + half * (D / 2);
+        float* tell = told + (x * 2 + half) * 128 + quarter * 32 + lane;
+        const float* other = told + (x * 2 + (half ^ 1)) * 128 + quarter * 32 + lane;
+        // q and the output pass through shared memory, PER lanes to a row of 16-byte chunks
+        constexpr int PER = D / 8, ROWS = 32 / PER;
+        uint8_t* staged = smem + x * C::kTile + quarter * 32 * 128;
+        const int mine = lane / PER, chunk = lane % PER;
+        auto stage_at = [&](int i) {  // this lane's 16 bytes of the warps' row i
+            return reinterpret_cast<uint4*>(staged + (chunk / 8) * kHalf + i * 128 + (((chunk & 7) ^ (i & 7)) << 4));
+        };
         int g = 0;   // key tiles of this row tile so far
         int gj = 0;  // key tiles of the CTA so far
         bool ok = true;
-        for (; !walk.done() && ok; walk.next(a)) {
+        auto wait = [&](const uint64_t* bar, int phase) {
+            if (ok) ok = __all_sync(0xffffffffu, pwait(bar, phase));
+            after_sync();
+        };
+        for (; !walk.done(); walk.next(a)) {
             if (x == 1 && walk.r.rows - walk.rt * kPromptRows <= 128) {
                 gj += walk.n;
                 continue;
             }
-            const int r = walk.rt * kPromptRows + x * 128 + rl;
-            const bool live = r < walk.r.rows;
-            const int token = live ? by_group(a, r) : 0, head = walk.head * a.group + (live ? r - token * a.group : 0);
-            Row row;
-            row.unit = 1.0f;
-            row.mr = -INFINITY;
-            row.l = 0.0f;
-            const int place = walk.r.begin + token;
-            row.hi = !live ? INT_MAX : a.causal ? min(place + 1, walk.r.length) : walk.r.length;
-            row.lo = !live ? 0 : max(walk.r.first, a.window > 0 ? place - a.window + 1 : 0);
-            // q: PER lanes read a row together, 16 bytes each
-            constexpr int PER = D / 8, ROWS = 32 / PER;
-            const int row0 = walk.rt * kPromptRows + x * 128 + (warp & 3) * 32;  // the warp's first row
+            const int row0 = walk.rt * kPromptRows + x * 128 + quarter * 32;  // the warps' first row
             auto row_at = [&](int i, int64_t token_stride, int64_t head_stride) {  // its row i's offset; -1: past the last
                 const int ri = row0 + i;
                 if (ri >= walk.r.rows) return int64_t(-1);
                 const int t = by_group(a, ri);
                 return (walk.r.token0 + t) * token_stride + (walk.head * a.group + ri - t * a.group) * head_stride;
             };
-            uint8_t* staged = smem + x * C::kTile + (warp & 3) * 32 * 128;  // q's rows, later the output's
-            const int mine = lane / PER, chunk = lane % PER;
-            auto stage_at = [&](int i) {  // this lane's 16 bytes of the warp's row i
-                return reinterpret_cast<uint4*>(staged + (chunk / 8) * kHalf + i * 128 + (((chunk & 7) ^ (i & 7)) << 4));
-            };
+            Row row;
+            row.unit = 1.0f;
+            row.mr = -INFINITY;
+            row.l = 0.0f;
+            const bool live = row0 + lane < walk.r.rows;
             {
-                uint4 v[PER];
+                const int place = walk.r.begin + by_group(a, live ? row0 + lane : 0);
+                row.hi = !live ? INT_MAX : a.causal ? min(place + 1, walk.r.length) : walk.r.length;
+                row.lo = !live ? 0 : max(walk.r.first, a.window > 0 ? place - a.window + 1 : 0);
+            }
+            {
+                uint4 v[PER / 2];  // each of the two warps brings every other load's rows
 #pragma unroll
-                for (int i = 0; i < PER; ++i) {
-                    const int64_t off = row_at(i * ROWS + mine, a.q.token_stride, a.q.head_stride);
+                for (int i = 0; i < PER / 2; ++i) {
+                    const int64_t off = row_at((2 * i + half) * ROWS + mine, a.q.token_stride, a.q.head_stride);
                     v[i] = off >= 0 ? __ldg(reinterpret_cast<const uint4*>(a.q.p + off) + chunk) : make_uint4(0, 0, 0, 0);
                 }
 #pragma unroll
-                for (int i = 0; i < PER; ++i) {
+                for (int i = 0; i < PER / 2; ++i) {
+                    const int ri = (2 * i + half) * ROWS + mine;
                     if constexpr (BF16) {
                         // over the power of two at the row's largest element, as in ebx_kv_attention.cu
                         const uint32_t m = 0x7fff7fffu;
@@ -367,56 +373,57 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                         for (int d = 1; d < PER; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
                         const uint32_t e = min(max(top >> 7, 1u), 253u);
                         const float down = __uint_as_float((254u - e) << 23);
-                        const uint32_t up = __shfl_sync(0xffffffffu, e << 23, (lane % ROWS) * PER);
-                        if (lane / ROWS == i) row.unit = __uint_as_float(up);
-                        auto half = [&](uint32_t b) {
+                        if (chunk == 0) told[x * 256 + quarter * 32 + ri] = __uint_as_float(e << 23);
+                        auto halves = [&](uint32_t b) {
                             return pack_half2(__uint_as_float(b << 16) * down, __uint_as_float(b & 0xffff0000u) * down);
                         };
-                        v[i] = make_uint4(half(v[i].x), half(v[i].y), half(v[i].z), half(v[i].w));
+                        v[i] = make_uint4(halves(v[i].x), halves(v[i].y), halves(v[i].z), halves(v[i].w));
                     }
-                    *stage_at(i * ROWS + mine) = v[i];
+                    *stage_at(ri) = v[i];
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(q_full + x));
+                if constexpr (BF16) {
+                    pair_sync(pair);
+                    row.unit = told[x * 256 + quarter * 32 + lane];
+                    pair_sync(pair);
+                }
             }
             // keys that every row of the warp sees
             const int all_lo = __reduce_max_sync(0xffffffffu, row.lo), all_hi = __reduce_min_sync(0xffffffffu, row.hi);
-            // moves mr of the rows whose t reached `top`, and what was summed with the old one
-            auto raise = [&](float top, int j) {
-                const bool up = top > row.mr + (kLag + kShift);
-                const float mr = up ? top - kShift : row.mr;
-                const float f = up ? ex2(row.mr - mr) : 1.0f;
-                row.mr = mr;
-                row.l *= f;
-                if (j == 0) return true;
-                if (!__all_sync(0xffffffffu, pwait(o_done + x, g - 1))) return false;
-                after_sync();
-#pragma unroll 1
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t v[32];
-                    tmem_ld32(o_addr + c * 32, v);
-                    tmem_wait(v);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-                    tmem_st32(o_addr + c * 32, v);
-                }
-                return true;
-            };
             for (int j = 0; j < walk.n; ++j, ++g, ++gj) {
-                ok = pwait(s_full + x, g) && pwait(tab_full + gj % kTabs, gj / kTabs);
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
-                    break;
-                }
-                after_sync();
-                const float4* tab = tabs + (gj % kTabs) * 8;
-                const int key0 = (walk.t0 + j) * kPromptKeys;
-                const bool mask = key0 < all_lo || key0 + kPromptKeys > all_hi;
+                wait(s_full + x, g);
+                wait(tab_full + gj % kTabs, gj / kTabs);
+                const float4* tab = tabs + (gj % kTabs) * 8 + half * 4;
+                const int key0 = (walk.t0 + j) * kPromptKeys + half * 64;
+                const bool mask = key0 < all_lo || key0 + 64 > all_hi;
                 const float mr = row.mr == -INFINITY ? 0.0f : row.mr;
-                const float top = mr + (mask ? largest<true>(s_addr, tab, row, mr, key0) : largest<false>(s_addr, tab, row, mr, key0));
-                if (__any_sync(0xffffffffu, top > row.mr + (kLag + kShift)))
-                    if (!(ok = raise(top, j))) break;
+                float top = mr + (mask ? largest<true>(s_addr, tab, row, mr, key0) : largest<false>(s_addr, tab, row, mr, key0));
+                if (pair_any(pair, top > row.mr + (kLag + kShift))) {
+                    // mr moves in the rows whose t grew, and with it what was summed
+                    *tell = top;
+                    pair_sync(pair);
+                    top = fmaxf(top, *other);
+                    const bool up = top > row.mr + (kLag + kShift);
+                    const float next = up ? top - kShift : row.mr;
+                    const float f = up ? ex2(row.mr - next) : 1.0f;
+                    row.mr = next;
+                    row.l *= f;
+                    if (j > 0) {
+                        wait(o_done + x, g - 1);
+#pragma unroll 1
+                        for (int c = 0; c < D / 2; c += 16) {
+                            uint32_t v[16];
+                            tmem_ld16(o_addr + c, v, 0);
+                            tmem_wait<16>(v);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                            tmem_st16(o_addr + c, v);
+                        }
+                    }
+                    pair_sync(pair);  // `told` is free again
+                }
                 const float now = row.mr == -INFINITY ? 0.0f : row.mr;
                 row.l += mask ? weigh<true>(s_addr, tab, row, now, key0) : weigh<false>(s_addr, tab, row, now, key0);
                 asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
@@ -424,59 +431,61 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(p_full + x));
             }
-            if (!ok) break;
-            if (!__all_sync(0xffffffffu, pwait(o_done + x, g - 1))) {
-                ok = false;
-                break;
-            }
-            after_sync();
+            // the sums of both halves, and O
+            *tell = row.l;
+            pair_sync(pair);
+            const float l = half ? *other + row.l : row.l + *other;
+            wait(o_done + x, g - 1);
             const bool whole = walk.whole();
             const int slot = walk.begins ? 1 : 0;
-            const float inv = row.l == 0.0f ? 0.0f : 1.0f / row.l;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             float4* part = whole ? nullptr
-                                 : reinterpret_cast<float4*>(kv_part<D, kPromptRows>(a, blockIdx.x, slot)) + x * 128 + rl;
+                                 : reinterpret_cast<float4*>(kv_part<D, kPromptRows>(a, blockIdx.x, slot)) + x * 128 + quarter * 32 + lane;
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-                uint32_t v[32];
-                tmem_ld32(o_addr + c * 32, v);
-                tmem_wait(v);
+            for (int c = 0; c < D / 2; c += 16) {
+                uint32_t v[16];
+                tmem_ld16(o_addr + c, v, 0);
+                tmem_wait<16>(v);
+                const int d0 = half * (D / 2) + c;
                 if (whole) {  // through shared memory, so that rows are written whole
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < 2; ++i) {
                         uint32_t h[4];
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             h[k] = pack16<BF16>(__uint_as_float(v[8 * i + 2 * k]) * inv, __uint_as_float(v[8 * i + 2 * k + 1]) * inv);
-                        const int q = 4 * c + i;
+                        const int q = d0 / 8 + i;
                         *reinterpret_cast<uint4*>(staged + (q / 8) * kHalf + lane * 128 + (((q & 7) ^ (lane & 7)) << 4)) =
                             make_uint4(h[0], h[1], h[2], h[3]);
                     }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        part[(8 * c + i) * kPromptRows] =
+                    for (int i = 0; i < 4; ++i)
+                        part[(d0 / 4 + i) * kPromptRows] =
                             make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
                                         __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
                 }
             }
-            __syncwarp();
-            if (whole) {
-#pragma unroll
-                for (int i = 0; i < PER; ++i) {
-                    const int64_t off = row_at(i * ROWS + mine, int64_t(a.heads) * D, D);
-                    if (off >= 0) *(reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + off) + chunk) = *stage_at(i * ROWS + mine);
-                }
-            }
-            const int64_t at_row = int64_t(walk.r.token0 + token) * a.heads + head;
             before_sync();
-            if (live && whole && a.lse)
-                a.lse[at_row] = row.l == 0.0f ? -INFINITY : (row.mr + lg2(row.l)) * 0.6931471805599453f;
-            if (!whole) kv_part_ml<D, kPromptRows>(a, blockIdx.x, slot)[x * 128 + rl] = make_float2(row.mr, row.l);
+            pair_sync(pair);
+            if (whole) {
+#pragma unroll 1
+                for (int i = 0; i < PER / 2; ++i) {
+                    const int ri = (2 * i + half) * ROWS + mine;
+                    const int64_t off = row_at(ri, int64_t(a.heads) * D, D);
+                    if (off >= 0) *(reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + off) + chunk) = *stage_at(ri);
+                }
+                pair_sync(pair);  // the staged rows are free again
+            }
+            if (half == 0 && live && whole && a.lse)
+                a.lse[row_at(lane, a.heads, 1)] = l == 0.0f ? -INFINITY : (row.mr + lg2(l)) * 0.6931471805599453f;
+            if (half == 0 && !whole)
+                kv_part_ml<D, kPromptRows>(a, blockIdx.x, slot)[x * 128 + quarter * 32 + lane] = make_float2(row.mr, l);
             if (walk.begins && !whole && threadIdx.x == 0)
                 a.desc[blockIdx.x] = kv_desc(walk.r, walk.rt, kPromptRows, walk.head, walk.last() - int(blockIdx.x));
         }
-    } else if (warp >= 12) {
-        if (warp == 12) {
+    } else if (warp >= kLoad) {
+        if (warp == kLoad) {
             // ---------------- loader ----------------
             const int bsize = a.pool.block_size, none = a.pool.blocks;
             const int64_t past_pool = int64_t(none) * a.pool.kv_heads * bsize;  // TMA fills with zeros
@@ -524,7 +533,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 }
             }
             asm volatile("cp.async.wait_all;\n" ::: "memory");
-        } else if (warp == 13) {
+        } else if (warp == kIssue) {
             // ---------------- products: the warp together, one elected lane issues ----------------
             const uint64_t q0 = tile_desc(smem_u32(smem)), buf0 = tile_desc(smem_u32(smem + C::kBufOff));
             int it = 0;            // fp16 tiles used: key and value tiles in turn
@@ -551,7 +560,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 if (elected()) {
 #pragma unroll
                     for (int i = 0; i < kPromptKeys / 16; ++i)
-                        mma_ts(d, w + i * 8, v + i * (2048 >> 4), C::kIdescO, i == 0 ? !first : 1);
+                        mma_ts(d, w + (i / 4) * 64 + (i % 4) * 8, v + i * (2048 >> 4), C::kIdescO, i == 0 ? !first : 1);
                     commit(o_done + x);
                 }
                 __syncwarp();
@@ -604,7 +613,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
     } else {
         // ---------------- codes to fp16 ----------------
-        const int w = warp - 8;
+        const int w = warp - kConvert;
         int it = 0, gj = 0;
         bool ok = true;
         for (; !walk.done() && ok; walk.next(a)) {
@@ -669,7 +678,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 
     before_sync();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == kLoad) {
         after_sync();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
     }

@@ -75,7 +75,7 @@ struct KvShare {
 // tiles are the CTA's.  Every warp keeps its own copy.
 template <int RT, int KT, int EXTRA>
 struct KvWalk {
-    int64_t left;        // units from here to the CTA's end
+    int left;            // units from here to the CTA's end
     int per, request, head, rt;
     KvRequest r;
     int skip;
@@ -85,7 +85,7 @@ struct KvWalk {
     bool begins;         // it holds the row tile's first key tile
 
     __device__ __forceinline__ void start(const KvAttnArgs& a, const KvShare& s) {
-        left = s.units;
+        left = int(s.units);  // at most per
         per = s.per;
         request = s.request;
         head = s.head;
@@ -104,9 +104,9 @@ struct KvWalk {
         begins = before == 0;
         t0 += before;
         n -= before;
-        const int64_t room = left - max(EXTRA - skip, 0);
+        const int room = left - max(EXTRA - skip, 0);
         if (room < n) {
-            rest = n - max(int(room), 0);
+            rest = n - max(room, 0);
             n -= rest;
             if (n == 0) left = 0;  // the share ends ahead of the first key tile
         }
@@ -148,7 +148,7 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, 
     int* tiles = scratch;                       // row tiles of the window's requests ahead of i
     int* units = scratch + kShareWindow;        // key tiles of one head of request i
     int64_t* sums = reinterpret_cast<int64_t*>(scratch + 2 * kShareWindow);  // [W] and the answer
-    static_assert(W + 4 <= 64, "scratch of kv_share");
+    static_assert(W + 3 <= 64, "scratch of kv_share");
     // exclusive scan over the block; total receives the sum
     auto scan = [&](int64_t v, int64_t& total) {
         int64_t x = v;
