@@ -89,6 +89,23 @@ uint64_t kv_prompt_workspace_bytes(int head_dim, int sms);
 cudaError_t launch_kv_prompt(const KvAttnArgs& a, bool bf16, void* ws, int dev, cudaStream_t s);
 cudaError_t read_kv_prompt_status(int* status, bool clear, cudaStream_t s);
 
+// A launch that may begin while the grid before it ends: the kernel waits (griddepcontrol.wait)
+// for that grid's end before it touches memory that calls share.
+template <class... P, class... A>
+cudaError_t launch_early(void (*kern)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, const A&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(unsigned(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, P(args)...);
+}
+
 // ebx_gemm.cu: cuTensorMapEncodeTiled of the loaded driver (null without one).
 void* tensor_map_encoder();
 int gemm_sm_count(int dev);

@@ -106,6 +106,7 @@ __global__ void __launch_bounds__(kStepThreads, (StepCfg<D, NQ>::PER_SM))
         }
         fence_proxy_async_smem();
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // nothing of the call's inputs is read before
     const KvShare share = kv_share<kRows, KT, kStepExtra, kStepThreads>(a, least, reinterpret_cast<int*>(smem));
     fence_proxy_async_smem();  // the ring's copies may overwrite what kv_share kept there
     if (threadIdx.x == 0 && !a.whole) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -457,8 +458,7 @@ cudaError_t launch_step(KvAttnArgs a, int rows, void* ws, int dev, cudaStream_t 
     const int grid = gemm_sm_count(dev) * C::PER_SM;
     a.desc = static_cast<int4*>(ws);
     a.part = reinterpret_cast<float*>(a.desc + grid);
-    kern<<<grid, kStepThreads, C::kSmem, s>>>(mk, mv, a, kStepLeast);
-    cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch_early(kern, dim3(grid), kStepThreads, C::kSmem, s, mk, mv, a, kStepLeast);
     if (e != cudaSuccess) return e;
     return launch_join<D, C::ROWS, 4, BF16>(a, grid, std::min(rows, C::ROWS), s);
 }

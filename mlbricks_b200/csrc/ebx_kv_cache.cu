@@ -45,6 +45,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* warp_sums, int
 // Every CTA computes the sums for itself (a few loads per thread: cheaper than a second
 // launch or a grid barrier) and then writes its share of the tokens.
 __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
     extern __shared__ int32_t plan_smem[];
     int32_t* s_start = plan_smem;                 // [requests]: first token
     int32_t* s_before = s_start + a.requests;     // blocks taken ahead of it, -1: refused
@@ -197,6 +198,7 @@ __device__ __forceinline__ uint2 quant8(const uint4& x, float s, float r) {
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kAppendWarps * 32)
     kv_append_kernel(KvPool pool, KvRows k, KvRows v, const int64_t* slots, int64_t tokens, int span) {
+    asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
     constexpr int kLanes = D / 8;         // lanes that share a token, 8 values each
     constexpr int kPer = 32 / kLanes;     // tokens in a warp's load
     constexpr int kHold = 8;              // loads held in registers
@@ -335,6 +337,7 @@ template <int DT>
 __global__ void __launch_bounds__(kMatThreads)
     kv_materialize_kernel(KvPool pool, const int32_t* tables, int width, const int32_t* starts,
                           const int32_t* first, int requests, int64_t tokens, void* k, void* v) {
+    asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
     __shared__ int64_t s_slot[kMatTokens];
     const int64_t t0 = int64_t(blockIdx.x) * kMatTokens;
     if (threadIdx.x < kMatTokens) {
@@ -397,8 +400,7 @@ cudaError_t launch_kv_plan(const KvPlanArgs& a, cudaStream_t s) {
     }
     const int64_t work = std::max<int64_t>(a.tokens, a.requests);
     const int64_t grid = std::min<int64_t>((work + kPlanThreads - 1) / kPlanThreads, 592);
-    kv_plan_kernel<<<unsigned(std::max<int64_t>(grid, 1)), kPlanThreads, smem, s>>>(a);
-    return cudaGetLastError();
+    return launch_early(kv_plan_kernel, dim3(unsigned(std::max<int64_t>(grid, 1))), kPlanThreads, smem, s, a);
 }
 
 cudaError_t launch_kv_append(const KvPool& pool, const KvRows& k, const KvRows& v, const int64_t* slots,
@@ -410,15 +412,15 @@ cudaError_t launch_kv_append(const KvPool& pool, const KvRows& k, const KvRows& 
     const int64_t grid = (items + kAppendWarps - 1) / kAppendWarps;
     if (grid > INT32_MAX) return cudaErrorInvalidValue;
     const dim3 g{unsigned(grid), 2};
-#define EBX_KV_APPEND(DD, BB) \
-    kv_append_kernel<DD, BB><<<g, kAppendWarps * 32, 0, s>>>(pool, k, v, slots, tokens, span)
+#define EBX_KV_APPEND(DD)                                                                            \
+    bf16 ? launch_early(kv_append_kernel<DD, true>, g, kAppendWarps * 32, 0, s, pool, k, v, slots, tokens, span) \
+         : launch_early(kv_append_kernel<DD, false>, g, kAppendWarps * 32, 0, s, pool, k, v, slots, tokens, span)
     switch (pool.head_dim) {
-        case 32: bf16 ? EBX_KV_APPEND(32, true) : EBX_KV_APPEND(32, false); break;
-        case 64: bf16 ? EBX_KV_APPEND(64, true) : EBX_KV_APPEND(64, false); break;
-        default: bf16 ? EBX_KV_APPEND(128, true) : EBX_KV_APPEND(128, false); break;
+        case 32: return EBX_KV_APPEND(32);
+        case 64: return EBX_KV_APPEND(64);
+        default: return EBX_KV_APPEND(128);
     }
 #undef EBX_KV_APPEND
-    return cudaGetLastError();
 }
 
 cudaError_t launch_kv_materialize(const KvPool& pool, const int32_t* tables, int width,
@@ -429,8 +431,7 @@ cudaError_t launch_kv_materialize(const KvPool& pool, const int32_t* tables, int
     if (grid > INT32_MAX) return cudaErrorInvalidValue;
     auto kern = dtype == kKvF32 ? kv_materialize_kernel<kKvF32>
                 : dtype == kKvF16 ? kv_materialize_kernel<kKvF16> : kv_materialize_kernel<kKvBF16>;
-    kern<<<unsigned(grid), kMatThreads, 0, s>>>(pool, tables, width, starts, first, requests, tokens, k, v);
-    return cudaGetLastError();
+    return launch_early(kern, dim3(unsigned(grid)), kMatThreads, 0, s, pool, tables, width, starts, first, requests, tokens, k, v);
 }
 
 }  // namespace ebx

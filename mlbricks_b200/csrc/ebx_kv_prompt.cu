@@ -33,7 +33,7 @@ constexpr int kPromptKeys = 128;
 constexpr int kRowWarps = 16, kConvert = 16, kLoad = 20, kIssue = 21;  // first warps of the roles
 constexpr int kPromptThreads = 24 * 32;
 constexpr int kHalf = 128 * 128;   // bytes of 128 rows x 64 fp16
-constexpr int kPromptExtra = 3;    // a row tile's begin and end, in key tiles
+constexpr int kPromptExtra = 2;    // a row tile's begin and end, in key tiles
 constexpr int kRaw = 4;            // int8 tiles in flight
 constexpr int kBufs = 3;           // fp16 tiles: a value tile, the next key tile, and one being filled
 constexpr int kTabs = 4;           // scale tables of key tiles
@@ -200,25 +200,9 @@ __device__ __forceinline__ float largest(uint32_t s, const float4* tab, const Ro
     return fmaxf(top0, top1);
 }
 
-// 2^t of two values on the FMA units: t = n + f with n its nearest integer (added to 1.5 * 2^23, so
-// that the sum's low bits are n), a polynomial of degree 4 for 2^f on [-1/2, 1/2] (minimax in the
-// relative error, 2.6e-6, by Remez' exchange) and n added to the exponent field.  t < -126 gives
-// 2^-126, and so does a NaN.
-__device__ __forceinline__ uint64_t ex2_pair(uint64_t t) {
-    const uint64_t x = pack2f(fmaxf(lo2(t), -126.0f), fmaxf(hi2(t), -126.0f));
-    const uint64_t n = add2(x, pack2f(12582912.0f, 12582912.0f));
-    const uint64_t f = fma2(add2(n, pack2f(-12582912.0f, -12582912.0f)), pack2f(-1.0f, -1.0f), x);
-    uint64_t p = fma2(f, pack2f(0x1.3997d6p-7f, 0x1.3997d6p-7f), pack2f(0x1.ca1440p-5f, 0x1.ca1440p-5f));
-    p = fma2(p, f, pack2f(0x1.ec06dap-3f, 0x1.ec06dap-3f));
-    p = fma2(p, f, pack2f(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
-    p = fma2(p, f, pack2f(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
-    return uint64_t(uint32_t(p) + (uint32_t(n) << 23)) | uint64_t(uint32_t(p >> 32) + (uint32_t(n >> 32) << 23)) << 32;
-}
-
 // Weights 2^(t - mr) as fp16 pairs over the columns of S that were read, and their sum over vs.
-// Without a mask one pair in kPolyEvery goes to the FMA units: the exponential unit's 16 a clock
-// bound this loop.  (A NaN unit still shows through the other pairs.)
-constexpr int kPolyEvery = 4;
+// (A quarter of the exponentials as polynomials on the FMA units made this loop slower, 1103 ->
+// 1152 us for a chunk of 4096 tokens behind 12000: it is instructions that it lacks time for.)
 
 template <bool MASK>
 __device__ __forceinline__ float weigh(uint32_t s, const float4* tab, const Row& row, float mr, int key0) {
@@ -231,10 +215,9 @@ __device__ __forceinline__ float weigh(uint32_t s, const float4* tab, const Row&
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
             const uint64_t t2 = t_pair<MASK>(v, i, c2, b2, seen);
-            const uint64_t w = !MASK && (i / 2) % kPolyEvery == kPolyEvery - 1 ? ex2_pair(t2)
-                                                                              : pack2f(ex2(lo2(t2)), ex2(hi2(t2)));
-            w2 = add2(w2, w);
-            p[i / 2] = pack_half2(lo2(w), hi2(w));  // 11 bits, as the codes' operands need
+            const float w0 = ex2(lo2(t2)), w1 = ex2(hi2(t2));
+            w2 = add2(w2, pack2f(w0, w1));
+            p[i / 2] = pack_half2(w0, w1);  // 11 bits, as the codes' operands need
         }
         l = fmaf(lo2(w2) + hi2(w2), e.z, l);
         tmem_st8(s + at / 2, p);
@@ -296,6 +279,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // nothing of the call's inputs is read before
     const KvShare share = kv_share<kPromptRows, kPromptKeys, kPromptExtra, kPromptThreads>(a, least, reinterpret_cast<int*>(smem));
     fence_proxy_async_smem();  // copies will overwrite what kv_share kept there
     if (threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -704,8 +688,7 @@ cudaError_t launch_prompt(KvAttnArgs a, void* ws, int dev, cudaStream_t s) {
     const int grid = gemm_sm_count(dev);
     a.desc = static_cast<int4*>(ws);
     a.part = reinterpret_cast<float*>(a.desc + grid);
-    kern<<<grid, kPromptThreads, C::kSmem, s>>>(mk, mv, a, kPromptLeast);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch_early(kern, dim3(grid), kPromptThreads, C::kSmem, s, mk, mv, a, kPromptLeast);
     if (e != cudaSuccess) return e;
     return launch_join<D, kPromptRows, 4, BF16>(a, grid, kPromptRows, s);
 }

@@ -343,7 +343,7 @@ __device__ __forceinline__ uint32_t codes_to_half2(uint32_t w, uint32_t sel) {
 // WAYS parts at a time.
 template <int D, int RT, int WAYS, bool BF16>
 __global__ void __launch_bounds__(32 * WAYS) kv_join_kernel(const __grid_constant__ KvAttnArgs a) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
     constexpr int COLS = D / 32;  // float4 columns of a thread: groups of 8 apart
     __shared__ float2 s_ml[WAYS][8][4];
     __shared__ float4 s_o[COLS][WAYS][8][4];
@@ -438,16 +438,7 @@ inline bool code_map(CUtensorMap* map, const int8_t* codes, const KvPool& p, int
 template <int D, int RT, int WAYS, bool BF16>
 cudaError_t launch_join(const KvAttnArgs& a, int ctas, int rows, cudaStream_t s) {
     if (a.whole) return cudaSuccess;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(ctas), unsigned((rows + 3) / 4));
-    cfg.blockDim = dim3(32 * WAYS);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kv_join_kernel<D, RT, WAYS, BF16>, a);
+    return launch_early(kv_join_kernel<D, RT, WAYS, BF16>, dim3(unsigned(ctas), unsigned((rows + 3) / 4)), 32 * WAYS, 0, s, a);
 }
 
 // Reads (and clears) a translation unit's status word; synchronizes `s`.
