@@ -243,4 +243,62 @@ def attention(q: torch.Tensor, pool: KVPool, tables: torch.Tensor, lengths: torc
     return out if lse is None else (out, lse)
 
 
-__all__ = ["BLOCK_SIZES", "HEAD_DIMS", "KVPlan", "KVPool", "append", "attention", "materialize", "plan"]
+class KVCache:
+    """Pools, block table and free ring of a model with ``layers`` layers, for up to ``requests``
+    requests of up to ``max_length`` tokens at a time.
+
+    A step is ``plan(new)`` and then, layer by layer, ``append`` and ``attention``; ``new[i]`` is the
+    number of tokens that request i brings (0: it rests, -1: it is done and gives its blocks back).
+    The state stays in the same tensors, so a step with fixed sizes can be captured in a CUDA graph
+    and replayed.  One stream at a time; more than one needs the caller's events."""
+
+    def __init__(self, layers: int, blocks: int, kv_heads: int, head_dim: int, *, requests: int, max_length: int,
+                 block_size: int = 64, device="cuda") -> None:
+        _check(layers > 0 and requests > 0 and max_length > 0, "layers, requests and max_length must be positive")
+        self.pools = [KVPool.empty(blocks, kv_heads, block_size, head_dim, device) for _ in range(layers)]
+        self.block_size, self.max_length = block_size, max_length
+        where = self.pools[0].k_codes.device
+        self.tables = torch.full((requests, -(-max_length // block_size)), -1, dtype=torch.int32, device=where)
+        self.lengths = torch.zeros(requests, dtype=torch.int32, device=where)
+        self.free = torch.arange(blocks, dtype=torch.int32, device=where)
+        self.ring = torch.tensor([0, blocks, 0, 0], dtype=torch.int64, device=where)
+        self.step: KVPlan | None = None
+        self._max_new = 0
+
+    def plan(self, new, tokens: int | None = None, max_new: int | None = None) -> KVPlan:
+        """Blocks and slots for a step.  ``new``: a list, or an int32 tensor on the GPU with
+        ``tokens`` (room for all its tokens) and, if known, ``max_new``.  ``ring[2]`` of the result is
+        the number of blocks that were missing: requests that got none keep their length."""
+        if not isinstance(new, torch.Tensor):
+            counts = [max(int(n), 0) for n in new]
+            tokens, max_new = sum(counts), max(counts, default=0)
+            new = torch.tensor([int(n) for n in new], dtype=torch.int32).to(self.lengths.device, non_blocking=True)
+        _check(tokens is not None, "a tensor of new tokens needs `tokens`")
+        self.step = plan(self.lengths, new, self.tables, self.free, self.ring, block_size=self.block_size, tokens=tokens)
+        self.lengths.copy_(self.step.lengths)
+        self.ring.copy_(self.step.ring)
+        self._max_new = max_new or 0
+        return self.step
+
+    def _planned(self) -> KVPlan:
+        if self.step is None:
+            raise RuntimeError("KVCache: plan a step first")
+        return self.step
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        """The step's keys and values [tokens, kv_heads, head_dim] into the layer's pool."""
+        append(k, v, self.pools[layer], self._planned().slots)
+
+    def attention(self, layer: int, q: torch.Tensor, **options):
+        """The step's queries [tokens, heads, head_dim] over the layer's cache (``attention``'s options)."""
+        step = self._planned()
+        return attention(q, self.pools[layer], self.tables, step.lengths, step.starts, max_new=self._max_new,
+                         max_length=self.max_length, **options)
+
+    def materialize(self, layer: int, starts: torch.Tensor, *, tokens: int, first: torch.Tensor | None = None,
+                    dtype: torch.dtype = torch.float16) -> tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values that the layer holds (``materialize``'s arguments)."""
+        return materialize(self.pools[layer], self.tables, starts, first=first, tokens=tokens, dtype=dtype)
+
+
+__all__ = ["BLOCK_SIZES", "HEAD_DIMS", "KVCache", "KVPlan", "KVPool", "append", "attention", "materialize", "plan"]
