@@ -234,6 +234,16 @@ __device__ __forceinline__ bool pair_any(int id, bool mine) {
     return any != 0;
 }
 
+// The segment's key tiles [j0, j1), at least one, counted from its first, that rows of row tile x
+// see: the rows of the other tile may begin earlier or end later.
+using PromptWalk = KvWalk<kPromptRows, kPromptKeys, kPromptExtra>;
+__device__ __forceinline__ void tiles_seen(const KvAttnArgs& a, const PromptWalk& w, int x, int& j0, int& j1) {
+    int t0, n;
+    kv_key_tiles<128, kPromptKeys>(a, w.r, 2 * w.rt + x, t0, n);
+    j0 = min(max(t0 - w.t0, 0), w.n - 1);
+    j1 = max(min(t0 + n - w.t0, w.n), j0 + 1);
+}
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kPromptThreads, 1)
     kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -288,7 +298,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     __syncthreads();
     after_sync();
     const uint32_t tmem = *tmem_slot;
-    KvWalk<kPromptRows, kPromptKeys, kPromptExtra> walk;
+    PromptWalk walk;
     walk.start(a, share);
 
     if (warp < kRowWarps) {
@@ -322,29 +332,24 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 continue;
             }
             const int row0 = walk.rt * kPromptRows + x * 128 + quarter * 32;  // the warps' first row
-            auto row_at = [&](int i, int64_t token_stride, int64_t head_stride) {  // its row i's offset; -1: past the last
-                const int ri = row0 + i;
-                if (ri >= walk.r.rows) return int64_t(-1);
-                const int t = by_group(a, ri);
-                return (walk.r.token0 + t) * token_stride + (walk.head * a.group + ri - t * a.group) * head_stride;
-            };
+            // this lane's row; past the last one: the last, whose result is not kept
+            const bool live = row0 + lane < walk.r.rows;
+            const int token = by_group(a, min(row0 + lane, walk.r.rows - 1));
+            const int head = walk.head * a.group + min(row0 + lane, walk.r.rows - 1) - token * a.group;
             Row row;
             row.unit = 1.0f;
             row.mr = -INFINITY;
             row.l = 0.0f;
-            const bool live = row0 + lane < walk.r.rows;
+            const int place = walk.r.begin + token;
+            row.hi = !live ? INT_MAX : a.causal ? min(place + 1, walk.r.length) : walk.r.length;
+            row.lo = !live ? 0 : max(walk.r.first, a.window > 0 ? place - a.window + 1 : 0);
             {
-                const int place = walk.r.begin + by_group(a, live ? row0 + lane : 0);
-                row.hi = !live ? INT_MAX : a.causal ? min(place + 1, walk.r.length) : walk.r.length;
-                row.lo = !live ? 0 : max(walk.r.first, a.window > 0 ? place - a.window + 1 : 0);
-            }
-            {
+                const int64_t off = (walk.r.token0 + token) * a.q.token_stride + head * a.q.head_stride;
                 uint4 v[PER / 2];  // each of the two warps brings every other load's rows
 #pragma unroll
-                for (int i = 0; i < PER / 2; ++i) {
-                    const int64_t off = row_at((2 * i + half) * ROWS + mine, a.q.token_stride, a.q.head_stride);
-                    v[i] = off >= 0 ? __ldg(reinterpret_cast<const uint4*>(a.q.p + off) + chunk) : make_uint4(0, 0, 0, 0);
-                }
+                for (int i = 0; i < PER / 2; ++i)
+                    v[i] = __ldg(reinterpret_cast<const uint4*>(
+                                     a.q.p + __shfl_sync(0xffffffffu, off, (2 * i + half) * ROWS + mine)) + chunk);
 #pragma unroll
                 for (int i = 0; i < PER / 2; ++i) {
                     const int ri = (2 * i + half) * ROWS + mine;
@@ -376,10 +381,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
             // keys that every row of the warp sees
             const int all_lo = __reduce_max_sync(0xffffffffu, row.lo), all_hi = __reduce_min_sync(0xffffffffu, row.hi);
-            for (int j = 0; j < walk.n; ++j, ++g, ++gj) {
+            int j0, j1;
+            tiles_seen(a, walk, x, j0, j1);
+            for (int j = j0; j < j1; ++j, ++g) {
+                const int at = gj + j;
                 wait(s_full + x, g);
-                wait(tab_full + gj % kTabs, gj / kTabs);
-                const float4* tab = tabs + (gj % kTabs) * 8 + half * 4;
+                wait(tab_full + at % kTabs, at / kTabs);
+                const float4* tab = tabs + (at % kTabs) * 8 + half * 4;
                 const int key0 = (walk.t0 + j) * kPromptKeys + half * 64;
                 const bool mask = key0 < all_lo || key0 + 64 > all_hi;
                 const float mr = row.mr == -INFINITY ? 0.0f : row.mr;
@@ -394,7 +402,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     const float f = up ? ex2(row.mr - next) : 1.0f;
                     row.mr = next;
                     row.l *= f;
-                    if (j > 0) {
+                    if (j > j0) {
                         wait(o_done + x, g - 1);
 #pragma unroll 1
                         for (int c = 0; c < D / 2; c += 16) {
@@ -415,12 +423,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(p_full + x));
             }
+            gj += walk.n;
             // the sums of both halves, and O
             *tell = row.l;
             pair_sync(pair);
             const float l = half ? *other + row.l : row.l + *other;
             wait(o_done + x, g - 1);
             const bool whole = walk.whole();
+            const int64_t at_row = int64_t(walk.r.token0 + token) * a.heads + head;
             const int slot = walk.begins ? 1 : 0;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             float4* part = whole ? nullptr
@@ -453,16 +463,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             before_sync();
             pair_sync(pair);
             if (whole) {
-#pragma unroll 1
+#pragma unroll
                 for (int i = 0; i < PER / 2; ++i) {
                     const int ri = (2 * i + half) * ROWS + mine;
-                    const int64_t off = row_at(ri, int64_t(a.heads) * D, D);
-                    if (off >= 0) *(reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + off) + chunk) = *stage_at(ri);
+                    const int64_t to = __shfl_sync(0xffffffffu, at_row, ri);
+                    if (row0 + ri < walk.r.rows) *(reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + to * D) + chunk) = *stage_at(ri);
                 }
                 pair_sync(pair);  // the staged rows are free again
             }
             if (half == 0 && live && whole && a.lse)
-                a.lse[row_at(lane, a.heads, 1)] = l == 0.0f ? -INFINITY : (row.mr + lg2(l)) * 0.6931471805599453f;
+                a.lse[at_row] = l == 0.0f ? -INFINITY : (row.mr + lg2(l)) * 0.6931471805599453f;
             if (half == 0 && !whole)
                 kv_part_ml<D, kPromptRows>(a, blockIdx.x, slot)[x * 128 + quarter * 32 + lane] = make_float2(row.mr, l);
             if (walk.begins && !whole && threadIdx.x == 0)
@@ -560,35 +570,40 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             };
             for (; !walk.done() && ok; walk.next(a)) {
                 const bool two = walk.r.rows - walk.rt * kPromptRows > 128;
-                ok = wait(buf_full + it % kBufs, it / kBufs) && wait(q_full, seg);
-                ++seg;
+                int from[2], to[2];  // the segment's key tiles that either row tile sees
+                tiles_seen(a, walk, 0, from[0], to[0]);
+                tiles_seen(a, walk, 1, from[1], to[1]);
+                if (!two) from[1] = to[1] = 0;
+                // S of every row tile that begins at key tile j (counted from the segment's first)
+                auto step = [&](int x, int j, int buf, int phase) {
+                    if (j < from[x] || j >= to[x]) return true;
+                    if (!wait(buf_full + buf, phase)) return false;
+                    if (j == from[x] && !(x == 0 ? wait(q_full, seg++) : wait(q_full + 1, segb++))) return false;
+                    scores(x, buf);
+                    return true;
+                };
+                // every buffer is waited for, used or not, so that its phases are never overrun
+                ok = wait(buf_full + it % kBufs, it / kBufs) && step(0, 0, it % kBufs, it / kBufs) && step(1, 0, it % kBufs, it / kBufs);
                 if (!ok) break;
-                scores(0, it % kBufs);
-                if (two) {
-                    if (!(ok = wait(q_full + 1, segb))) break;
-                    ++segb;
-                    scores(1, it % kBufs);
-                }
                 release(it % kBufs);
                 ++it;
                 for (int j = 0; j < walk.n; ++j) {
                     const int vb = it % kBufs, kb = (it + 1) % kBufs;
                     const bool more = j + 1 < walk.n;
-                    if (!(ok = wait(buf_full + vb, it / kBufs) && wait(p_full, g[0]))) break;
-                    ++g[0];
-                    values(0, vb, j == 0);
-                    if (more) {
-                        if (!(ok = wait(buf_full + kb, (it + 1) / kBufs))) break;
-                        scores(0, kb);  // after the product above, which reads the same columns
+                    if (!(ok = wait(buf_full + vb, it / kBufs))) break;
+                    for (int x = 0; x < 2 && ok; ++x) {
+                        if (j >= from[x] && j < to[x]) {
+                            if (!(ok = wait(p_full + x, g[x]))) break;
+                            ++g[x];
+                            values(x, vb, j == from[x]);
+                        }
+                        // after the product above, which reads the same columns
+                        if (more) ok = step(x, j + 1, kb, (it + 1) / kBufs);
                     }
-                    if (two) {
-                        if (!(ok = wait(p_full + 1, g[1]))) break;
-                        ++g[1];
-                        values(1, vb, j == 0);
-                    }
+                    if (!ok) break;
                     release(vb);
                     if (more) {
-                        if (two) scores(1, kb);
+                        if (!(ok = wait(buf_full + kb, (it + 1) / kBufs))) break;
                         release(kb);
                     }
                     it += more ? 2 : 1;
