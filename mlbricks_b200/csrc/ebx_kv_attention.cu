@@ -34,7 +34,7 @@ constexpr int kConsumers = 4;    // warps that compute; one more loads
 constexpr int kStepThreads = 32 * (kConsumers + 1);
 constexpr int kStages = 3;
 constexpr int kStepLeast = 4;   // units a CTA takes at least: a partial result costs about as much
-constexpr int kStepExtra = 1;   // a row tile's begin and end, in key tiles
+constexpr int kStepExtra = 2;   // a row tile's begin and end, in key tiles (64 requests: 0 / 1 / 2: 112 / 109 / 106 us)
 
 // D: head_dim; NQ: blocks of 8 rows (queries) in a row tile, the N of mma.m16n8k16, whose M is 16
 // keys of the first product and 16 dimensions of the second.
@@ -467,10 +467,14 @@ cudaError_t launch_step(KvAttnArgs a, int rows, void* ws, int dev, cudaStream_t 
 
 namespace {
 
-// Row tiles of 256 rows on tcgen05 from kPromptMin rows of a request on; below, tiles of 8 or 16.
-constexpr int kPromptMin = 33;
+// From kPromptMin rows of a request and head on, row tiles of 256 rows on tcgen05; below, tiles of 8
+// or 16.  Measured with the rule at 17 and at 65 rows (step / prompt kernel): 16 requests of 4000
+// tokens, 8 heads of 128, 32 rows 66 / 95 us, 48 rows 94 / 96, 64 rows 119 / 97; 64 requests of 2000
+// tokens, 2 heads of 64, 48 rows 39 / 54, 64 rows 47 / 54; one request of 16000, 48 rows 31 / 41.
+constexpr int kPromptMin = 49;
 
-// Short requests: a second launch, to join, would cost more than sharing row tiles gains.
+// Short requests: a second launch, to join, would cost more than sharing row tiles gains (8
+// requests of 600 tokens over one head of 32: 17.1 us in place of 20.5).
 bool takes_whole(int head_dim, int max_length) {
     constexpr int kTiles = 4;
     return max_length > 0 && max_length <= kTiles * (8192 / head_dim);

@@ -338,8 +338,8 @@ __device__ __forceinline__ uint32_t codes_to_half2(uint32_t w, uint32_t sel) {
     return hsub2_u(__byte_perm(w, 0x64646464u, sel), 0x64806480u);  // - 1152
 }
 
-// Row tiles that several CTAs worked on: CTA (c, y) joins rows 4 y .. 4 y + 3 of the one that begins
-// in CTA c, c's part 1 and then part 0 of the CTAs behind it.  Threads: 4 rows x 8 column groups x
+// Row tiles that several CTAs worked on: CTA (c, y) joins rows 4 y .. 4 y + 3 (and so on, gridDim.y
+// fours at a time: the grid goes by what the caller says of the rows) of the one that begins in CTA c, c's part 1 and then part 0 of the CTAs behind it.  Threads: 4 rows x 8 column groups x
 // WAYS parts at a time.
 template <int D, int RT, int WAYS, bool BF16>
 __global__ void __launch_bounds__(32 * WAYS) kv_join_kernel(const __grid_constant__ KvAttnArgs a) {
@@ -350,10 +350,10 @@ __global__ void __launch_bounds__(32 * WAYS) kv_join_kernel(const __grid_constan
     const int c = blockIdx.x;
     const int4 d = a.desc[c];
     const int rows = d.w & 0xffff, last = c + (d.w >> 16);
-    if (d.x == 0 || int(blockIdx.y) * 4 >= rows) return;
+    if (d.x == 0) return;
     const int ri = threadIdx.x & 3, col = (threadIdx.x >> 2) & 7, way = threadIdx.x >> 5;
-    {
-        const int r = blockIdx.y * 4 + ri;
+    for (int r0 = blockIdx.y * 4; r0 < rows; r0 += gridDim.y * 4) {
+        const int r = r0 + ri;
         float m = -INFINITY, l = 0.0f;
         float4 o[COLS];
 #pragma unroll
@@ -415,6 +415,7 @@ __global__ void __launch_bounds__(32 * WAYS) kv_join_kernel(const __grid_constan
             }
             if (a.lse && col == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + lg2(l)) * 0.6931471805599453f;
         }
+        __syncthreads();
     }
 }
 

@@ -184,6 +184,12 @@ def test_hints_change_nothing(new):
         assert (out.float() - outs[0][0].float()).abs().max() <= 2.0**-8 * outs[0][0].float().abs().max()
 
 
+@pytest.mark.parametrize("new", [2, 3, 9])
+def test_a_hint_that_is_too_small_leaves_no_row_out(new):
+    run_attention([20011, 3000], [new, new], heads=2, group=4, dim=128, block=64, max_new=1)
+    run_attention([20011, 3000], [new, new], heads=1, group=5, dim=32, block=16, max_new=1, max_length=9)
+
+
 @pytest.mark.parametrize("requests", [1, 300])
 def test_long_requests_are_split_and_joined(requests):
     lengths = [20011] if requests == 1 else [1 + (37 * i) % 900 for i in range(requests)]
