@@ -19,6 +19,7 @@ mlbricks/cache.py, are whole 16-bit tensors).
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import NamedTuple
 
@@ -47,9 +48,16 @@ def _check(cond: bool, msg: str) -> None:
         raise ValueError(msg)
 
 
-def _check_int(t: torch.Tensor, dtype: torch.dtype, device: int, name: str) -> None:
-    if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor on cuda:{device}")
+# These calls are made every step and every layer, so what can be wrong is looked for in one
+# expression, and told apart only when something is.
+def _int_ok(t: torch.Tensor, dtype: torch.dtype, device: int) -> bool:
+    return t.dtype is dtype and t.get_device() == device and t.is_contiguous()
+
+
+def _refuse_ints(device: int, **tensors) -> None:
+    for name, (t, dtype) in tensors.items():
+        if t is not None and not _int_ok(t, dtype, device):
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor on cuda:{device}")
 
 
 class KVPool:
@@ -61,14 +69,12 @@ class KVPool:
     def __init__(self, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
                  v_scales: torch.Tensor) -> None:
         shape, device = k_codes.shape, k_codes.get_device()
-        if device < 0 or len(shape) != 4:
-            raise ValueError("codes must be CUDA tensors [blocks, kv_heads, block_size, head_dim]")
-        for t, dtype, name in ((k_codes, torch.int8, "k_codes"), (v_codes, torch.int8, "v_codes"),
-                               (k_scales, torch.float32, "k_scales"), (v_scales, torch.float32, "v_scales")):
-            if (t.dtype is not dtype or t.get_device() != device or not t.is_contiguous()
-                    or t.shape != (shape if dtype is torch.int8 else shape[:2])):
-                raise ValueError(f"{name} must be a contiguous {dtype} tensor "
-                                 f"{tuple(shape if dtype is torch.int8 else shape[:2])} on cuda:{device}")
+        scales = shape[:2]
+        if not (len(shape) == 4 and device >= 0 and v_codes.shape == shape and k_scales.shape == scales
+                and v_scales.shape == scales and _int_ok(k_codes, torch.int8, device)
+                and _int_ok(v_codes, torch.int8, device) and _int_ok(k_scales, torch.float32, device)
+                and _int_ok(v_scales, torch.float32, device)):
+            self._refuse(k_codes, k_scales, v_codes, v_scales)
         blocks, kv_heads, block_size, head_dim = shape
         if block_size not in BLOCK_SIZES:
             raise ValueError(f"block_size must be one of {BLOCK_SIZES}, got {block_size}")
@@ -81,6 +87,17 @@ class KVPool:
         self._c = _ebx.KVPool(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
                               blocks, kv_heads, block_size, head_dim, device, 0)
         self._ref = ctypes.byref(self._c)
+
+    @staticmethod
+    def _refuse(k_codes, k_scales, v_codes, v_scales) -> None:
+        shape, device = k_codes.shape, k_codes.get_device()
+        if len(shape) != 4 or device < 0:
+            raise ValueError("codes must be CUDA tensors [blocks, kv_heads, block_size, head_dim]")
+        for name, t, dtype, want in (("k_codes", k_codes, torch.int8, shape), ("v_codes", v_codes, torch.int8, shape),
+                                     ("k_scales", k_scales, torch.float32, shape[:2]),
+                                     ("v_scales", v_scales, torch.float32, shape[:2])):
+            if t.shape != want or not _int_ok(t, dtype, device):
+                raise ValueError(f"{name} must be a contiguous {dtype} tensor {tuple(want)} on cuda:{device}")
 
     @classmethod
     def empty(cls, blocks: int, kv_heads: int, block_size: int, head_dim: int, device="cuda") -> "KVPool":
@@ -108,7 +125,17 @@ class KVPool:
 
 
 def _stream(device: int) -> int:
-    return _ebx.stream_ptr(device=device)
+    return _RAW_STREAM(device) if _RAW_STREAM is not None else _ebx.stream_ptr(device=device)
+
+
+_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(device: int, kv_heads: int, head_dim: int, heads: int, tokens: int, max_new: int,
+                     max_length: int) -> int:
+    pool = _ebx.KVPool(16, 16, 16, 16, 1, kv_heads, BLOCK_SIZES[0], head_dim, device, 0)  # only its sizes count
+    return int(_ebx.load().ebx_kv_attention_workspace_bytes(ctypes.byref(pool), heads, tokens, max_new, max_length))
 
 
 def plan(past: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, free: torch.Tensor, ring: torch.Tensor, *,
@@ -126,18 +153,19 @@ def plan(past: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, free: torc
     The inputs ``past`` and ``ring`` are not changed; the next step takes the result's ``lengths``
     and ``ring`` in their place."""
     device = past.get_device()
-    if not past.is_cuda:
+    if device < 0:
         raise ValueError("plan needs CUDA tensors")
-    requests = past.numel()
-    _check_int(past, torch.int32, device, "past")
-    _check_int(new, torch.int32, device, "new")
-    _check_int(tables, torch.int32, device, "tables")
-    _check_int(free, torch.int32, device, "free")
-    _check_int(ring, torch.int64, device, "ring")
-    _check(new.numel() == requests and tables.dim() == 2 and tables.shape[0] == requests,
-           "past, new and the rows of tables must be as many")
-    _check(ring.numel() >= 2 and tokens >= 0, "ring holds at least its front and back, and tokens >= 0")
-    _check(block_size in BLOCK_SIZES, f"block_size must be one of {BLOCK_SIZES}, got {block_size}")
+    int32, requests = torch.int32, past.numel()
+    if not (_int_ok(past, int32, device) and _int_ok(new, int32, device) and _int_ok(tables, int32, device)
+            and _int_ok(free, int32, device) and _int_ok(ring, torch.int64, device)):
+        _refuse_ints(device, past=(past, int32), new=(new, int32), tables=(tables, int32), free=(free, int32),
+                     ring=(ring, torch.int64))
+    if new.numel() != requests or tables.dim() != 2 or tables.shape[0] != requests:
+        raise ValueError("past, new and the rows of tables must be as many")
+    if ring.numel() < 2 or tokens < 0:
+        raise ValueError("ring holds at least its front and back, and tokens >= 0")
+    if block_size not in BLOCK_SIZES:
+        raise ValueError(f"block_size must be one of {BLOCK_SIZES}, got {block_size}")
     # new_empty: the cheapest way to a tensor, and this call is made every step
     lengths, starts, positions = past.new_empty(requests), past.new_empty(requests + 1), past.new_empty(tokens)
     slots, out = ring.new_empty(tokens), ring.new_empty(4)
@@ -161,7 +189,8 @@ def append(k: torch.Tensor, v: torch.Tensor, pool: KVPool, slots: torch.Tensor) 
     tokens = k.shape[0]
     if v.shape[0] != tokens or v.dtype is not k.dtype:
         raise ValueError("k and v must have the same tokens and dtype")
-    _check_int(slots, torch.int64, pool.device, "slots")
+    if not _int_ok(slots, torch.int64, pool.device):
+        _refuse_ints(pool.device, slots=(slots, torch.int64))
     if slots.numel() != tokens:
         raise ValueError("slots must have one entry for each token")
     if tokens == 0:
@@ -180,18 +209,19 @@ def materialize(pool: KVPool, tables: torch.Tensor, starts: torch.Tensor, *, fir
     if dtype not in _DTYPES:
         raise ValueError("dtype must be float32, float16 or bfloat16")
     requests = starts.numel() - 1
-    _check_int(starts, torch.int32, pool.device, "starts")
-    _check_int(tables, torch.int32, pool.device, "tables")
-    _check(requests >= 0 and tables.dim() == 2 and tables.shape[0] == requests and tokens >= 0,
-           "tables must have a row, and starts an entry, for each request (and one more); tokens >= 0")
-    if first is not None:
-        _check_int(first, torch.int32, pool.device, "first")
-        _check(first.numel() == requests, "first must have one entry for each request")
+    int32, device = torch.int32, pool.device
+    if not (_int_ok(starts, int32, device) and _int_ok(tables, int32, device)
+            and (first is None or _int_ok(first, int32, device))):
+        _refuse_ints(device, starts=(starts, int32), tables=(tables, int32), first=(first, int32))
+    if requests < 0 or tables.dim() != 2 or tables.shape[0] != requests or tokens < 0:
+        raise ValueError("tables must have a row, and starts an entry, for each request (and one more); tokens >= 0")
+    if first is not None and first.numel() != requests:
+        raise ValueError("first must have one entry for each request")
     shape = (tokens, pool._c.kv_heads, pool._c.head_dim)
     k, v = starts.new_empty(shape, dtype=dtype), starts.new_empty(shape, dtype=dtype)
     st = _ebx.load().ebx_kv_materialize(
         pool._ref, tables.data_ptr(), tables.shape[1], starts.data_ptr(), None if first is None else first.data_ptr(),
-        requests, tokens, _DTYPES[dtype], k.data_ptr(), v.data_ptr(), _stream(pool.device))
+        requests, tokens, _DTYPES[dtype], k.data_ptr(), v.data_ptr(), _stream(device))
     if st:
         _ebx.check(st)
     return k, v
@@ -213,16 +243,16 @@ def attention(q: torch.Tensor, pool: KVPool, tables: torch.Tensor, lengths: torc
     device = pool.device
     tokens, heads, dim = q.shape
     requests = lengths.numel()
-    _check_int(tables, torch.int32, device, "tables")
-    _check_int(lengths, torch.int32, device, "lengths")
-    _check_int(starts, torch.int32, device, "starts")
+    int32 = torch.int32
+    if not (_int_ok(tables, int32, device) and _int_ok(lengths, int32, device) and _int_ok(starts, int32, device)
+            and (first is None or _int_ok(first, int32, device))):
+        _refuse_ints(device, tables=(tables, int32), lengths=(lengths, int32), starts=(starts, int32), first=(first, int32))
     if heads == 0 or heads % pool._c.kv_heads:
         raise ValueError(f"heads ({heads}) must be a multiple of kv_heads ({pool._c.kv_heads})")
     if starts.numel() != requests + 1 or tables.dim() != 2 or tables.shape[0] != requests:
         raise ValueError("lengths and the rows of tables must be as many, and starts one more")
-    if first is not None:
-        _check_int(first, torch.int32, device, "first")
-        _check(first.numel() == requests, "first must have one entry for each request")
+    if first is not None and first.numel() != requests:
+        raise ValueError("first must have one entry for each request")
     if out is None:
         out = q.new_empty((tokens, heads, dim))
     elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != device or not out.is_contiguous():
@@ -230,7 +260,7 @@ def attention(q: torch.Tensor, pool: KVPool, tables: torch.Tensor, lengths: torc
     lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
     if tokens and requests:
         lib = _ebx.load()
-        nbytes = lib.ebx_kv_attention_workspace_bytes(pool._ref, heads, tokens, max_new, max_length)
+        nbytes = _workspace_bytes(device, pool._c.kv_heads, dim, heads, tokens, max_new, max_length)
         ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         st = lib.ebx_kv_attention(
             pool._ref, q.data_ptr(), q.stride(0), q.stride(1), heads, _ROW_DTYPES[q.dtype], tables.data_ptr(),
