@@ -43,7 +43,9 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* warp_sums, int
 // its blocks go behind the ring's tail.  A new block always begins with a new token, so the
 // threads that write the tokens' slots also write the table.
 // Every CTA computes the sums for itself (a few loads per thread: cheaper than a second
-// launch or a grid barrier) and then writes its share of the tokens.
+// launch or a grid barrier) and then writes its share of the tokens.  What bounds it is latency: the
+// lengths, the sums, a token's binary search, its block (64 requests of one token 7 us, 1000 requests
+// with 120 thousand tokens 12 us, from cold caches; the 1.5 MB alone would take 0.2 us).
 __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
     asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
     extern __shared__ int32_t plan_smem[];
@@ -195,6 +197,11 @@ __device__ __forceinline__ uint2 quant8(const uint4& x, float s, float r) {
 // s_old = the block's scale if the run does not begin the block (its earlier tokens then keep
 // their codes, or are moved to the larger scale: rint(code * s_old / s)), else 0.  A value that
 // is not finite makes the scale NaN, so that whatever reads the block shows it.
+// Runs, not blocks, are the unit because the slots alone then say everything: no atomics, no second
+// pass over other warps' tokens.  A run's values stay in registers between the largest and the codes
+// (up to 16 tokens at head_dim 128; longer ones are read again from L2).  What bounds it: 27 424
+// tokens of 8 heads of 128 in bf16 take 42 us = 4.0 TB/s of 168 MB, the integer pipe half busy and
+// the issue slots 62 %; with a division for each value it was 78 us.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kAppendWarps * 32)
     kv_append_kernel(KvPool pool, KvRows k, KvRows v, const int64_t* slots, int64_t tokens, int span) {
@@ -337,6 +344,8 @@ __device__ __forceinline__ void store8(void* out, int64_t at, uint32_t lo, uint3
 
 // out[t, h, :] = code * scale, rounded once: token t is place first[i] + t - starts[i] of the
 // request i that it falls into.  Tokens that no request has, or whose place has no block, are 0.
+// One pass: 499 MB in 86 us = 5.8 TB/s, 0.89 of a copy's rate.  One item a thread at a time: two or
+// four unrolled, or smaller and larger CTAs, were 2 to 14 % slower.
 template <int DT>
 __global__ void __launch_bounds__(kMatThreads)
     kv_materialize_kernel(KvPool pool, const int32_t* tables, int width, const int32_t* starts,

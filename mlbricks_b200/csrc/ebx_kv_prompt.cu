@@ -14,8 +14,13 @@
 //     passes over S in tensor memory: the largest t; the weights and their sum.  O is rescaled (in
 //     tensor memory) only when t grew by more than the lag.
 // What bounds it: the chain S -> weights -> O of a row tile, of which the products of the other row
-// tile cover only a part.  Two threads a row halve the weights' part of it (one thread a row: 570 +
-// 1500 clocks for 128 keys, where the exponential unit alone would take 1000).
+// tile cover only a part, and the issue slots when both compute weights.  A key tile takes some 5000
+// clocks for both row tiles: the products 2500 of them (8 of 128 x 128 x 16 take 670 from shared
+// memory, 600 with the weights in tensor memory), the largest and the weights 2700, the way from one
+// to the other the rest.  4096 tokens behind 12000, 32 heads over 8 of 128: 1.12 ms, 841 TFLOP/s.
+// Measured and not kept, for that case: one thread a row 1274 us; the row in registers (one read of
+// S) 1299; S of 64 keys twice over, so that the weights never wait for it, 1277 (a product of 64
+// columns takes as long as one of 128).
 // Every mbarrier wait is bounded; a timeout sets the device status word, after which the row warps
 // wait no more but still meet each other's barriers, and the other roles leave.
 #include <algorithm>
