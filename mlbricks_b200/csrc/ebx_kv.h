@@ -57,6 +57,7 @@ struct KvAttnArgs {
     int requests, width, heads, group;
     int causal, window;
     int whole;             // row tiles are not shared among CTAs
+    int least_rows, most_rows;  // the launch takes requests with that many rows (tokens * group)
     float scale_log2;      // softmax scale * log2(e)
     uint32_t group_mul, group_shift;  // n / group = n * group_mul >> group_shift
     // partial results of row tiles that several CTAs share

@@ -495,6 +495,15 @@ int64_t most_rows(int group, int64_t tokens, int max_new) {
     return (max_new > 0 ? std::min<int64_t>(max_new, tokens) : tokens) * group;
 }
 
+// A prompt or two among decode steps: if the other requests bring fewer than kPromptMin / 2 rows on
+// average, both kernels run, each for its own requests: a decode row streams at a third of its rate
+// in the prompt kernel.  Measured, both / the prompt kernel alone, 32 heads over 8 of 128: 63 requests
+// of 4000 tokens and a prompt of 2048 188 / 383 us, of 256 141 / 310; 200 of 500 and one of 300 101 / 189.
+bool takes_both(int group, int requests, int64_t tokens, int max_new) {
+    return requests > 1 && max_new > 0 && tokens > max_new && int64_t(max_new) * group >= kPromptMin &&
+           (tokens - max_new) * group * 2 < int64_t(requests - 1) * kPromptMin;
+}
+
 }  // namespace
 
 uint64_t kv_attention_workspace_bytes(int head_dim, int group, int64_t tokens, int max_new, int max_length) {
@@ -502,7 +511,7 @@ uint64_t kv_attention_workspace_bytes(int head_dim, int group, int64_t tokens, i
     if (cudaGetDevice(&dev) != cudaSuccess) return 0;
     const int sms = gemm_sm_count(dev);
     const int64_t most = most_rows(group, tokens, max_new);
-    if (most >= kPromptMin) return kv_prompt_workspace_bytes(head_dim, sms);
+    if (most >= kPromptMin) return kv_prompt_workspace_bytes(head_dim, sms);  // more than the step kernel's
     if (takes_whole(head_dim, max_length)) return 0;
     const int nq = most <= 8 ? 1 : 2, ctas = sms * (nq == 1 ? StepCfg<32, 1>::PER_SM : StepCfg<32, 2>::PER_SM);
     return uint64_t(round_up(int64_t(ctas) * int64_t(sizeof(int4) + 2 * 8 * nq * (head_dim + 2) * sizeof(float)), 256));
@@ -511,15 +520,26 @@ uint64_t kv_attention_workspace_bytes(int head_dim, int group, int64_t tokens, i
 cudaError_t launch_kv_attention(KvAttnArgs a, bool bf16, int max_new, int max_length, void* ws, cudaStream_t s) {
     if (a.tokens <= 0 || a.requests <= 0) return cudaSuccess;
     int dev = 0;
-    const cudaError_t e = cudaGetDevice(&dev);
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    if (most_rows(a.group, a.tokens, max_new) >= kPromptMin) return launch_kv_prompt(a, bf16, ws, dev, s);
+    a.least_rows = 0;
+    a.most_rows = INT_MAX;
+    int rows = int(most_rows(a.group, a.tokens, max_new));
+    if (rows >= kPromptMin) {
+        const bool both = takes_both(a.group, a.requests, a.tokens, max_new);
+        if (both) a.least_rows = kPromptMin;
+        e = launch_kv_prompt(a, bf16, ws, dev, s);
+        if (e != cudaSuccess || !both) return e;
+        a.least_rows = 0;
+        a.most_rows = kPromptMin - 1;
+        rows = a.group <= 8 ? a.group : kPromptMin - 1;  // most are single tokens; others take more row tiles
+    } else {
+        a.whole = takes_whole(a.pool.head_dim, max_length);
+    }
+    const bool few = rows <= 8;
 #define EBX_KV_STEP(DD)                                                                              \
     (few ? (bf16 ? launch_step<DD, 1, true>(a, rows, ws, dev, s) : launch_step<DD, 1, false>(a, rows, ws, dev, s)) \
          : (bf16 ? launch_step<DD, 2, true>(a, rows, ws, dev, s) : launch_step<DD, 2, false>(a, rows, ws, dev, s)))
-    const int rows = int(most_rows(a.group, a.tokens, max_new));
-    const bool few = rows <= 8;
-    a.whole = takes_whole(a.pool.head_dim, max_length);
     switch (a.pool.head_dim) {
         case 32: return EBX_KV_STEP(32);
         case 64: return EBX_KV_STEP(64);

@@ -30,6 +30,11 @@ struct KvRequest {
     int first;    // keys ahead of it are not seen
 };
 
+// Does this launch take a request with n new tokens?
+__device__ __forceinline__ bool kv_taken(const KvAttnArgs& a, int64_t n) {
+    return n * a.group >= a.least_rows && n * a.group <= a.most_rows;
+}
+
 __device__ __forceinline__ KvRequest kv_request(const KvAttnArgs& a, int i) {
     KvRequest r;
     const int64_t s0 = a.starts[i], s1 = a.starts[i + 1];
@@ -39,7 +44,7 @@ __device__ __forceinline__ KvRequest kv_request(const KvAttnArgs& a, int i) {
     const int len = a.lengths[i];
     r.length = len < 0 ? 0 : int64_t(len) > cap ? int(cap) : len;
     r.begin = r.length - n;
-    r.rows = n * a.group;
+    r.rows = kv_taken(a, n) ? n * a.group : 0;
     r.token0 = int(lo);
     r.first = a.first ? max(a.first[i], 0) : 0;
     return r;
@@ -177,7 +182,7 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, 
             int64_t rts = 0, total;
             if (i < n) {
                 const int64_t s0 = max(a.starts[i0 + i], 0), s1 = min(int64_t(a.starts[i0 + i + 1]), a.tokens);
-                rts = s1 > s0 ? ((s1 - s0) * a.group + RT - 1) / RT : 0;
+                rts = s1 > s0 && kv_taken(a, s1 - s0) ? ((s1 - s0) * a.group + RT - 1) / RT : 0;
             }
             const int64_t ahead = all + scan(rts, total);
             if (i < n) {

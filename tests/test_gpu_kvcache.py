@@ -190,6 +190,16 @@ def test_a_hint_that_is_too_small_leaves_no_row_out(new):
     run_attention([20011, 3000], [new, new], heads=1, group=5, dim=32, block=16, max_new=1, max_length=9)
 
 
+@pytest.mark.parametrize("dim,group,heads", [(128, 4, 2), (32, 12, 1), (64, 1, 3)])
+@pytest.mark.parametrize("many", [3, 40])
+def test_a_prompt_among_steps(many, dim, group, heads):
+    """One prompt and `many` requests with a token or a few: both kernels, each for its own."""
+    lengths = [20 + (331 * i) % 3000 for i in range(many)] + [400]
+    new = [0 if i == 1 else 7 if i == 2 else 1 for i in range(many)] + [300]
+    run_attention(lengths, new, heads=heads, group=group, dim=dim, block=32, max_new=300, max_length=3020)
+    run_attention(lengths[::-1], new[::-1], heads=heads, group=group, dim=dim, block=32, max_new=300, window=70)
+
+
 @pytest.mark.parametrize("requests", [1, 300])
 def test_long_requests_are_split_and_joined(requests):
     lengths = [20011] if requests == 1 else [1 + (37 * i) % 900 for i in range(requests)]
