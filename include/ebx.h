@@ -384,8 +384,9 @@ EBX_API uint64_t ebx_kv_attention_workspace_bytes(const ebx_kv_pool* pool, int32
  * first[i] <= j (first may be NULL) and j < lengths[i], and if causal j <= p, and if
  * window > 0 (causal only) j > p - window.
  *     out[t, h] = softmax_j(scale * q . k_j) v_j,  lse[t, h] = log sum_j exp(...)
- * out [tokens, heads, head_dim] in q's dtype, lse fp32 (may be NULL); a query that sees
- * nothing gets out = 0 and lse = -infinity.  Sums, maxima and scales are fp32, the
+ * out [tokens, heads, head_dim] in q's dtype, apart from q, and lse fp32 (may be NULL); a
+ * query that sees nothing gets out = 0 and lse = -infinity, rows of no request are left as
+ * they are.  Sums, maxima and scales are fp32, the
  * weights of the values fp16.  max_new / max_length (0: unknown) are the largest number
  * of new tokens and the largest length of a request where the caller knows them; they
  * choose the kernel and never change what is computed. */

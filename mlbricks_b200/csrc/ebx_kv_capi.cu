@@ -155,7 +155,7 @@ ebx_status ebx_kv_attention(const ebx_kv_pool* pool, const void* q, int64_t q_to
         tokens < 0 || tokens * (heads / p.kv_heads) > INT32_MAX / 2)
         return invalid("ebx_kv_attention: requests, table width or tokens out of range");
     if (window < 0 || (window > 0 && !causal)) return invalid("ebx_kv_attention: a window is causal and > 0");
-    if (!std::isfinite(scale)) return invalid("ebx_kv_attention: scale must be finite");
+    if (!std::isfinite(scale * 1.4426950408889634f)) return invalid("ebx_kv_attention: scale must be finite");
     if (max_new < 0 || max_length < 0) return invalid("ebx_kv_attention: max_new and max_length are >= 0");
     if (tokens == 0) return EBX_OK;
     if (!out || !starts || requests == 0 || !tables || !lengths) return invalid("null argument");
@@ -185,7 +185,7 @@ ebx_status ebx_kv_attention(const ebx_kv_pool* pool, const void* q, int64_t q_to
     a.heads = heads;
     a.set_group(heads / p.kv_heads);
     a.causal = causal != 0;
-    a.window = window;
+    a.window = window < int64_t(width) * p.block_size ? window : 0;  // longer than any request: no window
     a.scale_log2 = scale * 1.4426950408889634f;
     return launched(ebx::launch_kv_attention(a, dtype == ebx::kKvBF16, max_new, max_length, workspace,
                                              static_cast<cudaStream_t>(stream)), "ebx_kv_attention");

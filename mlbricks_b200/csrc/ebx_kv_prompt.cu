@@ -17,7 +17,7 @@
 // tile cover only a part, and the issue slots when both compute weights.  A key tile takes some 5000
 // clocks for both row tiles: the products 2500 of them (8 of 128 x 128 x 16 take 670 from shared
 // memory, 600 with the weights in tensor memory), the largest and the weights 2700, the way from one
-// to the other the rest.  4096 tokens behind 12000, 32 heads over 8 of 128: 1.12 ms, 841 TFLOP/s.
+// to the other the rest.  4096 tokens behind 12000, 32 heads over 8 of 128: 1.10 ms, 850 TFLOP/s.
 // Measured and not kept, for that case: one thread a row 1274 us; the row in registers (one read of
 // S) 1299; S of 64 keys twice over, so that the weights never wait for it, 1277 (a product of 64
 // columns takes as long as one of 128).
@@ -162,21 +162,18 @@ __device__ __forceinline__ uint32_t seen32(const Row& row, int key0) {
 template <bool MASK, class F>
 __device__ __forceinline__ void columns(uint32_t s, const float4* tab, const Row& row, int key0, F f) {
     uint32_t v[32];
-    float4 e0 = tab[0], e1;
     tmem_ld16(s, v, 0);
 #pragma unroll 1
     for (int c = 0; c < 64; c += 32) {
         const uint32_t seen = MASK ? seen32(row, key0 + c) : 0u;
         tmem_wait<16>(v, 0);
         tmem_ld16(s + c + 16, v, 16);
-        e1 = tab[c / 16 + 1];
-        f(v, e0, c, seen);
+        f(v, tab[c / 16], c, seen);
         tmem_wait<16>(v, 16);
         if (c == 0) {
             tmem_ld16(s + c + 32, v, 0);
-            e0 = tab[c / 16 + 2];
         }
-        f(v + 16, e1, c + 16, seen >> 16);
+        f(v + 16, tab[c / 16 + 1], c + 16, seen >> 16);
     }
 }
 
@@ -188,21 +185,28 @@ __device__ __forceinline__ uint64_t t_pair(const uint32_t* v, int i, uint64_t c2
     return pack2f(seen & (1u << i) ? lo2(t2) : -INFINITY, seen & (2u << i) ? hi2(t2) : -INFINITY);
 }
 
-// The largest t - mr of the 64 columns.
+// The largest t of the 64 columns.  t = c S + b grows with S (c >= 0: a negative scale is a negative
+// q), and rounding keeps the order, so of a unit only the largest S is scaled.  A NaN c is not seen
+// here but in the weights.
 template <bool MASK>
-__device__ __forceinline__ float largest(uint32_t s, const float4* tab, const Row& row, float mr, int key0) {
-    float top0 = -INFINITY, top1 = -INFINITY;
+__device__ __forceinline__ float largest(uint32_t s, const float4* tab, const Row& row, int key0) {
+    float top = -INFINITY;
     columns<MASK>(s, tab, row, key0, [&](const uint32_t* v, const float4& e, int, uint32_t seen) {
-        const float c = e.x * row.unit, b = e.y - mr;
-        const uint64_t c2 = pack2f(c, c), b2 = pack2f(b, b);
+        float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
-            const uint64_t t = t_pair<MASK>(v, i, c2, b2, seen), u = t_pair<MASK>(v, i + 2, c2, b2, seen);
-            top0 = fmaxf(top0, fmaxf(lo2(t), hi2(t)));
-            top1 = fmaxf(top1, fmaxf(lo2(u), hi2(u)));
+            float x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                x[k] = __uint_as_float(v[i + k]);
+                if constexpr (MASK) x[k] = seen & (1u << (i + k)) ? x[k] : -INFINITY;
+            }
+            most[0] = fmaxf(most[0], fmaxf(x[0], x[1]));
+            most[1] = fmaxf(most[1], fmaxf(x[2], x[3]));
         }
+        top = fmaxf(top, fmaf(fmaxf(most[0], most[1]), e.x * row.unit, e.y));
     });
-    return fmaxf(top0, top1);
+    return top;
 }
 
 // Weights 2^(t - mr) as fp16 pairs over the columns of S that were read, and their sum over vs.
@@ -373,7 +377,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                         };
                         v[i] = make_uint4(halves(v[i].x), halves(v[i].y), halves(v[i].z), halves(v[i].w));
                     }
-                    *stage_at(ri) = v[i];
+                    const uint32_t sign = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
+                    *stage_at(ri) = make_uint4(v[i].x ^ sign, v[i].y ^ sign, v[i].z ^ sign, v[i].w ^ sign);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -395,8 +400,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 const float4* tab = tabs + (at % kTabs) * 8 + half * 4;
                 const int key0 = (walk.t0 + j) * kPromptKeys + half * 64;
                 const bool mask = key0 < all_lo || key0 + 64 > all_hi;
-                const float mr = row.mr == -INFINITY ? 0.0f : row.mr;
-                float top = mr + (mask ? largest<true>(s_addr, tab, row, mr, key0) : largest<false>(s_addr, tab, row, mr, key0));
+                float top = mask ? largest<true>(s_addr, tab, row, key0) : largest<false>(s_addr, tab, row, key0);
                 if (pair_any(pair, top > row.mr + (kLag + kShift))) {
                     // mr moves in the rows whose t grew, and with it what was summed
                     *tell = top;
@@ -636,7 +640,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                             const float vsc = vs < 0x1p-100f ? 0x1p-100f : vs;  // NaN stays
                             // NaN goes through t, where the mask stops it, and not through 1 / vs
                             tabs[(gj % kTabs) * 8 + lane] =
-                                make_float4(none ? 0.0f : ks * a.scale_log2, none ? -INFINITY : lg2(vsc),
+                                make_float4(none ? 0.0f : ks * fabsf(a.scale_log2), none ? -INFINITY : lg2(vsc),
                                             none ? 0.0f : vs == vs ? 1.0f / vsc : 1.0f, 0.0f);
                         }
                         __syncwarp();

@@ -46,7 +46,7 @@ __device__ __forceinline__ KvRequest kv_request(const KvAttnArgs& a, int i) {
     r.begin = r.length - n;
     r.rows = kv_taken(a, n) ? n * a.group : 0;
     r.token0 = int(lo);
-    r.first = a.first ? max(a.first[i], 0) : 0;
+    r.first = a.first ? min(max(a.first[i], 0), r.length) : 0;
     return r;
 }
 

@@ -236,7 +236,8 @@ def attention(q: torch.Tensor, pool: KVPool, tables: torch.Tensor, lengths: torc
     lengths[i] tokens; heads / kv_heads query heads share a key/value head.  A query at position p
     sees the keys j < lengths[i] with j >= first[i] (if given), j <= p (``causal``) and
     j > p - window (``window`` > 0).  A query that sees nothing gets 0 (log-sum-exp -infinity); rows
-    of no request are left as they are.  ``scale`` defaults to 1 / sqrt(head_dim).  ``max_new`` and
+    of no request are left as they are, and ``out``, if given, is not q's memory.  ``scale`` defaults to
+    1 / sqrt(head_dim).  ``max_new`` and
     ``max_length``, where the caller knows the largest number of new tokens and the largest length,
     choose the kernel and change no result.  Returns out, or (out, lse [tokens, heads] fp32)."""
     q = pool._rows(q, None, "q")

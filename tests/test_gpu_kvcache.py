@@ -154,12 +154,25 @@ def test_without_causal_mask(new):
     run_attention([500, 7, 129, 301], new, heads=2, group=2, dim=128, block=64, causal=False)
 
 
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 0.5])
+@pytest.mark.parametrize("new", [[1, 1, 1], [40, 129, 300]])
+def test_any_scale(new, scale):
+    run_attention([500, 129, 301], new, heads=2, group=4, dim=64, block=16, scale=scale)
+    run_attention([500, 129, 301], new, heads=1, group=5, dim=128, block=32, scale=scale, dtype=torch.bfloat16)
+
+
 @pytest.mark.parametrize("new", [[1, 1, 1, 1, 1], [40, 7, 129, 300, 64]])
 @pytest.mark.parametrize("window", [0, 33])
 def test_first_leaves_rows_empty(new, window):
     # first past the length: nothing to see; in the middle of a prompt: its first rows see nothing
     run_attention([500, 7, 129, 301, 64], new, heads=2, group=4, dim=64, block=32, first=[3, 1000, 128, 150, 64],
                   window=window)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [40, 300]])
+def test_numbers_as_large_as_they_go(new):
+    most = 2**31 - 1
+    run_attention([500, 200], new, heads=1, group=4, dim=64, block=32, first=[0, most], window=most)
 
 
 def test_requests_without_tokens():
