@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
     __shared__ int s_taken, s_short;
     const int tid = threadIdx.x;
     const int bsize = 1 << a.shift;
-    const int64_t head = a.ring[0], tail = a.ring[1];
+    const int64_t head = a.ring[0] < 0 ? 0 : a.ring[0], tail = a.ring[1] < head ? head : a.ring[1];
     const int64_t avail = tail - head;
     if (tid == 0) s_taken = s_short = 0;
     int64_t tokens = 0, blocks = 0, released = 0;
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
     // released blocks, a warp to a request
     for (int64_t i = gtid >> 5; i < a.requests; i += gthreads >> 5) {
         if (a.added[i] >= 0) continue;
-        const int had = min((max(a.past[i], 0) + bsize - 1) >> a.shift, a.width);
+        const int had = int(min((int64_t(max(a.past[i], 0)) + bsize - 1) >> a.shift, int64_t(a.width)));
         for (int j = tid & 31; j < had; j += 32)
             a.free_ring[(tail + s_gone[i] + j) % a.free_size] = a.tables[i * a.width + j];
     }
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
             const int before = s_before[lo];
             if (before >= 0) {
                 const int column = place >> a.shift;
-                const int fresh = column - ((past + bsize - 1) >> a.shift);
+                const int fresh = column - int((int64_t(past) + bsize - 1) >> a.shift);
                 int32_t* entry = a.tables + int64_t(lo) * a.width + column;
                 int id;
                 if (fresh >= 0) {

@@ -494,6 +494,17 @@ def test_plan_with_no_requests_and_no_tokens():
     assert step.lengths.tolist() == [16]
 
 
+def test_plan_with_numbers_out_of_range():
+    """Lengths that no table holds, a ring that ends ahead of its front: nobody gets a block, nothing is followed."""
+    most = 2**31 - 1
+    tables, free = i32([[0, 1], [2, 3], [4, 5]]), i32([6, 7, 8])
+    step = kv.plan(i32([most, -3, 40]), i32([5, 4, -1]), tables, free, torch.tensor([-9, -20], device="cuda"),
+                   block_size=16, tokens=9)
+    assert step.lengths.tolist() == [most, 0, 0] and step.slots.tolist() == [-1] * 9
+    assert step.ring.tolist()[:2] == [0, 2]  # the third's two blocks (its row holds no more) join the ring
+    assert free.tolist() == [4, 5, 8] and tables.tolist() == [[0, 1], [2, 3], [4, 5]]
+
+
 # ---- refusals and streams -------------------------------------------------------------------
 
 
