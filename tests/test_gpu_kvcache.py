@@ -219,6 +219,12 @@ def test_long_requests_are_split_and_joined(requests):
     run_attention(lengths, [1] * requests, heads=2, group=4, dim=128, block=64, q_size=2.0)
 
 
+@pytest.mark.parametrize("new", [1, 60])
+def test_more_requests_than_a_window_of_the_shares(new):
+    lengths = [new + (29 * i) % 90 for i in range(2100)]
+    run_attention(lengths, [new if i % 3 == 0 or new == 1 else 0 for i in range(2100)], heads=1, group=1, dim=32, block=16)
+
+
 def test_same_inputs_same_bits():
     q, pool, tables, starts, out, lse = run_attention([5000, 17, 900], [1, 1, 40], heads=4, group=4, dim=128, block=16)
     for _ in range(3):
