@@ -166,14 +166,14 @@ __device__ __forceinline__ void columns(uint32_t s, const float4* tab, const Row
 #pragma unroll 1
     for (int c = 0; c < 64; c += 32) {
         const uint32_t seen = MASK ? seen32(row, key0 + c) : 0u;
+        const float4 e0 = tab[c / 16];  // ahead of the wait: both take their time
         tmem_wait<16>(v, 0);
         tmem_ld16(s + c + 16, v, 16);
-        f(v, tab[c / 16], c, seen);
+        f(v, e0, c, seen);
+        const float4 e1 = tab[c / 16 + 1];
         tmem_wait<16>(v, 16);
-        if (c == 0) {
-            tmem_ld16(s + c + 32, v, 0);
-        }
-        f(v + 16, tab[c / 16 + 1], c + 16, seen >> 16);
+        if (c == 0) tmem_ld16(s + c + 32, v, 0);
+        f(v + 16, e1, c + 16, seen >> 16);
     }
 }
 
