@@ -60,28 +60,31 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
     const int64_t avail = tail - head;
     if (tid == 0) s_taken = s_short = 0;
     int64_t tokens = 0, blocks = 0, released = 0;
+    constexpr int64_t most = INT32_MAX;  // a token's number has 31 bits: nobody whose tokens pass them gets a block
     for (int base = 0; base < a.requests; base += kPlanThreads) {
         const int i = base + tid;
         int64_t add = 0, need = 0, wanted = 0, gone = 0;
-        bool wide = false, live = false;
+        bool refused = false, live = false;
         if (i < a.requests) {
-            const int64_t past = max(a.past[i], 0);
-            const int64_t had = (past + bsize - 1) >> a.shift;
             live = a.added[i] >= 0;
             add = live ? a.added[i] : 0;
-            gone = live ? 0 : min(had, int64_t(a.width));
-            wanted = ((past + add + bsize - 1) >> a.shift) - had;
-            wide = had + wanted > a.width;
-            need = wide ? 0 : wanted;
         }
         int64_t t_tok, t_need, t_gone;
         const int64_t i_tok = block_scan(add, warp_sums, t_tok);
+        if (i < a.requests) {
+            const int64_t past = max(a.past[i], 0);
+            const int64_t had = (past + bsize - 1) >> a.shift;
+            gone = live ? 0 : min(had, int64_t(a.width));
+            wanted = ((past + add + bsize - 1) >> a.shift) - had;
+            refused = had + wanted > a.width || (add > 0 && tokens + i_tok > most);
+            need = refused ? 0 : wanted;
+        }
         const int64_t i_need = block_scan(need, warp_sums, t_need);
         const int64_t i_gone = block_scan(gone, warp_sums, t_gone);
         if (i < a.requests) {
             const int64_t before = blocks + i_need - need;
-            const bool fits = live && !wide && (need == 0 || before + need <= avail);
-            s_start[i] = int32_t(tokens + i_tok - add);
+            const bool fits = live && !refused && (need == 0 || before + need <= avail);
+            s_start[i] = int32_t(min(tokens + i_tok - add, most));
             s_before[i] = fits ? int32_t(before) : -1;
             s_gone[i] = int32_t(released + i_gone - gone);
             if (fits && need > 0) atomicMax(&s_taken, int(before + need));
@@ -96,7 +99,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
     const int64_t gtid = int64_t(blockIdx.x) * kPlanThreads + tid;
     const int64_t gthreads = int64_t(gridDim.x) * kPlanThreads;
     if (gtid == 0) {
-        a.starts[a.requests] = int32_t(tokens);
+        a.starts[a.requests] = int32_t(min(tokens, most));
         a.ring_out[0] = head + s_taken;
         a.ring_out[1] = tail + released;
         a.ring_out[2] = s_short;

@@ -1,0 +1,53 @@
+"""What the 8-bit cache does with numbers on the device that nobody means: counts, rings and lengths out of
+range are not followed, and nothing around the tensors changes."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+kv = pytest.importorskip("mlbricks_b200.kvcache")
+MOST = 2**31 - 1
+
+
+@pytest.fixture(autouse=True)
+def _cuda(cuda_ok):
+    torch.manual_seed(0)
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def i64(x):
+    return torch.tensor(x, dtype=torch.int64, device="cuda")
+
+
+def guarded(rows, width, value=-1):
+    """A table [rows, width] of `value` in the middle of a larger tensor, and that tensor."""
+    around = torch.full((rows * width + 8192,), 77, dtype=torch.int32, device="cuda")
+    table = around[4096:4096 + rows * width].view(rows, width)
+    table.fill_(value)
+    return table, around
+
+
+def test_plan_with_more_tokens_than_31_bits_count():
+    """The first two want more than a row holds, and with the second the sum passes 2^31 - 1: nobody gets a block,
+    and no token of the room belongs to the last two."""
+    tables, around = guarded(4, 1)
+    before, free = around.clone(), i32(list(range(8)))
+    step = kv.plan(i32([0] * 4), i32([MOST, MOST, 1, 1]), tables, free, i64([0, 8]), block_size=16, tokens=64)
+    assert torch.equal(around, before) and free.tolist() == list(range(8))
+    assert step.lengths.tolist() == [0] * 4 and step.slots.tolist() == [-1] * 64
+    starts = step.starts.tolist()
+    assert starts[0] == 0 and starts == sorted(starts)
+    assert step.ring[:2].tolist() == [0, 8] and step.ring[3] == 2 * MOST + 2
+
+
+def test_plan_serves_those_ahead_of_a_sum_that_is_too_large():
+    tables, around = guarded(4, 2)
+    step = kv.plan(i32([0, 5, 0, 0]), i32([3, 0, MOST, 1]), tables, i32([4, 5, 6]), i64([0, 3]), block_size=16, tokens=3)
+    assert step.lengths.tolist() == [3, 5, 0, 0] and step.slots.tolist() == [64, 65, 66]
+    assert tables.tolist() == [[4, -1], [-1, -1], [-1, -1], [-1, -1]]
+    assert step.ring[:2].tolist() == [1, 3] and step.starts[:3].tolist() == [0, 3, 3]
