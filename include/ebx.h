@@ -336,13 +336,15 @@ typedef struct {
  * wait in free_ring (int32 [free_size], room for every block of the pool) at places
  * ring[0] .. ring[1] - 1 modulo free_size.  Requests are served in order: each takes
  * the blocks that it lacks from the ring's front into its row of `tables`, or, when
- * they are not there or its row is too short, nothing (its tokens get slot -1 and its
- * length stays).  Released blocks join the ring's back, for later calls; a released
+ * they are not there, its row is too short or its tokens do not all lie below `tokens`,
+ * nothing (its tokens get slot -1 and its length stays).  Released blocks join the ring's back, for later calls; a released
  * row's entries are left as they are.
- * Written: ring_out[4] = {front, back, blocks that were missing, tokens}, lengths
- * [requests] (after the step; 0 when released), starts[requests + 1] (first token of
- * each request among the step's tokens), and for t < `tokens` slots[t] = block *
- * block_size + offset and positions[t] (slot -1, position 0 past the last token).
+ * Written: ring_out[4] = {front, back, blocks that were missing, sum of the new tokens},
+ * lengths [requests] (after the step; 0 when released), starts[requests + 1] (first token
+ * of each request among the step's tokens, `tokens` at most), and for t < `tokens` slots[t]
+ * = block * block_size + offset and positions[t] (slot -1, position 0 past the last token).
+ * `tokens` is the room of slots and positions: the sum of the new tokens or more.  If
+ * ring_out[3] is larger, requests were refused for want of room.
  * ring_out and lengths must not overlap ring and past.  requests <= 16384. */
 EBX_API ebx_status ebx_kv_plan(const int32_t* past, const int32_t* added, int32_t requests,
                                int32_t* tables, int32_t width, int32_t block_size, int32_t* free_ring,

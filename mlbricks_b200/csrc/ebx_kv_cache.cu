@@ -39,8 +39,9 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* warp_sums, int
 // Request i holds past[i] tokens and adds added[i]; it needs ceil((past + added) / B) -
 // ceil(past / B) more blocks.  With before[i] the sum of the needs of the requests ahead of it,
 // it gets entries before[i].. of the free ring if they are there, so requests are served in
-// order and the exclusive sums alone say who gets what.  added[i] < 0 releases the request:
-// its blocks go behind the ring's tail.  A new block always begins with a new token, so the
+// order and the exclusive sums alone say who gets what.  A request that needs more blocks than its
+// row holds, or whose tokens end past the room for slots (which counts in 31 bits), gets nothing;
+// starts end at the room.  added[i] < 0 releases the request: its blocks go behind the ring's tail.  A new block always begins with a new token, so the
 // threads that write the tokens' slots also write the table.
 // Every CTA computes the sums for itself (a few loads per thread: cheaper than a second
 // launch or a grid barrier) and then writes its share of the tokens.  What bounds it is latency: the
@@ -60,7 +61,6 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
     const int64_t avail = tail - head;
     if (tid == 0) s_taken = s_short = 0;
     int64_t tokens = 0, blocks = 0, released = 0;
-    constexpr int64_t most = INT32_MAX;  // a token's number has 31 bits: nobody whose tokens pass them gets a block
     for (int base = 0; base < a.requests; base += kPlanThreads) {
         const int i = base + tid;
         int64_t add = 0, need = 0, wanted = 0, gone = 0;
@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
             const int64_t had = (past + bsize - 1) >> a.shift;
             gone = live ? 0 : min(had, int64_t(a.width));
             wanted = ((past + add + bsize - 1) >> a.shift) - had;
-            refused = had + wanted > a.width || (add > 0 && tokens + i_tok > most);
+            refused = had + wanted > a.width || (add > 0 && tokens + i_tok > a.tokens);
             need = refused ? 0 : wanted;
         }
         const int64_t i_need = block_scan(need, warp_sums, t_need);
@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
         if (i < a.requests) {
             const int64_t before = blocks + i_need - need;
             const bool fits = live && !refused && (need == 0 || before + need <= avail);
-            s_start[i] = int32_t(min(tokens + i_tok - add, most));
+            s_start[i] = int32_t(min(tokens + i_tok - add, a.tokens));
             s_before[i] = fits ? int32_t(before) : -1;
             s_gone[i] = int32_t(released + i_gone - gone);
             if (fits && need > 0) atomicMax(&s_taken, int(before + need));
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
     const int64_t gtid = int64_t(blockIdx.x) * kPlanThreads + tid;
     const int64_t gthreads = int64_t(gridDim.x) * kPlanThreads;
     if (gtid == 0) {
-        a.starts[a.requests] = int32_t(min(tokens, most));
+        a.starts[a.requests] = int32_t(min(tokens, a.tokens));
         a.ring_out[0] = head + s_taken;
         a.ring_out[1] = tail + released;
         a.ring_out[2] = s_short;

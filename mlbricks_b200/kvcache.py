@@ -145,10 +145,12 @@ def plan(past: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, free: torc
     Request i holds ``past[i]`` tokens and brings ``new[i]``; ``new[i] < 0`` releases it.  Free
     blocks wait in the ring ``free`` (int32, room for every block) from ``ring[0]`` up to
     ``ring[1]``, modulo its size.  In order, each request takes the blocks that it lacks into its
-    row of ``tables`` (written in place) -- or nothing, if they are not all there or the row is too
-    short: its tokens then get slot -1, its length stays, and ``ring[2]`` of the result counts the
-    missing blocks.  Released blocks join the ring's back.  ``tokens`` is the room for slots and
-    positions: the sum of the new tokens, or more (the rest is slot -1, position 0).
+    row of ``tables`` (written in place) -- or nothing, if they are not all there, the row is too
+    short, or its tokens do not fit ``tokens``: they then get slot -1, its length stays, and ``ring[2]``
+    of the result counts the missing blocks.  Released blocks join the ring's back.  ``tokens`` is the
+    room for slots and positions: the sum of the new tokens, or more (the rest is slot -1, position 0);
+    ``ring[3]`` of the result is that sum, so ``ring[3] > tokens`` says that requests were refused for
+    want of room.
 
     The inputs ``past`` and ``ring`` are not changed; the next step takes the result's ``lengths``
     and ``ring`` in their place."""
@@ -298,7 +300,7 @@ class KVCache:
 
     def plan(self, new, tokens: int | None = None, max_new: int | None = None) -> KVPlan:
         """Blocks and slots for a step.  ``new``: a list, or an int32 tensor on the GPU with
-        ``tokens`` (room for all its tokens) and, if known, ``max_new``.  ``ring[2]`` of the result is
+        ``tokens`` (room for all its tokens; requests that end past it are refused) and, if known, ``max_new``.  ``ring[2]`` of the result is
         the number of blocks that were missing: requests that got none keep their length."""
         if not isinstance(new, torch.Tensor):
             counts = [max(int(n), 0) for n in new]

@@ -51,3 +51,25 @@ def test_plan_serves_those_ahead_of_a_sum_that_is_too_large():
     assert step.lengths.tolist() == [3, 5, 0, 0] and step.slots.tolist() == [64, 65, 66]
     assert tables.tolist() == [[4, -1], [-1, -1], [-1, -1], [-1, -1]]
     assert step.ring[:2].tolist() == [1, 3] and step.starts[:3].tolist() == [0, 3, 3]
+
+
+def test_plan_with_room_for_fewer_tokens_than_there_are():
+    """The second request's 17 tokens end past the room for 2: it is refused, and so is the third; the first and
+    the one that rests are served, and what leaves the ring is in the table."""
+    tables, around = guarded(4, 2, value=55)
+    step = kv.plan(i32([0, 0, 0, 9]), i32([1, 17, 1, 0]), tables, i32(list(range(8))), i64([0, 8]), block_size=16, tokens=2)
+    assert step.lengths.tolist() == [1, 0, 0, 9] and step.starts.tolist() == [0, 1, 2, 2, 2]
+    assert step.slots.tolist() == [0, -1] and step.positions.tolist() == [0, 0]
+    assert tables.tolist() == [[0, 55], [55, 55], [55, 55], [55, 55]]
+    assert step.ring.tolist() == [1, 8, 3, 19]
+    assert (around[:4096] == 77).all() and (around[4104:] == 77).all()
+
+
+def test_plan_of_a_cache_with_room_for_one_token_a_row():
+    """A step captured for one token a row is given two in one row: that row waits, nothing of it is overwritten."""
+    cache = kv.KVCache(1, blocks=4, kv_heads=1, head_dim=32, requests=2, max_length=64, block_size=16)
+    cache.plan([15, 16])
+    step = cache.plan(i32([1, 2]), tokens=2)
+    assert cache.lengths.tolist() == [16, 16] and step.slots.tolist() == [15, -1]
+    assert cache.ring.tolist() == [2, 4, 1, 3]
+    assert cache.plan(i32([0, 2]), tokens=2).ring.tolist() == [3, 4, 0, 2] and cache.lengths.tolist() == [16, 18]
