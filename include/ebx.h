@@ -338,7 +338,8 @@ typedef struct {
  * the blocks that it lacks from the ring's front into its row of `tables`, or, when
  * they are not there, its row is too short or its tokens do not all lie below `tokens`,
  * nothing (its tokens get slot -1 and its length stays).  Released blocks join the ring's back, for later calls; a released
- * row's entries are left as they are.
+ * row's entries are left as they are.  A ring holds free_size blocks at most: of one that
+ * claims more the first free_size are used, and released blocks without a place are dropped.
  * Written: ring_out[4] = {front, back, blocks that were missing, sum of the new tokens},
  * lengths [requests] (after the step; 0 when released), starts[requests + 1] (first token
  * of each request among the step's tokens, `tokens` at most), and for t < `tokens` slots[t]

@@ -57,8 +57,15 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
     __shared__ int s_taken, s_short;
     const int tid = threadIdx.x;
     const int bsize = 1 << a.shift;
-    const int64_t head = a.ring[0] < 0 ? 0 : a.ring[0], tail = a.ring[1] < head ? head : a.ring[1];
-    const int64_t avail = tail - head;
+    // A ring that claims more blocks than its size holds the first of them.  Counters past 2^62 begin
+    // anew at their place, so that they never pass 2^63.
+    const int64_t begin = max(a.ring[0], int64_t(0));
+    const int64_t avail = min(max(a.ring[1], begin) - begin, int64_t(a.free_size));  // blocks to give
+    const int64_t room = a.free_size - avail;                                        // places for released ones
+    const int64_t head = begin >> 62 ? begin % a.free_size : begin, tail = head + avail;
+    const uint32_t size = uint32_t(a.free_size);
+    const uint32_t front = uint32_t(head % a.free_size), back = uint32_t(tail % a.free_size);
+    auto wrapped = [&](uint32_t place) { return place < size ? place : place - size; };  // place < 2 size < 2^32
     if (tid == 0) s_taken = s_short = 0;
     int64_t tokens = 0, blocks = 0, released = 0;
     for (int base = 0; base < a.requests; base += kPlanThreads) {
@@ -85,8 +92,8 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
             const int64_t before = blocks + i_need - need;
             const bool fits = live && !refused && (need == 0 || before + need <= avail);
             s_start[i] = int32_t(min(tokens + i_tok - add, a.tokens));
-            s_before[i] = fits ? int32_t(before) : -1;
-            s_gone[i] = int32_t(released + i_gone - gone);
+            s_before[i] = !fits ? -1 : need > 0 ? int32_t(before) : 0;
+            s_gone[i] = int32_t(min(released + i_gone - gone, room));
             if (fits && need > 0) atomicMax(&s_taken, int(before + need));
             if (!fits && wanted > 0) atomicAdd(&s_short, int(wanted));
         }
@@ -101,7 +108,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
     if (gtid == 0) {
         a.starts[a.requests] = int32_t(min(tokens, a.tokens));
         a.ring_out[0] = head + s_taken;
-        a.ring_out[1] = tail + released;
+        a.ring_out[1] = tail + min(released, room);
         a.ring_out[2] = s_short;
         a.ring_out[3] = tokens;
     }
@@ -113,9 +120,10 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
     // released blocks, a warp to a request
     for (int64_t i = gtid >> 5; i < a.requests; i += gthreads >> 5) {
         if (a.added[i] >= 0) continue;
-        const int had = int(min((int64_t(max(a.past[i], 0)) + bsize - 1) >> a.shift, int64_t(a.width)));
-        for (int j = tid & 31; j < had; j += 32)
-            a.free_ring[(tail + s_gone[i] + j) % a.free_size] = a.tables[i * a.width + j];
+        const int64_t had = min((int64_t(max(a.past[i], 0)) + bsize - 1) >> a.shift, int64_t(a.width));
+        const int left = int(min(had, room - s_gone[i]));
+        for (int j = tid & 31; j < left; j += 32)
+            a.free_ring[wrapped(back + s_gone[i] + j)] = a.tables[i * a.width + j];
     }
     for (int64_t t = gtid; t < a.tokens; t += gthreads) {
         int64_t slot = -1;
@@ -135,7 +143,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
                 int32_t* entry = a.tables + int64_t(lo) * a.width + column;
                 int id;
                 if (fresh >= 0) {
-                    id = a.free_ring[(head + before + fresh) % a.free_size];
+                    id = a.free_ring[wrapped(front + before + fresh)];
                     if ((place & (bsize - 1)) == 0) *entry = id;
                 } else {
                     id = *entry;

@@ -73,3 +73,31 @@ def test_plan_of_a_cache_with_room_for_one_token_a_row():
     assert cache.lengths.tolist() == [16, 16] and step.slots.tolist() == [15, -1]
     assert cache.ring.tolist() == [2, 4, 1, 3]
     assert cache.plan(i32([0, 2]), tokens=2).ring.tolist() == [3, 4, 0, 2] and cache.lengths.tolist() == [16, 18]
+
+
+def test_plan_with_a_ring_that_claims_more_than_it_holds():
+    """Four blocks, a back 100 places on: nobody gets a block twice, in this step or the next."""
+    tables, free = i32([[-1] * 8, [-1] * 8]), i32([0, 1, 2, 3])
+    step = kv.plan(i32([0, 0]), i32([128, 0]), tables, free, i64([0, 100]), block_size=16, tokens=128)
+    assert step.lengths.tolist() == [0, 0] and step.ring.tolist() == [0, 4, 8, 128]
+    assert step.slots.tolist() == [-1] * 128 and (tables == -1).all()
+    step = kv.plan(i32([0, 0]), i32([40, 10]), tables, free, i64([1, 100]), block_size=16, tokens=50)
+    assert step.lengths.tolist() == [40, 10] and step.ring.tolist() == [5, 5, 0, 50]
+    assert tables[:, :4].tolist() == [[1, 2, 3, -1], [0, -1, -1, -1]]
+    step = kv.plan(step.lengths, i32([16, 16]), tables, free, step.ring, block_size=16, tokens=32)
+    assert step.lengths.tolist() == [40, 10] and step.ring.tolist() == [5, 5, 2, 32]
+
+
+def test_plan_with_counters_near_their_end():
+    """A front and a back at 2^63 - 1, an odd size: the released blocks go to places of the ring."""
+    around = torch.full((4096 * 2 + 3,), 77, dtype=torch.int32, device="cuda")
+    free = around[4096:4099]
+    step = kv.plan(i32([32]), i32([-1]), i32([[8, 9]]), free, i64([2**63 - 1, 2**63 - 1]), block_size=16, tokens=0)
+    assert sorted(free.tolist()) == [8, 9, 77] and (around == 77).sum() == around.numel() - 2
+    assert step.lengths.tolist() == [0] and int(step.ring[1] - step.ring[0]) == 2
+
+
+def test_plan_does_not_release_more_than_the_ring_has_places_for():
+    free = i32([7, 8, 9])
+    step = kv.plan(i32([16, 32]), i32([-1, -1]), i32([[1, 2], [3, 4]]), free, i64([2, 4]), block_size=16, tokens=0)
+    assert free.tolist() == [7, 1, 9] and step.ring.tolist() == [2, 5, 0, 0]
