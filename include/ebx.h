@@ -346,7 +346,8 @@ typedef struct {
  * = block * block_size + offset and positions[t] (slot -1, position 0 past the last token).
  * `tokens` is the room of slots and positions: the sum of the new tokens or more.  If
  * ring_out[3] is larger, requests were refused for want of room.
- * ring_out and lengths must not overlap ring and past.  requests <= 16384. */
+ * ring_out and lengths must not overlap ring and past.  requests <= 16384, width *
+ * block_size <= 2^31 - 1. */
 EBX_API ebx_status ebx_kv_plan(const int32_t* past, const int32_t* added, int32_t requests,
                                int32_t* tables, int32_t width, int32_t block_size, int32_t* free_ring,
                                int32_t free_size, const int64_t* ring, int64_t* ring_out,

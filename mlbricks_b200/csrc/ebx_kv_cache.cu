@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
                 if (s_start[mid] <= t) lo = mid; else hi = mid;
             }
             const int past = max(a.past[lo], 0);
-            place = past + int(t - s_start[lo]);
+            place = int(min(past + t - s_start[lo], int64_t(INT32_MAX)));  // past it: a refused request's
             const int before = s_before[lo];
             if (before >= 0) {
                 const int column = place >> a.shift;

@@ -81,6 +81,8 @@ ebx_status ebx_kv_plan(const int32_t* past, const int32_t* added, int32_t reques
         return invalid("null argument");
     if (requests < 0 || requests > ebx::kKvMaxRequests) return invalid("ebx_kv_plan: need 0 <= requests <= 16384");
     if (width < 1 || free_size < 1) return invalid("ebx_kv_plan: need width >= 1 and free_size >= 1");
+    // lengths and positions have 31 bits, so a row that holds more could carry a request past them
+    if (int64_t(width) * block_size > INT32_MAX) return invalid("ebx_kv_plan: need width * block_size < 2^31");
     if (tokens < 0 || tokens > INT32_MAX) return invalid("ebx_kv_plan: need 0 <= tokens < 2^31");
     if (log2_of(block_size) < 0) return invalid("ebx_kv_plan: block_size must be 16, 32, 64 or 128");
     if (ring_out == ring || (requests > 0 && lengths == past))

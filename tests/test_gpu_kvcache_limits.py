@@ -101,3 +101,10 @@ def test_plan_does_not_release_more_than_the_ring_has_places_for():
     free = i32([7, 8, 9])
     step = kv.plan(i32([16, 32]), i32([-1, -1]), i32([[1, 2], [3, 4]]), free, i64([2, 4]), block_size=16, tokens=0)
     assert free.tolist() == [7, 1, 9] and step.ring.tolist() == [2, 5, 0, 0]
+
+
+def test_plan_keeps_positions_within_31_bits():
+    """A length that no table holds: the refused tokens' positions end at 2^31 - 1."""
+    step = kv.plan(i32([MOST - 2]), i32([5]), i32([[1]]), i32([2]), i64([0, 1]), block_size=16, tokens=5)
+    assert step.positions.tolist() == [MOST - 2, MOST - 1, MOST, MOST, MOST] and step.slots.tolist() == [-1] * 5
+    assert step.lengths.tolist() == [MOST - 2]
