@@ -54,7 +54,8 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
     int32_t* s_before = s_start + a.requests;     // blocks taken ahead of it, -1: refused
     int32_t* s_gone = s_before + a.requests;      // blocks released ahead of it
     __shared__ int64_t warp_sums[kPlanThreads / 32];
-    __shared__ int s_taken, s_short;
+    __shared__ int s_taken;
+    __shared__ unsigned long long s_short;  // whole rows of counts may be out of range, and still add up
     const int tid = threadIdx.x;
     const int bsize = 1 << a.shift;
     // A ring that claims more blocks than its size holds the first of them.  Counters past 2^62 begin
@@ -66,7 +67,10 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
     const uint32_t size = uint32_t(a.free_size);
     const uint32_t front = uint32_t(head % a.free_size), back = uint32_t(tail % a.free_size);
     auto wrapped = [&](uint32_t place) { return place < size ? place : place - size; };  // place < 2 size < 2^32
-    if (tid == 0) s_taken = s_short = 0;
+    if (tid == 0) {
+        s_taken = 0;
+        s_short = 0;
+    }
     int64_t tokens = 0, blocks = 0, released = 0;
     for (int base = 0; base < a.requests; base += kPlanThreads) {
         const int i = base + tid;
@@ -95,7 +99,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
             s_before[i] = !fits ? -1 : need > 0 ? int32_t(before) : 0;
             s_gone[i] = int32_t(min(released + i_gone - gone, room));
             if (fits && need > 0) atomicMax(&s_taken, int(before + need));
-            if (!fits && wanted > 0) atomicAdd(&s_short, int(wanted));
+            if (!fits && wanted > 0) atomicAdd(&s_short, static_cast<unsigned long long>(wanted));
         }
         tokens += t_tok;
         blocks += t_need;
@@ -109,7 +113,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(KvPlanArgs a) {
         a.starts[a.requests] = int32_t(min(tokens, a.tokens));
         a.ring_out[0] = head + s_taken;
         a.ring_out[1] = tail + min(released, room);
-        a.ring_out[2] = s_short;
+        a.ring_out[2] = int64_t(s_short);
         a.ring_out[3] = tokens;
     }
     for (int64_t i = gtid; i < a.requests; i += gthreads) {

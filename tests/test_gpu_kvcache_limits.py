@@ -108,3 +108,10 @@ def test_plan_keeps_positions_within_31_bits():
     step = kv.plan(i32([MOST - 2]), i32([5]), i32([[1]]), i32([2]), i64([0, 1]), block_size=16, tokens=5)
     assert step.positions.tolist() == [MOST - 2, MOST - 1, MOST, MOST, MOST] and step.slots.tolist() == [-1] * 5
     assert step.lengths.tolist() == [MOST - 2]
+
+
+def test_plan_counts_missing_blocks_past_31_bits():
+    """Twenty requests that lack 2^27 blocks each."""
+    step = kv.plan(i32([0] * 20), i32([MOST] * 20), i32([[-1]] * 20), i32([0]), i64([0, 1]), block_size=16, tokens=1)
+    assert step.ring.tolist() == [0, 1, 20 * 2**27, 20 * MOST]
+    assert step.lengths.tolist() == [0] * 20 and step.slots.tolist() == [-1]
