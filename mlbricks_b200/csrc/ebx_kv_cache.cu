@@ -323,6 +323,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32)
                 *reinterpret_cast<uint2*>(dst + (off + j) * D + part * 8) = c;
             }
         }
+        __syncwarp();  // every lane has read the old scale
         if (lane == 0) scales[cell] = s;
     }
 }
