@@ -134,7 +134,8 @@ ebx_status ebx_kv_materialize(const ebx_kv_pool* pool, const int32_t* tables, in
 uint64_t ebx_kv_attention_workspace_bytes(const ebx_kv_pool* pool, int32_t heads, int64_t tokens,
                                           int32_t max_new, int32_t max_length) {
     ebx::KvPool p;
-    if (pool_of(pool, p) || heads < 1 || heads % p.kv_heads != 0 || tokens < 0 || max_new < 0 || max_length < 0)
+    if (pool_of(pool, p) || heads < 1 || heads % p.kv_heads != 0 || tokens < 0 || tokens > INT32_MAX ||
+        max_new < 0 || max_length < 0)
         return 0;
     Device d(pool->device);
     if (d.err != cudaSuccess) return 0;
@@ -154,7 +155,7 @@ ebx_status ebx_kv_attention(const ebx_kv_pool* pool, const void* q, int64_t q_to
     if (heads < 1 || heads % p.kv_heads != 0 || heads > (1 << 20))
         return invalid("ebx_kv_attention: heads must be a multiple of kv_heads");
     if (requests < 0 || requests > (1 << 20) || width < 1 || int64_t(width) * p.block_size > INT32_MAX / 2 ||
-        tokens < 0 || tokens * (heads / p.kv_heads) > INT32_MAX / 2)
+        tokens < 0 || tokens > INT32_MAX || tokens * (heads / p.kv_heads) > INT32_MAX / 2)
         return invalid("ebx_kv_attention: requests, table width or tokens out of range");
     if (window < 0 || (window > 0 && !causal)) return invalid("ebx_kv_attention: a window is causal and > 0");
     if (!std::isfinite(scale * 1.4426950408889634f)) return invalid("ebx_kv_attention: scale must be finite");

@@ -1,6 +1,8 @@
 """Sizes that the cache's C entries refuse before anything reaches a GPU."""
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 
 from mlbricks_b200 import _ebx
@@ -17,3 +19,18 @@ def test_plan_refuses_rows_that_hold_more_tokens_than_a_length_counts(width, blo
     entries lie ahead of the table."""
     lib = _ebx.load()
     refused(lib.ebx_kv_plan(4, 4, 1, 4, width, block, 4, 1, 8, 16, 8, 4, 8, 4, 1, 0, None), "2^31")
+
+
+def pool(**change):
+    fields = dict(k_codes=16, k_scales=4, v_codes=16, v_scales=4, blocks=8, kv_heads=2, block_size=16, head_dim=64,
+                  device=0, reserved=0)
+    return ctypes.byref(_ebx.KVPool(*{**fields, **change}.values()))
+
+
+@pytest.mark.parametrize("tokens", [2**31, 2**62, 2**63 - 1])
+def test_attention_refuses_more_rows_than_it_counts(tokens):
+    """2^62 tokens of four heads a key/value head are 2^64 rows, which 64 bits show as none."""
+    lib = _ebx.load()
+    refused(lib.ebx_kv_attention(pool(), 16, 256, 64, 8, 1, 4, 1, 4, 4, None, 1, tokens, 1, 0, 1.0, 0, 0, 16, None, None,
+                                 0, None), "out of range")
+    assert lib.ebx_kv_attention_workspace_bytes(pool(), 8, tokens, 0, 0) == 0
