@@ -122,6 +122,9 @@ ebx_status ebx_kv_materialize(const ebx_kv_pool* pool, const int32_t* tables, in
         return invalid("ebx_kv_materialize: dtype must be fp32, fp16 or bf16");
     if (requests < 0 || width < 1 || tokens < 0 || tokens > INT32_MAX)
         return invalid("ebx_kv_materialize: need requests >= 0, width >= 1 and 0 <= tokens < 2^31");
+    // a CTA counts the elements of its tokens, kv_heads * head_dim of them, in 31 bits
+    if (int64_t(p.kv_heads) * p.head_dim > INT32_MAX / 2)
+        return invalid("ebx_kv_materialize: need kv_heads * head_dim < 2^30");
     if (tokens == 0) return EBX_OK;
     if (!starts || !k || !v || (requests > 0 && !tables)) return invalid("null argument");
     if (!aligned16(k) || !aligned16(v)) return invalid("ebx_kv_materialize: outputs must be 16-byte aligned");

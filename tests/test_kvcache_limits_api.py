@@ -34,3 +34,11 @@ def test_attention_refuses_more_rows_than_it_counts(tokens):
     refused(lib.ebx_kv_attention(pool(), 16, 256, 64, 8, 1, 4, 1, 4, 4, None, 1, tokens, 1, 0, 1.0, 0, 0, 16, None, None,
                                  0, None), "out of range")
     assert lib.ebx_kv_attention_workspace_bytes(pool(), 8, tokens, 0, 0) == 0
+
+
+@pytest.mark.parametrize("kv_heads,head_dim", [(2**24, 128), (2**27 - 1, 32)])
+def test_materialize_refuses_tokens_wider_than_it_counts(kv_heads, head_dim):
+    """The elements of a CTA's 16 tokens, 16 to a thread, would pass 31 bits, and nothing would be written."""
+    lib = _ebx.load()
+    wide = pool(blocks=1, kv_heads=kv_heads, head_dim=head_dim)
+    refused(lib.ebx_kv_materialize(wide, 4, 1, 4, None, 1, 1, 1, 16, 16, None), "2^30")
