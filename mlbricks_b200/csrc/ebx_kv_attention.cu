@@ -180,6 +180,8 @@ __global__ void __launch_bounds__(kStepThreads, (StepCfg<D, NQ>::PER_SM))
             }
         }
         asm volatile("cp.async.wait_all;\n" ::: "memory");
+        if (!ok)  // given up: copies on their way land before this shared memory is another CTA's
+            for (int i = max(it - kStages, 0); i < it; ++i) kv_wait(smem_u32(&full[i % kStages]), uint32_t((i / kStages) & 1));
         return;
     }
 
