@@ -144,15 +144,18 @@ struct KvWalk {
 // that one long prompt and many short requests cost the same few loads a thread.  `scratch`:
 // kShareInts ints of shared memory, free again when the last barrier in here is passed.
 constexpr int kShareWindow = 1024;
-constexpr int kShareInts = 2 * kShareWindow + 128;
+constexpr int kShareInts = 3 * kShareWindow + 128;
 
 template <int RT, int KT, int EXTRA, int NT>
 __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, int* scratch) {
     constexpr int W = NT / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int* tiles = scratch;                       // row tiles of the window's requests ahead of i
-    int* units = scratch + kShareWindow;        // key tiles of one head of request i
-    int64_t* sums = reinterpret_cast<int64_t*>(scratch + 2 * kShareWindow);  // [W] and the answer
+    // key tiles of one head of request i, low and high words (a long prompt in tiles of 8 rows passes 2^32)
+    uint32_t* units = reinterpret_cast<uint32_t*>(scratch + kShareWindow);
+    uint32_t* carry = units + kShareWindow;
+    auto units_of = [&](int i) { return int64_t(carry[i]) << 32 | units[i]; };
+    int64_t* sums = reinterpret_cast<int64_t*>(scratch + 3 * kShareWindow);  // [W] and the answer
     static_assert(W + 3 <= 64, "scratch of kv_share");
     // exclusive scan over the block; total receives the sum
     auto scan = [&](int64_t v, int64_t& total) {
@@ -187,7 +190,7 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, 
             const int64_t ahead = all + scan(rts, total);
             if (i < n) {
                 tiles[i] = int(ahead);
-                units[i] = 0;
+                units[i] = carry[i] = 0;
             }
             all += total;
         }
@@ -200,7 +203,8 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, 
             }
             int t0, k;
             kv_key_tiles<RT, KT>(a, kv_request(a, i0 + lo), int(x) - tiles[lo], t0, k);
-            atomicAdd(units + lo, a.whole ? 1 : k + EXTRA);
+            const uint32_t more = a.whole ? 1 : k + EXTRA;
+            if (atomicAdd(units + lo, more) > ~more) atomicAdd(carry + lo, 1u);
         }
         __syncthreads();
     };
@@ -209,7 +213,7 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, 
         const int n = min(kShareWindow, a.requests - i0);
         count(i0, n);
         int64_t mine = 0, all;
-        for (int i = tid; i < n; i += NT) mine += units[i];
+        for (int i = tid; i < n; i += NT) mine += units_of(i);
         scan(mine, all);
         total += all * a.pool.kv_heads;
     }
@@ -232,14 +236,14 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, 
         bool found = false;
         for (int b = 0; b < n; b += NT) {
             const int i = b + tid;
-            const int64_t u = i < n ? int64_t(units[i]) * a.pool.kv_heads : 0;
+            const int64_t u = i < n ? units_of(i) * a.pool.kv_heads : 0;
             int64_t all;
             const int64_t begin = base + scan(u, all);
             if (u > 0 && begin <= w0 && w0 < begin + u) {  // exactly one thread
                 const int64_t at = w0 - begin;
                 sums[W] = i0 + i;
-                sums[W + 1] = at / units[i];
-                sums[W + 2] = at % units[i];
+                sums[W + 1] = at / units_of(i);
+                sums[W + 2] = at % units_of(i);
             }
             base += all;
             found = base > w0;
@@ -251,7 +255,7 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, 
     out.request = int(sums[W]);
     out.head = int(sums[W + 1]);
     // the row tile: each warp for itself, 32 at a time
-    int rest = int(sums[W + 2]);
+    int64_t rest = sums[W + 2];
     const KvRequest r = kv_request(a, out.request);
     for (int rt0 = 0;; rt0 += 32) {
         int t0, k = 0;
@@ -269,7 +273,7 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, 
         if (past) {
             const int f = __ffs(past) - 1;
             out.rt = rt0 + f;
-            out.skip = rest - __shfl_sync(0xffffffffu, x - k, f);
+            out.skip = int(rest) - __shfl_sync(0xffffffffu, x - k, f);
             break;
         }
         rest -= __shfl_sync(0xffffffffu, x, 31);

@@ -115,3 +115,26 @@ def test_plan_counts_missing_blocks_past_31_bits():
     step = kv.plan(i32([0] * 20), i32([MOST] * 20), i32([[-1]] * 20), i32([0]), i64([0, 1]), block_size=16, tokens=1)
     assert step.ring.tolist() == [0, 1, 20 * 2**27, 20 * MOST]
     assert step.lengths.tolist() == [0] * 20 and step.slots.tolist() == [-1]
+
+
+def test_attention_with_more_key_tiles_than_31_bits_count():
+    """A prompt of 540 thousand tokens in tiles of 8 rows (what a wrong `max_new` leads to): 2.3e9 tiles of 64 keys.
+
+    Tolerance: a weight is rounded to 11 bits (2^-11 of it) and the products' sums to 24 bits, over some 2^13 key
+    tiles 2^-11 of their sizes at most; the output's own rounding is 2^-11 of it."""
+    n, heads, dim, block = 540_000, 8, 128, 128
+    blocks = -(-n // block)
+    pool = kv.KVPool(*(t for _ in "kv" for t in (
+        torch.randint(-127, 128, (blocks, 1, block, dim), dtype=torch.int8, device="cuda"),
+        0.02 * torch.exp(torch.randn(blocks, 1, device="cuda")))))
+    table = torch.randperm(blocks, device="cuda").int().view(1, -1)
+    q = torch.randn(n, heads, dim, device="cuda", dtype=torch.float16)
+    out = torch.full_like(q, 77.0)
+    kv.attention(q, pool, table, i32([n]), i32([0, n]), max_new=1, out=out)
+    ids = table[0].long()
+    k, v = (c[ids].double().mul_(s[ids].double()[..., None, None]).view(-1, dim)[:n]
+            for c, s in ((pool.k_codes, pool.k_scales), (pool.v_codes, pool.v_scales)))
+    for t in (0, 1, 1000, n // 3, n // 2 + 7, n - 2, n - 1):
+        w = torch.softmax(q[t].double() @ k[:t + 1].T / dim**0.5, 1)
+        want, size = w @ v[:t + 1], w @ v[:t + 1].abs()
+        assert ((out[t].double() - want).abs() <= 2.0**-10 * size + 2.0**-11 * want.abs() + 2.0**-24).all(), t
