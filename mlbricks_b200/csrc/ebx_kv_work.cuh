@@ -291,8 +291,8 @@ __device__ __forceinline__ int4 kv_desc(const KvRequest& r, int rt, int rt_rows,
 }
 
 // Weights are 2^(t - m + kShift), m at most kLag below the maximum so far: the largest is below
-// 2^15, and of the fp16 range nothing is left unused below it (a weight 2^-22 of the largest
-// still has all its 11 bits).
+// 2^15 and at least 2^kShift, so that a weight 2^-21 of the largest (2^-14: the smallest normal
+// fp16) still has all its 11 bits.
 constexpr float kLag = 8.0f, kShift = 7.0f;
 // V scale of 16 tokens that no block holds: their keys are not seen.
 constexpr float kKvNone = -1.0f;
