@@ -109,11 +109,13 @@ def serve(steps: int = 24) -> dict:
 
     def decode():
         cache.plan(ones, tokens=rows, max_new=1)
+        missing.add_(cache.ring[2])
         logits.copy_(model(ids, cache=cache))
         ids.copy_(logits.argmax(-1))
 
     logits = torch.empty(rows, VOCAB, dtype=torch.float16, device="cuda")
-    state = [t.clone() for t in (cache.lengths, cache.ring, cache.tables, cache.free, ids)]
+    missing = torch.zeros((), dtype=torch.int64, device="cuda")  # blocks that were not there, over all steps
+    state = [t.clone() for t in (cache.lengths, cache.ring, cache.tables, cache.free, ids, missing)]
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -122,7 +124,7 @@ def serve(steps: int = 24) -> dict:
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         decode()
-    for now, then in zip((cache.lengths, cache.ring, cache.tables, cache.free, ids), state):
+    for now, then in zip((cache.lengths, cache.ring, cache.tables, cache.free, ids, missing), state):
         now.copy_(then)
 
     def run(n):
@@ -138,13 +140,12 @@ def serve(steps: int = 24) -> dict:
     admit([200 if i == 1 else 0 for i in range(rows)])
     ids.copy_(torch.stack([t[-1] for t in texts]))
     run(steps - steps // 2)
-    missing = int(cache.ring[2])
 
     errors = []
     for i in range(rows):
         want = model(texts[i][:-1])[-1].float()
         errors.append(float((logits[i].float() - want).norm() / want.norm()))
-    return {"lengths": cache.lengths.tolist(), "texts": [t.numel() for t in texts], "errors": errors, "missing": missing,
+    return {"lengths": cache.lengths.tolist(), "texts": [t.numel() for t in texts], "errors": errors, "missing": int(missing),
             "free": int(cache.ring[1] - cache.ring[0])}
 
 
