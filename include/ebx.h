@@ -315,6 +315,9 @@ EBX_API ebx_status ebx_exchange_allreduce(ebx_exchange* ex, const float* partial
  * [blocks][kv_heads][block_size][head_dim] and one fp32 scale for each (block,
  * head); value = code * scale.  Row i of a block table (int32 [requests, width])
  * names the blocks that hold request i's tokens, block_size tokens in each.
+ * Scales are >= 0 (ebx_kv_append writes no others but NaN): attention takes V scales
+ * below 2^-100 for 2^-100 and a block with a negative one for no block, and has no
+ * meaning for negative K scales; ebx_kv_materialize multiplies by whatever is there.
  * All pointers are DEVICE memory; every call is stream-ordered on `device` and
  * allocates nothing.  A number on the device that is out of range (a block id, a
  * slot, a length) is never followed: such a token is not written, and not seen. */
@@ -337,12 +340,15 @@ typedef struct {
  * ring[0] .. ring[1] - 1 modulo free_size.  Requests are served in order: each takes
  * the blocks that it lacks from the ring's front into its row of `tables`, or, when
  * they are not there, its row is too short or its tokens do not all lie below `tokens`,
- * nothing (its tokens get slot -1 and its length stays).  Released blocks join the ring's back, for later calls; a released
+ * nothing (its tokens get slot -1 and its length stays).  Nobody overtakes: what a
+ * request needs and does not find still counts for those behind it, so that after the
+ * first one which finds too few, no later one gets a block in this call either; those
+ * that need none go on.  Released blocks join the ring's back, for later calls; a released
  * row's entries are left as they are.  A ring holds free_size blocks at most: of one that
  * claims more the first free_size are used, and released blocks without a place are dropped.
- * Written: ring_out[4] = {front, back, blocks that were missing, sum of the new tokens},
- * lengths [requests] (after the step; 0 when released), starts[requests + 1] (first token
- * of each request among the step's tokens, `tokens` at most), and for t < `tokens` slots[t]
+ * Written: ring_out[4] = {front, back, blocks that the refused requests needed (all of
+ * them, not what the ring was short of), sum of the new tokens}, lengths [requests] (after the step; 0 when released), starts[requests + 1] (first token
+ * of each request among the step's tokens, refused ones too, `tokens` at most), and for t < `tokens` slots[t]
  * = block * block_size + offset and positions[t] (slot -1, position 0 past the last token).
  * `tokens` is the room of slots and positions: the sum of the new tokens or more.  If
  * ring_out[3] is larger, requests were refused for want of room.
@@ -370,7 +376,10 @@ EBX_API ebx_status ebx_kv_append(const ebx_kv_pool* pool, const void* k, int64_t
 /* Keys and values back as code * scale, rounded once to dtype (0 = fp32, 1 = fp16,
  * 2 = bf16): k, v [tokens, kv_heads, head_dim]; row t is place first[i] + t - starts[i]
  * (first NULL: 0) of the request i with starts[i] <= t < starts[i + 1].  Rows of no
- * request, and places without a block, are 0. */
+ * request, and places whose table entry is no block, are 0.  The call knows no lengths:
+ * past what a request holds it reads what the table names there, and entries that are
+ * not yet or no longer the request's (a released row keeps its own) may name another's
+ * block.  The caller keeps first and starts within the lengths. */
 EBX_API ebx_status ebx_kv_materialize(const ebx_kv_pool* pool, const int32_t* tables, int32_t width,
                                       const int32_t* starts, const int32_t* first, int32_t requests,
                                       int64_t tokens, int32_t dtype, void* k, void* v, void* stream);
@@ -384,16 +393,25 @@ EBX_API uint64_t ebx_kv_attention_workspace_bytes(const ebx_kv_pool* pool, int32
 /* Attention of the new tokens' queries over the cache: request i's queries are rows
  * starts[i] .. starts[i + 1] - 1 of q [tokens, heads, head_dim] (strides and dtype as in
  * ebx_kv_append), at the last positions of its lengths[i] tokens; query head h reads
- * key/value head h / (heads / kv_heads).  A query at position p sees keys j with
+ * key/value head h / (heads / kv_heads).  starts do not decrease.  A query at position p sees keys j with
  * first[i] <= j (first may be NULL) and j < lengths[i], and if causal j <= p, and if
  * window > 0 (causal only) j > p - window.
  *     out[t, h] = softmax_j(scale * q . k_j) v_j,  lse[t, h] = log sum_j exp(...)
  * out [tokens, heads, head_dim] in q's dtype, apart from q, and lse fp32 (may be NULL); a
  * query that sees nothing gets out = 0 and lse = -infinity, rows of no request are left as
  * they are.  Sums, maxima and scales are fp32, the
- * weights of the values fp16.  max_new / max_length (0: unknown) are the largest number
- * of new tokens and the largest length of a request where the caller knows them; they
- * choose the kernel and never change what is computed. */
+ * weights of the values fp16, bf16 queries fp16 over the largest power of two in their row
+ * (elements below 2^-14 of it lose bits).
+ * A request that ebx_kv_plan refused still has its rows in starts, and its old length: its
+ * queries are then taken for the last of the tokens that it holds, and the result means
+ * nothing.  The caller drops it (its slots are -1), or gives first[i] = lengths[i], with
+ * which such a request sees nothing.
+ * max_new / max_length (0: unknown) are the largest number of new tokens and the largest
+ * length of a request where the caller knows them; they choose the kernel, and with it
+ * the order of sums, but not the formula: results agree to the roundings above, not bit
+ * for bit.  Without max_new, `tokens` is taken for it, and calls of 49 rows (tokens *
+ * heads / kv_heads) and more go to the kernel for prompts, which takes about three times
+ * as long over single tokens. */
 EBX_API ebx_status ebx_kv_attention(const ebx_kv_pool* pool, const void* q, int64_t q_token_stride,
                                     int64_t q_head_stride, int32_t heads, int32_t dtype,
                                     const int32_t* tables, int32_t width, const int32_t* lengths,

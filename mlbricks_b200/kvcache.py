@@ -62,7 +62,8 @@ def _refuse_ints(device: int, **tensors) -> None:
 
 class KVPool:
     """One layer's cache: int8 codes [blocks, kv_heads, block_size, head_dim] and fp32 scales
-    [blocks, kv_heads], of keys and of values.  Holds the tensors; copies nothing."""
+    [blocks, kv_heads], of keys and of values.  Holds the tensors; copies nothing.  Scales are >= 0, or
+    NaN for a block that holds a value that is not finite, as ``append`` writes them."""
 
     __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "device", "_c", "_ref")
 
@@ -147,7 +148,10 @@ def plan(past: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, free: torc
     ``ring[1]``, modulo its size.  In order, each request takes the blocks that it lacks into its
     row of ``tables`` (written in place) -- or nothing, if they are not all there, the row is too
     short, or its tokens do not fit ``tokens``: they then get slot -1, its length stays, and ``ring[2]``
-    of the result counts the missing blocks.  Released blocks join the ring's back.  ``tokens`` is the
+    of the result counts the blocks that it needed.  Nobody overtakes: behind the first request that
+    finds too few blocks, no other gets one in this step; those that need none go on.  Refused tokens
+    keep their rows (``starts``), so what ``attention`` returns there means nothing: leave out rows with
+    slot -1.  Released blocks join the ring's back.  ``tokens`` is the
     room for slots and positions: the sum of the new tokens, or more (the rest is slot -1, position 0);
     ``ring[3]`` of the result is that sum, so ``ring[3] > tokens`` says that requests were refused for
     want of room.
@@ -207,7 +211,8 @@ def append(k: torch.Tensor, v: torch.Tensor, pool: KVPool, slots: torch.Tensor) 
 def materialize(pool: KVPool, tables: torch.Tensor, starts: torch.Tensor, *, first: torch.Tensor | None = None,
                 tokens: int, dtype: torch.dtype = torch.float16) -> tuple[torch.Tensor, torch.Tensor]:
     """Keys and values [tokens, kv_heads, head_dim] as code * scale, rounded once to ``dtype``:
-    rows starts[i] .. starts[i + 1] - 1 are the places first[i] (default 0) on of request i."""
+    rows starts[i] .. starts[i + 1] - 1 are the places first[i] (default 0) on of request i.  The caller
+    keeps them within what the request holds: behind that the table may name other requests' blocks."""
     if dtype not in _DTYPES:
         raise ValueError("dtype must be float32, float16 or bfloat16")
     requests = starts.numel() - 1
@@ -241,7 +246,9 @@ def attention(q: torch.Tensor, pool: KVPool, tables: torch.Tensor, lengths: torc
     of no request are left as they are, and ``out``, if given, is not q's memory.  ``scale`` defaults to
     1 / sqrt(head_dim).  ``max_new`` and
     ``max_length``, where the caller knows the largest number of new tokens and the largest length,
-    choose the kernel and change no result.  Returns out, or (out, lse [tokens, heads] fp32)."""
+    choose the kernel: they change the order of sums, not the formula.  Without ``max_new`` a batch of
+    49 rows (tokens * heads / kv_heads) and more is taken for a prompt, which costs single tokens about three
+    times their time.  Returns out, or (out, lse [tokens, heads] fp32)."""
     q = pool._rows(q, None, "q")
     device = pool.device
     tokens, heads, dim = q.shape
@@ -300,8 +307,9 @@ class KVCache:
 
     def plan(self, new, tokens: int | None = None, max_new: int | None = None) -> KVPlan:
         """Blocks and slots for a step.  ``new``: a list, or an int32 tensor on the GPU with
-        ``tokens`` (room for all its tokens; requests that end past it are refused) and, if known, ``max_new``.  ``ring[2]`` of the result is
-        the number of blocks that were missing: requests that got none keep their length."""
+        ``tokens`` (room for all its tokens; requests that end past it are refused) and ``max_new``, without which ``attention`` takes a batch
+        of single tokens for a prompt.  ``ring[2]`` of the result is the number of blocks that refused requests
+        needed: they keep their length, their tokens have slot -1, and their rows of ``attention`` mean nothing."""
         if not isinstance(new, torch.Tensor):
             counts = [max(int(n), 0) for n in new]
             tokens, max_new = sum(counts), max(counts, default=0)

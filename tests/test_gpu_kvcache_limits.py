@@ -138,3 +138,30 @@ def test_attention_with_more_key_tiles_than_31_bits_count():
         w = torch.softmax(q[t].double() @ k[:t + 1].T / dim**0.5, 1)
         want, size = w @ v[:t + 1], w @ v[:t + 1].abs()
         assert ((out[t].double() - want).abs() <= 2.0**-10 * size + 2.0**-11 * want.abs() + 2.0**-24).all(), t
+
+
+def test_nobody_overtakes_a_request_that_finds_too_few_blocks():
+    """The first lacks 63 blocks of 3; the second needs one and waits, the third needs none and goes on."""
+    tables = i32([[5] + [-1] * 63, [6, -1] + [-1] * 62, [7] + [-1] * 63])
+    step = kv.plan(i32([16, 16, 3]), i32([1000, 1, 2]), tables, i32([1, 2, 3, 0]), i64([0, 3]), block_size=16, tokens=1003)
+    assert step.lengths.tolist() == [16, 16, 5] and step.ring.tolist() == [0, 3, 64, 1003]
+    assert step.starts.tolist() == [0, 1000, 1001, 1003]
+    assert (step.slots[:1001] == -1).all() and step.slots[1001:].tolist() == [7 * 16 + 3, 7 * 16 + 4]
+
+
+@pytest.mark.parametrize("new", [1, 60])
+def test_a_refused_request_sees_nothing_from_its_length_on(new):
+    cache = kv.KVCache(1, blocks=6, kv_heads=1, head_dim=32, requests=2, max_length=96, block_size=16)
+    x = torch.randn(42, 1, 32, device="cuda", dtype=torch.float16)
+    cache.plan([32, 10])
+    cache.append(0, x, x)
+    held = cache.lengths.clone()
+    step = cache.plan([80, new])  # the first does not fit its row; the second may find its blocks
+    fits = new == 1
+    assert cache.lengths.tolist() == [32, 10 + new if fits else 10]
+    q = torch.randn(80 + new, 2, 32, device="cuda", dtype=torch.float16)
+    refused = step.lengths == held
+    out, lse = cache.attention(0, q, first=torch.where(refused, step.lengths, 0).int(), return_lse=True)
+    gone = step.slots < 0
+    assert gone.sum() == (80 if fits else 80 + new)
+    assert not out[gone].any() and (lse[gone] == -torch.inf).all() and lse[~gone].isfinite().all()
