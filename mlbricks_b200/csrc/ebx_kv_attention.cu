@@ -485,8 +485,10 @@ namespace {
 // tokens, 2 heads of 64, 48 rows 39 / 54, 64 rows 47 / 54; one request of 16000, 48 rows 31 / 41.
 constexpr int kPromptMin = 49;
 
-// Short requests: a second launch, to join, would cost more than sharing row tiles gains (8
-// requests of 600 tokens over one head of 32: 17.1 us in place of 20.5).
+// Short requests: a second launch, to join, would cost more than sharing row tiles gains.  With / without
+// this, captured: 8 requests of 600 tokens, 12 heads over one of 32, 9.5 / 12.5 us; 8 of 256, 32 heads over 8 of 128,
+// 7.7 / 11.4; 64 of 100 11.7 / 12.8, of 256 15.4 / 14.9.  At twice the length it depends on how many there are:
+// 8 of 512 9.9 / 12.0, 64 of 512 23.2 / 19.8.
 bool takes_whole(int head_dim, int max_length) {
     constexpr int kTiles = 4;
     return max_length > 0 && max_length <= kTiles * (8192 / head_dim);

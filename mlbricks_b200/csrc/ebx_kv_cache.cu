@@ -2,7 +2,6 @@
 // keys and values (append), and reading them back (materialize).  No reference counterpart:
 // the reference's caches (mlbricks/cache.py) hold whole 16-bit tensors.
 #include <algorithm>
-#include <atomic>
 
 #include "ebx_common.cuh"
 #include "ebx_kv.h"
@@ -215,8 +214,10 @@ __device__ __forceinline__ uint2 quant8(const uint4& x, float s, float r) {
 // Runs, not blocks, are the unit because the slots alone then say everything: no atomics, no second
 // pass over other warps' tokens.  A run's values stay in registers between the largest and the codes
 // (up to 16 tokens at head_dim 128; longer ones are read again from L2).  What bounds it: 27 424
-// tokens of 8 heads of 128 in bf16 take 42 us = 4.0 TB/s of 168 MB, the integer pipe half busy and
-// the issue slots 62 %; with a division for each value it was 78 us.
+// tokens of 8 heads of 128 in bf16 take 42 us = 4.0 TB/s of 168 MB.  Nothing is full (DRAM 40 %, the
+// integer pipe 51 %, the issue slots 62 %): a warp takes its runs in turn, load, largest, codes, store,
+// and waits for memory at each, with a third of an SM's warps there to fill in.  With a division for
+// each value it was 78 us.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kAppendWarps * 32)
     kv_append_kernel(KvPool pool, KvRows k, KvRows v, const int64_t* slots, int64_t tokens, int span) {
@@ -426,6 +427,9 @@ cudaError_t launch_kv_plan(const KvPlanArgs& a, cudaStream_t s) {
         if (e != cudaSuccess) return e;
     }
     const int64_t work = std::max<int64_t>(a.tokens, a.requests);
+    // Every CTA repeats the sums, so more of them pay where the tokens are many and the requests few.
+    // At most 148 / 592 / 1184 of them, captured: 64 requests of 2048 tokens 5.3 / 4.9 / 4.9 us, 16 of 8000
+    // 4.9 / 4.6 / 4.6, but 1000 of 120 9.5 / 12.8 / 12.8.
     const int64_t grid = std::min<int64_t>((work + kPlanThreads - 1) / kPlanThreads, 592);
     return launch_early(kv_plan_kernel, dim3(unsigned(std::max<int64_t>(grid, 1))), kPlanThreads, smem, s, a);
 }
@@ -433,7 +437,11 @@ cudaError_t launch_kv_plan(const KvPlanArgs& a, cudaStream_t s) {
 cudaError_t launch_kv_append(const KvPool& pool, const KvRows& k, const KvRows& v, const int64_t* slots,
                              int64_t tokens, bool bf16, cudaStream_t s) {
     if (tokens <= 0) return cudaSuccess;
-    // a warp looks through `span` tokens for the runs that begin there: one when there are few
+    // A warp looks through `span` tokens for the runs that begin there: 16, or one when there are few.  The
+    // host does not know whether the tokens follow one another.  If they do, 16 spares reading slots (8 heads of
+    // 128, 16 / one: 512 tokens 9.4 / 10.6 us, 2048 tokens 18.5 / 24.0); if each is in a block of its own, a warp has
+    // 16 runs to take in turn (64 tokens 19.8 / 3.2 us, 512 tokens 20.2 / 7.0, 2048 tokens 30.2 / 21.6).  So
+    // one for as many tokens as steps bring.
     const int span = tokens * pool.kv_heads <= 4096 ? 1 : 16;
     const int64_t items = (tokens + span - 1) / span * pool.kv_heads;
     const int64_t grid = (items + kAppendWarps - 1) / kAppendWarps;
