@@ -163,8 +163,8 @@ ebx_status ebx_kv_attention(const ebx_kv_pool* pool, const void* q, int64_t q_to
     if (window < 0 || (window > 0 && !causal)) return invalid("ebx_kv_attention: a window is causal and > 0");
     if (!std::isfinite(scale * 1.4426950408889634f)) return invalid("ebx_kv_attention: scale must be finite");
     if (max_new < 0 || max_length < 0) return invalid("ebx_kv_attention: max_new and max_length are >= 0");
-    if (tokens == 0) return EBX_OK;
-    if (!out || !starts || requests == 0 || !tables || !lengths) return invalid("null argument");
+    if (tokens == 0 || requests == 0) return EBX_OK;  // rows of no request are left as they are
+    if (!out || !starts || !tables || !lengths) return invalid("null argument");
     ebx::KvRows rows;
     if (const char* msg = rows_of(q, q_token_stride, q_head_stride, rows)) return invalid(msg);
     if (!aligned16(out) || !aligned16(workspace))

@@ -42,3 +42,10 @@ def test_materialize_refuses_tokens_wider_than_it_counts(kv_heads, head_dim):
     lib = _ebx.load()
     wide = pool(blocks=1, kv_heads=kv_heads, head_dim=head_dim)
     refused(lib.ebx_kv_materialize(wide, 4, 1, 4, None, 1, 1, 1, 16, 16, None), "2^30")
+
+
+def test_attention_without_requests_has_nothing_to_do():
+    """Rows of no request are left as they are: that is no error."""
+    lib = _ebx.load()
+    assert lib.ebx_kv_attention(pool(), 16, 256, 64, 4, 1, None, 1, None, 4, None, 0, 5, 1, 0, 1.0, 0, 0, 16, None, None,
+                                0, None) == _ebx.EBX_OK
