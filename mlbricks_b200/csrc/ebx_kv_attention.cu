@@ -37,7 +37,7 @@ __device__ __forceinline__ bool kv_wait(uint32_t bar, uint32_t parity) {
 // 8 queries its columns, so a group of four heads fills half of the product and not a quarter of one
 // with 16 rows (166 -> 112 us for 64 requests), and V is never transposed: its fragments are byte
 // permutes of four rows.  What bounds it: 64 requests of 1 to 8192 tokens, 8 heads of 128, stream
-// 568 MB in 93 us inside the kernel = 6.1 TB/s, 0.93 of a copy's rate; the call takes 107 us with its
+// 568 MB in 93 to 96 us inside the kernel = 6.0 TB/s, 0.91 of a copy's rate; the call takes 107 us with its
 // launch, the shares and the join.  Two CTAs with four stages 114 us, four CTAs with two 120 us.
 
 constexpr int kConsumers = 4;    // warps that compute; one more loads
