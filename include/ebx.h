@@ -420,6 +420,31 @@ EBX_API ebx_status ebx_kv_attention(const ebx_kv_pool* pool, const void* q, int6
                                     int32_t max_new, int32_t max_length, void* out, float* lse,
                                     void* workspace, uint64_t workspace_bytes, void* stream);
 
+/* ---- rotary positions --------------------------------------------------------
+ * No reference counterpart.  A pair (a, b) of a head's elements, of a token at
+ * position p, with the pair's frequency f (radians a position), becomes
+ *     scale * (a cos(p f) - b sin(p f)),  scale * (b cos(p f) + a sin(p f)).
+ * Pair i of rotary_dim / 2 is elements (i, rotary_dim / 2 + i), or (2 i, 2 i + 1) if
+ * interleaved; elements from rotary_dim on are copied.  p f is reduced to one turn in
+ * 64 bits, products and sums are fp32, rounded once to dtype (0 = fp32, 1 = fp16,
+ * 2 = bf16).  positions: int32 or int64 [tokens], any sign; frequencies: fp32 or fp64
+ * [rotary_dim / 2].  A side is [tokens, heads, head_dim] whose last dimension is
+ * contiguous; strides in elements.  out is in, with the same strides, or shares no
+ * element with it; no two sides share elements.  k may be NULL, heads may be 0.
+ * 16-byte aligned bases, strides of 16 bytes and rotary_dim / 2 of as many are fastest. */
+typedef struct {
+    const void* in;
+    void* out;
+    int64_t in_token_stride, in_head_stride, out_token_stride, out_head_stride;
+    int32_t heads;
+    int32_t reserved;
+} ebx_rotary_side;
+
+EBX_API ebx_status ebx_rotate(const ebx_rotary_side* q, const ebx_rotary_side* k, int32_t head_dim,
+                              int32_t rotary_dim, int32_t dtype, const void* positions,
+                              int32_t position_bits, const void* frequencies, int32_t frequency_bits,
+                              int64_t tokens, int32_t interleaved, float scale, int32_t device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -68,6 +68,22 @@ class KVPool(ctypes.Structure):  # ebx_kv_pool
 
 _KV = ctypes.POINTER(KVPool)
 
+
+class RotarySide(ctypes.Structure):  # ebx_rotary_side
+    _fields_ = [
+        ("input", ctypes.c_void_p),
+        ("output", ctypes.c_void_p),
+        ("in_token_stride", ctypes.c_int64),
+        ("in_head_stride", ctypes.c_int64),
+        ("out_token_stride", ctypes.c_int64),
+        ("out_head_stride", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+_ROT = ctypes.POINTER(RotarySide)
+
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ebx_version": (ctypes.c_char_p, []),
     "ebx_last_error": (ctypes.c_size_t, [ctypes.c_char_p, ctypes.c_size_t]),
@@ -106,6 +122,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ebx_kv_attention": (
         _ST, [_KV, _P, _I64, _I64, _I32, _I32, _P, _I32, _P, _P, _P, _I32, _I64, _I32, _I32,
               ctypes.c_float, _I32, _I32, _P, _P, _P, _U64, _P]),
+    "ebx_rotate": (
+        _ST, [_ROT, _ROT, _I32, _I32, _I32, _P, _I32, _P, _I32, _I64, _I32, ctypes.c_float, _I32, _P]),
     "ebx_elastic_linear_packed": (
         _ST, [_P, _I32, _I64, _P, _P, _I32, _P, _I32, _I64, _I64, _I64, _P, _P]),
 }
@@ -162,4 +180,4 @@ def stream_ptr(stream=None, device: int | None = None) -> int:
     return int(torch.cuda.current_stream(device).cuda_stream)
 
 
-__all__ = ["LIB_PATH", "KVPool", "MatrixInfo", "SIGNATURES", "load", "last_error", "check", "stream_ptr"]
+__all__ = ["LIB_PATH", "KVPool", "MatrixInfo", "RotarySide", "SIGNATURES", "load", "last_error", "check", "stream_ptr"]

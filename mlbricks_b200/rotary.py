@@ -1,0 +1,119 @@
+"""Rotary positions of queries and keys (``libebx``, include/ebx.h ``ebx_rotate``).
+
+``rotate`` turns pairs of a head's elements by angles that grow with the token's position, in one launch
+for queries and keys: half and interleaved pairs, a part of the head, positions as
+``mlbricks_b200.kvcache.plan`` gives them.  ``frequencies`` gives the pairs' frequencies, scaled for
+contexts longer than those that a model was trained on.  Inference only, as the rest of the native route: no
+autograd.  The reference has no counterpart.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _ebx
+from .kvcache import _DTYPES, _stream
+
+SCALINGS = ("none", "linear", "base", "ramp")
+
+
+def frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str = "none", factor: float = 1.0,
+                trained_length: int = 0, slow: float = 1.0, fast: float = 32.0, device="cuda") -> torch.Tensor:
+    """Angles [rotary_dim / 2] (float64) of the pairs at position 1: base ** (-2 i / rotary_dim), and for
+    contexts ``factor`` times as long as trained
+
+    * ``"linear"``: all divided by ``factor``;
+    * ``"base"``: a larger base, with which the slowest pair is divided by ``factor`` and the fastest kept;
+    * ``"ramp"``: pairs that make ``slow`` turns or fewer within ``trained_length`` are divided by
+      ``factor``, those that make ``fast`` or more are kept, those between go from one to the other."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
+    if scaling not in SCALINGS:
+        raise ValueError(f"scaling must be one of {SCALINGS}, got {scaling!r}")
+    if not (base > 0 and math.isfinite(base) and factor > 0 and math.isfinite(factor)):
+        raise ValueError("base and factor must be positive and finite")
+    half = rotary_dim // 2
+    if scaling == "base" and half > 1:
+        base = base * factor ** (half / (half - 1))
+    freq = base ** (-torch.arange(half, dtype=torch.float64) / half)
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "ramp":
+        if trained_length <= 0 or not fast > slow:
+            raise ValueError("a ramp needs trained_length > 0 and fast > slow")
+        turns = trained_length * freq / (2 * math.pi)
+        keep = ((turns - slow) / (fast - slow)).clamp(0, 1)
+        freq = freq / factor * (1 - keep) + freq * keep
+    return freq.to(device)
+
+
+def _apart(x: torch.Tensor) -> bool:
+    """No two elements of x at one place."""
+    room = 1
+    for stride, size in sorted((s, n) for s, n in zip(x.stride(), x.shape) if n > 1):
+        if stride < room:
+            return False
+        room = stride * (size - 1) + room
+    return True
+
+
+def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, frequencies: torch.Tensor, *,
+           interleaved: bool = False, scale: float = 1.0, inplace: bool = False):
+    """Queries [tokens, heads, head_dim] and keys [tokens, kv_heads, head_dim] (fp16, bf16 or fp32, any
+    strides) turned by ``positions`` [tokens] (int32 or int64, any sign) times ``frequencies``
+    [rotary_dim / 2] (float64 or float32).  Pair i is elements (i, rotary_dim / 2 + i) of a head, or (2 i, 2 i + 1) if
+    ``interleaved``; elements from rotary_dim on stay as they are.  ``scale`` multiplies what was turned.
+
+    Returns (q, k) as new contiguous tensors, or, ``inplace``, the same tensors turned where they are (their
+    last dimension is then contiguous, and they share no elements).  ``k`` may be None."""
+    dtype, device, tokens = q.dtype, q.get_device(), q.shape[0] if q.dim() == 3 else -1
+    if device < 0:
+        raise ValueError("rotate needs CUDA tensors")
+    if dtype not in _DTYPES:
+        raise ValueError("q must be float32, float16 or bfloat16")
+    if tokens < 0 or (k is not None and (k.dim() != 3 or k.shape[0] != tokens or k.shape[2] != q.shape[2])):
+        raise ValueError("q and k must be [tokens, heads, head_dim] with the same tokens and head_dim")
+    if k is not None and (k.dtype is not dtype or k.get_device() != device):
+        raise ValueError("q and k must have the same dtype and device")
+    dim = q.shape[2]
+    if (positions.dtype not in (torch.int32, torch.int64) or positions.get_device() != device
+            or positions.dim() != 1 or positions.shape[0] != tokens or not positions.is_contiguous()):
+        raise ValueError(f"positions must be a contiguous int32 or int64 tensor [{tokens}] on cuda:{device}")
+    if (frequencies.dtype not in (torch.float32, torch.float64) or frequencies.get_device() != device
+            or frequencies.dim() != 1 or not frequencies.is_contiguous()):
+        raise ValueError(f"frequencies must be a contiguous float64 or float32 tensor on cuda:{device}")
+    part = 2 * frequencies.shape[0]
+    if not 2 <= part <= dim:
+        raise ValueError(f"frequencies must be 1 to {dim // 2}, half of the elements that turn, got {part // 2}")
+    if inplace and k is not None and q.data_ptr() == k.data_ptr() and q.numel() and k.numel():
+        raise ValueError("q and k must not be the same memory")
+    sides, out, copies = [], [], []
+    for x in (q, k):
+        if x is None:
+            sides.append(None)
+            out.append(None)
+            continue
+        if inplace:
+            if (dim > 1 and x.stride(2) != 1) or not _apart(x):
+                raise ValueError("a tensor that is turned in place has a contiguous last dimension and no element twice")
+            y = x
+        else:
+            if x.stride(2) != 1:
+                x = x.contiguous()
+                copies.append(x)  # until the launch, or its memory may become an output's
+            y = torch.empty(x.shape, dtype=dtype, device=x.device)
+        sides.append(_ebx.RotarySide(x.data_ptr(), y.data_ptr(), x.stride(0), x.stride(1), y.stride(0), y.stride(1),
+                                     x.shape[1], 0))
+        out.append(y)
+    st = _ebx.load().ebx_rotate(
+        ctypes.byref(sides[0]), None if k is None else ctypes.byref(sides[1]), dim, part, _DTYPES[dtype],
+        positions.data_ptr(), 64 if positions.dtype is torch.int64 else 32, frequencies.data_ptr(),
+        64 if frequencies.dtype is torch.float64 else 32, tokens, interleaved, scale, device, _stream(device))
+    if st:
+        _ebx.check(st)
+    return out[0], out[1]
+
+
+__all__ = ["SCALINGS", "frequencies", "rotate"]
