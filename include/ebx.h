@@ -420,6 +420,52 @@ EBX_API ebx_status ebx_kv_attention(const ebx_kv_pool* pool, const void* q, int6
                                     int32_t max_new, int32_t max_length, void* out, float* lse,
                                     void* workspace, uint64_t workspace_bytes, void* stream);
 
+/* ---- requests that share cache blocks ------------------------------------------
+ * No reference counterpart.  `shares` (int32 [blocks]) holds for every block the
+ * number of rows beyond the first that hold it: 0 for a free block, and for one that a
+ * single row holds, so ebx_kv_plan need not know of it, except that rows are then
+ * released by ebx_kv_fork and not by ebx_kv_plan.  Only full blocks are shared.
+ *
+ * Row r of the table goes on from the first keep[r] tokens (keep NULL, or more than
+ * there are: all) of what row parents[r] held: itself, another row, or none (a
+ * number that is no row) for a row that is done.  Full blocks are shared.  Of a block that
+ * is begun and that no row now holds whole, the first row that wants it keeps it, the parent itself
+ * ahead of others; every other row gets a block from the ring's front in its place, in row
+ * order, with a copy to be made by ebx_kv_copy.  Where no block is left the row holds nothing
+ * afterwards (length 0), and ring_out[2] counts it.  Blocks that nobody holds any more join
+ * the ring's back by rising number, for later calls.  The ring is ebx_kv_plan's.
+ * Written: out_lengths [requests], out_tables [requests, width] (-1 behind what a row
+ * holds), out_shares [blocks], ring_out[4] = {front, back, blocks that were missing, copies},
+ * sources and targets [requests] (block numbers, -1 behind the last copy).  No output is an
+ * input.  Entries that are no block are kept and not counted.  workspace: 4 * blocks bytes.
+ * requests <= 16384, width * block_size and blocks * block_size < 2^31. */
+EBX_API ebx_status ebx_kv_fork(const int32_t* lengths, const int32_t* tables, int32_t width,
+                               int32_t block_size, const int32_t* shares, int32_t blocks,
+                               int32_t* free_ring, int32_t free_size, const int64_t* ring,
+                               const int32_t* parents, const int32_t* keep, int32_t requests,
+                               int32_t* out_lengths, int32_t* out_tables, int32_t* out_shares,
+                               int64_t* ring_out, int32_t* sources, int32_t* targets,
+                               void* workspace, uint64_t workspace_bytes, int32_t device, void* stream);
+
+/* New numbers for the blocks that rows hold, so that they are the pool's first: of H held
+ * blocks those numbered H or more move to the free numbers below H, in order, with copies to be
+ * made by ebx_kv_copy.  Every other block is free afterwards, also one that neither a
+ * row nor the ring had: free_out [blocks] holds their numbers, rising, then -1, and
+ * ring_out[4] = {0, blocks - H, 0, copies}.  out_tables as in ebx_kv_fork; sources and targets
+ * [blocks / 2], -1 behind the last copy.  No output is an input; workspace and limits as above. */
+EBX_API ebx_status ebx_kv_compact(const int32_t* lengths, const int32_t* tables, int32_t width,
+                                  int32_t block_size, const int32_t* shares, int32_t blocks,
+                                  int32_t requests, int32_t* out_tables, int32_t* out_shares,
+                                  int32_t* free_out, int64_t* ring_out, int32_t* sources,
+                                  int32_t* targets, void* workspace, uint64_t workspace_bytes,
+                                  int32_t device, void* stream);
+
+/* Blocks sources[j] to targets[j] of each of `layers` pools (equal sizes, one device), codes and
+ * scales, j < n and, if count is not NULL, j < *count (DEVICE).  Pairs with a number that is no
+ * block are skipped.  No target is another pair's source or target. */
+EBX_API ebx_status ebx_kv_copy(const ebx_kv_pool* pools, int32_t layers, const int32_t* sources,
+                               const int32_t* targets, const int64_t* count, int32_t n, void* stream);
+
 /* ---- rotary positions --------------------------------------------------------
  * No reference counterpart.  A pair (a, b) of a head's elements, of a token at
  * position p, with the pair's frequency f (radians a position), becomes

@@ -1,0 +1,111 @@
+// ebx_kv_share_capi.cu -- the extern "C" entries for requests that share cache blocks (include/ebx.h): every
+// check that the host can make, then the launch.
+#include <algorithm>
+
+#include "ebx_kv_check.h"
+#include "ebx_kv_share.h"
+
+namespace {
+
+// Null, or what is wrong with a table of `requests` rows over `blocks` blocks.
+const char* table_of(int32_t requests, int32_t width, int32_t block_size, int32_t blocks) {
+    if (requests < 0 || requests > ebx::kKvMaxRequests) return "kv tables: need 0 <= requests <= 16384";
+    if (log2_of(block_size) < 0) return "kv tables: block_size must be 16, 32, 64 or 128";
+    if (width < 1 || int64_t(width) * block_size > INT32_MAX) return "kv tables: need width >= 1 and width * block_size < 2^31";
+    if (blocks < 1 || int64_t(blocks) * block_size > INT32_MAX) return "kv tables: need blocks >= 1 and blocks * block_size < 2^31";
+    return nullptr;
+}
+
+}  // namespace
+
+extern "C" {
+
+ebx_status ebx_kv_fork(const int32_t* lengths, const int32_t* tables, int32_t width, int32_t block_size,
+                       const int32_t* shares, int32_t blocks, int32_t* free_ring, int32_t free_size,
+                       const int64_t* ring, const int32_t* parents, const int32_t* keep, int32_t requests,
+                       int32_t* out_lengths, int32_t* out_tables, int32_t* out_shares, int64_t* ring_out,
+                       int32_t* sources, int32_t* targets, void* workspace, uint64_t workspace_bytes,
+                       int32_t device, void* stream) {
+    if (const char* msg = table_of(requests, width, block_size, blocks)) return invalid(msg);
+    if (!shares || !free_ring || !ring || !out_shares || !ring_out || !workspace ||
+        (requests > 0 && (!lengths || !tables || !parents || !out_lengths || !out_tables || !sources || !targets)))
+        return invalid("null argument");
+    if (free_size < 1) return invalid("ebx_kv_fork: need free_size >= 1");
+    if (out_shares == shares || ring_out == ring ||
+        (requests > 0 && (out_lengths == lengths || out_tables == tables)))
+        return invalid("ebx_kv_fork: outputs must not be inputs");
+    if (workspace_bytes < uint64_t(blocks) * 4) {
+        ebx::set_error("ebx_kv_fork: workspace smaller than 4 * blocks bytes");
+        return EBX_ERR_WORKSPACE;
+    }
+    Device d(device);
+    if (d.err != cudaSuccess) return launched(d.err, "cudaSetDevice");
+    const ebx::KvForkArgs a{lengths, tables, shares, free_ring, ring, parents, keep, out_lengths, out_tables, out_shares,
+                            ring_out, sources, targets, static_cast<int32_t*>(workspace), requests, width,
+                            log2_of(block_size), blocks, free_size};
+    return launched(ebx::launch_kv_fork(a, static_cast<cudaStream_t>(stream)), "ebx_kv_fork");
+}
+
+ebx_status ebx_kv_compact(const int32_t* lengths, const int32_t* tables, int32_t width, int32_t block_size,
+                          const int32_t* shares, int32_t blocks, int32_t requests, int32_t* out_tables,
+                          int32_t* out_shares, int32_t* free_out, int64_t* ring_out, int32_t* sources,
+                          int32_t* targets, void* workspace, uint64_t workspace_bytes, int32_t device, void* stream) {
+    if (const char* msg = table_of(requests, width, block_size, blocks)) return invalid(msg);
+    if (!shares || !out_shares || !free_out || !ring_out || !workspace || (blocks > 1 && (!sources || !targets)) ||
+        (requests > 0 && (!lengths || !tables || !out_tables)))
+        return invalid("null argument");
+    if (out_shares == shares || (requests > 0 && out_tables == tables))
+        return invalid("ebx_kv_compact: outputs must not be inputs");
+    if (workspace_bytes < uint64_t(blocks) * 4) {
+        ebx::set_error("ebx_kv_compact: workspace smaller than 4 * blocks bytes");
+        return EBX_ERR_WORKSPACE;
+    }
+    Device d(device);
+    if (d.err != cudaSuccess) return launched(d.err, "cudaSetDevice");
+    const ebx::KvCompactArgs a{lengths, tables, shares, out_tables, out_shares, free_out, ring_out, sources, targets,
+                               static_cast<int32_t*>(workspace), requests, width, log2_of(block_size), blocks};
+    return launched(ebx::launch_kv_compact(a, static_cast<cudaStream_t>(stream)), "ebx_kv_compact");
+}
+
+ebx_status ebx_kv_copy(const ebx_kv_pool* pools, int32_t layers, const int32_t* sources, const int32_t* targets,
+                       const int64_t* count, int32_t n, void* stream) {
+    if (layers < 0 || n < 0) return invalid("ebx_kv_copy: need layers >= 0 and n >= 0");
+    if (layers == 0) return EBX_OK;
+    if (!pools) return invalid("null argument");
+    for (int32_t i = 0; i < layers; ++i) {
+        ebx::KvPool p;
+        if (const char* msg = pool_of(pools + i, p)) return invalid(msg);
+        if (pools[i].blocks != pools->blocks || pools[i].kv_heads != pools->kv_heads ||
+            pools[i].block_size != pools->block_size || pools[i].head_dim != pools->head_dim ||
+            pools[i].device != pools->device)
+            return invalid("ebx_kv_copy: pools must have the same sizes and device");
+    }
+    if (n == 0) return EBX_OK;
+    if (!sources || !targets) return invalid("null argument");
+    Device d(pools->device);
+    if (d.err != cudaSuccess) return launched(d.err, "cudaSetDevice");
+    const int sms = ebx::gemm_sm_count(pools->device);
+    ebx::KvCopyArgs a{};
+    a.sources = sources;
+    a.targets = targets;
+    a.count = count;
+    a.bytes = int64_t(pools->kv_heads) * pools->block_size * pools->head_dim;
+    a.n = n;
+    a.blocks = pools->blocks;
+    a.kv_heads = pools->kv_heads;
+    for (int32_t first = 0; first < layers; first += ebx::kKvCopyLayers) {
+        a.layers = std::min(layers - first, int32_t(ebx::kKvCopyLayers));
+        for (int i = 0; i < a.layers; ++i) {
+            const ebx_kv_pool& p = pools[first + i];
+            a.layer[i].codes[0] = static_cast<int8_t*>(p.k_codes);
+            a.layer[i].codes[1] = static_cast<int8_t*>(p.v_codes);
+            a.layer[i].scales[0] = p.k_scales;
+            a.layer[i].scales[1] = p.v_scales;
+        }
+        const ebx_status st = launched(ebx::launch_kv_copy(a, sms, static_cast<cudaStream_t>(stream)), "ebx_kv_copy");
+        if (st != EBX_OK) return st;
+    }
+    return EBX_OK;
+}
+
+}  // extern "C"
