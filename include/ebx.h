@@ -466,6 +466,37 @@ EBX_API ebx_status ebx_kv_compact(const int32_t* lengths, const int32_t* tables,
 EBX_API ebx_status ebx_kv_copy(const ebx_kv_pool* pools, int32_t layers, const int32_t* sources,
                                const int32_t* targets, const int64_t* count, int32_t n, void* stream);
 
+/* Which of a step's requests share a prefix, for ebx_kv_shared_attention: starts and lengths as for
+ * ebx_kv_attention.  Requests that bring tokens and whose rows begin with the same block are candidates
+ * for a group, which shares as many full blocks, equal in all its members' rows and ahead of all
+ * its new tokens, as save most reading; who has fewer in common with the group's first request is left out.  Rows
+ * that share nothing are taken alone.  `prefixes` receives ebx_kv_prefixes_ints(requests, tokens) ints, whose
+ * layout is the library's own and which hold for one step: as long as tables (where blocks are shared), starts
+ * and `tokens` stay, for every layer.  workspace: 24 * requests + 4 * blocks bytes, 16-byte aligned. */
+EBX_API uint64_t ebx_kv_prefixes_ints(int32_t requests, int64_t tokens);
+EBX_API ebx_status ebx_kv_prefixes(const int32_t* tables, int32_t width, int32_t block_size,
+                                   int32_t blocks, const int32_t* lengths, const int32_t* starts,
+                                   int32_t requests, int64_t tokens, int32_t* prefixes, void* workspace,
+                                   uint64_t workspace_bytes, int32_t device, void* stream);
+
+/* ebx_kv_attention without window and `first`, for requests that share prefixes: the formula is the same,
+ * but a group's shared keys and values are read once for the rows of all its members, and
+ * the results over the prefix and over the rest joined in fp32.  Where a request brings many rows
+ * of its own (max_new, or without it `tokens`, times heads / kv_heads, 49 and more), requests go
+ * by themselves, as in ebx_kv_attention.  requests <= 16384.  `prefixes` of another step, or of other tables,
+ * make the result meaningless, but nothing outside the buffers is touched. */
+EBX_API uint64_t ebx_kv_shared_attention_workspace_bytes(const ebx_kv_pool* pool, int32_t heads,
+                                                         int64_t tokens, int32_t max_new,
+                                                         int32_t max_length);
+EBX_API ebx_status ebx_kv_shared_attention(const ebx_kv_pool* pool, const void* q,
+                                           int64_t q_token_stride, int64_t q_head_stride, int32_t heads,
+                                           int32_t dtype, const int32_t* tables, int32_t width,
+                                           const int32_t* lengths, const int32_t* starts,
+                                           const int32_t* prefixes, int32_t requests, int64_t tokens,
+                                           int32_t causal, float scale, int32_t max_new,
+                                           int32_t max_length, void* out, float* lse, void* workspace,
+                                           uint64_t workspace_bytes, void* stream);
+
 /* ---- rotary positions --------------------------------------------------------
  * No reference counterpart.  A pair (a, b) of a head's elements, of a token at
  * position p, with the pair's frequency f (radians a position), becomes

@@ -63,6 +63,17 @@ struct KvAttnArgs {
     // partial results of row tiles that several CTAs share
     float* part;           // [grid][2][rows][head_dim + 2]
     int4* desc;            // [grid]
+    // Requests that share prefixes: the kernels' requests 0 .. groups - 1 are then the groups, whose rows are the
+    // tokens in `list` and whose keys are those that the group shares, and the requests proper follow.
+    int groups;
+    const int32_t* group_starts;  // [groups + 1]
+    const int32_t* shared;        // [groups]: tokens that the group shares, in the row of its number
+    const int32_t* own_first;     // [groups]: a request's first token that it does not share
+    const int32_t* list;
+    const int32_t* state;         // [tokens], KvPrefixes
+    float* sums;                  // [2][tokens * heads][head_dim]: O of a row that one CTA has whole,
+    float2* sums_ml;              // [2][tokens * heads]: its {m, l}; of the prefix, and of what is the request's own
+    int2* where;                  // [2][tokens * heads]: which CTAs have a row's parts (kv_where)
 
     // With 2^(k-1) < g <= 2^k and mul = ceil(2^(31+k) / g), mul * g exceeds 2^(31+k) by less than
     // g <= 2^k, so n * mul >> (31 + k) is n / g for every n < 2^31.
@@ -83,11 +94,15 @@ cudaError_t launch_kv_materialize(const KvPool& pool, const int32_t* tables, int
                                   int64_t tokens, int dtype, void* k, void* v, cudaStream_t s);
 uint64_t kv_attention_workspace_bytes(int head_dim, int group, int64_t tokens, int max_new, int max_length);
 cudaError_t launch_kv_attention(KvAttnArgs a, bool bf16, int max_new, int max_length, void* ws, cudaStream_t s);
+// Over the prefixes that `a` names as well (state, list and so on).
+uint64_t kv_shared_workspace_bytes(int head_dim, int heads, int group, int64_t tokens, int max_new, int max_length);
+cudaError_t launch_kv_shared_attention(KvAttnArgs a, bool bf16, int max_new, int max_length, void* ws, cudaStream_t s);
 cudaError_t read_kv_status(int* status, bool clear, cudaStream_t s);
 
 // ebx_kv_prompt.cu: the same for many rows.
 uint64_t kv_prompt_workspace_bytes(int head_dim, int sms);
 cudaError_t launch_kv_prompt(const KvAttnArgs& a, bool bf16, void* ws, int dev, cudaStream_t s);
+cudaError_t launch_kv_prompt_shared(const KvAttnArgs& a, bool bf16, void* ws, int dev, cudaStream_t s);
 cudaError_t read_kv_prompt_status(int* status, bool clear, cudaStream_t s);
 
 // A launch that may begin while the grid before it ends: the kernel waits (griddepcontrol.wait)

@@ -90,7 +90,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     return r;
 }
 
-template <int D, int NQ, bool BF16>
+template <int D, int NQ, bool BF16, bool SHARED>
 __global__ void __launch_bounds__(kStepThreads, (StepCfg<D, NQ>::PER_SM))
     kv_step_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                    const __grid_constant__ KvAttnArgs a, int least) {
@@ -117,12 +117,12 @@ __global__ void __launch_bounds__(kStepThreads, (StepCfg<D, NQ>::PER_SM))
         fence_proxy_async_smem();
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");  // nothing of the call's inputs is read before
-    const KvShare share = kv_share<kRows, KT, kStepExtra, kStepThreads>(a, least, reinterpret_cast<int*>(smem));
+    const KvShare share = kv_share<kRows, KT, kStepExtra, kStepThreads, SHARED>(a, least, reinterpret_cast<int*>(smem));
     fence_proxy_async_smem();  // the ring's copies may overwrite what kv_share kept there
-    if (threadIdx.x == 0 && !a.whole) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (!SHARED && threadIdx.x == 0 && !a.whole) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join waits for this grid's end
     __syncthreads();
-    KvWalk<kRows, KT, kStepExtra> walk;
+    KvWalk<kRows, KT, kStepExtra, SHARED> walk;
     walk.start(a, share);
     const int bsize = a.pool.block_size;
 
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(kStepThreads, (StepCfg<D, NQ>::PER_SM))
         bool ok = true;
         const int none = a.pool.blocks;           // past the pool: TMA fills with zeros
         for (; !walk.done() && ok; walk.next(a)) {
-            const int32_t* row = a.tables + int64_t(walk.request) * a.width;
+            const int32_t* row = a.tables + int64_t(kv_table_row<SHARED>(a, walk.request)) * a.width;
             auto block_of = [&](int tile, int r) {  // the block of a key tile's token r
                 const int token = tile * KT + r, column = token >> a.pool.shift;
                 if (token >= walk.r.length || column >= a.width) return none;
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kStepThreads, (StepCfg<D, NQ>::PER_SM))
                 const int r = walk.rt * kRows + 8 * nq + n8;
                 const bool in = r < walk.r.rows;
                 const int token = in ? by_group(a, r) : 0;
-                const uint16_t* src = a.q.p + (walk.r.token0 + token) * a.q.token_stride +
+                const uint16_t* src = a.q.p + kv_token<SHARED>(a, walk.request, walk.r, token) * a.q.token_stride +
                                       (walk.head * a.group + (in ? r - token * a.group : 0)) * a.q.head_stride + c * KB;
 #pragma unroll
                 for (int l = 0; l < KL; ++l)
@@ -431,7 +431,22 @@ __global__ void __launch_bounds__(kStepThreads, (StepCfg<D, NQ>::PER_SM))
                 sum.z = fmaf(v.z, f, sum.z); sum.w = fmaf(v.w, f, sum.w);
                 ll = fmaf(y[D + 1], f, ll);
             }
-            if (whole) {
+            if constexpr (SHARED) {
+                const int row = walk.rt * kRows + r;
+                const int token = by_group(a, row), side = walk.request < a.groups ? 0 : 1;
+                const int64_t at_row = int64_t(kv_token<true>(a, walk.request, walk.r, token)) * a.heads + walk.head * a.group +
+                                       row - token * a.group;
+                if (whole) {
+                    const int64_t at = side * a.tokens * a.heads + at_row;
+                    *reinterpret_cast<float4*>(a.sums + at * D + d) = sum;
+                    if (d == 0) a.sums_ml[at] = make_float2(mm, ll);
+                } else {
+                    reinterpret_cast<float4*>(kv_part<D, kRows>(a, blockIdx.x, slot))[d / 4 * kRows + r] = sum;
+                    if (d == 0) kv_part_ml<D, kRows>(a, blockIdx.x, slot)[r] = make_float2(mm, ll);
+                }
+                if (d == 0 && whole) kv_whole(a, side, at_row);
+                else if (d == 0 && walk.begins) kv_begins(a, side, at_row, false, walk.last() - int(blockIdx.x), r);
+            } else if (whole) {
                 const int row = walk.rt * kRows + r;
                 const int token = by_group(a, row);
                 const int64_t at_row = int64_t(walk.r.token0 + token) * a.heads + walk.head * a.group + row - token * a.group;
@@ -446,16 +461,17 @@ __global__ void __launch_bounds__(kStepThreads, (StepCfg<D, NQ>::PER_SM))
                 if (d == 0) kv_part_ml<D, kRows>(a, blockIdx.x, slot)[r] = make_float2(mm, ll);
             }
         }
-        if (walk.begins && !whole && threadIdx.x == 0)
+        if (!SHARED && walk.begins && !whole && threadIdx.x == 0)
             a.desc[blockIdx.x] = kv_desc(walk.r, walk.rt, kRows, walk.head, walk.last() - int(blockIdx.x));
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kConsumers) : "memory");  // merge is free again
     }
 }
 
-template <int D, int NQ, bool BF16>
+// SHARED: `ws` holds the parts, and the caller joins.
+template <int D, int NQ, bool BF16, bool SHARED = false>
 cudaError_t launch_step(KvAttnArgs a, int rows, void* ws, int dev, cudaStream_t s) {
     using C = StepCfg<D, NQ>;
-    auto kern = kv_step_kernel<D, NQ, BF16>;
+    auto kern = kv_step_kernel<D, NQ, BF16, SHARED>;
     static std::atomic<uint64_t> configured{0};
     const uint64_t bit = 1ull << (dev & 63);
     if (!(configured.load(std::memory_order_relaxed) & bit)) {
@@ -469,10 +485,113 @@ cudaError_t launch_step(KvAttnArgs a, int rows, void* ws, int dev, cudaStream_t 
         return cudaErrorInvalidValue;
     const int grid = gemm_sm_count(dev) * C::PER_SM;
     a.desc = static_cast<int4*>(ws);
-    a.part = reinterpret_cast<float*>(a.desc + grid);
+    a.part = reinterpret_cast<float*>(SHARED ? a.desc : a.desc + grid);
     const cudaError_t e = launch_early(kern, dim3(grid), kStepThreads, C::kSmem, s, mk, mv, a, kStepLeast);
-    if (e != cudaSuccess) return e;
+    if (e != cudaSuccess || SHARED) return e;
     return launch_join<D, C::ROWS, 4, BF16>(a, grid, std::min(rows, C::ROWS), s);
+}
+
+// ---- the join of rows over a prefix and their own part -----------------------------------------
+
+struct SharedParts {
+    const float* step;     // parts of either kernel, row tiles of step_rows and of kPromptTile
+    const float* prompt;
+    int step_rows, step_ctas, prompt_ctas;
+};
+constexpr int kPromptTile = 256;
+constexpr int kJoinWays = 4;
+
+// CTA y joins rows 4 y .. 4 y + 3 of [tokens * heads]: 4 rows x 8 column groups x ways that take the row's
+// results in turn, those over the prefix first.  Only what the kernels before it wrote is followed.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(32 * kJoinWays) kv_shared_join_kernel(const __grid_constant__ KvAttnArgs a, SharedParts parts) {
+    asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
+    constexpr int COLS = D / 32;  // float4 columns of a thread: groups of 8 apart
+    __shared__ float2 s_ml[kJoinWays][8][4];
+    __shared__ float4 s_o[COLS][kJoinWays][8][4];
+    const int ri = threadIdx.x & 3, col = (threadIdx.x >> 2) & 7, way = threadIdx.x >> 5;
+    const int64_t rows = a.tokens * a.heads, row = int64_t(blockIdx.x) * 4 + ri;
+    const int state = row < rows ? a.state[row / a.heads] : 0;
+    int first[2], tile_row[2], count[2] = {0, 0};
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+        if (state < 2 - side) continue;
+        const int2 w = a.where[side * rows + row];
+        const int ctas = w.x < -1 ? parts.prompt_ctas : parts.step_ctas, c = w.x < -1 ? -2 - w.x : w.x;
+        first[side] = w.x;
+        tile_row[side] = w.y & 0xff;
+        count[side] = w.x == -1 ? 1 : c < ctas ? min(max(w.y >> 8, 0) + 1, ctas - c) : 0;
+        if (w.x != -1 && tile_row[side] >= (w.x < -1 ? kPromptTile : parts.step_rows)) count[side] = 0;
+    }
+    float m = -INFINITY, l = 0.0f;
+    float4 o[COLS];
+#pragma unroll
+    for (int x = 0; x < COLS; ++x) o[x] = make_float4(0, 0, 0, 0);
+    auto join = [&](float m1, float l1, const float4 (&v)[COLS]) {
+        const float mn = fmaxf(m, m1);
+        const float f0 = m == mn ? 1.0f : ex2(m - mn), f1 = m1 == mn ? 1.0f : ex2(m1 - mn);
+#pragma unroll
+        for (int x = 0; x < COLS; ++x) {
+            o[x].x = o[x].x * f0 + v[x].x * f1;
+            o[x].y = o[x].y * f0 + v[x].y * f1;
+            o[x].z = o[x].z * f0 + v[x].z * f1;
+            o[x].w = o[x].w * f0 + v[x].w * f1;
+        }
+        l = l * f0 + l1 * f1;
+        m = mn;
+    };
+    const int total = count[0] + count[1];
+    constexpr int AHEAD = 4;  // results on their way at once
+    for (int p0 = way; p0 < total; p0 += AHEAD * kJoinWays) {
+        float4 v[AHEAD][COLS];
+        float2 ml[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int p = p0 + i * kJoinWays;
+            if (p >= total) continue;
+            const int side = p < count[0] ? 0 : 1, k = side ? p - count[0] : p;
+            const int at = side ? first[1] : first[0], r = side ? tile_row[1] : tile_row[0];
+            const float4* src;
+            int stride;
+            if (at == -1) {
+                src = reinterpret_cast<const float4*>(a.sums + (side * rows + row) * D);
+                stride = 1;
+                ml[i] = a.sums_ml[side * rows + row];
+            } else {
+                const int tile = at < -1 ? kPromptTile : parts.step_rows;
+                const float* part = (at < -1 ? parts.prompt : parts.step) +
+                                    (2 * int64_t((at < -1 ? -2 - at : at) + k) + (k == 0)) * tile * (D + 2);
+                src = reinterpret_cast<const float4*>(part) + r;
+                stride = tile;
+                ml[i] = reinterpret_cast<const float2*>(part + tile * D)[r];
+            }
+#pragma unroll
+            for (int x = 0; x < COLS; ++x) v[i][x] = src[(x * 8 + col) * stride];
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (p0 + i * kJoinWays < total) join(ml[i].x, ml[i].y, v[i]);
+    }
+    s_ml[way][col][ri] = make_float2(m, l);
+#pragma unroll
+    for (int x = 0; x < COLS; ++x) s_o[x][way][col][ri] = o[x];
+    __syncthreads();
+    if (way != 0 || state == 0) return;
+    for (int w = 1; w < min(kJoinWays, total); ++w) {
+        float4 v[COLS];
+#pragma unroll
+        for (int x = 0; x < COLS; ++x) v[x] = s_o[x][w][col][ri];
+        join(s_ml[w][col][ri].x, s_ml[w][col][ri].y, v);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int x = 0; x < COLS; ++x) {
+        uint2 pk;
+        pk.x = pack16<BF16>(o[x].x * inv, o[x].y * inv);
+        pk.y = pack16<BF16>(o[x].z * inv, o[x].w * inv);
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + row * D + 4 * (x * 8 + col)) = pk;
+    }
+    if (a.lse && col == 0) a.lse[row] = l == 0.0f ? -INFINITY : (m + lg2(l)) * 0.6931471805599453f;
 }
 
 }  // namespace
@@ -550,6 +669,96 @@ cudaError_t launch_kv_attention(KvAttnArgs a, bool bf16, int max_new, int max_le
         default: return EBX_KV_STEP(128);
     }
 #undef EBX_KV_STEP
+}
+
+// ---- with prefixes ------------------------------------------------------------------------------
+
+namespace {
+
+// A request with many rows of its own fills row tiles by itself: nothing is gained by sharing.
+bool takes_prefixes(int group, int64_t tokens, int max_new) { return most_rows(group, tokens, max_new) < kPromptMin; }
+
+struct SharedPlan {
+    bool prompt;           // groups of kPromptMin rows and more may occur
+    int nq, step_ctas, prompt_ctas;
+    int64_t where, ml, sums, step, prompt_at, bytes;  // places in the workspace
+};
+
+SharedPlan shared_plan(int head_dim, int heads, int group, int64_t tokens, int max_new, int max_length, int sms) {
+    SharedPlan p;
+    p.prompt = tokens * group >= kPromptMin;
+    // rows of most row tiles: the requests' own, or, without the other kernel, also those of the groups
+    p.nq = (p.prompt ? most_rows(group, tokens, max_new) : tokens * group) <= 8 ? 1 : 2;
+    p.step_ctas = sms * (p.nq == 1 ? StepCfg<32, 1>::PER_SM : StepCfg<32, 2>::PER_SM);
+    p.prompt_ctas = p.prompt ? sms : 0;
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const int64_t here = at;
+        at += round_up(bytes, 256);
+        return here;
+    };
+    const int64_t rows = 2 * tokens * heads;
+    p.where = take(rows * int64_t(sizeof(int2)));
+    p.ml = take(rows * int64_t(sizeof(float2)));
+    p.sums = take(rows * head_dim * int64_t(sizeof(float)));
+    p.step = take(int64_t(p.step_ctas) * 2 * 8 * p.nq * (head_dim + 2) * int64_t(sizeof(float)));
+    p.prompt_at = take(int64_t(p.prompt_ctas) * 2 * kPromptTile * (head_dim + 2) * int64_t(sizeof(float)));
+    p.bytes = at;
+    return p;
+}
+
+template <int D, bool BF16>
+cudaError_t launch_shared(KvAttnArgs a, const SharedPlan& p, char* ws, int dev, cudaStream_t s) {
+    a.where = reinterpret_cast<int2*>(ws + p.where);
+    a.sums_ml = reinterpret_cast<float2*>(ws + p.ml);
+    a.sums = reinterpret_cast<float*>(ws + p.sums);
+    a.least_rows = 0;
+    a.most_rows = INT_MAX;
+    cudaError_t e = cudaSuccess;
+    const int requests = a.requests;
+    if (p.prompt) {
+        a.least_rows = kPromptMin;
+        a.requests = a.groups;  // groups only
+        e = launch_kv_prompt_shared(a, BF16, ws + p.prompt_at, dev, s);
+        if (e != cudaSuccess) return e;
+        a.least_rows = 0;
+        a.most_rows = kPromptMin - 1;
+    }
+    a.requests = a.groups + requests;
+    e = p.nq == 1 ? launch_step<D, 1, BF16, true>(a, 0, ws + p.step, dev, s)
+                  : launch_step<D, 2, BF16, true>(a, 0, ws + p.step, dev, s);
+    if (e != cudaSuccess) return e;
+    const int64_t grid = (a.tokens * a.heads + 3) / 4;
+    if (grid > INT32_MAX) return cudaErrorInvalidValue;
+    const SharedParts parts{reinterpret_cast<const float*>(ws + p.step), reinterpret_cast<const float*>(ws + p.prompt_at),
+                            8 * p.nq, p.step_ctas, p.prompt_ctas};
+    return launch_early(kv_shared_join_kernel<D, BF16>, dim3(unsigned(grid)), 32 * kJoinWays, 0, s, a, parts);
+}
+
+}  // namespace
+
+uint64_t kv_shared_workspace_bytes(int head_dim, int heads, int group, int64_t tokens, int max_new, int max_length) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    if (!takes_prefixes(group, tokens, max_new)) return kv_attention_workspace_bytes(head_dim, group, tokens, max_new, max_length);
+    return uint64_t(shared_plan(head_dim, heads, group, tokens, max_new, max_length, gemm_sm_count(dev)).bytes);
+}
+
+cudaError_t launch_kv_shared_attention(KvAttnArgs a, bool bf16, int max_new, int max_length, void* ws, cudaStream_t s) {
+    if (a.tokens <= 0 || a.requests <= 0) return cudaSuccess;
+    if (!takes_prefixes(a.group, a.tokens, max_new)) return launch_kv_attention(a, bf16, max_new, max_length, ws, s);
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const SharedPlan p = shared_plan(a.pool.head_dim, a.heads, a.group, a.tokens, max_new, max_length, gemm_sm_count(dev));
+    a.groups = a.requests;
+    a.whole = 0;
+    char* base = static_cast<char*>(ws);
+    switch (a.pool.head_dim) {
+        case 32: return bf16 ? launch_shared<32, true>(a, p, base, dev, s) : launch_shared<32, false>(a, p, base, dev, s);
+        case 64: return bf16 ? launch_shared<64, true>(a, p, base, dev, s) : launch_shared<64, false>(a, p, base, dev, s);
+        default: return bf16 ? launch_shared<128, true>(a, p, base, dev, s) : launch_shared<128, false>(a, p, base, dev, s);
+    }
 }
 
 cudaError_t read_kv_status(int* status, bool clear, cudaStream_t s) {

@@ -245,8 +245,10 @@ __device__ __forceinline__ bool pair_any(int id, bool mine) {
 
 // The segment's key tiles [j0, j1), at least one, counted from its first, that rows of row tile x
 // see: the rows of the other tile may begin earlier or end later.
-using PromptWalk = KvWalk<kPromptRows, kPromptKeys, kPromptExtra>;
-__device__ __forceinline__ void tiles_seen(const KvAttnArgs& a, const PromptWalk& w, int x, int& j0, int& j1) {
+template <bool SHARED>
+using PromptWalk = KvWalk<kPromptRows, kPromptKeys, kPromptExtra, SHARED>;
+template <bool SHARED>
+__device__ __forceinline__ void tiles_seen(const KvAttnArgs& a, const PromptWalk<SHARED>& w, int x, int& j0, int& j1) {
     int t0, n;
     kv_key_tiles<128, kPromptKeys>(a, w.r, 2 * w.rt + x, t0, n);
     j0 = min(max(t0 - w.t0, 0), w.n - 1);
@@ -267,7 +269,7 @@ __device__ __noinline__ void drain(const uint64_t* raw_full, const uint64_t* dra
     }
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool SHARED>
 __global__ void __launch_bounds__(kPromptThreads, 1)
     kv_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                      const __grid_constant__ KvAttnArgs a, int least) {
@@ -315,15 +317,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");  // nothing of the call's inputs is read before
-    const KvShare share = kv_share<kPromptRows, kPromptKeys, kPromptExtra, kPromptThreads>(a, least, reinterpret_cast<int*>(smem));
+    const KvShare share = kv_share<kPromptRows, kPromptKeys, kPromptExtra, kPromptThreads, SHARED>(a, least, reinterpret_cast<int*>(smem));
     fence_proxy_async_smem();  // copies will overwrite what kv_share kept there
-    if (threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (!SHARED && threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join waits for this grid's end
     before_sync();
     __syncthreads();
     after_sync();
     const uint32_t tmem = *tmem_slot;
-    PromptWalk walk;
+    PromptWalk<SHARED> walk;
     walk.start(a, share);
 
     if (warp < kRowWarps) {
@@ -366,10 +368,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             row.mr = -INFINITY;
             row.l = 0.0f;
             const int place = walk.r.begin + token;
+            auto q_token = [&] { return kv_token<SHARED>(a, walk.request, walk.r, token); };
             row.hi = !live ? INT_MAX : a.causal ? min(place + 1, walk.r.length) : walk.r.length;
             row.lo = !live ? 0 : max(walk.r.first, a.window > 0 ? place - a.window + 1 : 0);
             {
-                const int64_t off = (walk.r.token0 + token) * a.q.token_stride + head * a.q.head_stride;
+                const int64_t off = q_token() * a.q.token_stride + head * a.q.head_stride;
                 uint4 v[PER / 2];  // each of the two warps brings every other load's rows
 #pragma unroll
                 for (int i = 0; i < PER / 2; ++i)
@@ -408,7 +411,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             // keys that every row of the warp sees
             const int all_lo = __reduce_max_sync(0xffffffffu, row.lo), all_hi = __reduce_min_sync(0xffffffffu, row.hi);
             int j0, j1;
-            tiles_seen(a, walk, x, j0, j1);
+            tiles_seen<SHARED>(a, walk, x, j0, j1);
             for (int j = j0; j < j1; ++j, ++g) {
                 const int at = gj + j;
                 wait(s_full + x, g);
@@ -455,7 +458,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             const float l = half ? *other + row.l : row.l + *other;
             wait(o_done + x, g - 1);
             const bool whole = walk.whole();
-            const int64_t at_row = int64_t(walk.r.token0 + token) * a.heads + head;
+            const int64_t at_row = int64_t(q_token()) * a.heads + head;
             const int slot = walk.begins ? 1 : 0;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             float4* part = whole ? nullptr
@@ -466,7 +469,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 tmem_ld16(o_addr + c, v, 0);
                 tmem_wait<16>(v);
                 const int d0 = half * (D / 2) + c;
-                if (whole) {  // through shared memory, so that rows are written whole
+                if (SHARED && whole) {
+                    if (live) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            *reinterpret_cast<float4*>(a.sums + at_row * D + d0 + 4 * i) =
+                                make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
+                                            __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+                    }
+                } else if (whole) {  // through shared memory, so that rows are written whole
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         uint32_t h[4];
@@ -487,7 +498,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
             before_sync();
             pair_sync(pair);
-            if (whole) {
+            if (!SHARED && whole) {
 #pragma unroll
                 for (int i = 0; i < PER / 2; ++i) {
                     const int ri = (2 * i + half) * ROWS + mine;
@@ -496,11 +507,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 }
                 pair_sync(pair);  // the staged rows are free again
             }
-            if (half == 0 && live && whole && a.lse)
+            if constexpr (SHARED) {  // groups only: side 0
+                if (half == 0 && live) {
+                    if (whole) {
+                        a.sums_ml[at_row] = make_float2(row.mr, l);
+                        kv_whole(a, 0, at_row);
+                    } else if (walk.begins) {
+                        kv_begins(a, 0, at_row, true, walk.last() - int(blockIdx.x), x * 128 + quarter * 32 + lane);
+                    }
+                }
+            }
+            if (!SHARED && half == 0 && live && whole && a.lse)
                 a.lse[at_row] = l == 0.0f ? -INFINITY : (row.mr + lg2(l)) * 0.6931471805599453f;
             if (half == 0 && !whole)
                 kv_part_ml<D, kPromptRows>(a, blockIdx.x, slot)[x * 128 + quarter * 32 + lane] = make_float2(row.mr, l);
-            if (walk.begins && !whole && threadIdx.x == 0)
+            if (!SHARED && walk.begins && !whole && threadIdx.x == 0)
                 a.desc[blockIdx.x] = kv_desc(walk.r, walk.rt, kPromptRows, walk.head, walk.last() - int(blockIdx.x));
         }
     } else if (warp >= kLoad) {
@@ -512,7 +533,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             int it = 0;
             bool ok = true;
             for (; !walk.done() && ok; walk.next(a)) {
-                const int32_t* row = a.tables + int64_t(walk.request) * a.width;
+                const int32_t* row = a.tables + int64_t(kv_table_row<SHARED>(a, walk.request)) * a.width;
                 auto block_of = [&](int token) {
                     const int column = token >> a.pool.shift;
                     if (token >= walk.r.length || column >= a.width) return none;
@@ -597,8 +618,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             for (; !walk.done() && ok; walk.next(a)) {
                 const bool two = walk.r.rows - walk.rt * kPromptRows > 128;
                 int from[2], to[2];  // the segment's key tiles that either row tile sees
-                tiles_seen(a, walk, 0, from[0], to[0]);
-                tiles_seen(a, walk, 1, from[1], to[1]);
+                tiles_seen<SHARED>(a, walk, 0, from[0], to[0]);
+                tiles_seen<SHARED>(a, walk, 1, from[1], to[1]);
                 if (!two) from[1] = to[1] = 0;
                 // S of every row tile that begins at key tile j (counted from the segment's first)
                 auto step = [&](int x, int j, int buf, int phase) {
@@ -715,11 +736,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 // of 700 35 / 35 / 44 / 64, of 1500 60 / 60 / 60 / 66, three of 2048 184 with any).
 constexpr int kPromptLeast = 8;
 
-template <int D, bool BF16>
+// SHARED: `ws` holds the parts, and the caller joins.
+template <int D, bool BF16, bool SHARED = false>
 cudaError_t launch_prompt(KvAttnArgs a, void* ws, int dev, cudaStream_t s) {
     using C = PromptCfg<D>;
     static_assert(C::kSmem <= 227 * 1024, "shared memory of the prompt kernel");
-    auto kern = kv_prompt_kernel<D, BF16>;
+    auto kern = kv_prompt_kernel<D, BF16, SHARED>;
     static std::atomic<uint64_t> configured{0};
     const uint64_t bit = 1ull << (dev & 63);
     if (!(configured.load(std::memory_order_relaxed) & bit)) {
@@ -732,9 +754,9 @@ cudaError_t launch_prompt(KvAttnArgs a, void* ws, int dev, cudaStream_t s) {
         return cudaErrorInvalidValue;
     const int grid = gemm_sm_count(dev);
     a.desc = static_cast<int4*>(ws);
-    a.part = reinterpret_cast<float*>(a.desc + grid);
+    a.part = reinterpret_cast<float*>(SHARED ? a.desc : a.desc + grid);
     const cudaError_t e = launch_early(kern, dim3(grid), kPromptThreads, C::kSmem, s, mk, mv, a, kPromptLeast);
-    if (e != cudaSuccess) return e;
+    if (e != cudaSuccess || SHARED) return e;
     return launch_join<D, kPromptRows, 4, BF16>(a, grid, kPromptRows, s);
 }
 
@@ -749,6 +771,14 @@ cudaError_t launch_kv_prompt(const KvAttnArgs& a, bool bf16, void* ws, int dev, 
         case 32: return bf16 ? launch_prompt<32, true>(a, ws, dev, s) : launch_prompt<32, false>(a, ws, dev, s);
         case 64: return bf16 ? launch_prompt<64, true>(a, ws, dev, s) : launch_prompt<64, false>(a, ws, dev, s);
         default: return bf16 ? launch_prompt<128, true>(a, ws, dev, s) : launch_prompt<128, false>(a, ws, dev, s);
+    }
+}
+
+cudaError_t launch_kv_prompt_shared(const KvAttnArgs& a, bool bf16, void* ws, int dev, cudaStream_t s) {
+    switch (a.pool.head_dim) {
+        case 32: return bf16 ? launch_prompt<32, true, true>(a, ws, dev, s) : launch_prompt<32, false, true>(a, ws, dev, s);
+        case 64: return bf16 ? launch_prompt<64, true, true>(a, ws, dev, s) : launch_prompt<64, false, true>(a, ws, dev, s);
+        default: return bf16 ? launch_prompt<128, true, true>(a, ws, dev, s) : launch_prompt<128, false, true>(a, ws, dev, s);
     }
 }
 

@@ -64,6 +64,11 @@ struct KvPrefixes {
     int32_t* state;         // [tokens]: 0: of no request, 1: of a request by itself, 2: of one in a group
 };
 
+// All in one buffer of 3 * requests + 1 + 2 * tokens ints, in the order of the structure.
+inline KvPrefixes prefixes_at(int32_t* p, int64_t requests, int64_t tokens) {
+    return {p, p + requests + 1, p + 2 * requests + 1, p + 3 * requests + 1, p + 3 * requests + 1 + tokens};
+}
+
 struct KvPrefixArgs {
     const int32_t* tables;
     const int32_t* lengths;

@@ -1,6 +1,7 @@
 // ebx_kv_share_capi.cu -- the extern "C" entries for requests that share cache blocks (include/ebx.h): every
 // check that the host can make, then the launch.
 #include <algorithm>
+#include <cmath>
 
 #include "ebx_kv_check.h"
 #include "ebx_kv_share.h"
@@ -106,6 +107,106 @@ ebx_status ebx_kv_copy(const ebx_kv_pool* pools, int32_t layers, const int32_t* 
         if (st != EBX_OK) return st;
     }
     return EBX_OK;
+}
+
+uint64_t ebx_kv_prefixes_ints(int32_t requests, int64_t tokens) {
+    return requests < 0 || tokens < 0 ? 0 : 3 * uint64_t(requests) + 1 + 2 * uint64_t(tokens);
+}
+
+ebx_status ebx_kv_prefixes(const int32_t* tables, int32_t width, int32_t block_size, int32_t blocks,
+                           const int32_t* lengths, const int32_t* starts, int32_t requests, int64_t tokens,
+                           int32_t* prefixes, void* workspace, uint64_t workspace_bytes, int32_t device, void* stream) {
+    if (const char* msg = table_of(requests, width, block_size, blocks)) return invalid(msg);
+    if (tokens < 0 || tokens > INT32_MAX) return invalid("ebx_kv_prefixes: need 0 <= tokens < 2^31");
+    if (requests == 0) return EBX_OK;
+    if (!tables || !lengths || !starts || !prefixes || !workspace) return invalid("null argument");
+    if (reinterpret_cast<uintptr_t>(workspace) & 15) return invalid("ebx_kv_prefixes: workspace must be 16-byte aligned");
+    if (workspace_bytes < 4 * (uint64_t(ebx::kKvPrefixScratch) * requests + uint64_t(blocks))) {
+        ebx::set_error("ebx_kv_prefixes: workspace smaller than 24 * requests + 4 * blocks bytes");
+        return EBX_ERR_WORKSPACE;
+    }
+    Device d(device);
+    if (d.err != cudaSuccess) return launched(d.err, "cudaSetDevice");
+    ebx::KvPrefixArgs a{};
+    a.tables = tables;
+    a.lengths = lengths;
+    a.starts = starts;
+    a.out = ebx::prefixes_at(prefixes, requests, tokens);
+    a.scratch = static_cast<int32_t*>(workspace);
+    a.first_with = a.scratch + int64_t(ebx::kKvPrefixScratch) * requests;
+    a.tokens = tokens;
+    a.requests = requests;
+    a.width = width;
+    a.shift = log2_of(block_size);
+    a.blocks = blocks;
+    return launched(ebx::launch_kv_prefixes(a, static_cast<cudaStream_t>(stream)), "ebx_kv_prefixes");
+}
+
+uint64_t ebx_kv_shared_attention_workspace_bytes(const ebx_kv_pool* pool, int32_t heads, int64_t tokens,
+                                                 int32_t max_new, int32_t max_length) {
+    ebx::KvPool p;
+    if (pool_of(pool, p) || heads < 1 || heads % p.kv_heads != 0 || tokens < 0 || tokens > INT32_MAX ||
+        max_new < 0 || max_length < 0)
+        return 0;
+    Device d(pool->device);
+    if (d.err != cudaSuccess) return 0;
+    return ebx::kv_shared_workspace_bytes(p.head_dim, heads, heads / p.kv_heads, tokens, max_new, max_length);
+}
+
+ebx_status ebx_kv_shared_attention(const ebx_kv_pool* pool, const void* q, int64_t q_token_stride,
+                                   int64_t q_head_stride, int32_t heads, int32_t dtype, const int32_t* tables,
+                                   int32_t width, const int32_t* lengths, const int32_t* starts,
+                                   const int32_t* prefixes, int32_t requests, int64_t tokens, int32_t causal,
+                                   float scale, int32_t max_new, int32_t max_length, void* out, float* lse,
+                                   void* workspace, uint64_t workspace_bytes, void* stream) {
+    ebx::KvPool p;
+    if (const char* msg = pool_of(pool, p)) return invalid(msg);
+    if (dtype != ebx::kKvF16 && dtype != ebx::kKvBF16)
+        return invalid("ebx_kv_shared_attention: dtype must be fp16 or bf16");
+    if (heads < 1 || heads % p.kv_heads != 0 || heads > (1 << 20))
+        return invalid("ebx_kv_shared_attention: heads must be a multiple of kv_heads");
+    if (requests < 0 || requests > ebx::kKvMaxRequests || width < 1 || int64_t(width) * p.block_size > INT32_MAX / 2 ||
+        tokens < 0 || tokens > INT32_MAX || tokens * (heads / p.kv_heads) > INT32_MAX / 2)
+        return invalid("ebx_kv_shared_attention: requests, table width or tokens out of range");
+    if (!std::isfinite(scale * 1.4426950408889634f)) return invalid("ebx_kv_shared_attention: scale must be finite");
+    if (max_new < 0 || max_length < 0) return invalid("ebx_kv_shared_attention: max_new and max_length are >= 0");
+    if (tokens == 0 || requests == 0) return EBX_OK;  // rows of no request are left as they are
+    if (!out || !starts || !tables || !lengths || !prefixes) return invalid("null argument");
+    ebx::KvRows rows;
+    if (const char* msg = rows_of(q, q_token_stride, q_head_stride, rows)) return invalid(msg);
+    if (!aligned16(out) || !aligned16(workspace))
+        return invalid("ebx_kv_shared_attention: out and workspace must be 16-byte aligned");
+    Device d(pool->device);
+    if (d.err != cudaSuccess) return launched(d.err, "cudaSetDevice");
+    const int group = heads / p.kv_heads;
+    const uint64_t need = ebx::kv_shared_workspace_bytes(p.head_dim, heads, group, tokens, max_new, max_length);
+    if (need > 0 && (!workspace || workspace_bytes < need)) {
+        ebx::set_error("ebx_kv_shared_attention: workspace smaller than ebx_kv_shared_attention_workspace_bytes");
+        return EBX_ERR_WORKSPACE;
+    }
+    ebx::KvAttnArgs a{};
+    a.pool = p;
+    a.q = rows;
+    a.tables = tables;
+    a.lengths = lengths;
+    a.starts = starts;
+    a.out = out;
+    a.lse = lse;
+    a.tokens = tokens;
+    a.requests = requests;
+    a.width = width;
+    a.heads = heads;
+    a.set_group(group);
+    a.causal = causal != 0;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    const ebx::KvPrefixes found = ebx::prefixes_at(const_cast<int32_t*>(prefixes), requests, tokens);
+    a.group_starts = found.group_starts;
+    a.shared = found.shared;
+    a.own_first = found.own_first;
+    a.list = found.list;
+    a.state = found.state;
+    return launched(ebx::launch_kv_shared_attention(a, dtype == ebx::kKvBF16, max_new, max_length, workspace,
+                                                    static_cast<cudaStream_t>(stream)), "ebx_kv_shared_attention");
 }
 
 }  // extern "C"

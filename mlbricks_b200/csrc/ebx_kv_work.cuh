@@ -30,13 +30,30 @@ struct KvRequest {
     int first;    // keys ahead of it are not seen
 };
 
-// Does this launch take a request with n new tokens?
-__device__ __forceinline__ bool kv_taken(const KvAttnArgs& a, int64_t n) {
+// Does this launch take request i, with n new tokens?  SHARED: with prefixes, where it chooses among groups only.
+template <bool SHARED>
+__device__ __forceinline__ bool kv_taken(const KvAttnArgs& a, int i, int64_t n) {
+    if (SHARED && i >= a.groups) return true;
     return n * a.group >= a.least_rows && n * a.group <= a.most_rows;
 }
 
+template <bool SHARED>
 __device__ __forceinline__ KvRequest kv_request(const KvAttnArgs& a, int i) {
     KvRequest r;
+    if constexpr (SHARED) {
+        const bool whole = i < a.groups;  // a group: every key of it is ahead of every row
+        const int own = whole ? i : i - a.groups;
+        const int32_t* starts = (whole ? a.group_starts : a.starts) + own;
+        const int64_t lo = max(starts[0], 0), hi = min(int64_t(starts[1]), a.tokens);
+        const int n = hi > lo ? int(hi - lo) : 0;
+        const int64_t cap = int64_t(a.width) << a.pool.shift;
+        r.length = int(min(int64_t(max(whole ? a.shared[own] : a.lengths[own], 0)), cap));
+        r.begin = whole ? r.length : r.length - n;
+        r.rows = kv_taken<true>(a, i, n) ? n * a.group : 0;
+        r.token0 = int(lo);
+        r.first = whole ? 0 : min(max(a.own_first[own], 0), r.length);
+        return r;
+    }
     const int64_t s0 = a.starts[i], s1 = a.starts[i + 1];
     const int64_t lo = s0 < 0 ? 0 : s0, hi = s1 > a.tokens ? a.tokens : s1;
     const int n = hi > lo ? int(hi - lo) : 0;
@@ -44,10 +61,21 @@ __device__ __forceinline__ KvRequest kv_request(const KvAttnArgs& a, int i) {
     const int len = a.lengths[i];
     r.length = len < 0 ? 0 : int64_t(len) > cap ? int(cap) : len;
     r.begin = r.length - n;
-    r.rows = kv_taken(a, n) ? n * a.group : 0;
+    r.rows = kv_taken<false>(a, i, n) ? n * a.group : 0;
     r.token0 = int(lo);
     r.first = a.first ? min(max(a.first[i], 0), r.length) : 0;
     return r;
+}
+
+// The token of row tile rows whose number among the request's tokens is n; the table row of a request.
+template <bool SHARED>
+__device__ __forceinline__ int kv_token(const KvAttnArgs& a, int request, const KvRequest& r, int n) {
+    if (SHARED && request < a.groups) return min(max(a.list[r.token0 + n], 0), int(a.tokens) - 1);
+    return r.token0 + n;
+}
+template <bool SHARED>
+__device__ __forceinline__ int kv_table_row(const KvAttnArgs& a, int request) {
+    return SHARED && request >= a.groups ? request - a.groups : request;
 }
 
 // n / group for 0 <= n < 2^31 (KvAttnArgs::set_group).
@@ -78,7 +106,7 @@ struct KvShare {
 
 // A CTA's walk along the line: which (request, head, row tile) it is at, and which of its key
 // tiles are the CTA's.  Every warp keeps its own copy.
-template <int RT, int KT, int EXTRA>
+template <int RT, int KT, int EXTRA, bool SHARED = false>
 struct KvWalk {
     int left;            // units from here to the CTA's end
     int per, request, head, rt;
@@ -97,7 +125,7 @@ struct KvWalk {
         rt = s.rt;
         skip = s.skip;
         if (left <= 0) return;
-        r = kv_request(a, request);
+        r = kv_request<SHARED>(a, request);
         segment(a);
     }
     __device__ __forceinline__ void segment(const KvAttnArgs& a) {
@@ -131,7 +159,7 @@ struct KvWalk {
             if (++head == a.pool.kv_heads) {
                 head = 0;
                 do {  // units are left, so a request with rows follows
-                    r = kv_request(a, ++request);
+                    r = kv_request<SHARED>(a, ++request);
                 } while (r.rows == 0);
             }
         }
@@ -146,7 +174,7 @@ struct KvWalk {
 constexpr int kShareWindow = 1024;
 constexpr int kShareInts = 3 * kShareWindow + 128;
 
-template <int RT, int KT, int EXTRA, int NT>
+template <int RT, int KT, int EXTRA, int NT, bool SHARED = false>
 __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, int* scratch) {
     constexpr int W = NT / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -184,8 +212,13 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, 
             const int i = b + tid;
             int64_t rts = 0, total;
             if (i < n) {
-                const int64_t s0 = max(a.starts[i0 + i], 0), s1 = min(int64_t(a.starts[i0 + i + 1]), a.tokens);
-                rts = s1 > s0 && kv_taken(a, s1 - s0) ? ((s1 - s0) * a.group + RT - 1) / RT : 0;
+                const int32_t* starts = a.starts;
+                int at = i0 + i;
+                if constexpr (SHARED) {
+                    if (at < a.groups) starts = a.group_starts; else at -= a.groups;
+                }
+                const int64_t s0 = max(starts[at], 0), s1 = min(int64_t(starts[at + 1]), a.tokens);
+                rts = s1 > s0 && kv_taken<SHARED>(a, i0 + i, s1 - s0) ? ((s1 - s0) * a.group + RT - 1) / RT : 0;
             }
             const int64_t ahead = all + scan(rts, total);
             if (i < n) {
@@ -202,7 +235,7 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, 
                 if (tiles[mid] <= x) lo = mid; else hi = mid;
             }
             int t0, k;
-            kv_key_tiles<RT, KT>(a, kv_request(a, i0 + lo), int(x) - tiles[lo], t0, k);
+            kv_key_tiles<RT, KT>(a, kv_request<SHARED>(a, i0 + lo), int(x) - tiles[lo], t0, k);
             const uint32_t more = a.whole ? 1 : k + EXTRA;
             if (atomicAdd(units + lo, more) > ~more) atomicAdd(carry + lo, 1u);
         }
@@ -256,7 +289,7 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, 
     out.head = int(sums[W + 1]);
     // the row tile: each warp for itself, 32 at a time
     int64_t rest = sums[W + 2];
-    const KvRequest r = kv_request(a, out.request);
+    const KvRequest r = kv_request<SHARED>(a, out.request);
     for (int rt0 = 0;; rt0 += 32) {
         int t0, k = 0;
         if ((rt0 + lane) * RT < r.rows) {
@@ -306,6 +339,17 @@ __device__ __forceinline__ float* kv_part(const KvAttnArgs& a, int cta, int slot
 template <int D, int RT>
 __device__ __forceinline__ float2* kv_part_ml(const KvAttnArgs& a, int cta, int slot) {
     return reinterpret_cast<float2*>(kv_part<D, RT>(a, cta, slot) + RT * D);
+}
+
+// With prefixes a row of q has two results, over the prefix (side 0) and over what is its request's own (side 1), each whole or in
+// parts; kv_where says where: {-1, 0}: whole, in `sums`; else {first CTA, CTAs behind << 8 | row of the tile}, the
+// CTA of the kernel for prompts as ~CTA - 1.  kv_shared_join_kernel makes one of all.
+__device__ __forceinline__ void kv_whole(const KvAttnArgs& a, int side, int64_t row) {
+    a.where[side * a.tokens * a.heads + row] = make_int2(-1, 0);
+}
+__device__ __forceinline__ void kv_begins(const KvAttnArgs& a, int side, int64_t row, bool prompt, int behind, int tile_row) {
+    a.where[side * a.tokens * a.heads + row] =
+        make_int2(prompt ? -2 - int(blockIdx.x) : int(blockIdx.x), behind << 8 | tile_row);
 }
 
 template <bool BF16>

@@ -6,17 +6,22 @@ they hold the same blocks, each with a count of its holders:
 * ``fork``       lets rows go on from what other rows hold, rolls rows back, and frees them;
 * ``compact``    moves the blocks that rows hold to the front of the pool;
 * ``copy``       copies the blocks that either asks for, in all layers;
+* ``prefixes``   finds which of a step's requests share a prefix;
+* ``attention``  attends over the cache, reading what requests share once for all of them.
 
 Inference only: no autograd.  The reference has no counterpart.
 """
 from __future__ import annotations
 
+import ctypes
+import functools
+import math
 from typing import NamedTuple, Sequence
 
 import torch
 
 from . import _ebx
-from .kvcache import BLOCK_SIZES, KVPool, _int_ok, _refuse_ints, _stream
+from .kvcache import _ROW_DTYPES, BLOCK_SIZES, KVPool, _int_ok, _refuse_ints, _stream
 
 
 class KVMoves(NamedTuple):
@@ -127,4 +132,81 @@ def copy(pools: Sequence[KVPool], moves: KVMoves) -> None:
                                        None if count is None else count.data_ptr(), sources.numel(), _stream(device)))
 
 
-__all__ = ["KVCompact", "KVFork", "KVMoves", "compact", "copy", "fork"]
+class KVPrefixes:
+    """Which requests of a step share a prefix (``prefixes``)."""
+
+    __slots__ = ("data", "requests", "tokens")
+
+    def __init__(self, data: torch.Tensor, requests: int, tokens: int) -> None:
+        self.data, self.requests, self.tokens = data, requests, tokens
+
+
+def prefixes(tables: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor, *, block_size: int, blocks: int,
+             tokens: int) -> KVPrefixes:
+    """Which requests of a step share a prefix, for ``attention`` of every layer.
+
+    ``lengths`` and ``starts`` are the step's, as for ``kvcache.attention``; ``blocks`` is the pool's.  Requests that
+    bring tokens and whose rows of ``tables`` begin with the same block form a group, which shares as many full blocks ahead
+    of the new tokens as save most reading; rows with fewer in common are taken alone.  The result holds for this
+    step."""
+    int32, device, requests = torch.int32, tables.get_device(), lengths.numel()
+    if device < 0:
+        raise ValueError("tables must be a CUDA tensor")
+    if not (_int_ok(tables, int32, device) and _int_ok(lengths, int32, device) and _int_ok(starts, int32, device)):
+        _refuse_ints(device, tables=(tables, int32), lengths=(lengths, int32), starts=(starts, int32))
+    if starts.numel() != requests + 1 or tables.dim() != 2 or tables.shape[0] != requests or tokens < 0:
+        raise ValueError("lengths and the rows of tables must be as many, and starts one more; tokens >= 0")
+    data = starts.new_empty(3 * requests + 1 + 2 * tokens)
+    work = starts.new_empty(6 * requests + blocks) if blocks > 0 else data
+    _ebx.check(_ebx.load().ebx_kv_prefixes(
+        tables.data_ptr(), tables.shape[1], block_size, blocks, lengths.data_ptr(), starts.data_ptr(), requests, tokens,
+        data.data_ptr(), work.data_ptr(), 4 * work.numel(), device, _stream(device)))
+    return KVPrefixes(data, requests, tokens)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(device: int, kv_heads: int, head_dim: int, heads: int, tokens: int, max_new: int,
+                     max_length: int) -> int:
+    pool = _ebx.KVPool(16, 16, 16, 16, 1, kv_heads, BLOCK_SIZES[0], head_dim, device, 0)  # only its sizes count
+    return int(_ebx.load().ebx_kv_shared_attention_workspace_bytes(ctypes.byref(pool), heads, tokens, max_new, max_length))
+
+
+def attention(q: torch.Tensor, pool: KVPool, tables: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor,
+              shared: KVPrefixes, *, scale: float | None = None, causal: bool = True, max_new: int = 0, max_length: int = 0,
+              out: torch.Tensor | None = None, return_lse: bool = False):
+    """``kvcache.attention`` (without ``window`` and ``first``) that reads the prefixes that ``shared`` tells of, found
+    by ``prefixes`` for the same tables, lengths and starts, once for all requests that share them.
+
+    The formula is the same; the order of sums is not.  ``max_new``, the largest number of new tokens of a request, should be given: with
+    49 rows (max_new, or without it tokens, times heads / kv_heads) and more, requests fill the kernels' tiles by
+    themselves, and go alone."""
+    q = pool._rows(q, None, "q")
+    device, int32 = pool.device, torch.int32
+    tokens, heads, dim = q.shape
+    requests = lengths.numel()
+    if not (_int_ok(tables, int32, device) and _int_ok(lengths, int32, device) and _int_ok(starts, int32, device)
+            and _int_ok(shared.data, int32, device)):
+        _refuse_ints(device, tables=(tables, int32), lengths=(lengths, int32), starts=(starts, int32), shared=(shared.data, int32))
+    if heads == 0 or heads % pool._c.kv_heads:
+        raise ValueError(f"heads ({heads}) must be a multiple of kv_heads ({pool._c.kv_heads})")
+    if starts.numel() != requests + 1 or tables.dim() != 2 or tables.shape[0] != requests:
+        raise ValueError("lengths and the rows of tables must be as many, and starts one more")
+    if shared.requests != requests or shared.tokens != tokens or shared.data.numel() != 3 * requests + 1 + 2 * tokens:
+        raise ValueError("shared must be of this step: as many requests and tokens")
+    if out is None:
+        out = q.new_empty((tokens, heads, dim))
+    elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != device or not out.is_contiguous():
+        raise ValueError("out must be a contiguous tensor of q's shape and dtype")
+    lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
+    if tokens and requests:
+        nbytes = _workspace_bytes(device, pool._c.kv_heads, dim, heads, tokens, max_new, max_length)
+        ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        _ebx.check(_ebx.load().ebx_kv_shared_attention(
+            pool._ref, q.data_ptr(), q.stride(0), q.stride(1), heads, _ROW_DTYPES[q.dtype], tables.data_ptr(),
+            tables.shape[1], lengths.data_ptr(), starts.data_ptr(), shared.data.data_ptr(), requests, tokens, causal,
+            1.0 / math.sqrt(dim) if scale is None else scale, max_new, max_length, out.data_ptr(),
+            None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, _stream(device)))
+    return out if lse is None else (out, lse)
+
+
+__all__ = ["KVCompact", "KVFork", "KVMoves", "KVPrefixes", "attention", "compact", "copy", "fork", "prefixes"]
