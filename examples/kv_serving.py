@@ -18,18 +18,11 @@ from torch import nn
 sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
 
 import mlbricks_b200 as mlb  # noqa: E402
+from mlbricks_b200 import rotary  # noqa: E402
 from mlbricks_b200.kvcache import KVCache  # noqa: E402
 
 VOCAB, DIM, HEADS, KV_HEADS, LAYERS = 512, 384, 12, 1, 3
 HEAD_DIM = DIM // HEADS
-
-
-def rotate(x: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
-    """Rotary positions of x [tokens, heads, HEAD_DIM]."""
-    half = HEAD_DIM // 2
-    angle = positions[:, None, None] * (10000.0 ** (-torch.arange(half, device=x.device) / half))
-    a, b = x.float().chunk(2, -1)
-    return torch.cat([a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()], -1).to(x.dtype)
 
 
 class Layer(nn.Module):
@@ -39,11 +32,12 @@ class Layer(nn.Module):
         self.k, self.v = (nn.Linear(DIM, KV_HEADS * HEAD_DIM, bias=False) for _ in "kv")
         self.up, self.down = nn.Linear(DIM, 4 * DIM), nn.Linear(4 * DIM, DIM)
         self.n1, self.n2 = nn.RMSNorm(DIM), nn.RMSNorm(DIM)
+        self.frequencies = rotary.frequencies(HEAD_DIM)
 
     def forward(self, x, positions, attend):
         h = self.n1(x)
-        q = rotate(self.q(h).view(-1, HEADS, HEAD_DIM), positions)
-        k = rotate(self.k(h).view(-1, KV_HEADS, HEAD_DIM), positions)
+        q, k = self.q(h).view(-1, HEADS, HEAD_DIM), self.k(h).view(-1, KV_HEADS, HEAD_DIM)
+        q, k = rotary.rotate(q, k, positions, self.frequencies, inplace=True)
         x = x + self.o(attend(q, k, self.v(h).view(-1, KV_HEADS, HEAD_DIM)).reshape(x.shape))
         return x + self.down(torch.nn.functional.gelu(self.up(self.n2(x))))
 

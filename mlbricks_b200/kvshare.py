@@ -9,6 +9,8 @@ they hold the same blocks, each with a count of its holders:
 * ``prefixes``   finds which of a step's requests share a prefix;
 * ``attention``  attends over the cache, reading what requests share once for all of them.
 
+``SharedKVCache`` is a ``KVCache`` with all of them.
+
 Inference only: no autograd.  The reference has no counterpart.
 """
 from __future__ import annotations
@@ -21,7 +23,7 @@ from typing import NamedTuple, Sequence
 import torch
 
 from . import _ebx
-from .kvcache import _ROW_DTYPES, BLOCK_SIZES, KVPool, _int_ok, _refuse_ints, _stream
+from .kvcache import _ROW_DTYPES, BLOCK_SIZES, KVCache, KVPlan, KVPool, _int_ok, _refuse_ints, _stream
 
 
 class KVMoves(NamedTuple):
@@ -209,4 +211,76 @@ def attention(q: torch.Tensor, pool: KVPool, tables: torch.Tensor, lengths: torc
     return out if lse is None else (out, lse)
 
 
-__all__ = ["KVCompact", "KVFork", "KVMoves", "KVPrefixes", "attention", "compact", "copy", "fork", "prefixes"]
+class SharedKVCache(KVCache):
+    """A ``KVCache`` whose requests can share blocks.
+
+    ``fork`` makes rows go on from others, frees them and rolls them back, ``compact`` renumbers blocks; both
+    come between steps: a step is planned after them.  ``attention`` reads prefixes that requests share once."""
+
+    def __init__(self, layers: int, blocks: int, kv_heads: int, head_dim: int, *, requests: int, max_length: int,
+                 block_size: int = 64, device="cuda") -> None:
+        super().__init__(layers, blocks, kv_heads, head_dim, requests=requests, max_length=max_length,
+                         block_size=block_size, device=device)
+        where = self.lengths.device
+        self.shares = torch.zeros(blocks, dtype=torch.int32, device=where)
+        self._rows = torch.arange(requests, dtype=torch.int32, device=where)
+        self._shared: KVPrefixes | None = None
+
+    def plan(self, new, tokens: int | None = None, max_new: int | None = None, releases: bool = True) -> KVPlan:
+        """As ``KVCache.plan``, but a request that is done (-1) gives up blocks that it shares, and its blocks are there
+        for this step already.  With a tensor ``new`` that costs a launch or two more, unless ``releases`` is False:
+        then -1 is taken for 0."""
+        if isinstance(new, torch.Tensor):
+            if releases:
+                self.fork(torch.where(new < 0, -1, self._rows).to(torch.int32))
+            new = new.clamp(min=0)
+        else:
+            new = [int(n) for n in new]
+            if min(new, default=0) < 0:
+                self.fork([-1 if n < 0 else i for i, n in enumerate(new)])
+            new = [max(n, 0) for n in new]
+        self._shared = None
+        return super().plan(new, tokens, max_new)
+
+    def fork(self, parents, keep=None) -> KVFork:
+        """Row i goes on from the first ``keep[i]`` tokens (default: all) of row ``parents[i]``; -1 frees it.  Lists, or
+        int32 tensors on the GPU.  Returns ``fork``'s result, whose copies are made; ``ring[2]`` counts rows that found no block
+        and are empty now."""
+        parents, keep = (x if x is None or isinstance(x, torch.Tensor) else
+                         torch.tensor([int(n) for n in x], dtype=torch.int32).to(self.lengths.device, non_blocking=True)
+                         for x in (parents, keep))
+        done = fork(self.lengths, self.tables, self.shares, self.free, self.ring, parents, block_size=self.block_size, keep=keep)
+        copy(self.pools, done.moves)
+        self.lengths.copy_(done.lengths)
+        self._take(done)
+        return done
+
+    def compact(self) -> KVCompact:
+        """Moves the blocks that rows hold to the front of the pools.  Returns ``compact``'s result, whose copies are made."""
+        done = compact(self.lengths, self.tables, self.shares, block_size=self.block_size)
+        copy(self.pools, done.moves)
+        self.free.copy_(done.free)
+        self._take(done)
+        return done
+
+    def _take(self, done: KVFork | KVCompact) -> None:
+        self.tables.copy_(done.tables)
+        self.shares.copy_(done.shares)
+        self.ring.copy_(done.ring)
+        self.step = self._shared = None  # slots and prefixes of a step planned before are not this table's
+
+    def attention(self, layer: int, q: torch.Tensor, **options):
+        """The step's queries over the layer's cache, what requests share once; with ``window`` or ``first``, which
+        prefixes do not allow, as ``KVCache.attention``."""
+        if options.get("window") or options.get("first") is not None:
+            return super().attention(layer, q, **options)
+        options.pop("window", None), options.pop("first", None)
+        step = self._planned()
+        if self._shared is None:
+            self._shared = prefixes(self.tables, step.lengths, step.starts, block_size=self.block_size,
+                                    blocks=self.pools[layer].blocks, tokens=q.shape[0])
+        return attention(q, self.pools[layer], self.tables, step.lengths, step.starts, self._shared,
+                         max_new=self._max_new, max_length=self.max_length, **options)
+
+
+__all__ = ["KVCompact", "KVFork", "KVMoves", "KVPrefixes", "SharedKVCache", "attention", "compact", "copy", "fork", "prefixes"]

@@ -69,3 +69,49 @@ def test_argument_errors_without_gpu():
 @pytest.mark.parametrize("args", [(None, 1, None, None, None, 0)])
 def test_copy_without_pools(args):
     assert _ebx.load().ebx_kv_copy(ctypes.cast(None, ctypes.POINTER(_ebx.KVPool)), *args[1:], None) == _ebx.EBX_ERR_INVALID
+
+
+def test_prefix_errors_without_gpu():
+    lib = _ebx.load()
+
+    def refused(status, words, code=_ebx.EBX_ERR_INVALID):
+        assert status == code
+        assert words in _ebx.last_error()
+
+    def prefixes(tables=4, width=1, block=16, blocks=1, requests=1, tokens=1, out=4, work=16, work_bytes=28):
+        return lib.ebx_kv_prefixes(tables, width, block, blocks, 4, 4, requests, tokens, out, work, work_bytes, 0, None)
+
+    refused(prefixes(tables=None), "null")
+    refused(prefixes(out=None), "null")
+    refused(prefixes(width=0), "width")
+    refused(prefixes(block=1), "block_size")
+    refused(prefixes(blocks=0), "blocks")
+    refused(prefixes(requests=16385), "16384")
+    refused(prefixes(tokens=2**31), "tokens")
+    refused(prefixes(work=8), "aligned")
+    refused(prefixes(work_bytes=27), "workspace", _ebx.EBX_ERR_WORKSPACE)
+    assert prefixes(requests=0, tables=None) == _ebx.EBX_OK
+    assert lib.ebx_kv_prefixes_ints(3, 5) == 20 and lib.ebx_kv_prefixes_ints(-1, 5) == 0
+
+    def pool(**change):
+        fields = dict(k_codes=16, k_scales=4, v_codes=16, v_scales=4, blocks=8, kv_heads=2, block_size=16, head_dim=64,
+                      device=0, reserved=0)
+        return ctypes.byref(_ebx.KVPool(*{**fields, **change}.values()))
+
+    def attention(p, heads=4, dtype=1, width=1, scale=1.0, q=16, stride=256, tokens=1, requests=1, shared=4, max_new=0):
+        return lib.ebx_kv_shared_attention(p, q, stride, 64, heads, dtype, 4, width, 4, 4, shared, requests, tokens, 1, scale,
+                                           max_new, 0, 16, None, None, 0, None)
+
+    refused(attention(None), "null")
+    refused(attention(pool(head_dim=96)), "head_dim")
+    refused(attention(pool(), heads=3), "multiple of kv_heads")
+    refused(attention(pool(), dtype=0), "dtype")
+    refused(attention(pool(), scale=float("nan")), "scale")
+    refused(attention(pool(), q=8), "aligned")
+    refused(attention(pool(), stride=12), "multiples of 8")
+    refused(attention(pool(), width=2**27), "out of range")
+    refused(attention(pool(), requests=16385), "out of range")
+    refused(attention(pool(), shared=None), "null")
+    refused(attention(pool(), max_new=-1), ">= 0")
+    assert attention(pool(), tokens=0) == _ebx.EBX_OK
+    assert lib.ebx_kv_shared_attention_workspace_bytes(pool(head_dim=96), 4, 1, 1, 1) == 0
