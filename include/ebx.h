@@ -437,7 +437,7 @@ EBX_API ebx_status ebx_kv_attention(const ebx_kv_pool* pool, const void* q, int6
  * Written: out_lengths [requests], out_tables [requests, width] (-1 behind what a row
  * holds), out_shares [blocks], ring_out[4] = {front, back, blocks that were missing, copies},
  * sources and targets [requests] (block numbers, -1 behind the last copy).  No output is an
- * input.  Entries that are no block are kept and not counted.  workspace: 4 * blocks bytes.
+ * input.  Entries that are no block are kept and not counted.
  * requests <= 16384, width * block_size and blocks * block_size < 2^31. */
 EBX_API ebx_status ebx_kv_fork(const int32_t* lengths, const int32_t* tables, int32_t width,
                                int32_t block_size, const int32_t* shares, int32_t blocks,
@@ -445,14 +445,15 @@ EBX_API ebx_status ebx_kv_fork(const int32_t* lengths, const int32_t* tables, in
                                const int32_t* parents, const int32_t* keep, int32_t requests,
                                int32_t* out_lengths, int32_t* out_tables, int32_t* out_shares,
                                int64_t* ring_out, int32_t* sources, int32_t* targets,
-                               void* workspace, uint64_t workspace_bytes, int32_t device, void* stream);
+                               int32_t device, void* stream);
 
 /* New numbers for the blocks that rows hold, so that they are the pool's first: of H held
  * blocks those numbered H or more move to the free numbers below H, in order, with copies to be
  * made by ebx_kv_copy.  Every other block is free afterwards, also one that neither a
  * row nor the ring had: free_out [blocks] holds their numbers, rising, then -1, and
  * ring_out[4] = {0, blocks - H, 0, copies}.  out_tables as in ebx_kv_fork; sources and targets
- * [blocks / 2], -1 behind the last copy.  No output is an input; workspace and limits as above. */
+ * [blocks / 2], -1 behind the last copy.  No output is an input; limits as above.
+ * workspace: 4 * blocks bytes. */
 EBX_API ebx_status ebx_kv_compact(const int32_t* lengths, const int32_t* tables, int32_t width,
                                   int32_t block_size, const int32_t* shares, int32_t blocks,
                                   int32_t requests, int32_t* out_tables, int32_t* out_shares,
@@ -472,18 +473,18 @@ EBX_API ebx_status ebx_kv_copy(const ebx_kv_pool* pools, int32_t layers, const i
  * its new tokens, as save most reading; who has fewer in common with the group's first request is left out.  Rows
  * that share nothing are taken alone.  `prefixes` receives ebx_kv_prefixes_ints(requests, tokens) ints, whose
  * layout is the library's own and which hold for one step: as long as tables (where blocks are shared), starts
- * and `tokens` stay, for every layer.  workspace: 24 * requests + 4 * blocks bytes, 16-byte aligned. */
+ * and `tokens` stay, for every layer.  requests <= 8192. */
 EBX_API uint64_t ebx_kv_prefixes_ints(int32_t requests, int64_t tokens);
 EBX_API ebx_status ebx_kv_prefixes(const int32_t* tables, int32_t width, int32_t block_size,
                                    int32_t blocks, const int32_t* lengths, const int32_t* starts,
-                                   int32_t requests, int64_t tokens, int32_t* prefixes, void* workspace,
-                                   uint64_t workspace_bytes, int32_t device, void* stream);
+                                   int32_t requests, int64_t tokens, int32_t* prefixes, int32_t device,
+                                   void* stream);
 
 /* ebx_kv_attention without window and `first`, for requests that share prefixes: the formula is the same,
  * but a group's shared keys and values are read once for the rows of all its members, and
  * the results over the prefix and over the rest joined in fp32.  Where a request brings many rows
  * of its own (max_new, or without it `tokens`, times heads / kv_heads, 49 and more), requests go
- * by themselves, as in ebx_kv_attention.  requests <= 16384.  `prefixes` of another step, or of other tables,
+ * by themselves, as in ebx_kv_attention.  requests <= 8192.  `prefixes` of another step, or of other tables,
  * make the result meaningless, but nothing outside the buffers is touched. */
 EBX_API uint64_t ebx_kv_shared_attention_workspace_bytes(const ebx_kv_pool* pool, int32_t heads,
                                                          int64_t tokens, int32_t max_new,
@@ -508,7 +509,7 @@ EBX_API ebx_status ebx_kv_shared_attention(const ebx_kv_pool* pool, const void* 
  * [rotary_dim / 2].  A side is [tokens, heads, head_dim] whose last dimension is
  * contiguous; strides in elements.  out is in, with the same strides, or shares no
  * element with it; no two sides share elements.  k may be NULL, heads may be 0.
- * 16-byte aligned bases, strides of 16 bytes and rotary_dim / 2 of as many are fastest. */
+ * head_dim <= 4096, heads <= 65536.  16-byte aligned bases, strides of 16 bytes and rotary_dim / 2 of as many are fastest. */
 typedef struct {
     const void* in;
     void* out;

@@ -122,6 +122,20 @@ cudaError_t launch_early(void (*kern)(P...), dim3 grid, int threads, size_t smem
     return cudaLaunchKernelEx(&cfg, kern, P(args)...);
 }
 
+// ebx_kv_share.cu: that of the kernel that copies blocks.
+cudaError_t read_kv_copy_status(int* status, bool clear, cudaStream_t s);
+
+// Reads (and clears) a translation unit's status word; synchronizes `s`.
+inline cudaError_t read_status_word(const int& word, int* status, bool clear, cudaStream_t s) {
+    void* p = nullptr;
+    cudaError_t e = cudaGetSymbolAddress(&p, word);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(status, p, sizeof(int), cudaMemcpyDeviceToHost, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    if (e == cudaSuccess && clear) e = cudaMemsetAsync(p, 0, sizeof(int), s);
+    if (e == cudaSuccess && clear) e = cudaStreamSynchronize(s);
+    return e;
+}
+
 // ebx_gemm.cu: cuTensorMapEncodeTiled of the loaded driver (null without one).
 void* tensor_map_encoder();
 int gemm_sm_count(int dev);

@@ -762,10 +762,11 @@ cudaError_t launch_kv_shared_attention(KvAttnArgs a, bool bf16, int max_new, int
 }
 
 cudaError_t read_kv_status(int* status, bool clear, cudaStream_t s) {
-    int prompt = 0;
+    int prompt = 0, copy = 0;
     cudaError_t e = read_status_word(g_kv_status, status, clear, s);
     if (e == cudaSuccess) e = read_kv_prompt_status(&prompt, clear, s);
-    if (*status == 0) *status = prompt;
+    if (e == cudaSuccess) e = read_kv_copy_status(&copy, clear, s);
+    if (*status == 0) *status = prompt != 0 ? prompt : copy;
     return e;
 }
 

@@ -6,6 +6,7 @@
 // a fraction of a launch.  Counts are changed by atomic additions only, whose order does not change
 // them, and whatever is given an order (blocks to the ring, copies) gets it from sums over rows or ids.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 #include <cooperative_groups.h>
@@ -98,11 +99,15 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kShareThreads
     auto block = [&](int id) { return id >= 0 && id < a.blocks; };
     if (tid == 0) s_missing = 0;
 
-    for (int b = gtid; b < a.blocks; b += kAll) {
-        a.out_shares[b] = a.shares[b];
-        a.claim[b] = INT_MAX;
-    }
+    for (int b = gtid; b < a.blocks; b += kAll) a.out_shares[b] = a.shares[b];
     for (int r = gtid; r < a.requests; r += kAll) a.sources[r] = a.targets[r] = -1;
+    auto tail_of = [&](const ForkRow& f) { return a.tables[int64_t(f.parent) * a.width + (f.keep >> a.shift)]; };
+    ForkRow mine{};  // the row of this thread below
+    int my_tail = -1;
+    if (rank == 0 && tid < a.requests) {
+        mine = fork_row(a, tid);
+        if (mine.begun) my_tail = tail_of(mine);
+    }
     cluster.sync();
 
     for (int r = gwarp; r < a.requests; r += kAllWarps) {
@@ -127,41 +132,41 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kShareThreads
     }
     cluster.sync();
 
-    // who keeps a begun block that no row holds whole
-    auto key_of = [&](const ForkRow& f, int r) { return f.parent == r ? r : r + a.requests; };
-    auto tail_of = [&](const ForkRow& f) { return a.tables[int64_t(f.parent) * a.width + (f.keep >> a.shift)]; };
-    for (int r = gtid; r < a.requests; r += kAll) {
-        const ForkRow f = fork_row(a, r);
-        if (!f.begun) continue;
-        const int id = tail_of(f);
-        if (block(id) && a.out_shares[id] < 0) atomicMin(a.claim + id, key_of(f, r));
-    }
-    cluster.sync();
-
+    // Begun blocks, by the cluster's first CTA, a thread to a row.  Who keeps one that no row holds whole: its count, -1,
+    // becomes the lowest of the rows' claims.
     if (rank == 0) {
-        int64_t taken = 0;
-        for (int base = 0; base < a.requests; base += kShareThreads) {
-            const int r = base + tid;
-            bool need = false;
-            int id = -1, column = 0;
-            if (r < a.requests) {
-                const ForkRow f = fork_row(a, r);
-                if (f.begun) {
-                    id = tail_of(f);
-                    column = f.keep >> a.shift;
-                    need = block(id);
-                    if (need && a.claim[id] == key_of(f, r)) {
-                        atomicAdd(a.out_shares + id, 1);
-                        need = false;
-                    }
+        auto claim_of = [&](const ForkRow& f, int r) { return INT_MIN + (f.parent == r ? r : r + a.requests); };
+        auto each_row = [&](auto go) {  // the first kShareThreads rows are known already
+            for (int base = 0; base < a.requests; base += kShareThreads) {
+                const int r = base + tid;
+                ForkRow f = mine;
+                int id = my_tail;
+                if (base > 0) {
+                    f.begun = false;
+                    id = -1;
+                    if (r < a.requests) f = fork_row(a, r);
+                    if (f.begun) id = tail_of(f);
                 }
+                go(r, f, id);
+            }
+        };
+        each_row([&](int r, const ForkRow& f, int id) {
+            if (f.begun && block(id) && __ldcg(a.out_shares + id) < 0) atomicMin(a.out_shares + id, claim_of(f, r));
+        });
+        __syncthreads();
+        int64_t taken = 0;
+        each_row([&](int r, const ForkRow& f, int id) {
+            bool need = f.begun && block(id);
+            if (need && __ldcg(a.out_shares + id) == claim_of(f, r)) {  // no other row has that claim
+                a.out_shares[id] = 0;
+                need = false;
             }
             int total;
             const int64_t before = taken + block_sum(need, warp_sums, total);
             if (need) {
                 if (before < avail) {
                     const int fresh = a.free_ring[wrapped(front + before)];
-                    a.out_tables[int64_t(r) * a.width + column] = fresh;
+                    a.out_tables[int64_t(r) * a.width + (f.keep >> a.shift)] = fresh;
                     a.sources[before] = id;
                     a.targets[before] = fresh;
                 } else {
@@ -170,7 +175,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kShareThreads
                 }
             }
             taken += total;
-        }
+        });
         __syncthreads();
         if (tid == 0) {
             taken = min(taken, avail);
@@ -199,10 +204,9 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kShareThreads
     // a part of the blocks each: count those that nobody holds, then write them behind those of the parts before
     const int per = int((int64_t(a.blocks) + kCluster - 1) / kCluster);
     const int b0 = min(rank * int64_t(per), int64_t(a.blocks)), b1 = min(b0 + int64_t(per), int64_t(a.blocks));
-    int mine = 0;
-    for (int b = b0 + tid; b < b1; b += kShareThreads) mine += a.out_shares[b] < 0;
-    int total;
-    block_sum(mine, warp_sums, total);
+    int gone_here = 0, total;
+    for (int b = b0 + tid; b < b1; b += kShareThreads) gone_here += a.out_shares[b] < 0;
+    block_sum(gone_here, warp_sums, total);
     tell(cluster, counts, total);
     int64_t at = 0, all = 0;
     for (int c = 0; c < kCluster; ++c) {
@@ -318,168 +322,257 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kShareThreads
 
 // ---- copy ---------------------------------------------------------------------------------
 
-constexpr int kCopyThreads = 256;
-constexpr int kCopySegment = kCopyThreads * 16 * 4;  // bytes of a unit
+constexpr int kCopyThreads = 128;     // a warp for the codes, the others for scales
+constexpr int kCopySegment = 16384;   // bytes of a unit
+constexpr int kCopyStages = 4;
+constexpr int kCopyCtas = 3;          // of an SM
 
-// Unit: a segment of one side of one pair of blocks in one layer; the first segment brings the scales along.
+__device__ int g_kv_copy_status = 0;
+
+__device__ __forceinline__ bool copy_wait(uint32_t bar, uint32_t parity) {
+    if (mbar_wait_bounded(bar, parity)) return true;
+    atomicExch(&g_kv_copy_status, 0x7106);
+    return false;
+}
+
+// Unit: a segment of one side of one pair of blocks in one layer.  One thread sends a CTA's units through a ring of
+// shared memory by bulk copies, which need no registers on the way.
 __global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(const __grid_constant__ KvCopyArgs a) {
+    extern __shared__ __align__(128) uint8_t copy_smem[];
+    __shared__ uint64_t full[kCopyStages];
+    __shared__ int8_t* s_to[kCopyStages];
+    __shared__ uint32_t s_bytes[kCopyStages];
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kCopyStages; ++i) mbar_init(smem_u32(&full[i]), 1);
+        fence_proxy_async_smem();
+    }
     asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
     const int64_t pairs = a.count ? min(max(*a.count, int64_t(0)), int64_t(a.n)) : a.n;
+    auto block = [&](int id) { return id >= 0 && id < a.blocks; };
+    if (threadIdx.x >= 32) {
+        const int64_t all = pairs * a.layers * 2 * a.kv_heads, step = int64_t(gridDim.x) * (kCopyThreads - 32);
+        for (int64_t x = int64_t(blockIdx.x) * (kCopyThreads - 32) + threadIdx.x - 32; x < all; x += step) {
+            const int64_t cell = x / a.kv_heads, h = x - cell * a.kv_heads, unit = cell >> 1, pair = unit / a.layers;
+            const int from = a.sources[pair], to = a.targets[pair];
+            if (!block(from) || !block(to)) continue;
+            float* scales = a.layer[int(unit - pair * a.layers)].scales[cell & 1];
+            scales[int64_t(to) * a.kv_heads + h] = scales[int64_t(from) * a.kv_heads + h];
+        }
+        return;
+    }
+    if (threadIdx.x != 0) return;
     const int segments = int((a.bytes + kCopySegment - 1) / kCopySegment);
     const int64_t units = pairs * a.layers * 2 * segments;
-    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-        const int64_t side_unit = u / segments;
-        const int segment = int(u - side_unit * segments), side = int(side_unit & 1);
-        const int64_t layer_unit = side_unit >> 1;
-        const int64_t pair = layer_unit / a.layers;
-        const int layer = int(layer_unit - pair * a.layers);
-        const int from = a.sources[pair], to = a.targets[pair];
-        if (from < 0 || from >= a.blocks || to < 0 || to >= a.blocks || from == to) continue;
-        const int8_t* src = a.layer[layer].codes[side] + from * a.bytes;
-        int8_t* dst = a.layer[layer].codes[side] + to * a.bytes;
-        const int64_t first = int64_t(segment) * kCopySegment + threadIdx.x * 16;
-        uint4 v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (first + i * kCopyThreads * 16 < a.bytes) v[i] = *reinterpret_cast<const uint4*>(src + first + i * kCopyThreads * 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (first + i * kCopyThreads * 16 < a.bytes) *reinterpret_cast<uint4*>(dst + first + i * kCopyThreads * 16) = v[i];
-        if (segment == 0) {
-            float* scales = a.layer[layer].scales[side];
-            for (int h = threadIdx.x; h < a.kv_heads; h += kCopyThreads)
-                scales[int64_t(to) * a.kv_heads + h] = scales[int64_t(from) * a.kv_heads + h];
+    int64_t u = blockIdx.x;
+    const int8_t* src = nullptr;
+    int8_t* dst = nullptr;
+    uint32_t bytes = 0;
+    auto next = [&]() {  // the CTA's next unit that there is
+        for (; u < units; u += gridDim.x) {
+            const int64_t cell = u / segments, unit = cell >> 1, pair = unit / a.layers;
+            const int from = a.sources[pair], to = a.targets[pair];
+            if (!block(from) || !block(to) || from == to) continue;
+            const int64_t at = (u - cell * segments) * kCopySegment;
+            int8_t* codes = a.layer[int(unit - pair * a.layers)].codes[cell & 1];
+            src = codes + from * a.bytes + at;
+            dst = codes + to * a.bytes + at;
+            bytes = uint32_t(min(a.bytes - at, int64_t(kCopySegment)));
+            u += gridDim.x;
+            return true;
         }
+        return false;
+    };
+    bool more = next(), ok = true;
+    int sent = 0, stored = 0;  // units on their way here, and from here
+    for (;;) {
+        while (more && sent < stored + kCopyStages - 1) {
+            const int st = sent % kCopyStages;
+            // the stage's unit before, sent - kCopyStages <= stored - 2, has left: all but the last store have read theirs
+            if (sent >= kCopyStages) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            const uint32_t bar = smem_u32(&full[st]);
+            mbar_expect_tx(bar, bytes);
+            bulk_g2s(smem_u32(copy_smem + st * kCopySegment), src, bytes, bar);
+            s_to[st] = dst;
+            s_bytes[st] = bytes;
+            ++sent;
+            more = next();
+        }
+        if (stored == sent) break;
+        const int st = stored % kCopyStages;
+        ok = copy_wait(smem_u32(&full[st]), uint32_t((stored / kCopyStages) & 1));
+        if (!ok) break;
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n\tcp.async.bulk.commit_group;" ::"l"(s_to[st]),
+                     "r"(smem_u32(copy_smem + st * kCopySegment)), "r"(s_bytes[st]) : "memory");
+        ++stored;
     }
+    if (!ok)  // given up: what is on its way lands before this shared memory is another CTA's
+        for (; stored < sent; ++stored) copy_wait(smem_u32(&full[stored % kCopyStages]), uint32_t((stored / kCopyStages) & 1));
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 // ---- prefixes -----------------------------------------------------------------------------
 
+constexpr int kPrefixThreads = 512;
+constexpr int kPrefixColumns = 128;   // entries that a warp compares at a time
+
+// Ascending, in place; `size` a power of two.  Called by all threads of the block.
+__device__ __forceinline__ void sort(uint64_t* keys, int size) {
+    for (int k = 2; k <= size; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            __syncthreads();
+            for (int t = threadIdx.x; t < size / 2; t += kPrefixThreads) {
+                const int i = 2 * t - (t & (j - 1)), o = i + j;
+                const uint64_t x = keys[i], y = keys[o];
+                if ((x > y) == ((i & k) == 0)) {
+                    keys[i] = y;
+                    keys[o] = x;
+                }
+            }
+        }
+    __syncthreads();
+}
+
 // Requests that bring tokens and whose tables begin with the same block are compared with the first of
 // them: common[i] full blocks ahead of the new tokens are the same.  Of the lengths that occur, the one that
 // saves most reading, (members with at least that much in common - 1) * length, becomes the group's.
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kShareThreads, 1) kv_prefixes_kernel(const __grid_constant__ KvPrefixArgs a) {
-    asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
+//
+// Every CTA sorts the requests by their first blocks, so that each knows everyone's leader; the comparisons are shared
+// out among the cluster, and minima kept in the first CTA, which then sorts by leader and length: a request's place among
+// its leader's is one less than the members that its length would have.
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kPrefixThreads, 1)
+    kv_prefixes_kernel(const __grid_constant__ KvPrefixArgs a) {
     cg::cluster_group cluster = cg::this_cluster();
-    extern __shared__ int2 found[];  // [requests]: leader, blocks in common
+    extern __shared__ __align__(16) uint8_t prefix_smem[];
     __shared__ int warp_sums[32];
-    const int tid = threadIdx.x, lane = tid & 31, rank = int(cluster.block_rank());
-    const int gtid = rank * kShareThreads + tid, gwarp = gtid >> 5;
-    constexpr int kAll = kCluster * kShareThreads, kAllWarps = kAll / 32;
-    const int n = a.requests;
-    unsigned long long* best = reinterpret_cast<unsigned long long*>(a.scratch);  // [n]: saved << 14 | request
-    int2* pairs = reinterpret_cast<int2*>(a.scratch + 2 * n);                     // [n]: `found`
-    int* offset = a.scratch + 4 * n;                                              // [n]: tokens of the group ahead
-    int* totals = a.scratch + 5 * n;                                              // [n]: tokens of group i
-    auto from = [&](int i) { return int(min(max(int64_t(a.starts[i]), int64_t(0)), a.tokens)); };
-    auto brings = [&](int i) { return max(from(i + 1) - from(i), 0); };
-    auto ahead = [&](int i) {  // full blocks ahead of the new tokens
-        const int64_t cap = int64_t(a.width) << a.shift;
-        const int64_t past = min(int64_t(max(a.lengths[i], 0)), cap) - brings(i);
-        return past > 0 && brings(i) > 0 ? int(past >> a.shift) : 0;
-    };
-    auto block = [&](int id) { return id >= 0 && id < a.blocks; };
-    auto key_of = [&](int i) {
-        const int id = ahead(i) > 0 ? a.tables[int64_t(i) * a.width] : -1;
-        return block(id) ? id : -1;
-    };
-
-    for (int i = gtid; i < n; i += kAll) {
-        const int key = key_of(i);
-        if (key >= 0) a.first_with[key] = INT_MAX;
+    const int n = a.requests, size = a.size;
+    uint64_t* keys = reinterpret_cast<uint64_t*>(prefix_smem);                            // [size]
+    unsigned long long* best = reinterpret_cast<unsigned long long*>(keys + size);        // [n]: saved << 13 | place
+    int* full = reinterpret_cast<int*>(best + n);  // [n]: a request's full blocks ahead of its new tokens
+    int* common = full + n;                        // [n], then of a place: its leader's first place, its tokens' in the list
+    int* leader = common + n;                      // [n], then tokens of a group
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = int(cluster.block_rank());
+    constexpr int kWarps = kPrefixThreads / 32;
+    if (tid < 32) warp_sums[tid] = 0;
+    for (int i = tid; i < n; i += kPrefixThreads) {
+        common[i] = INT_MAX;
         best[i] = 0;
     }
-    for (int64_t t = gtid; t < a.tokens; t += kAll) a.out.state[t] = 0;
-    cluster.sync();
-    for (int i = gtid; i < n; i += kAll) {
-        const int key = key_of(i);
-        if (key >= 0) atomicMin(a.first_with + key, i);
-    }
-    cluster.sync();
-    for (int i = gwarp; i < n; i += kAllWarps) {
-        const int key = key_of(i);
-        const int leader = key >= 0 ? a.first_with[key] : -1;
-        int common = 0;
-        if (leader == i) common = ahead(i);
-        if (leader >= 0 && leader != i) {
-            const int most = min(ahead(i), ahead(leader));
-            const int32_t* x = a.tables + int64_t(i) * a.width;
-            const int32_t* y = a.tables + int64_t(leader) * a.width;
-            common = most;
-            for (int j0 = 0; j0 < most; j0 += 128) {
-                unsigned differ[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int j = j0 + q * 32 + lane;
-                    differ[q] = __ballot_sync(0xffffffffu, j < most && x[j] != y[j]);
-                }
-                int at = -1;
-#pragma unroll
-                for (int q = 3; q >= 0; --q)
-                    if (differ[q]) at = j0 + q * 32 + __ffs(differ[q]) - 1;
-                if (at >= 0) {
-                    common = at;
-                    break;
-                }
-            }
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");  // waited for ahead of the first minimum
+    asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
+    auto from = [&](int i) { return int(min(max(int64_t(a.starts[i]), int64_t(0)), a.tokens)); };
+    auto brings = [&](int i) { return max(from(i + 1) - from(i), 0); };
+
+    // keys: block << 13 | request; behind them those that share nothing, and none at all
+    constexpr uint64_t kAlone = uint64_t(1) << 44, kNone = ~uint64_t(0);
+    for (int i = tid; i < size; i += kPrefixThreads) {
+        uint64_t key = kNone;
+        if (i < n) {
+            const int64_t cap = int64_t(a.width) << a.shift;
+            const int count = brings(i);
+            const int64_t past = min(int64_t(max(a.lengths[i], 0)), cap) - count;
+            full[i] = past > 0 && count > 0 ? int(past >> a.shift) : 0;
+            const int id = full[i] > 0 ? a.tables[int64_t(i) * a.width] : -1;
+            key = (id >= 0 && id < a.blocks ? uint64_t(id) << 13 : kAlone) | uint64_t(i);
         }
-        if (lane == 0) pairs[i] = make_int2(leader, common);
+        keys[i] = key;
     }
-    cluster.sync();
-    for (int i = tid; i < n; i += kShareThreads) found[i] = pairs[i];
+    sort(keys, size);
+    // the first place in [0, p] whose key begins like that of place p
+    auto begins = [&](int p, int shift) {
+        int lo = -1, hi = p;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (keys[mid] >> shift == keys[p] >> shift) hi = mid; else lo = mid;
+        }
+        return hi;
+    };
+    for (int p = tid; p < n; p += kPrefixThreads)
+        if (keys[p] < kAlone) leader[keys[p] & 8191] = int(keys[begins(p, 13)] & 8191);
+    for (int64_t t = int64_t(rank) * kPrefixThreads + tid; t < a.tokens; t += kCluster * kPrefixThreads) a.out.state[t] = 0;
     __syncthreads();
-    for (int i = gtid; i < n; i += kAll) {
-        const int2 me = found[i];
-        if (me.x < 0) continue;
-        int members = 0;
-        for (int j = me.x; j < n; ++j) {
-            const int2 it = found[j];
-            members += it.x == me.x && it.y >= me.y;
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    // a warp to a piece of a row
+    int* minima = cluster.map_shared_rank(common, 0);
+    const int pieces = (a.width + kPrefixColumns - 1) / kPrefixColumns;
+    for (int64_t x = int64_t(rank) * kWarps + warp; x < int64_t(n) * pieces; x += kCluster * kWarps) {
+        const int place = int(x / pieces), j0 = int(x - int64_t(place) * pieces) * kPrefixColumns;
+        if (keys[place] >= kAlone) break;  // and all behind it
+        const int i = int(keys[place] & 8191), first = leader[i];
+        const int most = min(full[i], full[first]);
+        if (i == first || j0 >= most) continue;
+        const int32_t* mine = a.tables + int64_t(i) * a.width;
+        const int32_t* its = a.tables + int64_t(first) * a.width;
+        bool differ[kPrefixColumns / 32];
+#pragma unroll
+        for (int q = 0; q < kPrefixColumns / 32; ++q) {
+            const int j = j0 + q * 32 + lane;
+            differ[q] = j < most && mine[j] != its[j];
         }
-        if (members > 1) atomicMax(best + me.x, static_cast<unsigned long long>(int64_t(members - 1) * me.y) << 14 | unsigned(i));
+        int at = INT_MAX;
+#pragma unroll
+        for (int q = kPrefixColumns / 32 - 1; q >= 0; --q) {
+            const unsigned any = __ballot_sync(0xffffffffu, differ[q]);
+            if (any) at = j0 + q * 32 + __ffs(any) - 1;
+        }
+        if (lane == 0 && at != INT_MAX) atomicMin(minima + i, at);
     }
     cluster.sync();
-    // blocks that group g shares; 0: no group
-    auto depth = [&](int g) { return best[g] == 0 ? 0 : found[int(best[g] & 0x3fff)].y; };
-    auto grouped = [&](int i) { return found[i].x >= 0 && depth(found[i].x) > 0 && found[i].y >= depth(found[i].x); };
-    for (int i = gtid; i < n; i += kAll) {
-        const int2 me = found[i];
-        const bool in = grouped(i);
-        const int deep = in ? depth(me.x) : 0;
-        int ahead_of_me = 0, all = 0;
-        if (in) {
-            for (int j = me.x; j < (me.x == i ? n : i); ++j) {
-                const int2 it = found[j];
-                const int m = it.x == me.x && it.y >= deep ? brings(j) : 0;
-                if (j < i) ahead_of_me += m;
-                all += m;
-            }
-        }
-        offset[i] = ahead_of_me;
-        totals[i] = in && me.x == i ? all : 0;
-        a.out.shared[i] = in && me.x == i ? deep << a.shift : 0;
-        a.out.own_first[i] = deep << a.shift;
+    if (rank != 0) return;
+
+    // keys: leader << 40 | (kMost - length) << 13 | request; those that share nothing have the leader 8192
+    constexpr uint64_t kMost = (1 << 27) - 1;
+    for (int p = tid; p < n; p += kPrefixThreads) {
+        const int i = int(keys[p] & 8191);
+        const bool alone = keys[p] >= kAlone;
+        const int first = alone ? 8192 : leader[i];
+        const int length = alone ? 0 : min(common[i], min(full[i], full[first]));
+        keys[p] = uint64_t(first) << 40 | (kMost - uint64_t(length)) << 13 | uint64_t(i);
     }
-    cluster.sync();
-    // every CTA sums for itself; `found` then holds the groups' first tokens in place of the leaders
-    int base = 0;
-    for (int i0 = 0; i0 < n; i0 += kShareThreads) {
-        const int i = i0 + tid;
+    sort(keys, size);
+    auto length_of = [&](int p) { return int(kMost - (keys[p] >> 13 & kMost)); };
+    int* begin = common;
+    int* tokens = leader;
+    for (int p = tid; p < n; p += kPrefixThreads) {
+        tokens[p] = 0;
+        const int b = begins(p, 40);
+        begin[p] = b;
+        if (p > b) atomicMax(best + b, static_cast<unsigned long long>(int64_t(p - b) * length_of(p)) << 13 | unsigned(p));
+    }
+    __syncthreads();
+    int64_t listed = 0;
+    for (int p0 = 0; p0 < n; p0 += kPrefixThreads) {
+        const int p = p0 + tid;
+        int depth = 0, count = 0, total;
+        if (p < n) {
+            const unsigned long long b = best[begin[p]];
+            depth = b >> 13 ? length_of(int(b & 8191)) : 0;  // what the group shares
+            if (length_of(p) < depth) depth = 0;
+            if (depth > 0) count = brings(int(keys[p] & 8191));
+        }
+        const int64_t to = listed + block_sum(count, warp_sums, total);
+        listed += total;
+        if (p >= n) continue;
+        const int i = int(keys[p] & 8191), first = int(keys[p] >> 40);
+        a.out.shared[i] = first == i ? depth << a.shift : 0;
+        a.out.own_first[i] = depth << a.shift;
+        if (depth > 0) atomicAdd(tokens + first, count);
+        begin[p] = depth > 0 ? int(min(to, int64_t(INT_MAX))) : -1;
+    }
+    __syncthreads();
+    int64_t ahead = 0;
+    for (int g0 = 0; g0 < n; g0 += kPrefixThreads) {
+        const int g = g0 + tid;
         int total;
-        const int start = base + block_sum(i < n ? totals[i] : 0, warp_sums, total);
-        if (i < n && rank == 0) a.out.group_starts[i] = int(min(int64_t(start), a.tokens));
-        if (i < n) found[i].y = start;
-        base += total;
+        const int64_t start = ahead + block_sum(g < n ? tokens[g] : 0, warp_sums, total);
+        if (g < n) a.out.group_starts[g] = int(min(start, a.tokens));
+        ahead += total;
     }
-    if (gtid == 0) a.out.group_starts[n] = int(min(int64_t(base), a.tokens));
-    __syncthreads();
-    for (int i = gwarp; i < n; i += kAllWarps) {
-        const bool in = a.out.own_first[i] > 0;
-        const int64_t to = in ? int64_t(found[found[i].x].y) + offset[i] : 0;
-        const int t0 = from(i), count = brings(i);
+    if (tid == 0) a.out.group_starts[n] = int(min(ahead, a.tokens));
+    for (int p = warp; p < n; p += kWarps) {
+        const int i = int(keys[p] & 8191), to = begin[p], t0 = from(i), count = brings(i);
         for (int t = lane; t < count; t += 32) {
-            a.out.state[t0 + t] = in ? 2 : 1;
-            if (in && uint64_t(to + t) < uint64_t(a.tokens)) a.out.list[to + t] = t0 + t;
+            a.out.state[t0 + t] = to >= 0 ? 2 : 1;
+            if (to >= 0 && int64_t(to) + t < a.tokens) a.out.list[to + t] = t0 + t;
         }
     }
 }
@@ -494,22 +587,36 @@ cudaError_t launch_kv_compact(const KvCompactArgs& a, cudaStream_t s) {
     return launch_early(kv_compact_kernel, dim3(kCluster), kShareThreads, 0, s, a);
 }
 
-cudaError_t launch_kv_copy(const KvCopyArgs& a, int sms, cudaStream_t s) {
+cudaError_t launch_kv_copy(const KvCopyArgs& a, int sms, int dev, cudaStream_t s) {
     if (a.n <= 0 || a.layers <= 0) return cudaSuccess;
+    constexpr int kSmem = kCopyStages * kCopySegment;
+    static std::atomic<uint64_t> configured{0};
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(configured.load(std::memory_order_relaxed) & bit)) {
+        const cudaError_t e = cudaFuncSetAttribute(kv_copy_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        if (e != cudaSuccess) return e;
+        configured.fetch_or(bit);
+    }
     const int64_t segments = (a.bytes + kCopySegment - 1) / kCopySegment;
     const int64_t units = int64_t(a.n) * a.layers * 2 * segments;
-    const int64_t grid = std::min<int64_t>(units, int64_t(sms) * 8);
-    return launch_early(kv_copy_kernel, dim3(unsigned(grid)), kCopyThreads, 0, s, a);
+    const int64_t grid = std::min<int64_t>(units, int64_t(sms) * kCopyCtas);
+    return launch_early(kv_copy_kernel, dim3(unsigned(grid)), kCopyThreads, kSmem, s, a);
 }
 
-cudaError_t launch_kv_prefixes(const KvPrefixArgs& a, cudaStream_t s) {
-    const size_t smem = size_t(a.requests) * sizeof(int2);
-    if (smem > 40 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kv_prefixes_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   kKvMaxRequests * int(sizeof(int2)));
+cudaError_t read_kv_copy_status(int* status, bool clear, cudaStream_t s) {
+    return read_status_word(g_kv_copy_status, status, clear, s);
+}
+
+cudaError_t launch_kv_prefixes(KvPrefixArgs a, cudaStream_t s) {
+    a.size = 2;
+    while (a.size < a.requests) a.size *= 2;
+    constexpr int kMostSmem = kKvMostPrefixes * (8 + 8 + 3 * 4);
+    const size_t smem = size_t(a.size) * 8 + size_t(a.requests) * (8 + 3 * 4);
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kv_prefixes_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem);
         if (e != cudaSuccess) return e;
     }
-    return launch_early(kv_prefixes_kernel, dim3(kCluster), kShareThreads, smem, s, a);
+    return launch_early(kv_prefixes_kernel, dim3(kCluster), kPrefixThreads, smem, s, a);
 }
 
 }  // namespace ebx

@@ -22,7 +22,6 @@ struct KvForkArgs {
     int64_t* ring_out;
     int32_t* sources;         // [requests]
     int32_t* targets;
-    int32_t* claim;           // [blocks], scratch
     int requests, width, shift, blocks, free_size;
 };
 
@@ -74,16 +73,15 @@ struct KvPrefixArgs {
     const int32_t* lengths;
     const int32_t* starts;
     KvPrefixes out;
-    int32_t* first_with;    // [blocks], scratch
-    int32_t* scratch;       // [kKvPrefixScratch * requests]
     int64_t tokens;
     int requests, width, shift, blocks;
+    int size;               // a power of two, requests or more (set by the launch)
 };
-constexpr int kKvPrefixScratch = 6;
+constexpr int kKvMostPrefixes = 8192;  // requests that kv_prefixes sorts in shared memory
 
 cudaError_t launch_kv_fork(const KvForkArgs& a, cudaStream_t s);
 cudaError_t launch_kv_compact(const KvCompactArgs& a, cudaStream_t s);
-cudaError_t launch_kv_copy(const KvCopyArgs& a, int sms, cudaStream_t s);
-cudaError_t launch_kv_prefixes(const KvPrefixArgs& a, cudaStream_t s);
+cudaError_t launch_kv_copy(const KvCopyArgs& a, int sms, int dev, cudaStream_t s);
+cudaError_t launch_kv_prefixes(KvPrefixArgs a, cudaStream_t s);
 
 }  // namespace ebx

@@ -25,25 +25,19 @@ ebx_status ebx_kv_fork(const int32_t* lengths, const int32_t* tables, int32_t wi
                        const int32_t* shares, int32_t blocks, int32_t* free_ring, int32_t free_size,
                        const int64_t* ring, const int32_t* parents, const int32_t* keep, int32_t requests,
                        int32_t* out_lengths, int32_t* out_tables, int32_t* out_shares, int64_t* ring_out,
-                       int32_t* sources, int32_t* targets, void* workspace, uint64_t workspace_bytes,
-                       int32_t device, void* stream) {
+                       int32_t* sources, int32_t* targets, int32_t device, void* stream) {
     if (const char* msg = table_of(requests, width, block_size, blocks)) return invalid(msg);
-    if (!shares || !free_ring || !ring || !out_shares || !ring_out || !workspace ||
+    if (!shares || !free_ring || !ring || !out_shares || !ring_out ||
         (requests > 0 && (!lengths || !tables || !parents || !out_lengths || !out_tables || !sources || !targets)))
         return invalid("null argument");
     if (free_size < 1) return invalid("ebx_kv_fork: need free_size >= 1");
     if (out_shares == shares || ring_out == ring ||
         (requests > 0 && (out_lengths == lengths || out_tables == tables)))
         return invalid("ebx_kv_fork: outputs must not be inputs");
-    if (workspace_bytes < uint64_t(blocks) * 4) {
-        ebx::set_error("ebx_kv_fork: workspace smaller than 4 * blocks bytes");
-        return EBX_ERR_WORKSPACE;
-    }
     Device d(device);
     if (d.err != cudaSuccess) return launched(d.err, "cudaSetDevice");
     const ebx::KvForkArgs a{lengths, tables, shares, free_ring, ring, parents, keep, out_lengths, out_tables, out_shares,
-                            ring_out, sources, targets, static_cast<int32_t*>(workspace), requests, width,
-                            log2_of(block_size), blocks, free_size};
+                            ring_out, sources, targets, requests, width, log2_of(block_size), blocks, free_size};
     return launched(ebx::launch_kv_fork(a, static_cast<cudaStream_t>(stream)), "ebx_kv_fork");
 }
 
@@ -103,7 +97,7 @@ ebx_status ebx_kv_copy(const ebx_kv_pool* pools, int32_t layers, const int32_t* 
             a.layer[i].scales[0] = p.k_scales;
             a.layer[i].scales[1] = p.v_scales;
         }
-        const ebx_status st = launched(ebx::launch_kv_copy(a, sms, static_cast<cudaStream_t>(stream)), "ebx_kv_copy");
+        const ebx_status st = launched(ebx::launch_kv_copy(a, sms, pools->device, static_cast<cudaStream_t>(stream)), "ebx_kv_copy");
         if (st != EBX_OK) return st;
     }
     return EBX_OK;
@@ -115,16 +109,12 @@ uint64_t ebx_kv_prefixes_ints(int32_t requests, int64_t tokens) {
 
 ebx_status ebx_kv_prefixes(const int32_t* tables, int32_t width, int32_t block_size, int32_t blocks,
                            const int32_t* lengths, const int32_t* starts, int32_t requests, int64_t tokens,
-                           int32_t* prefixes, void* workspace, uint64_t workspace_bytes, int32_t device, void* stream) {
+                           int32_t* prefixes, int32_t device, void* stream) {
     if (const char* msg = table_of(requests, width, block_size, blocks)) return invalid(msg);
+    if (requests > ebx::kKvMostPrefixes) return invalid("ebx_kv_prefixes: need requests <= 8192");
     if (tokens < 0 || tokens > INT32_MAX) return invalid("ebx_kv_prefixes: need 0 <= tokens < 2^31");
     if (requests == 0) return EBX_OK;
-    if (!tables || !lengths || !starts || !prefixes || !workspace) return invalid("null argument");
-    if (reinterpret_cast<uintptr_t>(workspace) & 15) return invalid("ebx_kv_prefixes: workspace must be 16-byte aligned");
-    if (workspace_bytes < 4 * (uint64_t(ebx::kKvPrefixScratch) * requests + uint64_t(blocks))) {
-        ebx::set_error("ebx_kv_prefixes: workspace smaller than 24 * requests + 4 * blocks bytes");
-        return EBX_ERR_WORKSPACE;
-    }
+    if (!tables || !lengths || !starts || !prefixes) return invalid("null argument");
     Device d(device);
     if (d.err != cudaSuccess) return launched(d.err, "cudaSetDevice");
     ebx::KvPrefixArgs a{};
@@ -132,8 +122,6 @@ ebx_status ebx_kv_prefixes(const int32_t* tables, int32_t width, int32_t block_s
     a.lengths = lengths;
     a.starts = starts;
     a.out = ebx::prefixes_at(prefixes, requests, tokens);
-    a.scratch = static_cast<int32_t*>(workspace);
-    a.first_with = a.scratch + int64_t(ebx::kKvPrefixScratch) * requests;
     a.tokens = tokens;
     a.requests = requests;
     a.width = width;
@@ -165,7 +153,7 @@ ebx_status ebx_kv_shared_attention(const ebx_kv_pool* pool, const void* q, int64
         return invalid("ebx_kv_shared_attention: dtype must be fp16 or bf16");
     if (heads < 1 || heads % p.kv_heads != 0 || heads > (1 << 20))
         return invalid("ebx_kv_shared_attention: heads must be a multiple of kv_heads");
-    if (requests < 0 || requests > ebx::kKvMaxRequests || width < 1 || int64_t(width) * p.block_size > INT32_MAX / 2 ||
+    if (requests < 0 || requests > ebx::kKvMostPrefixes || width < 1 || int64_t(width) * p.block_size > INT32_MAX / 2 ||
         tokens < 0 || tokens > INT32_MAX || tokens * (heads / p.kv_heads) > INT32_MAX / 2)
         return invalid("ebx_kv_shared_attention: requests, table width or tokens out of range");
     if (!std::isfinite(scale * 1.4426950408889634f)) return invalid("ebx_kv_shared_attention: scale must be finite");

@@ -495,15 +495,4 @@ cudaError_t launch_join(const KvAttnArgs& a, int ctas, int rows, cudaStream_t s)
     return launch_early(kv_join_kernel<D, RT, WAYS, BF16>, dim3(unsigned(ctas), unsigned((rows + 3) / 4)), 32 * WAYS, 0, s, a);
 }
 
-// Reads (and clears) a translation unit's status word; synchronizes `s`.
-inline cudaError_t read_status_word(const int& word, int* status, bool clear, cudaStream_t s) {
-    void* p = nullptr;
-    cudaError_t e = cudaGetSymbolAddress(&p, word);
-    if (e == cudaSuccess) e = cudaMemcpyAsync(status, p, sizeof(int), cudaMemcpyDeviceToHost, s);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-    if (e == cudaSuccess && clear) e = cudaMemsetAsync(p, 0, sizeof(int), s);
-    if (e == cudaSuccess && clear) e = cudaStreamSynchronize(s);
-    return e;
-}
-
 }  // namespace ebx

@@ -18,6 +18,21 @@ namespace ebx {
 namespace {
 
 constexpr int kRotThreads = 256;
+constexpr int kRotCtas = 4;        // CTAs of an SM (4 / 5 / 6: 20000 tokens, below, 72 / 76 / 77 us, 6144 24.6 / 23.9 / 32)
+constexpr int kRotTable = 2048;    // pairs in a CTA's table: 16 KB
+constexpr int kRotMostDim = 2 * kRotTable;
+
+// n / d for n < 2^31: with 2^(k-1) < d <= 2^k and mul = ceil(2^(31+k) / d), mul * d exceeds 2^(31+k) by less than d.
+struct ByConstant {
+    uint32_t mul, shift;
+    void set(uint32_t d) {
+        uint32_t k = 0;
+        while ((uint64_t(1) << k) < d) ++k;
+        shift = 31 + k;
+        mul = uint32_t(((uint64_t(1) << shift) + d - 1) / d);
+    }
+    __device__ __forceinline__ uint32_t of(uint32_t n) const { return uint32_t(uint64_t(n) * mul >> shift); }
+};
 
 struct RotSide {
     const char* in;
@@ -31,9 +46,10 @@ struct RotArgs {
     const void* frequencies;
     int64_t tokens;
     int q_heads, heads;    // queries' heads, and all
-    int turning, chunks;   // chunks of V pairs that turn; these and the chunks of V elements behind them
+    int turning, chunks;   // a head's chunks that turn; these and those that are copied
     int dim, part;
-    int slices;            // threads that share a token's chunk, every slices-th head each
+    int64_t share, span;   // items of a CTA; tokens of a piece of them
+    ByConstant by_chunks, by_heads, by_half;
     int wide_positions, wide_frequencies;
     float scale;
 };
@@ -53,68 +69,108 @@ __device__ __forceinline__ T down(float x) {
     else return __float2bfloat16_rn(x);
 }
 
-// A thread has a chunk of V pairs of one token, whose angles it computes once, and every slices-th head.
+// An item: two vectors of V elements of a head, `second` apart, that have V pairs (in either layout the same vector of
+// both halves, but neighbours for interleaved elements one by one), or one vector that is copied.
+template <class T, int V>
+struct RotItem {
+    Pack<T, V> u, v;
+    T* to;
+    int at;  // its first entry in the table; -1: copied
+};
+
+// The items of all tokens, head by head, lie on one line, of which every CTA takes an equal share, in pieces whose tokens'
+// sines and cosines fit the table.  The next item of a thread is on its way while it turns one, and the first of
+// a piece while the table is filled.
+// What bounds it: reading and writing, 20000 tokens of 40 heads of 128 in fp16 72 us = 5.7 TB/s, 0.87 of a copy's rate; 6144
+// tokens (126 MB) 24.5 us; the smallest calls take a launch, 2 us.  A thread for each item, which computes its own
+// angles, 121 and 42 us: 40 heads use an angle, and a sine costs 40 instructions.  A thread that keeps its angles in registers
+// for every n-th head 68 to 95 and 30 to 54, as its number of waves has it; equal CTAs of 256 items that do not go on 88 to
+// 105 and 24: with a table each and half the bytes on their way.  Interleaved items of one vector 98: half the bytes again.
 template <class T, int V, bool PAIRS>
-__global__ void __launch_bounds__(kRotThreads) rotate_kernel(const __grid_constant__ RotArgs a) {
+__global__ void __launch_bounds__(kRotThreads, kRotCtas) rotate_kernel(const __grid_constant__ RotArgs a) {
     asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
     using P = Pack<T, V>;
-    const int64_t id = int64_t(blockIdx.x) * kRotThreads + threadIdx.x;
-    const int64_t rest = id / a.chunks;
-    const int chunk = int(id - rest * a.chunks);
-    const int64_t token = rest / a.slices;
-    const int slice = int(rest - token * a.slices);
-    if (token >= a.tokens) return;
-    if (chunk >= a.turning) {
-        const int e = a.part + (chunk - a.turning) * V;
-        for (int h = slice; h < a.heads; h += a.slices) {
-            const RotSide& x = h < a.q_heads ? a.q : a.k;
-            const int g = h < a.q_heads ? h : h - a.q_heads;
-            const T* in = reinterpret_cast<const T*>(x.in) + token * x.in_token + g * x.in_head + e;
-            T* out = reinterpret_cast<T*>(x.out) + token * x.out_token + g * x.out_head + e;
-            *reinterpret_cast<P*>(out) = *reinterpret_cast<const P*>(in);
+    constexpr bool SINGLE = PAIRS && V == 1;
+    constexpr int W = V >= 2 ? V / 2 : 1;   // table entries of an item, of two pairs each (one where V = 1)
+    using Entry = typename std::conditional<(V >= 2), float4, float2>::type;
+    using Item = RotItem<T, V>;
+    extern __shared__ __align__(16) uint8_t rot_smem[];
+    Entry* table = reinterpret_cast<Entry*>(rot_smem);  // [token][W][chunk]: neighbouring lanes read neighbours
+    const int64_t per_token = int64_t(a.heads) * a.chunks, total = a.tokens * per_token;
+    int64_t first = blockIdx.x * a.share;
+    const int64_t end = min(first + a.share, total);
+    const int half = a.part / 2, second = SINGLE ? 1 : half;
+    for (; first < end;) {
+        const int64_t t0 = first / per_token;
+        const uint32_t skip = uint32_t(first - t0 * per_token);  // items of its first token ahead of the piece
+        const uint32_t last = uint32_t(min(end - t0 * per_token, a.span * per_token));  // its end, counted from t0
+        auto load = [&](uint32_t item, Item& x) {
+            const uint32_t row = a.by_chunks.of(item), token = a.by_heads.of(row);
+            const int chunk = int(item - row * a.chunks), head = int(row - token * a.heads);
+            const bool q = head < a.q_heads, turns = chunk < a.turning;
+            const RotSide& side = q ? a.q : a.k;
+            const int h = q ? head : head - a.q_heads;
+            const int e0 = !turns ? a.part + (chunk - a.turning) * V : SINGLE ? 2 * chunk : chunk * V;
+            const T* in = reinterpret_cast<const T*>(side.in) + (t0 + token) * side.in_token + h * side.in_head + e0;
+            x.to = reinterpret_cast<T*>(side.out) + (t0 + token) * side.out_token + h * side.out_head + e0;
+            x.at = turns ? int(token) * W * a.turning + chunk : -1;
+            x.u = *reinterpret_cast<const P*>(in);
+            if (turns) x.v = *reinterpret_cast<const P*>(in + second);
+        };
+        Item x;
+        uint32_t item = skip + threadIdx.x;
+        if (item < last) load(item, x);
+        const uint32_t entries = (a.by_heads.of(a.by_chunks.of(last - 1)) + 1) * half;
+        for (uint32_t e = threadIdx.x; e < entries; e += kRotThreads) {
+            const uint32_t token = a.by_half.of(e);
+            const int pair = int(e - token * half);
+            // its item, and its place there: the first half of an item's interleaved pairs are the first vector's
+            const int back = PAIRS && V > 1 && pair >= half / 2, of = back ? pair - half / 2 : pair;
+            constexpr int N = PAIRS && V > 1 ? V / 2 : V;
+            const int chunk = of / N, i = of % N + (back ? N : 0);
+            const double p = a.wide_positions ? double(static_cast<const int64_t*>(a.positions)[t0 + token])
+                                              : double(static_cast<const int32_t*>(a.positions)[t0 + token]);
+            const double f = a.wide_frequencies ? static_cast<const double*>(a.frequencies)[pair]
+                                                : double(static_cast<const float*>(a.frequencies)[pair]);
+            const double turn = p * f * 0.15915494309189533577;  // 1 / (2 pi)
+            // half turns as 32 bits and what they leave: sin(pi (h + r)) = sin(pi h) + pi r cos(pi h) to 2^-48
+            const double half_turns = 2.0 * (turn - rint(turn));
+            const float h = float(half_turns), r = 3.14159265f * float(half_turns - double(h));
+            float sine, cosine;
+            sincospif(h, &sine, &cosine);
+            const float along = fmaf(-r, sine, cosine);
+            sine = fmaf(r, cosine, sine);
+            cosine = along;
+            float2* entry = reinterpret_cast<float2*>(table + (token * W + i / (V / W)) * a.turning + chunk);
+            entry[i % (V / W)] = make_float2(cosine * a.scale, sine * a.scale);
         }
-        return;
-    }
-    float c[V], s[V];
-    {
-        const double p = a.wide_positions ? double(static_cast<const int64_t*>(a.positions)[token])
-                                          : double(static_cast<const int32_t*>(a.positions)[token]);
+        __syncthreads();
+        while (item < last) {
+            Item y = x;
+            item += kRotThreads;
+            if (item < last) load(item, x);
+            if (y.at >= 0) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int at = chunk * V + i;
-            const double f = a.wide_frequencies ? static_cast<const double*>(a.frequencies)[at]
-                                                : double(static_cast<const float*>(a.frequencies)[at]);
-            const double turns = p * f * 0.15915494309189533577;  // 1 / (2 pi)
-            sincospif(float(2.0 * (turns - rint(turns))), &s[i], &c[i]);
-            s[i] *= a.scale;
-            c[i] *= a.scale;
-        }
-    }
-    const int e0 = PAIRS ? 2 * chunk * V : chunk * V, e1 = PAIRS ? e0 + V : e0 + a.part / 2;
-    for (int h = slice; h < a.heads; h += a.slices) {
-        const RotSide& x = h < a.q_heads ? a.q : a.k;
-        const int g = h < a.q_heads ? h : h - a.q_heads;
-        const T* in = reinterpret_cast<const T*>(x.in) + token * x.in_token + g * x.in_head;
-        T* out = reinterpret_cast<T*>(x.out) + token * x.out_token + g * x.out_head;
-        P u = *reinterpret_cast<const P*>(in + e0), v = *reinterpret_cast<const P*>(in + e1);
-        P y, z;
+                for (int w = 0; w < W; ++w) {
+                    const Entry e = table[y.at + w * a.turning];
+                    const float2* turn = reinterpret_cast<const float2*>(&e);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            // element j of u, v together: a pair is (j, j + 1) or one of each
-            T& ta = PAIRS ? (2 * i < V ? u.v[2 * i % V] : v.v[2 * i % V]) : u.v[i];
-            T& tb = PAIRS ? (2 * i + 1 < V ? u.v[(2 * i + 1) % V] : v.v[(2 * i + 1) % V]) : v.v[i];
-            const float fa = up(ta), fb = up(tb);
-            const T na = down<T>(fa * c[i] - fb * s[i]), nb = down<T>(fb * c[i] + fa * s[i]);
-            if constexpr (PAIRS) {
-                (2 * i < V ? y.v[2 * i % V] : z.v[2 * i % V]) = na;
-                (2 * i + 1 < V ? y.v[(2 * i + 1) % V] : z.v[(2 * i + 1) % V]) = nb;
-            } else {
-                y.v[i] = na;
-                z.v[i] = nb;
+                    for (int k = 0; k < V / W; ++k) {
+                        const int i = w * (V / W) + k;
+                        const float c = turn[k].x, s = turn[k].y;
+                        T& one = !PAIRS || SINGLE ? y.u.v[i] : (2 * i < V ? y.u : y.v).v[2 * i % V];
+                        T& other = !PAIRS || SINGLE ? y.v.v[i] : (2 * i < V ? y.u : y.v).v[(2 * i + 1) % V];
+                        const float fa = up(one), fb = up(other);
+                        one = down<T>(fa * c - fb * s);
+                        other = down<T>(fb * c + fa * s);
+                    }
+                }
+                *reinterpret_cast<P*>(y.to + second) = y.v;
             }
+            *reinterpret_cast<P*>(y.to) = y.u;
         }
-        *reinterpret_cast<P*>(out + e0) = y;
-        *reinterpret_cast<P*>(out + e1) = z;
+        first = t0 * per_token + last;
+        if (first < end) __syncthreads();  // the table is free again
     }
 }
 
@@ -131,25 +187,34 @@ int vector_of(const RotArgs& a, int size) {
 }
 
 template <class T, int V>
-cudaError_t launch(RotArgs a, bool pairs, bool in_place, cudaStream_t s) {
+cudaError_t launch(RotArgs a, bool pairs, bool in_place, int sms, cudaStream_t s) {
     a.turning = a.part / 2 / V;
     a.chunks = a.turning + (in_place ? 0 : (a.dim - a.part) / V);  // in place the part behind stays as it is
-    a.slices = a.heads;
-    const int64_t grid = (a.tokens * a.slices * a.chunks + kRotThreads - 1) / kRotThreads;
-    if (grid > INT32_MAX) return cudaErrorInvalidValue;
-    return pairs ? launch_early(rotate_kernel<T, V, true>, dim3(unsigned(grid)), kRotThreads, 0, s, a)
-                 : launch_early(rotate_kernel<T, V, false>, dim3(unsigned(grid)), kRotThreads, 0, s, a);
+    const int64_t per_token = int64_t(a.heads) * a.chunks, total = a.tokens * per_token;
+    a.by_chunks.set(a.chunks);
+    a.by_heads.set(a.heads);
+    a.by_half.set(uint32_t(a.part / 2));
+    // as many CTAs as run at once, with whole rounds of their threads
+    const int64_t most = int64_t(sms) * kRotCtas, rounds = (total + most * kRotThreads - 1) / (most * kRotThreads);
+    a.share = rounds * kRotThreads;
+    const dim3 grid{unsigned((total + a.share - 1) / a.share)};
+    // tokens of a piece: what the table holds and 31 bits count, and no more than a share may touch
+    a.span = std::min<int64_t>(std::max(kRotTable / (a.part / 2), 1), std::max<int64_t>(INT32_MAX / per_token - 1, 1));
+    a.span = std::min(a.span, a.share / per_token + 2);
+    const size_t smem = size_t(a.span) * (a.part / 2) * sizeof(float2);
+    return pairs ? launch_early(rotate_kernel<T, V, true>, grid, kRotThreads, smem, s, a)
+                 : launch_early(rotate_kernel<T, V, false>, grid, kRotThreads, smem, s, a);
 }
 
 template <class T>
-cudaError_t launch_type(const RotArgs& a, bool pairs, bool in_place, cudaStream_t s) {
+cudaError_t launch_type(const RotArgs& a, bool pairs, bool in_place, int sms, cudaStream_t s) {
     switch (vector_of(a, int(sizeof(T)))) {
         case 8:
-            if constexpr (sizeof(T) == 2) return launch<T, 8>(a, pairs, in_place, s);
+            if constexpr (sizeof(T) == 2) return launch<T, 8>(a, pairs, in_place, sms, s);
             return cudaErrorInvalidValue;
-        case 4: return launch<T, 4>(a, pairs, in_place, s);
-        case 2: return launch<T, 2>(a, pairs, in_place, s);
-        default: return launch<T, 1>(a, pairs, in_place, s);
+        case 4: return launch<T, 4>(a, pairs, in_place, sms, s);
+        case 2: return launch<T, 2>(a, pairs, in_place, sms, s);
+        default: return launch<T, 1>(a, pairs, in_place, sms, s);
     }
 }
 
@@ -160,7 +225,7 @@ RotSide side_of(const ebx_rotary_side& x) {
 
 // Null, or what is wrong with a side of elements of `size` bytes.
 const char* wrong(const ebx_rotary_side& x, int size, int64_t tokens) {
-    if (x.heads < 0 || x.heads > (1 << 20)) return "ebx_rotate: need 0 <= heads <= 2^20";
+    if (x.heads < 0 || x.heads > (1 << 16)) return "ebx_rotate: need 0 <= heads <= 65536";
     if (x.heads == 0 || tokens == 0) return nullptr;
     if (!x.in || !x.out) return "null argument";
     if (reinterpret_cast<uintptr_t>(x.in) % size || reinterpret_cast<uintptr_t>(x.out) % size)
@@ -177,8 +242,8 @@ extern "C" ebx_status ebx_rotate(const ebx_rotary_side* q, const ebx_rotary_side
                                  int64_t tokens, int32_t interleaved, float scale, int32_t device, void* stream) {
     if (!q) return invalid("null argument");
     if (dtype < ebx::kKvF32 || dtype > ebx::kKvBF16) return invalid("ebx_rotate: dtype must be fp32, fp16 or bf16");
-    if (head_dim < 2 || head_dim > (1 << 20) || rotary_dim < 2 || rotary_dim % 2 != 0 || rotary_dim > head_dim)
-        return invalid("ebx_rotate: need an even rotary_dim, 2 <= rotary_dim <= head_dim <= 2^20");
+    if (head_dim < 2 || head_dim > ebx::kRotMostDim || rotary_dim < 2 || rotary_dim % 2 != 0 || rotary_dim > head_dim)
+        return invalid("ebx_rotate: need an even rotary_dim, 2 <= rotary_dim <= head_dim <= 4096");
     if (position_bits != 32 && position_bits != 64) return invalid("ebx_rotate: positions have 32 or 64 bits");
     if (frequency_bits != 32 && frequency_bits != 64) return invalid("ebx_rotate: frequencies have 32 or 64 bits");
     if (!std::isfinite(scale)) return invalid("ebx_rotate: scale must be finite");
@@ -189,7 +254,7 @@ extern "C" ebx_status ebx_rotate(const ebx_rotary_side* q, const ebx_rotary_side
         if (const char* msg = ebx::wrong(*k, size, tokens)) return invalid(msg);
     ebx::RotArgs a{};
     a.q_heads = q->heads;
-    a.heads = q->heads + (k ? k->heads : 0);
+    a.heads = q->heads + (k ? k->heads : 0);  // at most 2^17 heads of 2^12 chunks: below 2^31 items a token
     if (tokens == 0 || a.heads == 0) return EBX_OK;
     if (!positions || !frequencies) return invalid("null argument");
     a.q = q->heads ? ebx::side_of(*q) : ebx::RotSide{};
@@ -209,7 +274,8 @@ extern "C" ebx_status ebx_rotate(const ebx_rotary_side* q, const ebx_rotary_side
     if (d.err != cudaSuccess) return launched(d.err, "cudaSetDevice");
     const bool in_place = stays(a.q) && stays(a.k), pairs = interleaved != 0;
     const auto s = static_cast<cudaStream_t>(stream);
-    return launched(dtype == ebx::kKvF32 ? ebx::launch_type<float>(a, pairs, in_place, s)
-                    : dtype == ebx::kKvF16 ? ebx::launch_type<__half>(a, pairs, in_place, s)
-                                           : ebx::launch_type<__nv_bfloat16>(a, pairs, in_place, s), "ebx_rotate");
+    const int sms = ebx::gemm_sm_count(device);
+    return launched(dtype == ebx::kKvF32 ? ebx::launch_type<float>(a, pairs, in_place, sms, s)
+                    : dtype == ebx::kKvF16 ? ebx::launch_type<__half>(a, pairs, in_place, sms, s)
+                                           : ebx::launch_type<__nv_bfloat16>(a, pairs, in_place, sms, s), "ebx_rotate");
 }

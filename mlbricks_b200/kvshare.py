@@ -26,6 +26,9 @@ from . import _ebx
 from .kvcache import _ROW_DTYPES, BLOCK_SIZES, KVCache, KVPlan, KVPool, _int_ok, _refuse_ints, _stream
 
 
+MOST_REQUESTS = 8192  # of a step whose prefixes are looked for
+
+
 class KVMoves(NamedTuple):
     """Blocks to copy (on the GPU)."""
 
@@ -54,20 +57,19 @@ class KVCompact(NamedTuple):
     moves: KVMoves
 
 
-def _state(lengths: torch.Tensor, tables: torch.Tensor, shares: torch.Tensor, block_size: int, **more) -> int:
-    """Checks what fork and compact have in common; the device."""
-    device = lengths.get_device()
+def _state(lengths, tables, shares, block_size, device) -> None:
+    """What fork and compact have in common."""
+    int32 = torch.int32
     if device < 0:
         raise ValueError("lengths must be a CUDA tensor")
-    int32 = torch.int32
-    _refuse_ints(device, lengths=(lengths, int32), tables=(tables, int32), shares=(shares, int32), **more)
+    if not (_int_ok(lengths, int32, device) and _int_ok(tables, int32, device) and _int_ok(shares, int32, device)):
+        _refuse_ints(device, lengths=(lengths, int32), tables=(tables, int32), shares=(shares, int32))
     if tables.dim() != 2 or lengths.numel() != tables.shape[0] or tables.shape[1] < 1:
         raise ValueError("tables must have a row for each of lengths, and a column")
     if block_size not in BLOCK_SIZES:
         raise ValueError(f"block_size must be one of {BLOCK_SIZES}, got {block_size}")
     if shares.numel() < 1:
         raise ValueError("shares must have an entry for each block")
-    return device
 
 
 def fork(lengths: torch.Tensor, tables: torch.Tensor, shares: torch.Tensor, free: torch.Tensor, ring: torch.Tensor,
@@ -84,39 +86,47 @@ def fork(lengths: torch.Tensor, tables: torch.Tensor, shares: torch.Tensor, free
     later calls.
 
     ``lengths``, ``tables``, ``shares`` and ``ring`` are not changed: the result's take their place."""
-    int32 = torch.int32
-    device = _state(lengths, tables, shares, block_size, free=(free, int32), ring=(ring, torch.int64),
-                    parents=(parents, int32), keep=(keep, int32))
+    int32, device = torch.int32, lengths.get_device()
+    _state(lengths, tables, shares, block_size, device)
+    if not (_int_ok(free, int32, device) and _int_ok(ring, torch.int64, device) and _int_ok(parents, int32, device)
+            and (keep is None or _int_ok(keep, int32, device))):
+        _refuse_ints(device, free=(free, int32), ring=(ring, torch.int64), parents=(parents, int32), keep=(keep, int32))
     requests, width = tables.shape
     if parents.numel() != requests or (keep is not None and keep.numel() != requests):
         raise ValueError("parents and keep must have one entry for each request")
     if ring.numel() < 2 or free.numel() < 1:
         raise ValueError("ring holds at least its front and back, and free at least one place")
     blocks = shares.numel()
-    out_lengths, out_tables, out_shares = lengths.new_empty(requests), tables.new_empty((requests, width)), shares.new_empty(blocks)
-    out_ring, moves, work = ring.new_empty(4), lengths.new_empty((2, requests)), shares.new_empty(blocks)
-    _ebx.check(_ebx.load().ebx_kv_fork(
+    out_lengths, sources, targets = lengths.new_empty((3, requests)).unbind()
+    out_tables, out_shares, out_ring = tables.new_empty((requests, width)), shares.new_empty(blocks), ring.new_empty(4)
+    st = _ebx.load().ebx_kv_fork(
         lengths.data_ptr(), tables.data_ptr(), width, block_size, shares.data_ptr(), blocks, free.data_ptr(), free.numel(),
         ring.data_ptr(), parents.data_ptr(), None if keep is None else keep.data_ptr(), requests, out_lengths.data_ptr(),
-        out_tables.data_ptr(), out_shares.data_ptr(), out_ring.data_ptr(), moves[0].data_ptr(), moves[1].data_ptr(),
-        work.data_ptr(), 4 * blocks, device, _stream(device)))
-    return KVFork(out_lengths, out_tables, out_shares, out_ring, KVMoves(moves[0], moves[1], out_ring[3:]))
+        out_tables.data_ptr(), out_shares.data_ptr(), out_ring.data_ptr(), sources.data_ptr(), targets.data_ptr(), device,
+        _stream(device))
+    if st:
+        _ebx.check(st)
+    return KVFork(out_lengths, out_tables, out_shares, out_ring, KVMoves(sources, targets, out_ring[3:]))
 
 
 def compact(lengths: torch.Tensor, tables: torch.Tensor, shares: torch.Tensor, *, block_size: int) -> KVCompact:
     """New numbers for the blocks that rows hold, so that they are the pool's first ones, with the fewest copies
     (the result's ``moves``, for ``copy``).  All others are free afterwards, and in the result's ring by rising number.
     The inputs are not changed: the result's tensors take their place."""
-    device = _state(lengths, tables, shares, block_size)
+    device = lengths.get_device()
+    _state(lengths, tables, shares, block_size, device)
     requests, width = tables.shape
     blocks = shares.numel()
-    out_tables, out_shares, free = tables.new_empty((requests, width)), shares.new_empty(blocks), shares.new_empty(blocks)
-    ring, moves, work = lengths.new_empty(4, dtype=torch.int64), lengths.new_empty((2, blocks // 2)), shares.new_empty(blocks)
-    _ebx.check(_ebx.load().ebx_kv_compact(
+    out_tables, ring = tables.new_empty((requests, width)), lengths.new_empty(4, dtype=torch.int64)
+    out_shares, free, work = shares.new_empty((3, blocks)).unbind()
+    sources, targets = shares.new_empty((2, blocks // 2)).unbind()
+    st = _ebx.load().ebx_kv_compact(
         lengths.data_ptr(), tables.data_ptr(), width, block_size, shares.data_ptr(), blocks, requests, out_tables.data_ptr(),
-        out_shares.data_ptr(), free.data_ptr(), ring.data_ptr(), moves[0].data_ptr(), moves[1].data_ptr(), work.data_ptr(),
-        4 * blocks, device, _stream(device)))
-    return KVCompact(out_tables, out_shares, free, ring, KVMoves(moves[0], moves[1], ring[3:]))
+        out_shares.data_ptr(), free.data_ptr(), ring.data_ptr(), sources.data_ptr(), targets.data_ptr(), work.data_ptr(),
+        4 * blocks, device, _stream(device))
+    if st:
+        _ebx.check(st)
+    return KVCompact(out_tables, out_shares, free, ring, KVMoves(sources, targets, ring[3:]))
 
 
 def copy(pools: Sequence[KVPool], moves: KVMoves) -> None:
@@ -126,12 +136,16 @@ def copy(pools: Sequence[KVPool], moves: KVMoves) -> None:
         return
     device = pools[0].device
     sources, targets, count = moves
-    _refuse_ints(device, sources=(sources, torch.int32), targets=(targets, torch.int32), count=(count, torch.int64))
+    if not (_int_ok(sources, torch.int32, device) and _int_ok(targets, torch.int32, device)
+            and (count is None or _int_ok(count, torch.int64, device))):
+        _refuse_ints(device, sources=(sources, torch.int32), targets=(targets, torch.int32), count=(count, torch.int64))
     if sources.numel() != targets.numel() or (count is not None and count.numel() < 1):
         raise ValueError("sources and targets must be as many, and count one number")
-    array = (_ebx.KVPool * len(pools))(*(p._c for p in pools))
-    _ebx.check(_ebx.load().ebx_kv_copy(array, len(pools), sources.data_ptr(), targets.data_ptr(),
-                                       None if count is None else count.data_ptr(), sources.numel(), _stream(device)))
+    array = (_ebx.KVPool * len(pools))(*[p._c for p in pools])
+    st = _ebx.load().ebx_kv_copy(array, len(pools), sources.data_ptr(), targets.data_ptr(),
+                                 None if count is None else count.data_ptr(), sources.numel(), _stream(device))
+    if st:
+        _ebx.check(st)
 
 
 class KVPrefixes:
@@ -150,7 +164,7 @@ def prefixes(tables: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor, 
     ``lengths`` and ``starts`` are the step's, as for ``kvcache.attention``; ``blocks`` is the pool's.  Requests that
     bring tokens and whose rows of ``tables`` begin with the same block form a group, which shares as many full blocks ahead
     of the new tokens as save most reading; rows with fewer in common are taken alone.  The result holds for this
-    step."""
+    step.  At most 8192 requests."""
     int32, device, requests = torch.int32, tables.get_device(), lengths.numel()
     if device < 0:
         raise ValueError("tables must be a CUDA tensor")
@@ -159,10 +173,10 @@ def prefixes(tables: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor, 
     if starts.numel() != requests + 1 or tables.dim() != 2 or tables.shape[0] != requests or tokens < 0:
         raise ValueError("lengths and the rows of tables must be as many, and starts one more; tokens >= 0")
     data = starts.new_empty(3 * requests + 1 + 2 * tokens)
-    work = starts.new_empty(6 * requests + blocks) if blocks > 0 else data
-    _ebx.check(_ebx.load().ebx_kv_prefixes(
-        tables.data_ptr(), tables.shape[1], block_size, blocks, lengths.data_ptr(), starts.data_ptr(), requests, tokens,
-        data.data_ptr(), work.data_ptr(), 4 * work.numel(), device, _stream(device)))
+    st = _ebx.load().ebx_kv_prefixes(tables.data_ptr(), tables.shape[1], block_size, blocks, lengths.data_ptr(), starts.data_ptr(),
+                                     requests, tokens, data.data_ptr(), device, _stream(device))
+    if st:
+        _ebx.check(st)
     return KVPrefixes(data, requests, tokens)
 
 
@@ -203,11 +217,13 @@ def attention(q: torch.Tensor, pool: KVPool, tables: torch.Tensor, lengths: torc
     if tokens and requests:
         nbytes = _workspace_bytes(device, pool._c.kv_heads, dim, heads, tokens, max_new, max_length)
         ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-        _ebx.check(_ebx.load().ebx_kv_shared_attention(
+        st = _ebx.load().ebx_kv_shared_attention(
             pool._ref, q.data_ptr(), q.stride(0), q.stride(1), heads, _ROW_DTYPES[q.dtype], tables.data_ptr(),
             tables.shape[1], lengths.data_ptr(), starts.data_ptr(), shared.data.data_ptr(), requests, tokens, causal,
             1.0 / math.sqrt(dim) if scale is None else scale, max_new, max_length, out.data_ptr(),
-            None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, _stream(device)))
+            None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, _stream(device))
+        if st:
+            _ebx.check(st)
     return out if lse is None else (out, lse)
 
 
@@ -272,7 +288,7 @@ class SharedKVCache(KVCache):
     def attention(self, layer: int, q: torch.Tensor, **options):
         """The step's queries over the layer's cache, what requests share once; with ``window`` or ``first``, which
         prefixes do not allow, as ``KVCache.attention``."""
-        if options.get("window") or options.get("first") is not None:
+        if options.get("window") or options.get("first") is not None or self.lengths.numel() > MOST_REQUESTS:
             return super().attention(layer, q, **options)
         options.pop("window", None), options.pop("first", None)
         step = self._planned()

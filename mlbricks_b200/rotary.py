@@ -66,54 +66,58 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
     [rotary_dim / 2] (float64 or float32).  Pair i is elements (i, rotary_dim / 2 + i) of a head, or (2 i, 2 i + 1) if
     ``interleaved``; elements from rotary_dim on stay as they are.  ``scale`` multiplies what was turned.
 
-    Returns (q, k) as new contiguous tensors, or, ``inplace``, the same tensors turned where they are (their
+    Returns (q, k) as new tensors, or, ``inplace``, the same tensors turned where they are (their
     last dimension is then contiguous, and they share no elements).  ``k`` may be None."""
-    dtype, device, tokens = q.dtype, q.get_device(), q.shape[0] if q.dim() == 3 else -1
+    dtype, device, shape = q.dtype, q.get_device(), q.shape
     if device < 0:
         raise ValueError("rotate needs CUDA tensors")
     if dtype not in _DTYPES:
         raise ValueError("q must be float32, float16 or bfloat16")
-    if tokens < 0 or (k is not None and (k.dim() != 3 or k.shape[0] != tokens or k.shape[2] != q.shape[2])):
+    if len(shape) != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != shape[0] or k.shape[2] != shape[2])):
         raise ValueError("q and k must be [tokens, heads, head_dim] with the same tokens and head_dim")
     if k is not None and (k.dtype is not dtype or k.get_device() != device):
         raise ValueError("q and k must have the same dtype and device")
-    dim = q.shape[2]
-    if (positions.dtype not in (torch.int32, torch.int64) or positions.get_device() != device
-            or positions.dim() != 1 or positions.shape[0] != tokens or not positions.is_contiguous()):
+    tokens, heads, dim = shape
+    wide = positions.dtype is torch.int64
+    if not ((wide or positions.dtype is torch.int32) and positions.get_device() == device and positions.shape == (tokens,)
+            and positions.is_contiguous()):
         raise ValueError(f"positions must be a contiguous int32 or int64 tensor [{tokens}] on cuda:{device}")
-    if (frequencies.dtype not in (torch.float32, torch.float64) or frequencies.get_device() != device
-            or frequencies.dim() != 1 or not frequencies.is_contiguous()):
+    double = frequencies.dtype is torch.float64
+    if not ((double or frequencies.dtype is torch.float32) and frequencies.get_device() == device and frequencies.dim() == 1
+            and frequencies.is_contiguous()):
         raise ValueError(f"frequencies must be a contiguous float64 or float32 tensor on cuda:{device}")
     part = 2 * frequencies.shape[0]
     if not 2 <= part <= dim:
         raise ValueError(f"frequencies must be 1 to {dim // 2}, half of the elements that turn, got {part // 2}")
-    if inplace and k is not None and q.data_ptr() == k.data_ptr() and q.numel() and k.numel():
-        raise ValueError("q and k must not be the same memory")
-    sides, out, copies = [], [], []
-    for x in (q, k):
-        if x is None:
-            sides.append(None)
-            out.append(None)
-            continue
-        if inplace:
-            if (dim > 1 and x.stride(2) != 1) or not _apart(x):
+    if inplace:
+        for x in (q, k):
+            if x is not None and (x.stride(2) != 1 or not _apart(x)):
                 raise ValueError("a tensor that is turned in place has a contiguous last dimension and no element twice")
-            y = x
-        else:
-            if x.stride(2) != 1:
-                x = x.contiguous()
-                copies.append(x)  # until the launch, or its memory may become an output's
-            y = torch.empty(x.shape, dtype=dtype, device=x.device)
-        sides.append(_ebx.RotarySide(x.data_ptr(), y.data_ptr(), x.stride(0), x.stride(1), y.stride(0), y.stride(1),
-                                     x.shape[1], 0))
-        out.append(y)
+        if k is not None and q.data_ptr() == k.data_ptr() and q.numel() and k.numel():
+            raise ValueError("q and k must not be the same memory")
+        a, b = q, k
+    else:  # whatever is copied first lives until the launch: its memory must not become an output's
+        if q.stride(2) != 1:
+            q = q.contiguous()
+        a, b = torch.empty_like(q), None
+        if k is not None:
+            if k.stride(2) != 1:
+                k = k.contiguous()
+            b = torch.empty_like(k)
+    i0, i1, _ = q.stride()
+    o0, o1, _ = a.stride()
+    side = _ebx.RotarySide(q.data_ptr(), a.data_ptr(), i0, i1, o0, o1, heads, 0)
+    other = None
+    if k is not None:
+        i0, i1, _ = k.stride()
+        o0, o1, _ = b.stride()
+        other = ctypes.byref(_ebx.RotarySide(k.data_ptr(), b.data_ptr(), i0, i1, o0, o1, k.shape[1], 0))
     st = _ebx.load().ebx_rotate(
-        ctypes.byref(sides[0]), None if k is None else ctypes.byref(sides[1]), dim, part, _DTYPES[dtype],
-        positions.data_ptr(), 64 if positions.dtype is torch.int64 else 32, frequencies.data_ptr(),
-        64 if frequencies.dtype is torch.float64 else 32, tokens, interleaved, scale, device, _stream(device))
+        ctypes.byref(side), other, dim, part, _DTYPES[dtype], positions.data_ptr(), 64 if wide else 32,
+        frequencies.data_ptr(), 64 if double else 32, tokens, interleaved, scale, device, _stream(device))
     if st:
         _ebx.check(st)
-    return out[0], out[1]
+    return a, b
 
 
 __all__ = ["SCALINGS", "frequencies", "rotate"]

@@ -25,12 +25,11 @@ def test_argument_errors_without_gpu():
         assert words in _ebx.last_error()
 
     def fork(lengths=4, tables=4, width=1, block=16, shares=8, blocks=1, ring_size=1, requests=1, out_lengths=8, out_tables=8,
-             out_shares=4, ring=8, ring_out=16, work=4, work_bytes=4):
+             out_shares=4, ring=8, ring_out=16):
         return lib.ebx_kv_fork(lengths, tables, width, block, shares, blocks, 4, ring_size, ring, 4, None, requests, out_lengths,
-                               out_tables, out_shares, ring_out, 4, 4, work, work_bytes, 0, None)
+                               out_tables, out_shares, ring_out, 4, 4, 0, None)
 
     refused(fork(lengths=None), "null")
-    refused(fork(work=None), "null")
     refused(fork(requests=16385), "16384")
     refused(fork(block=17), "block_size")
     refused(fork(width=2**27), "2^31")
@@ -41,7 +40,6 @@ def test_argument_errors_without_gpu():
     refused(fork(out_tables=4), "inputs")
     refused(fork(out_shares=8), "inputs")
     refused(fork(ring_out=8), "inputs")
-    refused(fork(blocks=2), "workspace", _ebx.EBX_ERR_WORKSPACE)
 
     def compact(width=1, blocks=1, out_tables=8, out_shares=4, work_bytes=8, sources=4):
         return lib.ebx_kv_compact(4, 4, width, 16, 8, blocks, 1, out_tables, out_shares, 4, 8, sources, sources, 4, work_bytes, 0, None)
@@ -78,18 +76,16 @@ def test_prefix_errors_without_gpu():
         assert status == code
         assert words in _ebx.last_error()
 
-    def prefixes(tables=4, width=1, block=16, blocks=1, requests=1, tokens=1, out=4, work=16, work_bytes=28):
-        return lib.ebx_kv_prefixes(tables, width, block, blocks, 4, 4, requests, tokens, out, work, work_bytes, 0, None)
+    def prefixes(tables=4, width=1, block=16, blocks=1, requests=1, tokens=1, out=4):
+        return lib.ebx_kv_prefixes(tables, width, block, blocks, 4, 4, requests, tokens, out, 0, None)
 
     refused(prefixes(tables=None), "null")
     refused(prefixes(out=None), "null")
     refused(prefixes(width=0), "width")
     refused(prefixes(block=1), "block_size")
     refused(prefixes(blocks=0), "blocks")
-    refused(prefixes(requests=16385), "16384")
+    refused(prefixes(requests=8193), "8192")
     refused(prefixes(tokens=2**31), "tokens")
-    refused(prefixes(work=8), "aligned")
-    refused(prefixes(work_bytes=27), "workspace", _ebx.EBX_ERR_WORKSPACE)
     assert prefixes(requests=0, tables=None) == _ebx.EBX_OK
     assert lib.ebx_kv_prefixes_ints(3, 5) == 20 and lib.ebx_kv_prefixes_ints(-1, 5) == 0
 
@@ -110,7 +106,7 @@ def test_prefix_errors_without_gpu():
     refused(attention(pool(), q=8), "aligned")
     refused(attention(pool(), stride=12), "multiples of 8")
     refused(attention(pool(), width=2**27), "out of range")
-    refused(attention(pool(), requests=16385), "out of range")
+    refused(attention(pool(), requests=8193), "out of range")
     refused(attention(pool(), shared=None), "null")
     refused(attention(pool(), max_new=-1), ">= 0")
     assert attention(pool(), tokens=0) == _ebx.EBX_OK

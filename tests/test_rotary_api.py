@@ -77,6 +77,8 @@ def test_argument_errors_without_gpu():
     refused(call(part=63), "even")
     refused(call(part=66), "even")
     refused(call(part=0), "even")
+    refused(call(dim=4098), "4096")
+    refused(call(q=side(heads=65537)), "65536")
     refused(call(dtype=3), "dtype")
     refused(call(position_bits=16), "positions")
     refused(call(frequency_bits=16), "frequencies")
