@@ -735,6 +735,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 // and end alone (2 / 4 / 8 / 16 units, 32 heads over 8 of 128, captured: a prompt of 200 tokens 29 / 32 / 42 / 59 us,
 // of 700 35 / 35 / 44 / 64, of 1500 60 / 60 / 60 / 66, three of 2048 184 with any).
 constexpr int kPromptLeast = 8;
+constexpr int kSharedLeast = 2;
 
 // SHARED: `ws` holds the parts, and the caller joins.
 template <int D, bool BF16, bool SHARED = false>
@@ -755,7 +756,7 @@ cudaError_t launch_prompt(KvAttnArgs a, void* ws, int dev, cudaStream_t s) {
     const int grid = gemm_sm_count(dev);
     a.desc = static_cast<int4*>(ws);
     a.part = reinterpret_cast<float*>(SHARED ? a.desc : a.desc + grid);
-    const cudaError_t e = launch_early(kern, dim3(grid), kPromptThreads, C::kSmem, s, mk, mv, a, kPromptLeast);
+    const cudaError_t e = launch_early(kern, dim3(grid), kPromptThreads, C::kSmem, s, mk, mv, a, SHARED ? kSharedLeast : kPromptLeast);
     if (e != cudaSuccess || SHARED) return e;
     return launch_join<D, kPromptRows, 4, BF16>(a, grid, kPromptRows, s);
 }

@@ -323,9 +323,9 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kShareThreads
 // ---- copy ---------------------------------------------------------------------------------
 
 constexpr int kCopyThreads = 128;     // a warp for the codes, the others for scales
-constexpr int kCopySegment = 16384;   // bytes of a unit
-constexpr int kCopyStages = 4;
-constexpr int kCopyCtas = 3;          // of an SM
+constexpr int kCopySegment = 4096;    // bytes of a unit
+constexpr int kCopyStages = 8;
+constexpr int kCopyCtas = 6;          // of an SM
 
 __device__ int g_kv_copy_status = 0;
 
