@@ -484,10 +484,14 @@ EBX_API ebx_status ebx_kv_prefixes(const int32_t* tables, int32_t width, int32_t
  * but a group's shared keys and values are read once for the rows of all its members, and
  * the results over the prefix and over the rest joined in fp32.  Where a request brings many rows
  * of its own (max_new, or without it `tokens`, times heads / kv_heads, 49 and more), requests go
- * by themselves, as in ebx_kv_attention.  requests <= 8192.  `prefixes` of another step, or of other tables,
- * make the result meaningless, but nothing outside the buffers is touched. */
+ * by themselves, as in ebx_kv_attention, and so they do where requests and max_length are so few
+ * (if max_length is given) that sharing could not pay: ebx_kv_takes_prefixes tells (1: prefixes are used,
+ * 0: not, and ebx_kv_prefixes need not be called).  requests <= 8192.  `prefixes` of another step, or of other
+ * tables, make the result meaningless, but nothing outside the buffers is touched. */
+EBX_API int32_t ebx_kv_takes_prefixes(const ebx_kv_pool* pool, int32_t heads, int32_t requests, int64_t tokens,
+                                      int32_t max_new, int32_t max_length);
 EBX_API uint64_t ebx_kv_shared_attention_workspace_bytes(const ebx_kv_pool* pool, int32_t heads,
-                                                         int64_t tokens, int32_t max_new,
+                                                         int32_t requests, int64_t tokens, int32_t max_new,
                                                          int32_t max_length);
 EBX_API ebx_status ebx_kv_shared_attention(const ebx_kv_pool* pool, const void* q,
                                            int64_t q_token_stride, int64_t q_head_stride, int32_t heads,

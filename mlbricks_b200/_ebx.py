@@ -129,7 +129,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ebx_kv_copy": (_ST, [_KV, _I32, _P, _P, _P, _I32, _P]),
     "ebx_kv_prefixes_ints": (_U64, [_I32, _I64]),
     "ebx_kv_prefixes": (_ST, [_P, _I32, _I32, _I32, _P, _P, _I32, _I64, _P, _I32, _P]),
-    "ebx_kv_shared_attention_workspace_bytes": (_U64, [_KV, _I32, _I64, _I32, _I32]),
+    "ebx_kv_takes_prefixes": (_I32, [_KV, _I32, _I32, _I64, _I32, _I32]),
+    "ebx_kv_shared_attention_workspace_bytes": (_U64, [_KV, _I32, _I32, _I64, _I32, _I32]),
     "ebx_kv_shared_attention": (
         _ST, [_KV, _P, _I64, _I64, _I32, _I32, _P, _I32, _P, _P, _P, _I32, _I64, _I32, ctypes.c_float, _I32, _I32, _P,
               _P, _P, _U64, _P]),

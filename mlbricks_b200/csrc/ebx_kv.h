@@ -95,7 +95,8 @@ cudaError_t launch_kv_materialize(const KvPool& pool, const int32_t* tables, int
 uint64_t kv_attention_workspace_bytes(int head_dim, int group, int64_t tokens, int max_new, int max_length);
 cudaError_t launch_kv_attention(KvAttnArgs a, bool bf16, int max_new, int max_length, void* ws, cudaStream_t s);
 // Over the prefixes that `a` names as well (state, list and so on).
-uint64_t kv_shared_workspace_bytes(int head_dim, int heads, int group, int64_t tokens, int max_new, int max_length);
+bool kv_takes_prefixes(const KvPool& pool, int heads, int requests, int64_t tokens, int max_new, int max_length);
+uint64_t kv_shared_workspace_bytes(const KvPool& pool, int heads, int requests, int64_t tokens, int max_new, int max_length);
 cudaError_t launch_kv_shared_attention(KvAttnArgs a, bool bf16, int max_new, int max_length, void* ws, cudaStream_t s);
 cudaError_t read_kv_status(int* status, bool clear, cudaStream_t s);
 

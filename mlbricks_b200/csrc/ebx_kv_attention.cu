@@ -675,8 +675,19 @@ cudaError_t launch_kv_attention(KvAttnArgs a, bool bf16, int max_new, int max_le
 
 namespace {
 
-// A request with many rows of its own fills row tiles by itself: nothing is gained by sharing.
-bool takes_prefixes(int group, int64_t tokens, int max_new) { return most_rows(group, tokens, max_new) < kPromptMin; }
+// Does reading prefixes once pay?  Not where a request brings many rows of its own, which fill row tiles by themselves; nor
+// where everything that the requests read (`most` bytes of codes, from L2) takes less time than the launches do that sharing
+// adds.  Captured, shared / each by itself, 32 heads over 8 of 128, and 16 of 64: 4 requests of 2050 tokens
+// (17 MB) 15.5 / 13.7 and 14.7 / 15.0 us, 12 of 2050 (50 MB) 17.6 / 17.9 and 16.5 / 21.4, 12 of 8050 (198 MB) 26 / 38
+// and 20 / 53.  With groups of kPromptMin rows and more, for which the other kernel is launched as well: 64 of 550 (72 MB)
+// 38 / 22 and 37 / 28, 64 of 1000 (131 MB) 43 / 27 and 43 / 34, 32 of 2050 (134 MB) 34 / 30 and 22 / 39, 64 of 2050 (269 MB)
+// 38 / 49 and 37 / 67, 200 of 8050 of 12 heads over one of 32 (103 MB) 47 / 62.
+bool takes_prefixes(const KvPool& pool, int group, int requests, int64_t tokens, int max_new, int max_length) {
+    if (most_rows(group, tokens, max_new) >= kPromptMin) return false;
+    if (max_length == 0) return true;  // unknown
+    const int64_t most = int64_t(requests) * max_length * pool.kv_heads * pool.head_dim * 2;
+    return most >= (tokens * group >= kPromptMin ? 128 : 48) * int64_t(1000000);
+}
 
 struct SharedPlan {
     bool prompt;           // groups of kPromptMin rows and more may occur
@@ -684,10 +695,11 @@ struct SharedPlan {
     int64_t where, ml, sums, step, prompt_at, bytes;  // places in the workspace
 };
 
-SharedPlan shared_plan(int head_dim, int heads, int group, int64_t tokens, int max_new, int max_length, int sms) {
+SharedPlan shared_plan(int head_dim, int heads, int group, int64_t tokens, int max_new, int sms) {
     SharedPlan p;
     p.prompt = tokens * group >= kPromptMin;
-    // rows of most row tiles: the requests' own, or, without the other kernel, also those of the groups
+    // Rows of most row tiles: the requests' own, or, without the other kernel, also those of the groups.  16 in either case:
+    // 64 requests behind 8192 tokens, 4 rows each, 63 us, not 58; 200 behind 500 82, not 69.
     p.nq = (p.prompt ? most_rows(group, tokens, max_new) : tokens * group) <= 8 ? 1 : 2;
     p.step_ctas = sms * (p.nq == 1 ? StepCfg<32, 1>::PER_SM : StepCfg<32, 2>::PER_SM);
     p.prompt_ctas = p.prompt ? sms : 0;
@@ -737,20 +749,27 @@ cudaError_t launch_shared(KvAttnArgs a, const SharedPlan& p, char* ws, int dev, 
 
 }  // namespace
 
-uint64_t kv_shared_workspace_bytes(int head_dim, int heads, int group, int64_t tokens, int max_new, int max_length) {
+bool kv_takes_prefixes(const KvPool& pool, int heads, int requests, int64_t tokens, int max_new, int max_length) {
+    return takes_prefixes(pool, heads / pool.kv_heads, requests, tokens, max_new, max_length);
+}
+
+uint64_t kv_shared_workspace_bytes(const KvPool& pool, int heads, int requests, int64_t tokens, int max_new, int max_length) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-    if (!takes_prefixes(group, tokens, max_new)) return kv_attention_workspace_bytes(head_dim, group, tokens, max_new, max_length);
-    return uint64_t(shared_plan(head_dim, heads, group, tokens, max_new, max_length, gemm_sm_count(dev)).bytes);
+    const int group = heads / pool.kv_heads;
+    if (!takes_prefixes(pool, group, requests, tokens, max_new, max_length))
+        return kv_attention_workspace_bytes(pool.head_dim, group, tokens, max_new, max_length);
+    return uint64_t(shared_plan(pool.head_dim, heads, group, tokens, max_new, gemm_sm_count(dev)).bytes);
 }
 
 cudaError_t launch_kv_shared_attention(KvAttnArgs a, bool bf16, int max_new, int max_length, void* ws, cudaStream_t s) {
     if (a.tokens <= 0 || a.requests <= 0) return cudaSuccess;
-    if (!takes_prefixes(a.group, a.tokens, max_new)) return launch_kv_attention(a, bf16, max_new, max_length, ws, s);
+    if (!takes_prefixes(a.pool, a.group, a.requests, a.tokens, max_new, max_length))
+        return launch_kv_attention(a, bf16, max_new, max_length, ws, s);
     int dev = 0;
     const cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    const SharedPlan p = shared_plan(a.pool.head_dim, a.heads, a.group, a.tokens, max_new, max_length, gemm_sm_count(dev));
+    const SharedPlan p = shared_plan(a.pool.head_dim, a.heads, a.group, a.tokens, max_new, gemm_sm_count(dev));
     a.groups = a.requests;
     a.whole = 0;
     char* base = static_cast<char*>(ws);

@@ -415,10 +415,36 @@ __global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(const __grid_cons
 constexpr int kPrefixThreads = 512;
 constexpr int kPrefixColumns = 128;   // entries that a warp compares at a time
 
-// Ascending, in place; `size` a power of two.  Called by all threads of the block.
+// Ascending, in place; `size` a power of two, 64 at least.  Called by all threads of the block.  Exchanges over less than 64
+// places are a warp's own, two keys a lane, without barriers: of 64 keys all 21.
 __device__ __forceinline__ void sort(uint64_t* keys, int size) {
-    for (int k = 2; k <= size; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // the exchanges over 32 and fewer places of the steps k0 .. k1
+    auto within = [&](int k0, int k1) {
+        for (int base = warp * 64; base < size; base += kPrefixThreads / 32 * 64) {
+            uint64_t x = keys[base + lane], y = keys[base + 32 + lane];
+            for (int k = k0; k <= k1; k <<= 1) {
+                const bool up_x = ((base + lane) & k) == 0, up_y = ((base + 32 + lane) & k) == 0;
+                if (k >= 64 && (x > y) == up_x) {
+                    const uint64_t z = x;
+                    x = y;
+                    y = z;
+                }
+                for (int j = min(k >> 1, 16); j > 0; j >>= 1) {
+                    const uint64_t ox = __shfl_xor_sync(0xffffffffu, x, j), oy = __shfl_xor_sync(0xffffffffu, y, j);
+                    const bool low = (lane & j) == 0;
+                    x = (low == up_x) == (x < ox) ? x : ox;
+                    y = (low == up_y) == (y < oy) ? y : oy;
+                }
+            }
+            keys[base + lane] = x;
+            keys[base + 32 + lane] = y;
+        }
+    };
+    __syncthreads();
+    within(2, 64);
+    for (int k = 128; k <= size; k <<= 1) {
+        for (int j = k >> 1; j >= 64; j >>= 1) {
             __syncthreads();
             for (int t = threadIdx.x; t < size / 2; t += kPrefixThreads) {
                 const int i = 2 * t - (t & (j - 1)), o = i + j;
@@ -429,6 +455,9 @@ __device__ __forceinline__ void sort(uint64_t* keys, int size) {
                 }
             }
         }
+        __syncthreads();
+        within(k, k);
+    }
     __syncthreads();
 }
 
@@ -446,21 +475,21 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kPrefixThread
     __shared__ int warp_sums[32];
     const int n = a.requests, size = a.size;
     uint64_t* keys = reinterpret_cast<uint64_t*>(prefix_smem);                            // [size]
-    unsigned long long* best = reinterpret_cast<unsigned long long*>(keys + size);        // [n]: saved << 13 | place
-    int* full = reinterpret_cast<int*>(best + n);  // [n]: a request's full blocks ahead of its new tokens
-    int* common = full + n;                        // [n], then of a place: its leader's first place, its tokens' in the list
-    int* leader = common + n;                      // [n], then tokens of a group
+    unsigned long long* best = reinterpret_cast<unsigned long long*>(keys + size);  // [n]: saved << 13 | place; before that
+    int* full = reinterpret_cast<int*>(best);  // [n]: a request's full blocks ahead of its new tokens
+    int* leader = full + n;                    // [n]
+    int* common = leader + n;                  // [n], then of a place: its leader's first place, its tokens' in the list
+    int* tokens = common + n;                  // [n], of a group
+    int* first_token = tokens + n;             // [n]
+    __shared__ int past_last;                  // first_token[n]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = int(cluster.block_rank());
     constexpr int kWarps = kPrefixThreads / 32;
     if (tid < 32) warp_sums[tid] = 0;
-    for (int i = tid; i < n; i += kPrefixThreads) {
-        common[i] = INT_MAX;
-        best[i] = 0;
-    }
+    for (int i = tid; i < n; i += kPrefixThreads) common[i] = INT_MAX;
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");  // waited for ahead of the first minimum
     asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
-    auto from = [&](int i) { return int(min(max(int64_t(a.starts[i]), int64_t(0)), a.tokens)); };
-    auto brings = [&](int i) { return max(from(i + 1) - from(i), 0); };
+    auto start_of = [&](int i) { return int(min(max(int64_t(a.starts[i]), int64_t(0)), a.tokens)); };
+    auto brings = [&](int i) { return max((i + 1 < n ? first_token[i + 1] : past_last) - first_token[i], 0); };
 
     // keys: block << 13 | request; behind them those that share nothing, and none at all
     constexpr uint64_t kAlone = uint64_t(1) << 44, kNone = ~uint64_t(0);
@@ -468,7 +497,9 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kPrefixThread
         uint64_t key = kNone;
         if (i < n) {
             const int64_t cap = int64_t(a.width) << a.shift;
-            const int count = brings(i);
+            const int begin = start_of(i), end = start_of(i + 1), count = max(end - begin, 0);
+            first_token[i] = begin;
+            if (i + 1 == n) past_last = end;
             const int64_t past = min(int64_t(max(a.lengths[i], 0)), cap) - count;
             full[i] = past > 0 && count > 0 ? int(past >> a.shift) : 0;
             const int id = full[i] > 0 ? a.tables[int64_t(i) * a.width] : -1;
@@ -528,10 +559,11 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kPrefixThread
         const int length = alone ? 0 : min(common[i], min(full[i], full[first]));
         keys[p] = uint64_t(first) << 40 | (kMost - uint64_t(length)) << 13 | uint64_t(i);
     }
+    __syncthreads();
+    for (int i = tid; i < n; i += kPrefixThreads) best[i] = 0;  // where leaders and full blocks were
     sort(keys, size);
     auto length_of = [&](int p) { return int(kMost - (keys[p] >> 13 & kMost)); };
     int* begin = common;
-    int* tokens = leader;
     for (int p = tid; p < n; p += kPrefixThreads) {
         tokens[p] = 0;
         const int b = begins(p, 40);
@@ -569,7 +601,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kPrefixThread
     }
     if (tid == 0) a.out.group_starts[n] = int(min(ahead, a.tokens));
     for (int p = warp; p < n; p += kWarps) {
-        const int i = int(keys[p] & 8191), to = begin[p], t0 = from(i), count = brings(i);
+        const int i = int(keys[p] & 8191), to = begin[p], t0 = first_token[i], count = brings(i);
         for (int t = lane; t < count; t += 32) {
             a.out.state[t0 + t] = to >= 0 ? 2 : 1;
             if (to >= 0 && int64_t(to) + t < a.tokens) a.out.list[to + t] = t0 + t;
@@ -608,7 +640,7 @@ cudaError_t read_kv_copy_status(int* status, bool clear, cudaStream_t s) {
 }
 
 cudaError_t launch_kv_prefixes(KvPrefixArgs a, cudaStream_t s) {
-    a.size = 2;
+    a.size = 64;
     while (a.size < a.requests) a.size *= 2;
     constexpr int kMostSmem = kKvMostPrefixes * (8 + 8 + 3 * 4);
     const size_t smem = size_t(a.size) * 8 + size_t(a.requests) * (8 + 3 * 4);

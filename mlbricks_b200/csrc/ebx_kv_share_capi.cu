@@ -17,6 +17,13 @@ const char* table_of(int32_t requests, int32_t width, int32_t block_size, int32_
     return nullptr;
 }
 
+// Can attention over prefixes be asked for with these sizes?
+bool shared_sizes(const ebx_kv_pool* pool, int32_t heads, int32_t requests, int64_t tokens, int32_t max_new, int32_t max_length,
+                  ebx::KvPool& p) {
+    return !pool_of(pool, p) && heads >= 1 && heads % p.kv_heads == 0 && requests >= 0 && requests <= ebx::kKvMostPrefixes &&
+           tokens >= 0 && tokens <= INT32_MAX && max_new >= 0 && max_length >= 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -130,15 +137,20 @@ ebx_status ebx_kv_prefixes(const int32_t* tables, int32_t width, int32_t block_s
     return launched(ebx::launch_kv_prefixes(a, static_cast<cudaStream_t>(stream)), "ebx_kv_prefixes");
 }
 
-uint64_t ebx_kv_shared_attention_workspace_bytes(const ebx_kv_pool* pool, int32_t heads, int64_t tokens,
-                                                 int32_t max_new, int32_t max_length) {
+uint64_t ebx_kv_shared_attention_workspace_bytes(const ebx_kv_pool* pool, int32_t heads, int32_t requests,
+                                                 int64_t tokens, int32_t max_new, int32_t max_length) {
     ebx::KvPool p;
-    if (pool_of(pool, p) || heads < 1 || heads % p.kv_heads != 0 || tokens < 0 || tokens > INT32_MAX ||
-        max_new < 0 || max_length < 0)
-        return 0;
+    if (!shared_sizes(pool, heads, requests, tokens, max_new, max_length, p)) return 0;
     Device d(pool->device);
     if (d.err != cudaSuccess) return 0;
-    return ebx::kv_shared_workspace_bytes(p.head_dim, heads, heads / p.kv_heads, tokens, max_new, max_length);
+    return ebx::kv_shared_workspace_bytes(p, heads, requests, tokens, max_new, max_length);
+}
+
+int32_t ebx_kv_takes_prefixes(const ebx_kv_pool* pool, int32_t heads, int32_t requests, int64_t tokens,
+                              int32_t max_new, int32_t max_length) {
+    ebx::KvPool p;
+    return shared_sizes(pool, heads, requests, tokens, max_new, max_length, p) &&
+           ebx::kv_takes_prefixes(p, heads, requests, tokens, max_new, max_length);
 }
 
 ebx_status ebx_kv_shared_attention(const ebx_kv_pool* pool, const void* q, int64_t q_token_stride,
@@ -167,7 +179,7 @@ ebx_status ebx_kv_shared_attention(const ebx_kv_pool* pool, const void* q, int64
     Device d(pool->device);
     if (d.err != cudaSuccess) return launched(d.err, "cudaSetDevice");
     const int group = heads / p.kv_heads;
-    const uint64_t need = ebx::kv_shared_workspace_bytes(p.head_dim, heads, group, tokens, max_new, max_length);
+    const uint64_t need = ebx::kv_shared_workspace_bytes(p, heads, requests, tokens, max_new, max_length);
     if (need > 0 && (!workspace || workspace_bytes < need)) {
         ebx::set_error("ebx_kv_shared_attention: workspace smaller than ebx_kv_shared_attention_workspace_bytes");
         return EBX_ERR_WORKSPACE;

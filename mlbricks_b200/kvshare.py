@@ -181,10 +181,19 @@ def prefixes(tables: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor, 
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace_bytes(device: int, kv_heads: int, head_dim: int, heads: int, tokens: int, max_new: int,
-                     max_length: int) -> int:
-    pool = _ebx.KVPool(16, 16, 16, 16, 1, kv_heads, BLOCK_SIZES[0], head_dim, device, 0)  # only its sizes count
-    return int(_ebx.load().ebx_kv_shared_attention_workspace_bytes(ctypes.byref(pool), heads, tokens, max_new, max_length))
+def _workspace(device: int, kv_heads: int, head_dim: int, heads: int, requests: int, tokens: int, max_new: int,
+               max_length: int) -> tuple[int, bool]:
+    """Bytes of workspace, and whether prefixes are used at all."""
+    pool = ctypes.byref(_ebx.KVPool(16, 16, 16, 16, 1, kv_heads, BLOCK_SIZES[0], head_dim, device, 0))  # only its sizes count
+    sizes, lib = (heads, requests, tokens, max_new, max_length), _ebx.load()
+    return int(lib.ebx_kv_shared_attention_workspace_bytes(pool, *sizes)), bool(lib.ebx_kv_takes_prefixes(pool, *sizes))
+
+
+def takes_prefixes(pool: KVPool, heads: int, requests: int, tokens: int, max_new: int = 0, max_length: int = 0) -> bool:
+    """Whether ``attention`` with these sizes uses prefixes; where it does not, ``prefixes`` need not be called."""
+    if heads <= 0 or heads % pool.kv_heads or min(requests, tokens, max_new, max_length) < 0 or requests > MOST_REQUESTS:
+        return False
+    return _workspace(pool.device, pool.kv_heads, pool.head_dim, heads, requests, tokens, max_new, max_length)[1]
 
 
 def attention(q: torch.Tensor, pool: KVPool, tables: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor,
@@ -195,7 +204,8 @@ def attention(q: torch.Tensor, pool: KVPool, tables: torch.Tensor, lengths: torc
 
     The formula is the same; the order of sums is not.  ``max_new``, the largest number of new tokens of a request, should be given: with
     49 rows (max_new, or without it tokens, times heads / kv_heads) and more, requests fill the kernels' tiles by
-    themselves, and go alone."""
+    themselves, and go alone; so they do where requests and ``max_length``, if given, are too few for sharing to pay
+    (``takes_prefixes``)."""
     q = pool._rows(q, None, "q")
     device, int32 = pool.device, torch.int32
     tokens, heads, dim = q.shape
@@ -215,7 +225,7 @@ def attention(q: torch.Tensor, pool: KVPool, tables: torch.Tensor, lengths: torc
         raise ValueError("out must be a contiguous tensor of q's shape and dtype")
     lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
     if tokens and requests:
-        nbytes = _workspace_bytes(device, pool._c.kv_heads, dim, heads, tokens, max_new, max_length)
+        nbytes = _workspace(device, pool._c.kv_heads, dim, heads, requests, tokens, max_new, max_length)[0]
         ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         st = _ebx.load().ebx_kv_shared_attention(
             pool._ref, q.data_ptr(), q.stride(0), q.stride(1), heads, _ROW_DTYPES[q.dtype], tables.data_ptr(),
@@ -286,12 +296,14 @@ class SharedKVCache(KVCache):
         self.step = self._shared = None  # slots and prefixes of a step planned before are not this table's
 
     def attention(self, layer: int, q: torch.Tensor, **options):
-        """The step's queries over the layer's cache, what requests share once; with ``window`` or ``first``, which
-        prefixes do not allow, as ``KVCache.attention``."""
-        if options.get("window") or options.get("first") is not None or self.lengths.numel() > MOST_REQUESTS:
+        """The step's queries over the layer's cache, what requests share once; as ``KVCache.attention`` with ``window`` or
+        ``first``, which prefixes do not allow, and where sharing could not pay."""
+        step = self._planned()
+        if (options.get("window") or options.get("first") is not None or q.dim() != 3
+                or not takes_prefixes(self.pools[layer], q.shape[1], self.lengths.numel(), q.shape[0], self._max_new,
+                                      self.max_length)):
             return super().attention(layer, q, **options)
         options.pop("window", None), options.pop("first", None)
-        step = self._planned()
         if self._shared is None:
             self._shared = prefixes(self.tables, step.lengths, step.starts, block_size=self.block_size,
                                     blocks=self.pools[layer].blocks, tokens=q.shape[0])
@@ -299,4 +311,5 @@ class SharedKVCache(KVCache):
                          max_new=self._max_new, max_length=self.max_length, **options)
 
 
-__all__ = ["KVCompact", "KVFork", "KVMoves", "KVPrefixes", "SharedKVCache", "attention", "compact", "copy", "fork", "prefixes"]
+__all__ = ["KVCompact", "KVFork", "KVMoves", "KVPrefixes", "SharedKVCache", "attention", "compact", "copy", "fork", "prefixes",
+           "takes_prefixes"]

@@ -77,7 +77,7 @@ def test_one_group(dtype, dim, heads, group):
         prefix = 3 * block + 5
         lengths = [prefix + 1 + 7 * i % 90 for i in range(members)]
         run([0] * members, [prefix], lengths, [1] * members, heads=heads, group=group, dim=dim, block=block, dtype=dtype,
-            grouped=members, max_new=1, max_length=max(lengths))
+            grouped=members, max_new=1)
 
 
 @pytest.mark.parametrize("block", [16, 32, 64, 128])

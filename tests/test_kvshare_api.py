@@ -110,4 +110,8 @@ def test_prefix_errors_without_gpu():
     refused(attention(pool(), shared=None), "null")
     refused(attention(pool(), max_new=-1), ">= 0")
     assert attention(pool(), tokens=0) == _ebx.EBX_OK
-    assert lib.ebx_kv_shared_attention_workspace_bytes(pool(head_dim=96), 4, 1, 1, 1) == 0
+    assert lib.ebx_kv_shared_attention_workspace_bytes(pool(head_dim=96), 4, 1, 1, 1, 1) == 0
+    takes = lib.ebx_kv_takes_prefixes
+    assert takes(pool(), 4, 40, 40, 1, 100000) == 1 and takes(pool(), 4, 40, 40, 1, 0) == 1  # much to read, or unknown
+    assert takes(pool(), 4, 40, 40, 1, 500) == 0 and takes(pool(), 4, 40, 40, 25, 100000) == 0  # little; many rows each
+    assert takes(pool(), 3, 40, 40, 1, 0) == 0 and takes(pool(), 4, 8193, 40, 1, 0) == 0 and takes(None, 4, 1, 1, 1, 0) == 0
