@@ -167,12 +167,20 @@ struct KvWalk {
     }
 };
 
-// This CTA's share.  Called by all NT threads of the block.  Two steps over windows of requests:
+// x / y of 64 bits, as 32 where they fit.
+__device__ __forceinline__ int64_t kv_divide(int64_t x, int64_t y) {
+    return ((x | y) >> 32) == 0 ? int64_t(uint32_t(x) / uint32_t(y)) : x / y;
+}
+
+// This CTA's share.  Called by all NT threads of the block.  Where there are no more requests than threads and
+// none has more than kShareFew row tiles, as in decode steps, a thread counts a request's key tiles: one pass over the
+// requests, one sum.  Else in two steps over windows of requests:
 // a thread per request counts its row tiles, then a thread per row tile counts its key tiles, so
 // that one long prompt and many short requests cost the same few loads a thread.  `scratch`:
 // kShareInts ints of shared memory, free again when the last barrier in here is passed.
 constexpr int kShareWindow = 1024;
 constexpr int kShareInts = 3 * kShareWindow + 128;
+constexpr int kShareFew = 4;
 
 template <int RT, int KT, int EXTRA, int NT, bool SHARED = false>
 __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, int* scratch) {
@@ -196,14 +204,15 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, 
         __syncthreads();
         if (lane == 31) sums[warp] = x;
         __syncthreads();
-        total = 0;
-        int64_t ahead = x - v;
+        int64_t y = lane < W ? sums[lane] : 0;
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-            if (w < warp) ahead += sums[w];
-            total += sums[w];
+        for (int d = 1; d < W; d <<= 1) {
+            const int64_t o = __shfl_up_sync(0xffffffffu, y, d);
+            if (lane >= d) y += o;
         }
-        return ahead;
+        total = __shfl_sync(0xffffffffu, y, W - 1);
+        const int64_t before = __shfl_sync(0xffffffffu, y, warp > 0 ? warp - 1 : 0);
+        return x - v + (warp > 0 ? before : 0);
     };
     // fills `units` for the requests [i0, i0 + n)
     auto count = [&](int i0, int n) {
@@ -241,8 +250,27 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, 
         }
         __syncthreads();
     };
-    int64_t total = 0;
-    for (int i0 = 0; i0 < a.requests; i0 += kShareWindow) {
+    int64_t total = 0, few_units = 0, few_ahead = 0;
+    bool few = a.requests <= NT;
+    if (few) {
+        bool many = false;
+        if (tid < a.requests) {
+            const KvRequest r = kv_request<SHARED>(a, tid);
+            many = r.rows > kShareFew * RT;
+            for (int rt = 0; rt * RT < r.rows && !many; ++rt) {
+                int t0, k;
+                kv_key_tiles<RT, KT>(a, r, rt, t0, k);
+                few_units += a.whole ? 1 : k + EXTRA;
+            }
+        }
+        few = !__syncthreads_or(many);
+    }
+    if (few) {
+        int64_t all;
+        few_ahead = scan(few_units, all);
+        total = all * a.pool.kv_heads;
+    }
+    for (int i0 = 0; i0 < a.requests && !few; i0 += kShareWindow) {
         const int n = min(kShareWindow, a.requests - i0);
         count(i0, n);
         int64_t mine = 0, all;
@@ -250,7 +278,7 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, 
         scan(mine, all);
         total += all * a.pool.kv_heads;
     }
-    int64_t per = (total + gridDim.x - 1) / gridDim.x;
+    int64_t per = kv_divide(total + gridDim.x - 1, gridDim.x);
     per = per < least && !a.whole ? least : per;
     const int64_t w0 = per * blockIdx.x;
     KvShare out;
@@ -262,8 +290,17 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnArgs& a, int64_t least, 
         __syncthreads();
         return out;
     }
+    if (few) {
+        const int64_t u = few_units * a.pool.kv_heads, begin = few_ahead * a.pool.kv_heads;
+        if (u > 0 && begin <= w0 && w0 < begin + u) {  // exactly one thread
+            const int64_t head = kv_divide(w0 - begin, few_units);
+            sums[W] = tid;
+            sums[W + 1] = head;
+            sums[W + 2] = w0 - begin - head * few_units;
+        }
+    }
     int64_t base = 0;  // units ahead of the window
-    for (int i0 = 0;; i0 += kShareWindow) {
+    for (int i0 = 0; !few; i0 += kShareWindow) {
         const int n = min(kShareWindow, a.requests - i0);
         if (a.requests > kShareWindow) count(i0, n);  // else they are still there
         bool found = false;
