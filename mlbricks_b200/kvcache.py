@@ -69,12 +69,13 @@ class KVPool:
 
     def __init__(self, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
                  v_scales: torch.Tensor) -> None:
-        shape, device = k_codes.shape, k_codes.get_device()
+        shape, device, int8, fp32 = k_codes.shape, k_codes.get_device(), torch.int8, torch.float32
         scales = shape[:2]
         if not (len(shape) == 4 and device >= 0 and v_codes.shape == shape and k_scales.shape == scales
-                and v_scales.shape == scales and _int_ok(k_codes, torch.int8, device)
-                and _int_ok(v_codes, torch.int8, device) and _int_ok(k_scales, torch.float32, device)
-                and _int_ok(v_scales, torch.float32, device)):
+                and v_scales.shape == scales and k_codes.dtype is int8 and v_codes.dtype is int8
+                and k_scales.dtype is fp32 and v_scales.dtype is fp32 and v_codes.get_device() == device
+                and k_scales.get_device() == device and v_scales.get_device() == device and k_codes.is_contiguous()
+                and v_codes.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous()):
             self._refuse(k_codes, k_scales, v_codes, v_scales)
         blocks, kv_heads, block_size, head_dim = shape
         if block_size not in BLOCK_SIZES:
