@@ -452,14 +452,13 @@ EBX_API ebx_status ebx_kv_fork(const int32_t* lengths, const int32_t* tables, in
  * made by ebx_kv_copy.  Every other block is free afterwards, also one that neither a
  * row nor the ring had: free_out [blocks] holds their numbers, rising, then -1, and
  * ring_out[4] = {0, blocks - H, 0, copies}.  out_tables as in ebx_kv_fork; sources and targets
- * [blocks / 2], -1 behind the last copy.  No output is an input; limits as above.
- * workspace: 4 * blocks bytes. */
+ * [blocks / 2], -1 behind the last copy.  No output is an input; limits as above,
+ * and blocks <= 524288. */
 EBX_API ebx_status ebx_kv_compact(const int32_t* lengths, const int32_t* tables, int32_t width,
                                   int32_t block_size, const int32_t* shares, int32_t blocks,
                                   int32_t requests, int32_t* out_tables, int32_t* out_shares,
                                   int32_t* free_out, int64_t* ring_out, int32_t* sources,
-                                  int32_t* targets, void* workspace, uint64_t workspace_bytes,
-                                  int32_t device, void* stream);
+                                  int32_t* targets, int32_t device, void* stream);
 
 /* Blocks sources[j] to targets[j] of each of `layers` pools (equal sizes, one device), codes and
  * scales, j < n and, if count is not NULL, j < *count (DEVICE).  Pairs with a number that is no

@@ -125,7 +125,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ebx_kv_fork": (
         _ST, [_P, _P, _I32, _I32, _P, _I32, _P, _I32, _P, _P, _P, _I32, _P, _P, _P, _P, _P, _P, _I32, _P]),
     "ebx_kv_compact": (
-        _ST, [_P, _P, _I32, _I32, _P, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _U64, _I32, _P]),
+        _ST, [_P, _P, _I32, _I32, _P, _I32, _I32, _P, _P, _P, _P, _P, _P, _I32, _P]),
     "ebx_kv_copy": (_ST, [_KV, _I32, _P, _P, _P, _I32, _P]),
     "ebx_kv_prefixes_ints": (_U64, [_I32, _I64]),
     "ebx_kv_prefixes": (_ST, [_P, _I32, _I32, _I32, _P, _P, _I32, _I64, _P, _I32, _P]),

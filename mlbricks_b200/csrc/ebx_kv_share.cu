@@ -5,6 +5,9 @@
 // rows or all blocks gave in the phase before, the data are a few hundred kilobytes, and a cluster's barrier costs
 // a fraction of a launch.  Counts are changed by atomic additions only, whose order does not change
 // them, and whatever is given an order (blocks to the ring, copies) gets it from sums over rows or ids.
+//
+// Each kernel lets the next one begin only after its own wait: kernels that begin while two others still run hold
+// places that the copies lack (690 blocks compacted in 2 layers, one call after the other, 91 us in place of 77).
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -81,8 +84,10 @@ __device__ __forceinline__ ForkRow fork_row(const KvForkArgs& a, int r) {
 // that wants it keeps it, the parent itself ahead of others; every other row gets a copy in a block
 // from the ring's front, in row order, or, when there are none left, nothing at all.  Blocks that nobody holds then go
 // to the ring's back in the order of their numbers.
+// What bounds it is latency: 16 or 128 rows 9.5 us, 11 from cold caches, a launch and five barriers of the cluster with
+// two or three dependent reads between each.
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kShareThreads, 1) kv_fork_kernel(const __grid_constant__ KvForkArgs a) {
-    asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
     cg::cluster_group cluster = cg::this_cluster();
     __shared__ int warp_sums[32];
     __shared__ int counts[kCluster];
@@ -231,87 +236,96 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kShareThreads
 // ---- compact ------------------------------------------------------------------------------
 
 // With H blocks held, those whose number is H or more move into the free ones below H, the first into the
-// first and so on: the fewest moves there can be, and no block is read and written.
+// first and so on: the fewest moves there can be, and no block is read and written.  Every CTA marks a part of the
+// rows' blocks in a bitmap of its own, puts the cluster's together and counts the bits ahead of each word; the rank of a
+// bit and the place of the k-th free number below H then answer everything without a list.  2900 blocks 8.8 us from cold
+// caches, and 5.7 us for a small cache's, both latency; with lists in global memory and six barriers 13.3 and 9.7.
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kShareThreads, 1) kv_compact_kernel(const __grid_constant__ KvCompactArgs a) {
-    asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
     cg::cluster_group cluster = cg::this_cluster();
+    extern __shared__ uint32_t bits[];     // [words]: this CTA's rows
     __shared__ int warp_sums[32];
-    __shared__ int counts[3][kCluster];
+    const int words = (a.blocks + 31) / 32;
+    uint32_t* held_bits = bits + words;                            // [words]: all rows
+    int* before = reinterpret_cast<int*>(held_bits + words);       // [words]: bits ahead of a word
     const int tid = threadIdx.x, lane = tid & 31, rank = int(cluster.block_rank());
     const int gtid = rank * kShareThreads + tid, gwarp = gtid >> 5;
     constexpr int kAll = kCluster * kShareThreads, kAllWarps = kAll / 32;
-    const int half = a.blocks / 2;
     auto block = [&](int id) { return id >= 0 && id < a.blocks; };
     auto held_by = [&](int r) {
         const int64_t n = (int64_t(max(a.lengths[r], 0)) + (1 << a.shift) - 1) >> a.shift;
         return int(min(n, int64_t(a.width)));
     };
-    for (int b = gtid; b < a.blocks; b += kAll) a.map[b] = -1;
-    for (int j = gtid; j < half; j += kAll) a.sources[j] = a.targets[j] = -1;
-    cluster.sync();
+    for (int w = tid; w < words; w += kShareThreads) bits[w] = 0;
+    __syncthreads();
     for (int r = gwarp; r < a.requests; r += kAllWarps) {
         const int n = held_by(r);
         for (int j = lane; j < n; j += 32) {
             const int id = a.tables[int64_t(r) * a.width + j];
-            if (block(id)) a.map[id] = 0;
+            if (block(id)) atomicOr(bits + (id >> 5), 1u << (id & 31));
         }
     }
     cluster.sync();
-    const int per = int((int64_t(a.blocks) + kCluster - 1) / kCluster);
-    const int b0 = min(rank * int64_t(per), int64_t(a.blocks)), b1 = min(b0 + int64_t(per), int64_t(a.blocks));
-    int mine = 0, total;
-    for (int b = b0 + tid; b < b1; b += kShareThreads) mine += a.map[b] >= 0;
-    block_sum(mine, warp_sums, total);
-    tell(cluster, counts[0], total);
     int held = 0;
-    for (int c = 0; c < kCluster; ++c) held += counts[0][c];
-    int high = 0, low = 0;
-    for (int b = b0 + tid; b < b1; b += kShareThreads) {
-        const bool is = a.map[b] >= 0;
-        high += is && b >= held;
-        low += !is && b < held;
-    }
-    int highs, lows;
-    block_sum(high, warp_sums, highs);
-    block_sum(low, warp_sums, lows);
-    tell(cluster, counts[1], highs);
-    tell(cluster, counts[2], lows);
-    int at_high = 0, at_low = 0, moves = 0;
-    for (int c = 0; c < kCluster; ++c) {
-        if (c < rank) {
-            at_high += counts[1][c];
-            at_low += counts[2][c];
+    for (int w0 = 0; w0 < words; w0 += kShareThreads) {
+        const int w = w0 + tid;
+        uint32_t x = 0;
+        if (w < words)
+            for (int c = 0; c < kCluster; ++c) x |= cluster.map_shared_rank(bits, c)[w];
+        int total;
+        const int ahead = block_sum(__popc(x), warp_sums, total);
+        if (w < words) {
+            held_bits[w] = x;
+            before[w] = held + ahead;
         }
-        moves += counts[1][c];
+        held += total;
     }
-    for (int base = b0; base < b1; base += kShareThreads) {
-        const int b = base + tid;
-        const bool is = b < b1 && a.map[b] >= 0;
-        const bool is_high = is && b >= held, is_low = b < b1 && !is && b < held;
-        const int h = at_high + block_sum(is_high, warp_sums, highs);
-        const int l = at_low + block_sum(is_low, warp_sums, lows);
-        if (is_high) {
-            a.sources[h] = b;
-            a.map[b] = h;
+    cluster.sync();  // also: nobody leaves while its bits are read
+    auto is_held = [&](int id) { return (held_bits[id >> 5] >> (id & 31) & 1) != 0; };
+    auto rank_of = [&](int id) {  // held blocks ahead of block id <= blocks
+        return (id >> 5) < words ? before[id >> 5] + __popc(held_bits[id >> 5] & ((1u << (id & 31)) - 1)) : held;
+    };
+    const int low = rank_of(held), moves = held - low;  // held ones below H stay
+    auto free_below = [&](int k) {  // the k-th number that is not held
+        int lo = 0, hi = words;     // the last word with at most k of them ahead
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (32 * mid - before[mid] <= k) lo = mid; else hi = mid;
         }
-        if (is_low) a.targets[l] = b;
-        at_high += highs;
-        at_low += lows;
-    }
-    cluster.sync();
-    auto moved = [&](int id) { return id < held ? id : a.targets[a.map[id]]; };
-    for (int64_t at = gwarp; at < a.requests; at += kAllWarps) {
-        const int n = held_by(int(at));
+        uint32_t x = ~held_bits[lo];
+        int left = k - (32 * lo - before[lo]), at = 0;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+            const int n = __popc(x & ((1u << d) - 1));
+            if (left >= n) {
+                left -= n;
+                at += d;
+                x >>= d;
+            }
+        }
+        return 32 * lo + at;
+    };
+    auto moved = [&](int id) { return id < held ? id : free_below(rank_of(id) - low); };
+    for (int at = gwarp; at < a.requests; at += kAllWarps) {
+        const int n = held_by(at);
         for (int j = lane; j < a.width; j += 32) {
-            const int id = j < n ? a.tables[at * a.width + j] : -1;
-            a.out_tables[at * a.width + j] = block(id) ? moved(id) : -1;
+            const int id = j < n ? a.tables[int64_t(at) * a.width + j] : -1;
+            a.out_tables[int64_t(at) * a.width + j] = block(id) ? moved(id) : -1;
         }
     }
     for (int b = gtid; b < a.blocks; b += kAll) {
-        if (a.map[b] >= 0) a.out_shares[moved(b)] = a.shares[b];
+        if (is_held(b)) {
+            const int to = moved(b);
+            a.out_shares[to] = a.shares[b];
+            if (b >= held) {
+                a.sources[rank_of(b) - low] = b;
+                a.targets[rank_of(b) - low] = to;
+            }
+        }
         if (b >= held) a.out_shares[b] = 0;
         a.free_out[b] = b < a.blocks - held ? held + b : -1;
     }
+    for (int j = moves + gtid; j < a.blocks / 2; j += kAll) a.sources[j] = a.targets[j] = -1;
     if (gtid == 0) {
         a.ring_out[0] = 0;
         a.ring_out[1] = a.blocks - held;
@@ -324,6 +338,8 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kShareThreads
 
 constexpr int kCopyThreads = 128;     // a warp for the codes, the others for scales
 constexpr int kCopySegment = 4096;    // bytes of a unit
+// Stages x segment x CTAs of an SM, for the two cases below and 1 KB blocks of 3 layers: 8 x 4 KB x 6 69.9, 93.1, 3.0 us;
+// 8 x 8 KB x 3 69.8, 93.1, 3.7; 4 x 16 KB x 3 74.9, 99.1, 3.7; 4 x 4 KB x 8 77.9, 114.7, 2.9; 6 x 32 KB x 1 72.6, 98.9, 7.3.
 constexpr int kCopyStages = 8;
 constexpr int kCopyCtas = 6;          // of an SM
 
@@ -336,7 +352,9 @@ __device__ __forceinline__ bool copy_wait(uint32_t bar, uint32_t parity) {
 }
 
 // Unit: a segment of one side of one pair of blocks in one layer.  One thread sends a CTA's units through a ring of
-// shared memory by bulk copies, which need no registers on the way.
+// shared memory by bulk copies, which need no registers on the way.  What bounds it is DRAM: 223 MB read and written in 70 us =
+// 6.4 TB/s, 0.98 of a copy's rate; 124 copies of 4 blocks (520 MB written, the sources from L2) 93 us = 5.6 TB/s of
+// writes.  Loads and stores of 16 bytes a thread, 64 KB an SM on their way, 86 and 115 us.
 __global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(const __grid_constant__ KvCopyArgs a) {
     extern __shared__ __align__(128) uint8_t copy_smem[];
     __shared__ uint64_t full[kCopyStages];
@@ -346,7 +364,7 @@ __global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(const __grid_cons
         for (int i = 0; i < kCopyStages; ++i) mbar_init(smem_u32(&full[i]), 1);
         fence_proxy_async_smem();
     }
-    asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
     const int64_t pairs = a.count ? min(max(*a.count, int64_t(0)), int64_t(a.n)) : a.n;
     auto block = [&](int id) { return id >= 0 && id < a.blocks; };
     if (threadIdx.x >= 32) {
@@ -467,7 +485,8 @@ __device__ __forceinline__ void sort(uint64_t* keys, int size) {
 //
 // Every CTA sorts the requests by their first blocks, so that each knows everyone's leader; the comparisons are shared
 // out among the cluster, and minima kept in the first CTA, which then sorts by leader and length: a request's place among
-// its leader's is one less than the members that its length would have.
+// its leader's is one less than the members that its length would have.  What bounds it is latency: 4 requests 6.3 us, 64
+// of 137 blocks 8.8, 4 of 2053 blocks 6.3 (a warp to a row 29), 200 12.
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kPrefixThreads, 1)
     kv_prefixes_kernel(const __grid_constant__ KvPrefixArgs a) {
     cg::cluster_group cluster = cg::this_cluster();
@@ -487,7 +506,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kPrefixThread
     if (tid < 32) warp_sums[tid] = 0;
     for (int i = tid; i < n; i += kPrefixThreads) common[i] = INT_MAX;
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");  // waited for ahead of the first minimum
-    asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
     auto start_of = [&](int i) { return int(min(max(int64_t(a.starts[i]), int64_t(0)), a.tokens)); };
     auto brings = [&](int i) { return max((i + 1 < n ? first_token[i + 1] : past_last) - first_token[i], 0); };
 
@@ -616,7 +635,13 @@ cudaError_t launch_kv_fork(const KvForkArgs& a, cudaStream_t s) {
 }
 
 cudaError_t launch_kv_compact(const KvCompactArgs& a, cudaStream_t s) {
-    return launch_early(kv_compact_kernel, dim3(kCluster), kShareThreads, 0, s, a);
+    const size_t smem = size_t((a.blocks + 31) / 32) * 3 * sizeof(uint32_t);
+    if (smem > 40 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kv_compact_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   kKvMostCompact / 32 * 3 * int(sizeof(uint32_t)));
+        if (e != cudaSuccess) return e;
+    }
+    return launch_early(kv_compact_kernel, dim3(kCluster), kShareThreads, smem, s, a);
 }
 
 cudaError_t launch_kv_copy(const KvCopyArgs& a, int sms, int dev, cudaStream_t s) {

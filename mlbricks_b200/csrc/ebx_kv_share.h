@@ -35,9 +35,9 @@ struct KvCompactArgs {
     int64_t* ring_out;
     int32_t* sources;         // [blocks / 2]
     int32_t* targets;
-    int32_t* map;             // [blocks], scratch
     int requests, width, shift, blocks;
 };
+constexpr int kKvMostCompact = 1 << 19;  // blocks whose bits kv_compact keeps in shared memory
 
 constexpr int kKvCopyLayers = 64;  // layers of a launch
 

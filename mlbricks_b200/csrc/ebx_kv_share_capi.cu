@@ -51,21 +51,18 @@ ebx_status ebx_kv_fork(const int32_t* lengths, const int32_t* tables, int32_t wi
 ebx_status ebx_kv_compact(const int32_t* lengths, const int32_t* tables, int32_t width, int32_t block_size,
                           const int32_t* shares, int32_t blocks, int32_t requests, int32_t* out_tables,
                           int32_t* out_shares, int32_t* free_out, int64_t* ring_out, int32_t* sources,
-                          int32_t* targets, void* workspace, uint64_t workspace_bytes, int32_t device, void* stream) {
+                          int32_t* targets, int32_t device, void* stream) {
     if (const char* msg = table_of(requests, width, block_size, blocks)) return invalid(msg);
-    if (!shares || !out_shares || !free_out || !ring_out || !workspace || (blocks > 1 && (!sources || !targets)) ||
+    if (blocks > ebx::kKvMostCompact) return invalid("ebx_kv_compact: need blocks <= 524288");
+    if (!shares || !out_shares || !free_out || !ring_out || (blocks > 1 && (!sources || !targets)) ||
         (requests > 0 && (!lengths || !tables || !out_tables)))
         return invalid("null argument");
     if (out_shares == shares || (requests > 0 && out_tables == tables))
         return invalid("ebx_kv_compact: outputs must not be inputs");
-    if (workspace_bytes < uint64_t(blocks) * 4) {
-        ebx::set_error("ebx_kv_compact: workspace smaller than 4 * blocks bytes");
-        return EBX_ERR_WORKSPACE;
-    }
     Device d(device);
     if (d.err != cudaSuccess) return launched(d.err, "cudaSetDevice");
     const ebx::KvCompactArgs a{lengths, tables, shares, out_tables, out_shares, free_out, ring_out, sources, targets,
-                               static_cast<int32_t*>(workspace), requests, width, log2_of(block_size), blocks};
+                               requests, width, log2_of(block_size), blocks};
     return launched(ebx::launch_kv_compact(a, static_cast<cudaStream_t>(stream)), "ebx_kv_compact");
 }
 

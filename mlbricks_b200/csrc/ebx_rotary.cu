@@ -88,7 +88,7 @@ struct RotItem {
 // 105 and 24: with a table each and half the bytes on their way.  Interleaved items of one vector 98: half the bytes again.
 template <class T, int V, bool PAIRS>
 __global__ void __launch_bounds__(kRotThreads, kRotCtas) rotate_kernel(const __grid_constant__ RotArgs a) {
-    asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
     using P = Pack<T, V>;
     constexpr bool SINGLE = PAIRS && V == 1;
     constexpr int W = V >= 2 ? V / 2 : 1;   // table entries of an item, of two pairs each (one where V = 1)

@@ -112,18 +112,18 @@ def fork(lengths: torch.Tensor, tables: torch.Tensor, shares: torch.Tensor, free
 def compact(lengths: torch.Tensor, tables: torch.Tensor, shares: torch.Tensor, *, block_size: int) -> KVCompact:
     """New numbers for the blocks that rows hold, so that they are the pool's first ones, with the fewest copies
     (the result's ``moves``, for ``copy``).  All others are free afterwards, and in the result's ring by rising number.
-    The inputs are not changed: the result's tensors take their place."""
+    The inputs are not changed: the result's tensors take their place.  At most 524288 blocks."""
     device = lengths.get_device()
     _state(lengths, tables, shares, block_size, device)
     requests, width = tables.shape
     blocks = shares.numel()
     out_tables, ring = tables.new_empty((requests, width)), lengths.new_empty(4, dtype=torch.int64)
-    out_shares, free, work = shares.new_empty((3, blocks)).unbind()
+    out_shares, free = shares.new_empty((2, blocks)).unbind()
     sources, targets = shares.new_empty((2, blocks // 2)).unbind()
     st = _ebx.load().ebx_kv_compact(
         lengths.data_ptr(), tables.data_ptr(), width, block_size, shares.data_ptr(), blocks, requests, out_tables.data_ptr(),
-        out_shares.data_ptr(), free.data_ptr(), ring.data_ptr(), sources.data_ptr(), targets.data_ptr(), work.data_ptr(),
-        4 * blocks, device, _stream(device))
+        out_shares.data_ptr(), free.data_ptr(), ring.data_ptr(), sources.data_ptr(), targets.data_ptr(), device,
+        _stream(device))
     if st:
         _ebx.check(st)
     return KVCompact(out_tables, out_shares, free, ring, KVMoves(sources, targets, ring[3:]))

@@ -231,7 +231,7 @@ def test_numbers_out_of_range_are_not_followed():
 @pytest.mark.parametrize("block", [16, 128])
 def test_compact(block):
     rng = random.Random(block + 1)
-    for requests, most, spare in ((1, 3 * block, 0), (1, 0, 1), (5, 4 * block, 0), (6, 9 * block, 100), (200, 5 * block, 700), (3, 2000 * block, 900)):
+    for requests, most, spare in ((1, 3 * block, 0), (1, 0, 1), (5, 4 * block, 0), (6, 9 * block, 100), (200, 5 * block, 700), (3, 2000 * block, 900), (2, 7 * block, 200000)):
         rows = random_rows(rng, requests, block, most, spare)
         width = max([len(r) for r in rows.rows] + [1]) + 2
         lengths, tables, shares, _, _ = rows.tensors(width)

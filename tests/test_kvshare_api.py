@@ -41,14 +41,14 @@ def test_argument_errors_without_gpu():
     refused(fork(out_shares=8), "inputs")
     refused(fork(ring_out=8), "inputs")
 
-    def compact(width=1, blocks=1, out_tables=8, out_shares=4, work_bytes=8, sources=4):
-        return lib.ebx_kv_compact(4, 4, width, 16, 8, blocks, 1, out_tables, out_shares, 4, 8, sources, sources, 4, work_bytes, 0, None)
+    def compact(width=1, blocks=1, out_tables=8, out_shares=4, sources=4):
+        return lib.ebx_kv_compact(4, 4, width, 16, 8, blocks, 1, out_tables, out_shares, 4, 8, sources, sources, 0, None)
 
     refused(compact(width=0), "width")
     refused(compact(out_tables=4), "inputs")
     refused(compact(out_shares=8), "inputs")
     refused(compact(blocks=2, sources=None), "null")
-    refused(compact(blocks=3), "workspace", _ebx.EBX_ERR_WORKSPACE)
+    refused(compact(blocks=524289), "524288")
 
     def pools(*changes):
         fields = dict(k_codes=16, k_scales=4, v_codes=16, v_scales=4, blocks=8, kv_heads=2, block_size=16, head_dim=64,
