@@ -71,6 +71,7 @@ struct KvAttnArgs {
     const int32_t* own_first;     // [groups]: a request's first token that it does not share
     const int32_t* list;
     const int32_t* state;         // [tokens], KvPrefixes
+    const int32_t* largest;       // tokens of the largest group
     float* sums;                  // [2][tokens * heads][head_dim]: O of a row that one CTA has whole,
     float2* sums_ml;              // [2][tokens * heads]: its {m, l}; of the prefix, and of what is the request's own
     int2* where;                  // [2][tokens * heads]: which CTAs have a row's parts (kv_where)

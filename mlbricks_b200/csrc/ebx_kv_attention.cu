@@ -192,6 +192,20 @@ __global__ void __launch_bounds__(kStepThreads, (StepCfg<D, NQ>::PER_SM))
     // the D / 8 bytes of a V row, and dimensions of O, of this lane
     const int vbyte = D == 128 ? 16 * ((n8 >> 1) | ((n8 & 1) << 2))
                       : D == 64 ? 8 * (2 * ((((n8 >> 1) & 1) << 1) | (n8 >> 2)) + (n8 & 1)) : 4 * n8;
+    // Where this lane's bytes of rows u * 16 + r and 8 rows on are: the swizzle there is that of row r.  Of 16 rows of a
+    // prefix (four requests of 131000 shared tokens) that is 73 us and not 75; decode steps of 8 rows have no
+    // registers for it (64 requests of up to 8192 tokens 96 us, not 95).
+    constexpr bool KEPT = SHARED && NQ == 2;
+    uint32_t k_at[KL];
+#pragma unroll
+    for (int x = 0; x < KL; ++x) k_at[x] = swz<D>(krow, x * 4 * KB + c * KB);
+    const uint32_t v_at[2] = {swz<D>(vrow0, vbyte), swz<D>(vrow1, vbyte)};
+    auto k_byte = [&](int u, int x, int on) {
+        return KEPT ? uint32_t(u * 16 * D) + k_at[x] + on * D : swz<D>(u * 16 + on + krow, x * 4 * KB + c * KB);
+    };
+    auto v_byte = [&](int u, int odd, int on) {
+        return KEPT ? uint32_t(u * 16 * D) + v_at[odd] + on * D : swz<D>(u * 16 + on + (odd ? vrow1 : vrow0), vbyte);
+    };
     int it = 0;
     bool ok = true;
     for (; !walk.done(); walk.next(a)) {
@@ -292,8 +306,8 @@ __global__ void __launch_bounds__(kStepThreads, (StepCfg<D, NQ>::PER_SM))
 #pragma unroll
                 for (int x = 0; x < KL; ++x) {
                     uint32_t w0[KW], w1[KW];
-                    lds<KB>(kbase + swz<D>(u * 16 + krow, x * 4 * KB + c * KB), w0);
-                    lds<KB>(kbase + swz<D>(u * 16 + 8 + krow, x * 4 * KB + c * KB), w1);
+                    lds<KB>(kbase + k_byte(u, x, 0), w0);
+                    lds<KB>(kbase + k_byte(u, x, 8), w1);
 #pragma unroll
                     for (int q = 0; q < KW; ++q) {
                         const uint32_t v0 = w0[q] ^ 0x80808080u, v1 = w1[q] ^ 0x80808080u;
@@ -304,10 +318,10 @@ __global__ void __launch_bounds__(kStepThreads, (StepCfg<D, NQ>::PER_SM))
                     }
                 }
                 uint32_t v00[VB / 4], v01[VB / 4], v10[VB / 4], v11[VB / 4];
-                lds<VB>(vbase + swz<D>(u * 16 + vrow0, vbyte), v00);
-                lds<VB>(vbase + swz<D>(u * 16 + vrow1, vbyte), v01);
-                lds<VB>(vbase + swz<D>(u * 16 + 8 + vrow0, vbyte), v10);
-                lds<VB>(vbase + swz<D>(u * 16 + 8 + vrow1, vbyte), v11);
+                lds<VB>(vbase + v_byte(u, 0, 0), v00);
+                lds<VB>(vbase + v_byte(u, 1, 0), v01);
+                lds<VB>(vbase + v_byte(u, 0, 8), v10);
+                lds<VB>(vbase + v_byte(u, 1, 8), v11);
                 const bool none = vs < 0.0f;  // kKvNone
                 const float vsc = vs < 0x1p-100f ? 0x1p-100f : vs;  // NaN stays
                 const float b = none ? -INFINITY : lg2(vsc);

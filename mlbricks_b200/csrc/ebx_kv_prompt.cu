@@ -317,6 +317,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");  // nothing of the call's inputs is read before
+    if constexpr (SHARED) {
+        if (int64_t(*a.largest) * a.group < a.least_rows) {  // the host does not know the groups
+            before_sync();
+            __syncthreads();
+            if (warp == kLoad) {
+                after_sync();
+                asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(*tmem_slot) : "memory");
+            }
+            return;
+        }
+    }
     const KvShare share = kv_share<kPromptRows, kPromptKeys, kPromptExtra, kPromptThreads, SHARED>(a, least, reinterpret_cast<int*>(smem));
     fence_proxy_async_smem();  // copies will overwrite what kv_share kept there
     if (!SHARED && threadIdx.x == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);

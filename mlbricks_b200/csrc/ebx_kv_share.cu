@@ -500,10 +500,11 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kPrefixThread
     int* common = leader + n;                  // [n], then of a place: its leader's first place, its tokens' in the list
     int* tokens = common + n;                  // [n], of a group
     int* first_token = tokens + n;             // [n]
-    __shared__ int past_last;                  // first_token[n]
+    __shared__ int past_last, s_largest;       // first_token[n]; tokens of the largest group
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = int(cluster.block_rank());
     constexpr int kWarps = kPrefixThreads / 32;
     if (tid < 32) warp_sums[tid] = 0;
+    if (tid == 0) s_largest = 0;
     for (int i = tid; i < n; i += kPrefixThreads) common[i] = INT_MAX;
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");  // waited for ahead of the first minimum
     asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
@@ -611,14 +612,20 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kPrefixThread
     }
     __syncthreads();
     int64_t ahead = 0;
+    int largest = 0;
     for (int g0 = 0; g0 < n; g0 += kPrefixThreads) {
         const int g = g0 + tid;
         int total;
+        largest = max(largest, g < n ? tokens[g] : 0);
         const int64_t start = ahead + block_sum(g < n ? tokens[g] : 0, warp_sums, total);
         if (g < n) a.out.group_starts[g] = int(min(start, a.tokens));
         ahead += total;
     }
+    largest = __reduce_max_sync(0xffffffffu, largest);
+    if (lane == 0 && largest > 0) atomicMax(&s_largest, largest);
     if (tid == 0) a.out.group_starts[n] = int(min(ahead, a.tokens));
+    __syncthreads();
+    if (tid == 0) *a.out.largest = s_largest;
     for (int p = warp; p < n; p += kWarps) {
         const int i = int(keys[p] & 8191), to = begin[p], t0 = first_token[i], count = brings(i);
         for (int t = lane; t < count; t += 32) {

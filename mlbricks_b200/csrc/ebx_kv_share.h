@@ -61,11 +61,13 @@ struct KvPrefixes {
     int32_t* own_first;     // [requests]: the first token that the request does not share
     int32_t* list;          // [tokens]: the groups' tokens
     int32_t* state;         // [tokens]: 0: of no request, 1: of a request by itself, 2: of one in a group
+    int32_t* largest;       // tokens of the largest group
 };
 
-// All in one buffer of 3 * requests + 1 + 2 * tokens ints, in the order of the structure.
+// All in one buffer of 3 * requests + 2 + 2 * tokens ints, in the order of the structure.
 inline KvPrefixes prefixes_at(int32_t* p, int64_t requests, int64_t tokens) {
-    return {p, p + requests + 1, p + 2 * requests + 1, p + 3 * requests + 1, p + 3 * requests + 1 + tokens};
+    return {p, p + requests + 1, p + 2 * requests + 1, p + 3 * requests + 1, p + 3 * requests + 1 + tokens,
+            p + 3 * requests + 1 + 2 * tokens};
 }
 
 struct KvPrefixArgs {

@@ -108,7 +108,7 @@ ebx_status ebx_kv_copy(const ebx_kv_pool* pools, int32_t layers, const int32_t* 
 }
 
 uint64_t ebx_kv_prefixes_ints(int32_t requests, int64_t tokens) {
-    return requests < 0 || tokens < 0 ? 0 : 3 * uint64_t(requests) + 1 + 2 * uint64_t(tokens);
+    return requests < 0 || tokens < 0 ? 0 : 3 * uint64_t(requests) + 2 + 2 * uint64_t(tokens);
 }
 
 ebx_status ebx_kv_prefixes(const int32_t* tables, int32_t width, int32_t block_size, int32_t blocks,
@@ -202,6 +202,7 @@ ebx_status ebx_kv_shared_attention(const ebx_kv_pool* pool, const void* q, int64
     a.own_first = found.own_first;
     a.list = found.list;
     a.state = found.state;
+    a.largest = found.largest;
     return launched(ebx::launch_kv_shared_attention(a, dtype == ebx::kKvBF16, max_new, max_length, workspace,
                                                     static_cast<cudaStream_t>(stream)), "ebx_kv_shared_attention");
 }

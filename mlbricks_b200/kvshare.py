@@ -172,7 +172,7 @@ def prefixes(tables: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor, 
         _refuse_ints(device, tables=(tables, int32), lengths=(lengths, int32), starts=(starts, int32))
     if starts.numel() != requests + 1 or tables.dim() != 2 or tables.shape[0] != requests or tokens < 0:
         raise ValueError("lengths and the rows of tables must be as many, and starts one more; tokens >= 0")
-    data = starts.new_empty(3 * requests + 1 + 2 * tokens)
+    data = starts.new_empty(3 * requests + 2 + 2 * tokens)
     st = _ebx.load().ebx_kv_prefixes(tables.data_ptr(), tables.shape[1], block_size, blocks, lengths.data_ptr(), starts.data_ptr(),
                                      requests, tokens, data.data_ptr(), device, _stream(device))
     if st:
@@ -217,7 +217,7 @@ def attention(q: torch.Tensor, pool: KVPool, tables: torch.Tensor, lengths: torc
         raise ValueError(f"heads ({heads}) must be a multiple of kv_heads ({pool._c.kv_heads})")
     if starts.numel() != requests + 1 or tables.dim() != 2 or tables.shape[0] != requests:
         raise ValueError("lengths and the rows of tables must be as many, and starts one more")
-    if shared.requests != requests or shared.tokens != tokens or shared.data.numel() != 3 * requests + 1 + 2 * tokens:
+    if shared.requests != requests or shared.tokens != tokens or shared.data.numel() != 3 * requests + 2 + 2 * tokens:
         raise ValueError("shared must be of this step: as many requests and tokens")
     if out is None:
         out = q.new_empty((tokens, heads, dim))

@@ -50,6 +50,11 @@ def make_tables(groups, lengths, prefix, block, spare=2, width=None):
     return tables.cuda(), count
 
 
+def states(found):
+    """Of each token: 0: of no request, 1: of a request by itself, 2: of one in a group."""
+    return found.data[-1 - found.tokens:-1]
+
+
 def run(groups, prefix, lengths, new, *, heads, group, dim, block, dtype=torch.float16, q_size=1.0, grouped=None, tail=0, **kw):
     tables, blocks = make_tables(groups, lengths, prefix, block)
     pool = make_pool(blocks, heads, block, dim)
@@ -59,7 +64,7 @@ def run(groups, prefix, lengths, new, *, heads, group, dim, block, dtype=torch.f
     starts = i32([sum(new[:i]) for i in range(len(new) + 1)])
     found = share.prefixes(tables, i32(lengths), starts, block_size=block, blocks=blocks, tokens=tokens)
     if grouped is not None:
-        assert int((found.data[-tokens:] == 2).sum()) == grouped
+        assert int((states(found) == 2).sum()) == grouped
     out = torch.full((tokens, heads * group, dim), 7.0, dtype=dtype, device="cuda")
     _, lse = share.attention(q, pool, tables, i32(lengths), starts, found, return_lse=True, out=out, **kw)
     kw.pop("max_new", None), kw.pop("max_length", None)
@@ -130,12 +135,12 @@ def test_who_joins():
     tables = i32([[1, 2, 3, 4, 5, 6], [1, 2, 3, 4, 7, 8], [1, 2, 3, 4, 9, 10], [1, 20, 21, 22, 23, 24], [1, 2, 3, 4, 11, 12], [1, 30, 31, 32, 33, 34]])
     starts = i32(range(7))
     shared = share.prefixes(tables, i32([90] * 6), starts, block_size=block, blocks=40, tokens=6)
-    state = shared.data[-6:].tolist()
+    state = states(shared).tolist()
     assert state == [2, 2, 2, 1, 2, 1]  # 3 * 4 blocks rather than 5 * 1
     shared = share.prefixes(tables, i32([90, 90, 90, 90, 64, 16]), starts, block_size=block, blocks=40, tokens=6)
-    assert shared.data[-6:].tolist() == [2, 2, 2, 1, 2, 1]  # 3 members of 4 blocks or 4 of 3: 8 or 9
+    assert states(shared).tolist() == [2, 2, 2, 1, 2, 1]  # 3 members of 4 blocks or 4 of 3: 8 or 9
     shared = share.prefixes(tables, i32([90, 90, 16, 16, 16, 16]), starts, block_size=block, blocks=40, tokens=6)
-    assert shared.data[-6:].tolist() == [2, 2, 1, 1, 1, 1]
+    assert states(shared).tolist() == [2, 2, 1, 1, 1, 1]
 
 
 def test_same_as_without_prefixes():

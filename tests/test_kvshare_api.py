@@ -87,7 +87,7 @@ def test_prefix_errors_without_gpu():
     refused(prefixes(requests=8193), "8192")
     refused(prefixes(tokens=2**31), "tokens")
     assert prefixes(requests=0, tables=None) == _ebx.EBX_OK
-    assert lib.ebx_kv_prefixes_ints(3, 5) == 20 and lib.ebx_kv_prefixes_ints(-1, 5) == 0
+    assert lib.ebx_kv_prefixes_ints(3, 5) == 21 and lib.ebx_kv_prefixes_ints(-1, 5) == 0
 
     def pool(**change):
         fields = dict(k_codes=16, k_scales=4, v_codes=16, v_scales=4, blocks=8, kv_heads=2, block_size=16, head_dim=64,
