@@ -228,3 +228,60 @@ def test_refusals():
             share.prefixes(**args)
     empty = share.prefixes(tables[:0], lengths[:0], starts[:1], block_size=16, blocks=5, tokens=0)
     assert share.attention(q[:0], pool, tables[:0], lengths[:0], starts[:1], empty).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("members", [4, 30])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_negative_and_zero_scale(members, dtype):
+    """Both kernels, whose signs are handled apart, and their join."""
+    for scale in (-0.3, 0.0):
+        run([0] * members, [300], [310 + 3 * i for i in range(members)], [1 + i % 2 for i in range(members)], heads=2, group=4, dim=64,
+            block=16, dtype=dtype, scale=scale, max_new=2, grouped=sum(1 + i % 2 for i in range(members)))
+
+
+def test_queries_of_any_strides():
+    """Rows that are not 16-byte aligned are copied first; others are read where they are."""
+    members, heads, dim = 20, 8, 64
+    q, pool, tables, starts, found, out, lse = run([0] * members, [200], [230] * members, [1] * members, heads=2, group=4, dim=dim,
+                                                   block=32, max_new=1)
+    lengths = i32([230] * members)
+    odd = torch.empty(members, heads, dim + 1, dtype=q.dtype, device="cuda")[..., 1:]
+    flat = torch.empty(heads, members, dim, dtype=q.dtype, device="cuda").transpose(0, 1)
+    for x in (odd, flat):
+        x.copy_(q)
+        assert torch.equal(share.attention(x, pool, tables, lengths, starts, found, max_new=1), out)
+
+
+def test_two_streams_at_once():
+    """Calls on two streams, each with its own prefixes and workspace, over one pool."""
+    one = run([0] * 40, [3000], [3100] * 40, [1] * 40, heads=2, group=4, dim=128, block=64, max_new=1)
+    q, pool, tables, starts, found, out, lse = one
+    lengths, streams, got = i32([3100] * 40), [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for stream, results in zip(streams, got):
+            with torch.cuda.stream(stream):
+                step = share.prefixes(tables, lengths, starts, block_size=64, blocks=pool.blocks, tokens=40)
+                results.append(share.attention(q, pool, tables, lengths, starts, step, max_new=1))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, out) for results in got for x in results)
+
+
+def test_hint_too_small():
+    """max_new chooses kernels; a request that brings more than it says is right all the same."""
+    groups, new = [0] * 12, [1] * 6 + [30] * 6
+    run(groups, [500], [560 + i for i in range(12)], new, heads=2, group=4, dim=64, block=16, max_new=1, grouped=sum(new))
+
+
+def test_largest_number_of_requests():
+    requests = 8192
+    tables = torch.arange(requests * 3, dtype=torch.int32, device="cuda").view(requests, 3)
+    tables[:, 0] = tables[0, 0]
+    tables[::2, 1] = tables[0, 1]
+    starts = torch.arange(requests + 1, dtype=torch.int32, device="cuda")
+    found = share.prefixes(tables, i32([48] * requests), starts, block_size=16, blocks=requests * 3, tokens=requests)
+    # 8191 times one block, or 4095 times two: the longer of what saves the same is not taken, the one that saves more is
+    assert (states(found) == 2).all()
+    with pytest.raises(ValueError, match="8192"):
+        share.prefixes(tables.repeat(2, 1), i32([48] * requests * 2), torch.arange(2 * requests + 1, dtype=torch.int32, device="cuda"),
+                       block_size=16, blocks=requests * 3, tokens=2 * requests)
