@@ -97,8 +97,11 @@ def fork(lengths: torch.Tensor, tables: torch.Tensor, shares: torch.Tensor, free
     if ring.numel() < 2 or free.numel() < 1:
         raise ValueError("ring holds at least its front and back, and free at least one place")
     blocks = shares.numel()
-    out_lengths, sources, targets = lengths.new_empty((3, requests)).unbind()
-    out_tables, out_shares, out_ring = tables.new_empty((requests, width)), shares.new_empty(blocks), ring.new_empty(4)
+    # one allocation: cheaper than five
+    cells = requests * width
+    out_lengths, sources, targets, out_shares, out_tables = lengths.new_empty(3 * requests + blocks + cells).split_with_sizes(
+        (requests, requests, requests, blocks, cells))
+    out_tables, out_ring = out_tables.view(requests, width), ring.new_empty(4)
     st = _ebx.load().ebx_kv_fork(
         lengths.data_ptr(), tables.data_ptr(), width, block_size, shares.data_ptr(), blocks, free.data_ptr(), free.numel(),
         ring.data_ptr(), parents.data_ptr(), None if keep is None else keep.data_ptr(), requests, out_lengths.data_ptr(),
@@ -117,9 +120,10 @@ def compact(lengths: torch.Tensor, tables: torch.Tensor, shares: torch.Tensor, *
     _state(lengths, tables, shares, block_size, device)
     requests, width = tables.shape
     blocks = shares.numel()
-    out_tables, ring = tables.new_empty((requests, width)), lengths.new_empty(4, dtype=torch.int64)
-    out_shares, free = shares.new_empty((2, blocks)).unbind()
-    sources, targets = shares.new_empty((2, blocks // 2)).unbind()
+    cells, half = requests * width, blocks // 2
+    out_shares, free, sources, targets, out_tables = lengths.new_empty(2 * blocks + 2 * half + cells).split_with_sizes(
+        (blocks, blocks, half, half, cells))
+    out_tables, ring = out_tables.view(requests, width), lengths.new_empty(4, dtype=torch.int64)
     st = _ebx.load().ebx_kv_compact(
         lengths.data_ptr(), tables.data_ptr(), width, block_size, shares.data_ptr(), blocks, requests, out_tables.data_ptr(),
         out_shares.data_ptr(), free.data_ptr(), ring.data_ptr(), sources.data_ptr(), targets.data_ptr(), device,
@@ -220,7 +224,9 @@ def attention(q: torch.Tensor, pool: KVPool, tables: torch.Tensor, lengths: torc
     if shared.requests != requests or shared.tokens != tokens or shared.data.numel() != 3 * requests + 2 + 2 * tokens:
         raise ValueError("shared must be of this step: as many requests and tokens")
     if out is None:
-        out = q.new_empty((tokens, heads, dim))
+        out = torch.empty_like(q)  # cheaper than new_empty, and contiguous unless q is dense in another order
+        if not out.is_contiguous():
+            out = q.new_empty((tokens, heads, dim))
     elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != device or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor of q's shape and dtype")
     lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
