@@ -513,24 +513,26 @@ struct SharedParts {
     int step_rows, step_ctas, prompt_ctas;
 };
 constexpr int kPromptTile = 256;
-constexpr int kJoinWays = 4;
 
-// CTA y joins rows 4 y .. 4 y + 3 of [tokens * heads]: 4 rows x 8 column groups x ways that take the row's
+// CTA y joins rows 4 y .. 4 y + 3 of [tokens * heads]: 4 rows x 8 column groups x WAYS that take the row's
 // results in turn, those over the prefix first.  Only what the kernels before it wrote is followed.
-template <int D, bool BF16>
-__global__ void __launch_bounds__(32 * kJoinWays) kv_shared_join_kernel(const __grid_constant__ KvAttnArgs a, SharedParts parts) {
+template <int D, bool BF16, int WAYS>
+__global__ void __launch_bounds__(32 * WAYS) kv_shared_join_kernel(const __grid_constant__ KvAttnArgs a, SharedParts parts) {
     asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
     constexpr int COLS = D / 32;  // float4 columns of a thread: groups of 8 apart
-    __shared__ float2 s_ml[kJoinWays][8][4];
-    __shared__ float4 s_o[COLS][kJoinWays][8][4];
+    __shared__ float2 s_ml[WAYS][8][4];
+    __shared__ float4 s_o[COLS][WAYS][8][4];
     const int ri = threadIdx.x & 3, col = (threadIdx.x >> 2) & 7, way = threadIdx.x >> 5;
     const int64_t rows = a.tokens * a.heads, row = int64_t(blockIdx.x) * 4 + ri;
     const int state = row < rows ? a.state[row / a.heads] : 0;
     int first[2], tile_row[2], count[2] = {0, 0};
+    int2 both[2];
+#pragma unroll
+    for (int side = 0; side < 2; ++side) both[side] = row < rows ? a.where[side * rows + row] : make_int2(0, 0);
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
-        if (state < 2 - side) continue;
-        const int2 w = a.where[side * rows + row];
+        if (state < 2 - side) continue;  // `where` then holds anything
+        const int2 w = both[side];
         const int ctas = w.x < -1 ? parts.prompt_ctas : parts.step_ctas, c = w.x < -1 ? -2 - w.x : w.x;
         first[side] = w.x;
         tile_row[side] = w.y & 0xff;
@@ -556,12 +558,12 @@ __global__ void __launch_bounds__(32 * kJoinWays) kv_shared_join_kernel(const __
     };
     const int total = count[0] + count[1];
     constexpr int AHEAD = 4;  // results on their way at once
-    for (int p0 = way; p0 < total; p0 += AHEAD * kJoinWays) {
+    for (int p0 = way; p0 < total; p0 += AHEAD * WAYS) {
         float4 v[AHEAD][COLS];
         float2 ml[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            const int p = p0 + i * kJoinWays;
+            const int p = p0 + i * WAYS;
             if (p >= total) continue;
             const int side = p < count[0] ? 0 : 1, k = side ? p - count[0] : p;
             const int at = side ? first[1] : first[0], r = side ? tile_row[1] : tile_row[0];
@@ -584,14 +586,14 @@ __global__ void __launch_bounds__(32 * kJoinWays) kv_shared_join_kernel(const __
         }
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i)
-            if (p0 + i * kJoinWays < total) join(ml[i].x, ml[i].y, v[i]);
+            if (p0 + i * WAYS < total) join(ml[i].x, ml[i].y, v[i]);
     }
     s_ml[way][col][ri] = make_float2(m, l);
 #pragma unroll
     for (int x = 0; x < COLS; ++x) s_o[x][way][col][ri] = o[x];
     __syncthreads();
     if (way != 0 || state == 0) return;
-    for (int w = 1; w < min(kJoinWays, total); ++w) {
+    for (int w = 1; w < min(WAYS, total); ++w) {
         float4 v[COLS];
 #pragma unroll
         for (int x = 0; x < COLS; ++x) v[x] = s_o[x][w][col][ri];
@@ -705,12 +707,13 @@ bool takes_prefixes(const KvPool& pool, int group, int requests, int64_t tokens,
 
 struct SharedPlan {
     bool prompt;           // groups of kPromptMin rows and more may occur
-    int nq, step_ctas, prompt_ctas;
+    int sms, nq, step_ctas, prompt_ctas;
     int64_t where, ml, sums, step, prompt_at, bytes;  // places in the workspace
 };
 
 SharedPlan shared_plan(int head_dim, int heads, int group, int64_t tokens, int max_new, int sms) {
     SharedPlan p;
+    p.sms = sms;
     p.prompt = tokens * group >= kPromptMin;
     // Rows of most row tiles: the requests' own, or, without the other kernel, also those of the groups.  16 in either case:
     // 64 requests behind 8192 tokens, 4 rows each, 63 us, not 58; 200 behind 500 82, not 69.
@@ -758,7 +761,10 @@ cudaError_t launch_shared(KvAttnArgs a, const SharedPlan& p, char* ws, int dev, 
     if (grid > INT32_MAX) return cudaErrorInvalidValue;
     const SharedParts parts{reinterpret_cast<const float*>(ws + p.step), reinterpret_cast<const float*>(ws + p.prompt_at),
                             8 * p.nq, p.step_ctas, p.prompt_ctas};
-    return launch_early(kv_shared_join_kernel<D, BF16>, dim3(unsigned(grid)), 32 * kJoinWays, 0, s, a, parts);
+    // Few rows have many parts each.  With 4 / 8 / 16 ways, the whole call: 128 rows of four requests behind 131000 tokens 73.0 /
+    // 70.6 / 71.1 us, 256 behind 8192 20.5 / 19.6 / 19.6; 2048 rows of 64 requests 54.7 / 56.2 / 62.3, 6400 66 / 72 / 84.
+    if (grid <= p.sms) return launch_early(kv_shared_join_kernel<D, BF16, 8>, dim3(unsigned(grid)), 32 * 8, 0, s, a, parts);
+    return launch_early(kv_shared_join_kernel<D, BF16, 4>, dim3(unsigned(grid)), 32 * 4, 0, s, a, parts);
 }
 
 }  // namespace
