@@ -329,3 +329,21 @@ def test_refusals():
     with pytest.raises(ValueError, match="sources"):
         share.copy([a], share.KVMoves(torch.zeros(1, dtype=torch.int32), i32([1]), None))
     share.copy([], moves)
+
+
+def test_offsets_past_32_bits():
+    """A pool of 8.6 GB of codes a side: blocks at both of its ends."""
+    blocks = 131072
+    pool = kv.KVPool(*(t for _ in "kv" for t in (torch.empty(blocks, 8, 64, 128, dtype=torch.int8, device="cuda"),
+                                                 torch.empty(blocks, 8, device="cuda"))))
+    for t in (pool.k_codes, pool.v_codes):
+        t[0].random_(-127, 128), t[-1].random_(-127, 128)
+    for t in (pool.k_scales, pool.v_scales):
+        t[0].uniform_(), t[-1].uniform_()
+    moves = share.KVMoves(i32([blocks - 1, 0]), i32([1, blocks - 2]), None)
+    share.copy([pool], moves)
+    for t in (pool.k_codes, pool.k_scales, pool.v_codes, pool.v_scales):
+        assert torch.equal(t[1], t[-1]) and torch.equal(t[-2], t[0])
+    got = share.compact(i32([200, 64]), i32([[blocks - 1, 5, blocks - 2, 0], [77777, -1, -1, -1]]), i32([0]).repeat(blocks), block_size=64)
+    assert got.tables.tolist() == [[4, 1, 3, 0], [2, -1, -1, -1]]  # 5, 77777 and the last two, in that order, to 1 .. 4
+    assert got.ring.tolist()[1] == blocks - 5

@@ -168,3 +168,16 @@ def test_other_stream_and_graph():
     graph.replay()
     fresh, _ = rotary.rotate(q, None, positions, freq)
     assert torch.equal(held, fresh)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^32 bytes and 2^31 elements: the last tokens as well as the first."""
+    tokens, heads, dim = 70001, 64, 512
+    q = torch.empty(tokens, heads, dim, dtype=torch.float16, device="cuda")
+    q[:3], q[-3:] = torch.randn(3, heads, dim, device="cuda").half(), torch.randn(3, heads, dim, device="cuda").half()
+    assert q.numel() > 2**31
+    positions, freq = torch.arange(tokens, dtype=torch.int32, device="cuda"), rotary.frequencies(dim)
+    ends = torch.tensor([0, 1, 2, tokens - 3, tokens - 2, tokens - 1], device="cuda")
+    before = q[ends].clone()
+    rotary.rotate(q, None, positions, freq, inplace=True)
+    check(before, q[ends], positions[ends], freq)
