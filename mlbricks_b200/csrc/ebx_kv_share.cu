@@ -432,6 +432,7 @@ __global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(const __grid_cons
 
 constexpr int kPrefixThreads = 512;
 constexpr int kPrefixColumns = 128;   // entries that a warp compares at a time
+constexpr int kPrefixFew = 8;         // tokens of a request that a thread writes
 
 // Ascending, in place; `size` a power of two, 64 at least.  Called by all threads of the block.  Exchanges over less than 64
 // places are a warp's own, two keys a lane, without barriers: of 64 keys all 21.
@@ -486,7 +487,8 @@ __device__ __forceinline__ void sort(uint64_t* keys, int size) {
 // Every CTA sorts the requests by their first blocks, so that each knows everyone's leader; the comparisons are shared
 // out among the cluster, and minima kept in the first CTA, which then sorts by leader and length: a request's place among
 // its leader's is one less than the members that its length would have.  What bounds it is latency: 4 requests 6.3 us, 64
-// of 137 blocks 8.8, 4 of 2053 blocks 6.3 (a warp to a row 29), 200 12.
+// of 137 blocks 8.5, 4 of 2053 blocks 6.5 (a warp to a row 29), 200 of 13 10.1 (12.1 with a warp to the tokens of each
+// request and an addition for each member).
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kPrefixThreads, 1)
     kv_prefixes_kernel(const __grid_constant__ KvPrefixArgs a) {
     cg::cluster_group cluster = cg::this_cluster();
@@ -500,11 +502,11 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kPrefixThread
     int* common = leader + n;                  // [n], then of a place: its leader's first place, its tokens' in the list
     int* tokens = common + n;                  // [n], of a group
     int* first_token = tokens + n;             // [n]
-    __shared__ int past_last, s_largest;       // first_token[n]; tokens of the largest group
+    __shared__ int past_last, s_largest, s_many;  // first_token[n]; tokens of the largest group; a request with many
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = int(cluster.block_rank());
     constexpr int kWarps = kPrefixThreads / 32;
     if (tid < 32) warp_sums[tid] = 0;
-    if (tid == 0) s_largest = 0;
+    if (tid == 0) s_largest = s_many = 0;
     for (int i = tid; i < n; i += kPrefixThreads) common[i] = INT_MAX;
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");  // waited for ahead of the first minimum
     asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
@@ -599,15 +601,21 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kPrefixThread
             const unsigned long long b = best[begin[p]];
             depth = b >> 13 ? length_of(int(b & 8191)) : 0;  // what the group shares
             if (length_of(p) < depth) depth = 0;
-            if (depth > 0) count = brings(int(keys[p] & 8191));
+            count = brings(int(keys[p] & 8191));
+            if (count > kPrefixFew) s_many = 1;
+            if (depth == 0) count = 0;
         }
         const int64_t to = listed + block_sum(count, warp_sums, total);
         listed += total;
+        // a group's members are neighbours: one addition for those of a warp
+        const int group = depth > 0 ? int(keys[p] >> 40) : -1;
+        const unsigned same = __match_any_sync(0xffffffffu, group);
+        const int64_t end = __shfl_sync(0xffffffffu, to + count, 31 - __clz(same));
+        if (group >= 0 && lane == __ffs(same) - 1) atomicAdd(tokens + group, int(min(end - to, int64_t(INT_MAX))));
         if (p >= n) continue;
         const int i = int(keys[p] & 8191), first = int(keys[p] >> 40);
         a.out.shared[i] = first == i ? depth << a.shift : 0;
         a.out.own_first[i] = depth << a.shift;
-        if (depth > 0) atomicAdd(tokens + first, count);
         begin[p] = depth > 0 ? int(min(to, int64_t(INT_MAX))) : -1;
     }
     __syncthreads();
@@ -626,13 +634,17 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kPrefixThread
     if (tid == 0) a.out.group_starts[n] = int(min(ahead, a.tokens));
     __syncthreads();
     if (tid == 0) *a.out.largest = s_largest;
-    for (int p = warp; p < n; p += kWarps) {
+    // tokens of a request: a thread, or, where a request has many, a warp
+    auto write = [&](int p, int t, int step, int least, int most) {
         const int i = int(keys[p] & 8191), to = begin[p], t0 = first_token[i], count = brings(i);
-        for (int t = lane; t < count; t += 32) {
+        if (count < least || count > most) return;
+        for (; t < count; t += step) {
             a.out.state[t0 + t] = to >= 0 ? 2 : 1;
             if (to >= 0 && int64_t(to) + t < a.tokens) a.out.list[to + t] = t0 + t;
         }
-    }
+    };
+    for (int p = tid; p < n; p += kPrefixThreads) write(p, 0, 1, 0, kPrefixFew);
+    for (int p = warp; p < n && s_many; p += kWarps) write(p, lane, 32, kPrefixFew + 1, INT_MAX);
 }
 
 }  // namespace
