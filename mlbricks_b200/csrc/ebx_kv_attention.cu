@@ -712,8 +712,8 @@ namespace {
 bool takes_prefixes(const KvPool& pool, int group, int requests, int64_t tokens, int max_new, int max_length) {
     if (most_rows(group, tokens, max_new) >= kPromptMin) return false;
     if (max_length == 0) return true;  // unknown
-    const int64_t most = int64_t(requests) * max_length * pool.kv_heads * pool.head_dim * 2;
-    return most >= (tokens * group >= kPromptMin ? 128 : 48) * int64_t(1000000);
+    const double most = double(requests) * max_length * pool.kv_heads * pool.head_dim * 2;  // passes 64 bits
+    return most >= (tokens * group >= kPromptMin ? 128e6 : 48e6);
 }
 
 struct SharedPlan {

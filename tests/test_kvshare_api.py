@@ -114,4 +114,6 @@ def test_prefix_errors_without_gpu():
     takes = lib.ebx_kv_takes_prefixes
     assert takes(pool(), 4, 40, 40, 1, 100000) == 1 and takes(pool(), 4, 40, 40, 1, 0) == 1  # much to read, or unknown
     assert takes(pool(), 4, 40, 40, 1, 500) == 0 and takes(pool(), 4, 40, 40, 25, 100000) == 0  # little; many rows each
+    assert takes(pool(blocks=1, kv_heads=2**26, block_size=16), 2**26, 8192, 8192, 0, 2**31 - 1) == 0  # many rows each
+    assert takes(pool(blocks=1, kv_heads=2**26, block_size=16), 2**26, 8192, 40, 1, 2**31 - 1) == 1  # a size past 64 bits
     assert takes(pool(), 3, 40, 40, 1, 0) == 0 and takes(pool(), 4, 8193, 40, 1, 0) == 0 and takes(None, 4, 1, 1, 1, 0) == 0
