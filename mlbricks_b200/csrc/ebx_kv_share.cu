@@ -433,6 +433,8 @@ __global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(const __grid_cons
 constexpr int kPrefixThreads = 512;
 constexpr int kPrefixColumns = 128;   // entries that a warp compares at a time
 constexpr int kPrefixFew = 8;         // tokens of a request that a thread writes
+// Dynamic shared memory that needs no leave: 48 KB hold the kernel's static shared memory as well.
+constexpr size_t kPrefixPlainSmem = 40 * 1024;
 
 // Ascending, in place; `size` a power of two, 64 at least.  Called by all threads of the block.  Exchanges over less than 64
 // places are a warp's own, two keys a lane, without barriers: of 64 keys all 21.
@@ -688,7 +690,7 @@ cudaError_t launch_kv_prefixes(KvPrefixArgs a, cudaStream_t s) {
     while (a.size < a.requests) a.size *= 2;
     constexpr int kMostSmem = kKvMostPrefixes * (8 + 8 + 3 * 4);
     const size_t smem = size_t(a.size) * 8 + size_t(a.requests) * (8 + 3 * 4);
-    if (smem > 48 * 1024) {
+    if (smem > kPrefixPlainSmem) {
         const cudaError_t e = cudaFuncSetAttribute(kv_prefixes_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem);
         if (e != cudaSuccess) return e;
     }
