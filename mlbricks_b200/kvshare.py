@@ -262,15 +262,28 @@ class SharedKVCache(KVCache):
         """As ``KVCache.plan``, but a request that is done (-1) gives up blocks that it shares, and its blocks are there
         for this step already.  With a tensor ``new`` that costs a launch or two more, unless ``releases`` is False:
         then -1 is taken for 0."""
-        if isinstance(new, torch.Tensor):
+        # all that can be refused is, before a row is freed
+        requests, where = self._rows.numel(), self.lengths.device
+        listed = not isinstance(new, torch.Tensor)
+        if listed:
+            new = [int(n) for n in new]
+            done = [-1 if n < 0 else i for i, n in enumerate(new)] if min(new, default=0) < 0 else None
+            counts = [max(n, 0) for n in new]
+            tokens, max_new = sum(counts), max(counts, default=0)
+            new = torch.tensor(counts, dtype=torch.int32).to(where, non_blocking=True)
+        elif not _int_ok(new, torch.int32, self.lengths.get_device()):
+            _refuse_ints(self.lengths.get_device(), new=(new, torch.int32))
+        if new.numel() != requests:
+            raise ValueError(f"new must have an entry for each of the {requests} requests")
+        if tokens is None or not 0 <= tokens < 2**31:
+            raise ValueError("a tensor of new tokens needs `tokens`, 0 <= tokens < 2^31")
+        if not listed:
+            new = new.view(-1)
             if releases:
                 self.fork(torch.where(new < 0, -1, self._rows).to(torch.int32))
             new = new.clamp(min=0)
-        else:
-            new = [int(n) for n in new]
-            if min(new, default=0) < 0:
-                self.fork([-1 if n < 0 else i for i, n in enumerate(new)])
-            new = [max(n, 0) for n in new]
+        elif done is not None:
+            self.fork(done)
         self._shared = None
         return super().plan(new, tokens, max_new)
 

@@ -148,3 +148,31 @@ def test_captured_steps_between_forks():
     cache.fork([0, 1, -1, -1, -1, -1])
     model.fork([0, 1, -1, -1, -1, -1], None)
     replay(3, 2)
+
+
+def forked(requests=7, heads=1, dim=64, block=16):
+    """A cache whose rows all share a prompt of five blocks and some, and one step of a token each behind it."""
+    cache = share.SharedKVCache(1, blocks=60, kv_heads=heads, head_dim=dim, requests=requests, max_length=70_000, block_size=block)
+    cache.plan([5 * block + 3] + [0] * (requests - 1))
+    cache.append(0, tokens_of(5 * block + 3, heads, dim), tokens_of(5 * block + 3, heads, dim))
+    cache.fork([0] * requests)
+    cache.plan([1] * requests)
+    cache.append(0, tokens_of(requests, heads, dim), tokens_of(requests, heads, dim))
+    return cache
+
+
+def test_a_refused_plan_frees_nothing():
+    """Calls of `plan` that are refused leave the rows that they would have released as they were."""
+    cache = forked()
+    state = [cache.lengths, cache.tables, cache.shares, cache.free, cache.ring]
+    before = [t.clone() for t in state]
+    ints = torch.tensor([-1, 1, -1, 1, 1, 1, 1], dtype=torch.int32, device="cuda")
+    for args, options in [((ints,), {}), ((ints.long(),), dict(tokens=5)), ((ints,), dict(tokens=-1)),
+                          ((ints.float(),), dict(tokens=5)), ((ints[:6],), dict(tokens=5)), ((ints[:1],), dict(tokens=5)),
+                          ((ints.repeat(2)[::2],), dict(tokens=5)), ((ints.cpu(),), dict(tokens=5)),
+                          (([-1, 1],), {}), (([-1] * 8,), {}), (([-1] + [2**31] + [1] * 5,), {})]:
+        with pytest.raises((ValueError, RuntimeError)):
+            cache.plan(*args, **options)
+        assert all(torch.equal(a, b) for a, b in zip(state, before)), (args, options)
+    assert cache.plan(ints.view(7, 1), tokens=5, max_new=1).ring.tolist()[2] == 0
+    assert cache.lengths.tolist() == [0, 85, 0, 85, 85, 85, 85]
