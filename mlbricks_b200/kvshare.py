@@ -323,7 +323,7 @@ class SharedKVCache(KVCache):
                                       self.max_length)):
             return super().attention(layer, q, **options)
         options.pop("window", None), options.pop("first", None)
-        if self._shared is None:
+        if self._shared is None or self._shared.tokens != q.shape[0]:  # a layer may bring fewer queries
             self._shared = prefixes(self.tables, step.lengths, step.starts, block_size=self.block_size,
                                     blocks=self.pools[layer].blocks, tokens=q.shape[0])
         return attention(q, self.pools[layer], self.tables, step.lengths, step.starts, self._shared,

@@ -161,6 +161,16 @@ def forked(requests=7, heads=1, dim=64, block=16):
     return cache
 
 
+def test_fewer_queries_than_the_step_has():
+    """Queries of the step's first requests only, and of all of them, in one step: as KVCache allows."""
+    cache = forked()
+    q = (0.01 * torch.randn(7, 4, 64, device="cuda")).half()
+    for n in (7, 5, 7, 2):
+        out, lse = cache.attention(0, q[:n].contiguous(), return_lse=True)
+        assert grouped(cache) == n
+        check_attention(q[:n], cache.pools[0], cache.tables, cache.lengths.tolist(), [1] * n + [0] * (7 - n), out, lse)
+
+
 def test_a_refused_plan_frees_nothing():
     """Calls of `plan` that are refused leave the rows that they would have released as they were."""
     cache = forked()
