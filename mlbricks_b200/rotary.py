@@ -3,8 +3,9 @@
 ``rotate`` turns pairs of a head's elements by angles that grow with the token's position, in one launch
 for queries and keys: half and interleaved pairs, a part of the head, positions as
 ``mlbricks_b200.kvcache.plan`` gives them.  ``frequencies`` gives the pairs' frequencies, scaled for
-contexts longer than those that a model was trained on.  Inference only, as the rest of the native route: no
-autograd.  The reference has no counterpart.
+contexts longer than those that a model was trained on.  Inference only, as the rest of the native route: there is no
+backward pass, and where one is being recorded ``rotate`` refuses tensors that require gradients.  The reference
+has no counterpart.
 """
 from __future__ import annotations
 
@@ -69,6 +70,8 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
     Returns (q, k) as new tensors, or, ``inplace``, the same tensors turned where they are (their
     last dimension is then contiguous, and they share no elements).  ``k`` may be None."""
     dtype, device, shape = q.dtype, q.get_device(), q.shape
+    if torch.is_grad_enabled() and (q.requires_grad or frequencies.requires_grad or (k is not None and k.requires_grad)):
+        raise ValueError("rotate has no backward pass: call it under torch.no_grad(), or with detached tensors")
     if device < 0:
         raise ValueError("rotate needs CUDA tensors")
     if dtype not in _DTYPES:
@@ -117,6 +120,8 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
         frequencies.data_ptr(), 64 if double else 32, tokens, interleaved, scale, device, _stream(device))
     if st:
         _ebx.check(st)
+    if inplace:  # a backward pass that saved them must know
+        torch.autograd.graph.increment_version(q if k is None else (q, k))
     return a, b
 
 

@@ -88,3 +88,15 @@ def test_argument_errors_without_gpu():
     refused(call(q=side(heads=-1)), "heads")
     assert call(tokens=0) == _ebx.EBX_OK
     assert call(q=side(heads=0, input=None)) == _ebx.EBX_OK
+
+
+def test_tensors_that_require_gradients_are_refused():
+    positions, freq = torch.zeros(1, dtype=torch.int32), torch.zeros(2)
+    x, g = torch.zeros(1, 1, 4), torch.zeros(1, 1, 4, requires_grad=True)
+    for args in ((g, None, positions, freq), (x, g, positions, freq), (g * 2, x, positions, freq),
+                 (x, None, positions, freq.clone().requires_grad_())):
+        for inplace in (False, True):
+            with pytest.raises(ValueError, match="backward"):
+                rotary.rotate(*args, inplace=inplace)
+            with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):  # the next check
+                rotary.rotate(*args, inplace=inplace)
