@@ -25,6 +25,21 @@ VOCAB, DIM, HEADS, KV_HEADS, LAYERS = 512, 384, 12, 1, 3
 HEAD_DIM = DIM // HEADS
 
 
+def turn(q, k, positions, frequencies):
+    """Rotary positions of q and k [tokens, heads, HEAD_DIM]: by one launch where nothing is differentiated, else
+    in torch."""
+    if q.is_cuda and not torch.is_grad_enabled():
+        return rotary.rotate(q, k, positions, frequencies, inplace=True)
+    angle = positions[:, None, None] * frequencies
+
+    def turned(x):
+        wide = torch.promote_types(x.dtype, torch.float32)
+        cosine, sine, (a, b) = angle.cos().to(wide), angle.sin().to(wide), x.to(wide).chunk(2, -1)
+        return torch.cat([a * cosine - b * sine, b * cosine + a * sine], -1).to(x.dtype)
+
+    return turned(q), turned(k)
+
+
 class Layer(nn.Module):
     def __init__(self) -> None:
         super().__init__()
@@ -32,12 +47,13 @@ class Layer(nn.Module):
         self.k, self.v = (nn.Linear(DIM, KV_HEADS * HEAD_DIM, bias=False) for _ in "kv")
         self.up, self.down = nn.Linear(DIM, 4 * DIM), nn.Linear(4 * DIM, DIM)
         self.n1, self.n2 = nn.RMSNorm(DIM), nn.RMSNorm(DIM)
-        self.frequencies = rotary.frequencies(HEAD_DIM)
+        self.frequencies = rotary.frequencies(HEAD_DIM, device="cpu")  # not a buffer: .half() is not for angles
 
     def forward(self, x, positions, attend):
         h = self.n1(x)
         q, k = self.q(h).view(-1, HEADS, HEAD_DIM), self.k(h).view(-1, KV_HEADS, HEAD_DIM)
-        q, k = rotary.rotate(q, k, positions, self.frequencies, inplace=True)
+        self.frequencies = self.frequencies.to(x.device)  # follows the module; copies only when that has moved
+        q, k = turn(q, k, positions, self.frequencies)
         x = x + self.o(attend(q, k, self.v(h).view(-1, KV_HEADS, HEAD_DIM)).reshape(x.shape))
         return x + self.down(torch.nn.functional.gelu(self.up(self.n2(x))))
 
