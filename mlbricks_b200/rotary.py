@@ -28,7 +28,12 @@ def frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str = "none"
     * ``"linear"``: all divided by ``factor``;
     * ``"base"``: a larger base, with which the slowest pair is divided by ``factor`` and the fastest kept;
     * ``"ramp"``: pairs that make ``slow`` turns or fewer within ``trained_length`` are divided by
-      ``factor``, those that make ``fast`` or more are kept, those between go from one to the other."""
+      ``factor``, those that make ``fast`` or more are kept, and those between go from one to the other linearly in their
+      number of turns.
+
+    The bounds of a ramp are part of what a model was trained with: give both as its configuration has them.  Configurations
+    whose ramp is linear in turns usually have ``slow=1, fast=4``.  Others, often with 1 and 32, mean a ramp that is linear in the
+    pair's index between the pairs that make so many turns: another formula, which this is not, with these numbers or any."""
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
     if scaling not in SCALINGS:
