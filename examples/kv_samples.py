@@ -1,7 +1,8 @@
 """Samples of one prompt over cache blocks that they share.
 
 The decoder of kv_serving.py reads a prompt once; five more rows fork it, so that its full blocks are held once,
-and all six are sampled together, one token at a time.  Attention reads the shared blocks once for all rows.
+and all six are sampled together, one token at a time.  (Attention would read the shared blocks once for all rows if they were
+many or long; for so few tokens ``takes_prefixes`` says that each row by itself is faster.)
 At the end the cache is compacted, and the logits are compared with those of the same model over 16-bit keys and values, without
 a cache.
 

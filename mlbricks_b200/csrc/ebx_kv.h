@@ -74,7 +74,7 @@ struct KvAttnArgs {
     const int32_t* largest;       // tokens of the largest group
     float* sums;                  // [2][tokens * heads][head_dim]: O of a row that one CTA has whole,
     float2* sums_ml;              // [2][tokens * heads]: its {m, l}; of the prefix, and of what is the request's own
-    int2* where;                  // [2][tokens * heads]: which CTAs have a row's parts (kv_where)
+    int2* where;                  // [2][tokens * heads]: which CTAs have a row's parts (kv_whole, kv_begins)
 
     // With 2^(k-1) < g <= 2^k and mul = ceil(2^(31+k) / g), mul * g exceeds 2^(31+k) by less than
     // g <= 2^k, so n * mul >> (31 + k) is n / g for every n < 2^31.

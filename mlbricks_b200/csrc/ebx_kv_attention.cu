@@ -702,13 +702,19 @@ cudaError_t launch_kv_attention(KvAttnArgs a, bool bf16, int max_new, int max_le
 
 namespace {
 
-// Does reading prefixes once pay?  Not where a request brings many rows of its own, which fill row tiles by themselves; nor
-// where everything that the requests read (`most` bytes of codes, from L2) takes less time than the launches do that sharing
-// adds.  Captured, shared / each by itself, 32 heads over 8 of 128, and 16 of 64: 4 requests of 2050 tokens
-// (17 MB) 15.5 / 13.7 and 14.7 / 15.0 us, 12 of 2050 (50 MB) 17.6 / 17.9 and 16.5 / 21.4, 12 of 8050 (198 MB) 26 / 38
+// Does reading prefixes once pay?  A request of kPromptMin rows and more is never taken: here the step kernel has every request's
+// own part, and a prompt's would take long.  That is simple, and for some steps it is lost: without it, `prefixes` included,
+// shared / each by itself, 32 heads over 8 of 128 behind 8192 shared tokens, 64 requests of 13 tokens (52 rows) 253 / 566 us, of 32
+// (128 rows) 544 / 570, 63 single tokens and a chunk of 512 202 / 267; 64 of 5 tokens of 32 heads over 2 112 / 159.
+// Nor does it pay where everything that the requests read (`most` bytes of codes, from L2) takes less time than the
+// launches do that sharing adds.  Captured, shared / each by itself, 32 heads over 8 of 128, and 16 of 64: 4 requests of 2050
+// tokens (17 MB) 15.5 / 13.7 and 14.7 / 15.0 us, 12 of 2050 (50 MB) 17.6 / 17.9 and 16.5 / 21.4, 12 of 8050 (198 MB) 26 / 38
 // and 20 / 53.  With groups of kPromptMin rows and more, for which the other kernel is launched as well: 64 of 550 (72 MB)
 // 38 / 22 and 37 / 28, 64 of 1000 (131 MB) 43 / 27 and 43 / 34, 32 of 2050 (134 MB) 34 / 30 and 22 / 39, 64 of 2050 (269 MB)
 // 38 / 49 and 37 / 67, 200 of 8050 of 12 heads over one of 32 (103 MB) 47 / 62.
+// `max_length` may be a capacity that the requests do not fill, as SharedKVCache's is; then the rule says yes too early, 32 heads
+// over 8 of 128: four requests of 600 tokens in a cache for 131072 11.5 us, and 6.6 for `prefixes` once a step, by themselves 11.0; 64
+// of 600 that share nothing, in one for 8192, 24.3 / 22.2, 12 of 4000 31.1 / 24.5.
 bool takes_prefixes(const KvPool& pool, int group, int requests, int64_t tokens, int max_new, int max_length) {
     if (most_rows(group, tokens, max_new) >= kPromptMin) return false;
     if (max_length == 0) return true;  // unknown

@@ -2,8 +2,9 @@
 // and finding the prefixes that requests share.  No reference counterpart.
 //
 // The bookkeeping kernels (fork, compact, prefixes) are one cluster of CTAs each: their phases need what all
-// rows or all blocks gave in the phase before, the data are a few hundred kilobytes, and a cluster's barrier costs
-// a fraction of a launch.  Counts are changed by atomic additions only, whose order does not change
+// rows or all blocks gave in the phase before, and a cluster's barrier costs a fraction of a launch.  That is for tables of
+// up to a few hundred kilobytes; a larger one is still read and written by eight SMs (fork, all rows staying: 128 rows of 64
+// blocks 8 us, 1024 of 256 16 us, 1024 of 2048, 8 MB, 68 us, 8192 of 1024 444 us).  Counts are changed by atomic additions only, whose order does not change
 // them, and whatever is given an order (blocks to the ring, copies) gets it from sums over rows or ids.
 //
 // Each kernel lets the next one begin only after its own wait: kernels that begin while two others still run hold
@@ -84,8 +85,8 @@ __device__ __forceinline__ ForkRow fork_row(const KvForkArgs& a, int r) {
 // that wants it keeps it, the parent itself ahead of others; every other row gets a copy in a block
 // from the ring's front, in row order, or, when there are none left, nothing at all.  Blocks that nobody holds then go
 // to the ring's back in the order of their numbers.
-// What bounds it is latency: 16 or 128 rows 9.5 us, 11 from cold caches, a launch and five barriers of the cluster with
-// two or three dependent reads between each.
+// What bounds it is latency: 16 or 128 rows 9.5 us, 11 from cold caches, a launch and four barriers of the cluster
+// (and one more where blocks are missing) with two or three dependent reads between each.
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kShareThreads, 1) kv_fork_kernel(const __grid_constant__ KvForkArgs a) {
     asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
     cg::cluster_group cluster = cg::this_cluster();

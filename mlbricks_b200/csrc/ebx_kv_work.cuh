@@ -379,7 +379,7 @@ __device__ __forceinline__ float2* kv_part_ml(const KvAttnArgs& a, int cta, int 
 }
 
 // With prefixes a row of q has two results, over the prefix (side 0) and over what is its request's own (side 1), each whole or in
-// parts; kv_where says where: {-1, 0}: whole, in `sums`; else {first CTA, CTAs behind << 8 | row of the tile}, the
+// parts; `where` says which, written by the two functions below: {-1, 0}: whole, in `sums`; else {first CTA, CTAs behind << 8 | row of the tile}, the
 // CTA of the kernel for prompts as ~CTA - 1.  kv_shared_join_kernel makes one of all.
 __device__ __forceinline__ void kv_whole(const KvAttnArgs& a, int side, int64_t row) {
     a.where[side * a.tokens * a.heads + row] = make_int2(-1, 0);

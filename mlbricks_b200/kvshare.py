@@ -207,9 +207,8 @@ def attention(q: torch.Tensor, pool: KVPool, tables: torch.Tensor, lengths: torc
     by ``prefixes`` for the same tables, lengths and starts, once for all requests that share them.
 
     The formula is the same; the order of sums is not.  ``out``, if given, is not q's memory.  ``max_new``, the largest number of new tokens of a request, should be given: with
-    49 rows (max_new, or without it tokens, times heads / kv_heads) and more, requests fill the kernels' tiles by
-    themselves, and go alone; so they do where requests and ``max_length``, if given, are too few for sharing to pay
-    (``takes_prefixes``)."""
+    49 rows (max_new, or without it tokens, times heads / kv_heads) and more of one request, all requests go by themselves; so they do where requests and ``max_length``, if given, are too few for sharing to pay
+    (``takes_prefixes``).  ``max_length`` decides best as the largest length that there is, not one that there may be."""
     q = pool._rows(q, None, "q")
     device, int32 = pool.device, torch.int32
     tokens, heads, dim = q.shape
@@ -247,7 +246,9 @@ class SharedKVCache(KVCache):
     """A ``KVCache`` whose requests can share blocks.
 
     ``fork`` makes rows go on from others, frees them and rolls them back, ``compact`` renumbers blocks; both
-    come between steps: a step is planned after them.  ``attention`` reads prefixes that requests share once."""
+    come between steps: a step is planned after them.  ``attention`` reads prefixes that requests share once, where
+    ``takes_prefixes`` says that it pays if requests are as long as ``max_length``: a cache much larger than what it holds
+    is better a ``KVCache`` if nothing is shared."""
 
     def __init__(self, layers: int, blocks: int, kv_heads: int, head_dim: int, *, requests: int, max_length: int,
                  block_size: int = 64, device="cuda") -> None:
