@@ -206,9 +206,11 @@ def attention(q: torch.Tensor, pool: KVPool, tables: torch.Tensor, lengths: torc
     """``kvcache.attention`` (without ``window`` and ``first``) that reads the prefixes that ``shared`` tells of, found
     by ``prefixes`` for the same tables, lengths and starts, once for all requests that share them.
 
-    The formula is the same; the order of sums is not.  ``out``, if given, is not q's memory.  ``max_new``, the largest number of new tokens of a request, should be given: with
-    49 rows (max_new, or without it tokens, times heads / kv_heads) and more of one request, all requests go by themselves; so they do where requests and ``max_length``, if given, are too few for sharing to pay
-    (``takes_prefixes``).  ``max_length`` decides best as the largest length that there is, not one that there may be."""
+    The formula is the same; the order of sums is not.  ``out``, if given, is not q's memory.  ``max_new``, the largest
+    number of new tokens of a request, should be given: with 49 rows (max_new, or without it tokens, times heads /
+    kv_heads) and more, all requests go by themselves; so they do where requests and ``max_length``, if given, are too
+    few for sharing to pay (``takes_prefixes``).  ``max_length`` decides best as the largest length that there is, not
+    one that there may be."""
     q = pool._rows(q, None, "q")
     device, int32 = pool.device, torch.int32
     tokens, heads, dim = q.shape
